@@ -65,6 +65,12 @@ class GrftInfo(ctypes.Structure):
                 ("session_id", ctypes.c_char_p)]
 
 
+class AttnDesc(ctypes.Structure):
+    _fields_ = [("B", _i32), ("T", _i32), ("n_q_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+                ("scale", _f32), ("causal", _i32), ("q_ld", _i64), ("k_ld", _i64), ("v_ld", _i64), ("o_ld", _i64),
+                ("seq_lens", _vp)]
+
+
 class LayerDesc(ctypes.Structure):
     _fields_ = [("B", _i32), ("T", _i32), ("n_q_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
                 ("rope_theta", _f32), ("rms_eps", _f32), ("mlp", MlpDesc)]
@@ -121,6 +127,9 @@ SIGNATURES = {
     "glt_rope_fwd": (_i32, [_vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _i32, _vp]),
     "glt_attention_fwd": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _sz, _vp]),
     "glt_attention_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
+    "glt_attention_train_fwd": (_i32, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "glt_attention_bwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc)]),
+    "glt_attention_bwd": (_i32, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "glt_grft_save": (_i32, [ctypes.c_char_p, ctypes.POINTER(GrftInfo), _vp, _i32, _vp]),
     "glt_grft_load": (_i32, [ctypes.c_char_p, ctypes.POINTER(GrftInfo), _vp, _i32, _vp]),
     "glt_grft_load_raw_f32": (_i32, [ctypes.c_char_p, ctypes.POINTER(GrftInfo), _vp, _i32, _vp]),

@@ -1,0 +1,501 @@
+// Attention backward for gfx950: the gradients of
+//   s = scale q . k^T (masked), p = exp(s - lse), out = p . v
+// with the probabilities recomputed from q, k and the forward's lse:
+//   D  = rowsum(dout * out)           (= rowsum(p * dp))
+//   dp = dout . v^T,  ds = p (dp - D)
+//   dq = scale ds . k,  dk = scale ds^T . q,  dv = p^T . dout
+// (k and v gradients summed over the query heads of their group.)
+//
+// Two kernels, no atomics: attn_dq_kernel owns query rows and walks the keys
+// (three products), attn_dkdv_kernel owns key rows and walks the queries of
+// every head of the group (four products). Seven products instead of the five
+// of one pass, but every sum has one fixed order: a pass that owns key rows
+// would add dq from many workgroups at once.
+//
+// In both, a wavefront owns 32 rows whose operands (q and dout, or k and v) and
+// accumulators stay in registers; the rows that it walks come through LDS in
+// tiles of 64, loaded once (direct to LDS, double buffered) and read in both
+// directions that the products need (attention_dev.hpp). The score products
+// are formed so that a lane holds one OWNED row: the packed p or ds is then the
+// next product's operand as it stands in the accumulator's layout.
+#include <algorithm>
+#include <atomic>
+
+#include "attention_dev.hpp"
+
+namespace glt {
+
+namespace {
+
+constexpr int kTile = 64;                     // walked rows per tile
+constexpr int kTileB = kTile * kHd * 2;       // 16 KB
+constexpr float kLog2e = 1.4426950408889634f;
+// Key tiles up to which a block of rows takes D from its own probabilities.
+constexpr int kExactTiles = 8;
+
+struct BwdArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* out;
+  const uint16_t* dout;
+  const float* lse;    // [B, Hq, T]
+  float* delta;        // [B, Hq, T]: D, written by the dq kernel
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  float* part;         // Hq > Hkv: dk, dv by query head, [2][B, T, Hq, 128]
+  const int32_t* seq_lens;
+  int64_t q_ld, k_ld, v_ld, o_ld;
+  int B, T, Hq, Hkv, causal;
+  float scale;
+};
+
+__device__ __forceinline__ int seq_len(const BwdArgs& a, int b) {
+  return a.seq_lens ? min(max(a.seq_lens[b], 0), a.T) : a.T;
+}
+
+// One tile (64 rows of a head, from byte row0_bytes) into LDS, by this
+// wavefront's share of the 16 loads of 1 KB (four rows each). off: this lane's
+// byte offset of its first load (tile_lane_off); a further load lies 4 WAVES
+// rows on, a multiple of 16, where tile_key is the same. Rows past the
+// descriptor are zeros.
+template <int WAVES>
+__device__ __forceinline__ void load_tile(__amdgpu_buffer_rsrc_t r, char* dst, int wave, uint32_t off, uint32_t row_bytes,
+                                          uint32_t row0_bytes) {
+#pragma unroll
+  for (int i = 0; i < 16 / WAVES; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + (WAVES * i + wave) * 1024), 16,
+                                             off + (row0_bytes + 4 * WAVES * i * row_bytes), 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t tile_lane_off(int wave, int lane, uint32_t row_bytes) {
+  const int row = 4 * wave + (lane >> 4);
+  return (uint32_t)row * row_bytes + (uint32_t)(((lane & 15) ^ tile_key(row)) << 4);
+}
+
+// A wavefront's 32 rows of 128 as MFMA operands: lane row (lane & 31),
+// elements 16 s + 8 (lane >> 5) .. +7; rows at or past the end are zeros.
+__device__ __forceinline__ void load_rows(bf16x8* f, const uint16_t* row, bool live, int lh) {
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const u32x4 x = live ? *reinterpret_cast<const u32x4*>(row + 16 * s + 8 * lh) : u32x4{0u, 0u, 0u, 0u};
+    f[s] = __builtin_bit_cast(bf16x8, x);
+  }
+}
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// elements 8 s2 .. +7 of an accumulator, rounded: the operand of 16 contracted
+// rows in the order that col_frag() reads them
+__device__ __forceinline__ bf16x8 pack_frag(const f32x16& x, int s2) {
+  const int o = 8 * s2;
+  return __builtin_bit_cast(bf16x8, u32x4{pack2_rne(x[o], x[o + 1]), pack2_rne(x[o + 2], x[o + 3]),
+                                          pack2_rne(x[o + 4], x[o + 5]), pack2_rne(x[o + 6], x[o + 7])});
+}
+
+// Score product of 32 walked rows: x += X . f^T over the 128 columns, the
+// fragments read kAhead steps ahead; between(i) is arithmetic that the
+// scheduler may put beside step i's matrix instruction. (The fence per step
+// keeps the reads from all being hoisted, which needs more registers than
+// there are.)
+constexpr int kAhead = 2;
+template <typename F>
+__device__ __forceinline__ void score_product(uint32_t X, const bf16x8* f, f32x16& x, F between) {
+  bf16x8 xa[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) xa[i] = row_frag(X, i);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x = mfma(xa[i % kAhead], f[i], x);
+    if (i + kAhead < 8) xa[i % kAhead] = row_frag(X, i + kAhead);
+    between(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+// an address that is worked out where it is used, not kept in a register for
+// every offset
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// Accumulator of a transposed product (lane: owned row, elements: d = 32 db +
+// 8 g + 4 lh + e) times `scale`, rounded once, to this lane's output row.
+__device__ __forceinline__ void store_rows(uint16_t* row, const f32x16* acc, float scale, int lh) {
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const u32x2a w = {pack2_rne(acc[db][4 * g] * scale, acc[db][4 * g + 1] * scale),
+                        pack2_rne(acc[db][4 * g + 2] * scale, acc[db][4 * g + 3] * scale)};
+      *reinterpret_cast<u32x2a*>(row + 32 * db + 8 * g + 4 * lh) = w;
+    }
+}
+
+// ------------------------------------------------------------------- dq
+// One workgroup per (batch, query head, block of 32 WAVES queries), longest
+// rows first. LDS: two buffers of a K and a V tile (64 KB).
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, lq = lane & 31, lh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nqb = (a.T + 32 * WAVES - 1) / (32 * WAVES);
+  const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
+  const int id = blockIdx.x, hb = id % nhb;
+  const int qb = nqb - 1 - id / nhb;
+  const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
+  const int q0 = qb * 32 * WAVES, wq0 = q0 + 32 * wave, myq = wq0 + lq;
+  const int len = seq_len(a, b);
+  const bool live = myq < len;
+  const int kv_end = q0 >= len ? 0 : a.causal ? min(len, q0 + 32 * WAVES) : len;
+  const int ntiles = (kv_end + kTile - 1) / kTile;
+  const int64_t tok = (int64_t)b * a.T + min(myq, a.T - 1);
+  const int64_t stat = ((int64_t)b * a.Hq + h) * a.T + min(myq, a.T - 1);
+
+  const __amdgpu_buffer_rsrc_t rk = uni_rsrc_a(a.k + (int64_t)b * a.T * a.k_ld + (int64_t)g * kHd, rows_extent(len, a.k_ld));
+  const __amdgpu_buffer_rsrc_t rv = uni_rsrc_a(a.v + (int64_t)b * a.T * a.v_ld + (int64_t)g * kHd, rows_extent(len, a.v_ld));
+  const uint32_t kb_ld = (uint32_t)(a.k_ld * 2), vb_ld = (uint32_t)(a.v_ld * 2);  // bytes
+  const uint32_t kof = tile_lane_off(wave, lane, kb_ld), vof = tile_lane_off(wave, lane, vb_ld);
+  auto load = [&](int t, int buf) {
+    char* dst = smem + buf * 2 * kTileB;
+    load_tile<WAVES>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
+    load_tile<WAVES>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
+  };
+  if (ntiles > 0) load(0, 0);
+
+  bf16x8 qf[8], dof[8];
+  load_rows(qf, a.q + tok * a.q_ld + (int64_t)h * kHd, live, lh);
+  load_rows(dof, a.dout + tok * a.o_ld + (int64_t)h * kHd, live, lh);
+  const float lse2 = live ? a.lse[stat] * kLog2e : 0.f;
+  // D of the lane's row: the diagonal of out . dout^T. The matrix product sums
+  // it in the order in which it sums dp, so a row whose output is one key's
+  // value (a single key) gets ds = 0 exactly.
+  float D;
+  {
+    bf16x8 of[8];
+    load_rows(of, a.out + tok * a.o_ld + (int64_t)h * kHd, live, lh);
+    f32x16 x{};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x = mfma(of[s], dof[s], x);
+    // row lq = 8 (lq >> 3) + 4 ((lq >> 2) & 1) + (lq & 3) of column lq
+    const int e = 4 * (lq >> 3) + (lq & 3);
+    float y = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) y = e == i ? x[i] : y;
+    D = pair_sum(((lq >> 2) & 1) == lh ? y : 0.f);
+  }
+
+  const uint32_t ro = lds_addr(smem) + row_frag_off(lane), co = lds_addr(smem) + col_frag_off(lane);
+  const float scale_log2 = a.scale * kLog2e;
+
+  // Score products of key block kb (32 keys) of tile t: p in s, dp.
+  auto probs = [&](int t, int kb, uint32_t row, f32x16& s, f32x16& dp) {
+    const int key0 = t * kTile + 32 * kb;
+    score_product(row, qf, s, [](int) {});
+    if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {
+      const int lim = (a.causal ? min(len, myq + 1) : len) - (key0 + 4 * lh);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < lim ? s[e] : -INFINITY;
+    }
+    // the exponentials beside the other product
+    score_product(row + kTileB, dof, dp, [&](int i) {
+#pragma unroll
+      for (int e = 2 * i; e < 2 * i + 2; ++e)
+        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale_log2, -lse2));
+    });
+  };
+  // Walks the tiles; step u of the workgroup uses buffer u & 1. block(t, kb,
+  // row, col) gets each 32-key block that this wavefront's rows read.
+  auto walk = [&](int u0, bool last, auto block) {
+    for (int t = 0; t < ntiles; ++t) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
+      phase_barrier();  // this step's tiles are whole, and every wavefront is done with the step before
+      const int u = u0 + t;
+      if (t + 1 < ntiles) load(t + 1, (u + 1) & 1);
+      else if (!last) load(0, (u + 1) & 1);
+      const uint32_t buf = (u & 1) * 2 * kTileB;  // K tile, V tile
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int key0 = t * kTile + 32 * kb;
+        if (key0 >= kv_end || (a.causal && key0 > wq0 + 31)) continue;
+        block(t, kb, opaque(ro + buf + kb * 8192), opaque(co + buf + kb * 8192));
+      }
+    }
+  };
+
+  // D from out carries out's rounding, which counts where few keys share a
+  // row's weight: dp - D nearly cancels there. Such rows take it from the
+  // probabilities, as D + sum p (dp - D), in a walk of their own.
+  const bool exact = ntiles <= kExactTiles;
+  if (exact) {
+    float d = 0.f;
+    walk(0, false, [&](int t, int kb, uint32_t row, uint32_t) {
+      f32x16 s{}, dp{};
+      probs(t, kb, row, s, dp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) d = __builtin_fmaf(s[e], dp[e] - D, d);
+    });
+    D += pair_sum(d);
+  }
+  if (lh == 0 && myq < a.T) a.delta[stat] = live ? D : 0.f;
+
+  f32x16 dq[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
+  walk(exact ? ntiles : 0, true, [&](int t, int kb, uint32_t row, uint32_t col) {
+    f32x16 s{}, dp{};
+    probs(t, kb, row, s, dp);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] *= dp[e] - D;
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      const bf16x8 f = pack_frag(s, s2);
+#pragma unroll
+      for (int db = 0; db < 4; ++db) dq[db] = mfma(col_frag(col, db, s2), f, dq[db]);
+    }
+  });
+  if (myq < a.T) {
+    if (!live)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
+    store_rows(a.dq + tok * a.q_ld + (int64_t)h * kHd, dq, a.scale, lh);
+  }
+}
+
+// ---------------------------------------------------------------- dk, dv
+// One workgroup per (batch, query head, block of 32 WAVES keys), the blocks
+// with the most queries first. LDS: two buffers of a Q and a dout tile and their
+// 64 lse and D values. Where query heads share a kv head, each writes its f32
+// part and attn_dkdv_sum_kernel adds the parts in head order: a workgroup that
+// walked the group's heads one after the other would leave too few workgroups
+// for the chip (2 x 4096 tokens, 8 kv heads: 256 of very different length),
+// and a cut that depends on the batch would make the sums' order depend on it.
+constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
+
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) attn_dkdv_kernel(const BwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, lq = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
+  const int id = blockIdx.x, hb = id % nhb, kb = id / nhb;
+  const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
+  const int k0 = kb * 32 * WAVES, wk0 = k0 + 32 * wave;
+  const int len = seq_len(a, b);
+
+  bf16x8 kf[8], vf[8];
+  {
+    const int64_t tok = (int64_t)b * a.T + min(wk0 + lq, a.T - 1);
+    load_rows(kf, a.k + tok * a.k_ld + (int64_t)g * kHd, wk0 + lq < len, lane >> 5);
+    load_rows(vf, a.v + tok * a.v_ld + (int64_t)g * kHd, wk0 + lq < len, lane >> 5);
+  }
+
+  // query tiles of this workgroup
+  const int qt0 = a.causal ? k0 / kTile : 0;
+  const int qt1 = k0 < len ? (len + kTile - 1) / kTile : qt0;
+  const uint32_t qb_ld = (uint32_t)(a.q_ld * 2), ob_ld = (uint32_t)(a.o_ld * 2);  // bytes
+  // rows at or past len read as zeros, lse and D too: p = 1 there, dp - D = 0
+  // and dout = 0, so they add nothing
+  const __amdgpu_buffer_rsrc_t rq = uni_rsrc_a(a.q + (int64_t)b * a.T * a.q_ld + (int64_t)h * kHd, rows_extent(len, a.q_ld));
+  const __amdgpu_buffer_rsrc_t rdo = uni_rsrc_a(a.dout + (int64_t)b * a.T * a.o_ld + (int64_t)h * kHd, rows_extent(len, a.o_ld));
+  const __amdgpu_buffer_rsrc_t rs = uni_rsrc_a((wave & 1 ? a.delta : a.lse) + ((int64_t)b * a.Hq + h) * a.T, (uint32_t)len * 4);
+  auto load = [&](int qt, int buf) {
+    char* dst = smem + buf * kDkdvBuf;
+    const int l = opaque(threadIdx.x) & 63;
+    load_tile<WAVES>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld);
+    load_tile<WAVES>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld);
+    if (wave < 2)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + 2 * kTileB + wave * kTile * 4), 4,
+                                               (uint32_t)(qt * kTile + l) * 4, 0, 0, 0);
+  };
+  if (qt0 < qt1) load(qt0, 0);
+
+  const uint32_t ro = lds_addr(smem) + row_frag_off(lane), co = lds_addr(smem) + col_frag_off(lane);
+  f32x16 dk[4], dv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dk[i] = dv[i] = f32x16{};
+  const float scale_log2 = a.scale * kLog2e;
+
+  for (int qt = qt0; qt < qt1; ++qt) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
+    phase_barrier();  // tile qt is whole, and every wavefront is done with tile qt - 1
+    const int q0t = qt * kTile, cur = (qt - qt0) & 1;
+    if (qt + 1 < qt1) load(qt + 1, cur ^ 1);
+    const uint32_t buf = cur * kDkdvBuf;  // Q tile, dout tile, lse, D
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const int q0 = q0t + 32 * qb;
+      if (q0 >= len || (a.causal && q0 + 31 < wk0)) continue;
+      f32x16 s{}, dp{};
+      const uint32_t row = opaque(ro + buf + qb * 8192);
+      score_product(row, kf, s, [](int) {});
+      if (a.causal && q0 < wk0 + 31) {  // row q0 + 8 (e >> 2) + 4 lh + (e & 3) reads keys up to itself
+        const int l = opaque(threadIdx.x) & 63;
+        const int lim = wk0 + (l & 31) - (q0 + 4 * (l >> 5));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= lim ? s[e] : -INFINITY;
+      }
+      // the exponentials beside the other product; elements 4 i .. + 3 are
+      // query rows 8 i + 4 lh .. + 3
+      const uint32_t st = opaque(lds_addr(smem) + buf + 2 * kTileB + 128 * qb + 16 * (lane >> 5));
+      score_product(row + kTileB, vf, dp, [&](int i) {
+        const f32x2 l = *reinterpret_cast<const lds_f32x2*>((uintptr_t)(st + 32 * (i >> 1) + 8 * (i & 1)));
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s[2 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + e], scale_log2, -l[e] * kLog2e));
+      });
+      u32x4 pw[2], dw[2];  // packed p and ds
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 D = *reinterpret_cast<const lds_f32x4*>((uintptr_t)(st + 32 * i + kTile * 4));
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const int x = 4 * i + e, w = 2 * (i & 1) + e / 2;
+          pw[i >> 1][w] = pack2_rne(s[x], s[x + 1]);
+          dw[i >> 1][w] = pack2_rne(s[x] * (dp[x] - D[e]), s[x + 1] * (dp[x + 1] - D[e + 1]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const uint32_t col = opaque(co + buf + qb * 8192);
+      bf16x8 oa[kAhead], qa[kAhead];  // step i: 16 query rows i >> 2, d block i & 3
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        oa[i] = col_frag(col + kTileB, i & 3, i >> 2);
+        qa[i] = col_frag(col, i & 3, i >> 2);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dv[i & 3] = mfma(oa[i % kAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), dv[i & 3]);
+        dk[i & 3] = mfma(qa[i % kAhead], __builtin_bit_cast(bf16x8, dw[i >> 2]), dk[i & 3]);
+        if (i + kAhead < 8) {
+          oa[i % kAhead] = col_frag(col + kTileB, (i + kAhead) & 3, (i + kAhead) >> 2);
+          qa[i % kAhead] = col_frag(col, (i + kAhead) & 3, (i + kAhead) >> 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  // the output rows' addresses are worked out again here: kept across the
+  // loop they cost registers that it does not have
+  const int tid = opaque(threadIdx.x);
+  const int lh = (tid >> 5) & 1, myk = k0 + 32 * (tid >> 6) + (tid & 31);
+  const int64_t tok = (int64_t)b * a.T + myk;
+  if (myk >= a.T) return;
+  if (myk >= len)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dk[i] = dv[i] = f32x16{};
+  if (rep == 1) {
+    store_rows(a.dk + tok * a.k_ld + (int64_t)g * kHd, dk, a.scale, lh);
+    store_rows(a.dv + tok * a.v_ld + (int64_t)g * kHd, dv, 1.0f, lh);
+    return;
+  }
+  float* pk = a.part + (tok * a.Hq + h) * kHd + 4 * lh;
+  float* pv = pk + (int64_t)a.B * a.T * a.Hq * kHd;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<f32x4*>(pk + 32 * db + 8 * i) = f32x4{dk[db][4 * i], dk[db][4 * i + 1], dk[db][4 * i + 2], dk[db][4 * i + 3]};
+      *reinterpret_cast<f32x4*>(pv + 32 * db + 8 * i) = f32x4{dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]};
+    }
+}
+
+// dk (blockIdx.y 0) or dv (1): the parts of a group's query heads added in head
+// order, rounded once; a thread takes 8 elements of a token's kv head.
+__global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int rep = a.Hq / a.Hkv, cols = a.Hkv * (kHd / 8);
+  if (i >= (int64_t)a.B * a.T * cols) return;
+  const int64_t row = i / cols;
+  const int c = (int)(i - row * cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
+  const float* p = a.part + ((blockIdx.y ? (int64_t)a.B * a.T : 0) + row) * a.Hq * kHd + (int64_t)g * rep * kHd + e;
+  f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+  for (int s = 1; s < rep; ++s) {
+    x += *reinterpret_cast<const f32x4*>(p + s * kHd);
+    y += *reinterpret_cast<const f32x4*>(p + s * kHd + 4);
+  }
+  const float f = blockIdx.y ? 1.0f : a.scale;
+  uint16_t* dst = blockIdx.y ? a.dv + row * a.v_ld : a.dk + row * a.k_ld;
+  *reinterpret_cast<u32x4*>(dst + g * kHd + e) =
+      u32x4{pack2_rne(x[0] * f, x[1] * f), pack2_rne(x[2] * f, x[3] * f), pack2_rne(y[0] * f, y[1] * f),
+            pack2_rne(y[2] * f, y[3] * f)};
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t delta_bytes(const glt_attn_desc* d) { return round256((size_t)d->B * d->n_q_heads * d->T * sizeof(float)); }
+size_t part_bytes(const glt_attn_desc* d) {
+  return d->n_q_heads > d->n_kv_heads ? (size_t)2 * d->B * d->T * d->n_q_heads * kHd * sizeof(float) : 0;
+}
+
+template <int WAVES>
+glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
+  constexpr int kDqLds = 4 * kTileB, kDkdvLds = 2 * kDkdvBuf;
+  // the dynamic-LDS limit is a per-device attribute of the kernels
+  static std::atomic<bool> attr_set[64];
+  int dev = 0;
+  GLT_TRY_HIP(hipGetDevice(&dev));
+  GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_attention_bwd: device index %d out of range", dev);
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_dq_kernel<WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, kDqLds));
+    GLT_TRY_HIP(
+        hipFuncSetAttribute((const void*)attn_dkdv_kernel<WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  const unsigned nb = (unsigned)cdiv(a.T, 32 * WAVES);
+  GLT_LAUNCH("attn_dq", attn_dq_kernel<WAVES>, dim3(nb * a.Hq * a.B), dim3(WAVES * 64), kDqLds, st, a);
+  GLT_LAUNCH_CHECK("attn_dq");
+  GLT_LAUNCH("attn_dkdv", attn_dkdv_kernel<WAVES>, dim3(nb * a.Hq * a.B), dim3(WAVES * 64), kDkdvLds, st, a);
+  GLT_LAUNCH_CHECK("attn_dkdv");
+  if (a.Hq > a.Hkv) {
+    const int64_t chunks = (int64_t)a.B * a.T * a.Hkv * (kHd / 8);
+    GLT_LAUNCH("attn_dkdv_sum", attn_dkdv_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
+    GLT_LAUNCH_CHECK("attn_dkdv_sum");
+  }
+  return GLT_OK;
+}
+
+}  // namespace
+
+}  // namespace glt
+
+using namespace glt;
+
+extern "C" size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d) {
+  if (!d || d->B <= 0 || d->T <= 0 || d->n_q_heads <= 0 || d->n_kv_heads <= 0) return 256;
+  return delta_bytes(d) + part_bytes(d);
+}
+
+extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
+                                        const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                        void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  const glt_status s = check_attn_desc(d, "glt_attention_bwd");
+  if (s != GLT_OK) return s;
+  if (d->B == 0 || d->T == 0) return GLT_OK;
+  GLT_CHECK(q && k && v && out && lse && dout && dq && dk && dv, GLT_ERR_INVALID_ARG, "glt_attention_bwd: null pointer");
+  const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq |
+                        (uintptr_t)dk | (uintptr_t)dv;
+  GLT_CHECK(all % 16 == 0 && (uintptr_t)lse % 4 == 0 && (uintptr_t)d->seq_lens % 4 == 0, GLT_ERR_ALIGNMENT,
+            "glt_attention_bwd: tensors must be 16-byte aligned");
+  const size_t need = glt_attention_bwd_workspace_size(d);
+  GLT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, GLT_ERR_WORKSPACE,
+            "glt_attention_bwd: needs %zu workspace bytes, 256-byte aligned", need);
+  BwdArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<const uint16_t*>(out);
+  a.dout = static_cast<const uint16_t*>(dout);
+  a.lse = lse;
+  a.delta = static_cast<float*>(workspace);
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(d));
+  a.seq_lens = d->seq_lens;
+  a.q_ld = d->q_ld; a.k_ld = d->k_ld; a.v_ld = d->v_ld; a.o_ld = d->o_ld;
+  a.B = d->B; a.T = d->T; a.Hq = d->n_q_heads; a.Hkv = d->n_kv_heads;
+  a.causal = d->causal; a.scale = d->scale;
+  return launch_bwd<8>(a, as_stream(stream));
+}

@@ -220,6 +220,116 @@ def attention(q, k, v, causal=True, scale=None):
     return out
 
 
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _workspace(ws, nbytes, device):
+    """ws where it is given (uint8, on the device, at least nbytes), else new."""
+    if ws is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if ws.dtype != torch.uint8 or ws.device != device or not ws.is_contiguous() or ws.numel() < nbytes:
+        raise ValueError(f"workspace: {nbytes} contiguous uint8 on {device}")
+    return ws
+
+
+def _call_on(t, name, *args):
+    """The entry point on t's device and that device's current stream, which
+    is passed last."""
+    if t.device.index == torch.cuda.current_device():
+        F.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(t.device):
+            F.call(name, *args, _stream())
+
+
+def _heads_ld(name, t, B, T, device):
+    """Elements between the tokens of t [B, T, heads, head_dim]; heads lie
+    next to each other, sequences T tokens apart."""
+    shape = t.shape
+    if len(shape) != 4 or shape[0] != B or shape[1] != T or t.dtype != torch.bfloat16 or t.device != device:
+        raise ValueError(f"{name}: bf16 [{B}, {T}, heads, head_dim] on {device}, not {t.dtype} {tuple(shape)} on "
+                         f"{t.device}")
+    H, hd = shape[2], shape[3]
+    if B * T == 0:
+        return H * hd
+    sb, st, sh, se = t.stride()
+    ld = st if T > 1 else sb if B > 1 else H * hd
+    if (hd > 1 and se != 1) or (H > 1 and sh != hd) or (B > 1 and sb != T * ld):
+        raise ValueError(f"{name}: strides {t.stride()} (a token's heads contiguous, tokens evenly spaced)")
+    return ld
+
+
+def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
+    _need(q.dim() == 4 and q.is_cuda, "q: [B, T, heads, head_dim] on a GPU")
+    B, T, Hq, hd = q.shape
+    dev = q.device
+    lds = (_heads_ld("q", q, B, T, dev), _heads_ld("k", k, B, T, dev), _heads_ld("v", v, B, T, dev),
+           _heads_ld("out", out, B, T, dev))
+    _need(k.shape == v.shape and k.shape[3] == hd and out.shape == q.shape, "k, v and out do not fit q")
+    if seq_lens is not None and not (seq_lens.dtype == torch.int32 and tuple(seq_lens.shape) == (B,)
+                                     and seq_lens.device == dev and seq_lens.is_contiguous()):
+        raise ValueError(f"seq_lens: contiguous int32 [{B}] on {dev}")
+    return F.AttnDesc(B, T, Hq, k.shape[2], hd, hd ** -0.5 if scale is None else scale, 1 if causal else 0, *lds,
+                      _p(seq_lens))
+
+
+def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
+    """GQA attention forward of a training step: (out [B,T,Hq,hd] bf16, lse
+    [B,Hq,T] f32) for attention_bwd. q [B,T,Hq,hd], k/v [B,T,Hkv,hd] bf16, also
+    as views of one projection output [B,T,(Hq+2Hkv)*hd]. seq_lens int32 [B]:
+    the lengths of a padded batch (rows past them: zero output, lse -inf)."""
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    d = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
+    lse = torch.empty((d.B, d.n_q_heads, d.T), dtype=torch.float32, device=q.device)
+    _call_on(q, "glt_attention_train_fwd", ctypes.byref(d), _p(q), _p(k), _p(v), _p(out), _p(lse))
+    return out, lse
+
+
+def _attn_grad_buffers(q, k, v, d):
+    """Gradients with the strides of q, k, v: parts of one buffer where q, k, v
+    are parts of one (that do not overlap)."""
+    ld, rows = d.q_ld, d.B * d.T
+    if ld == d.k_ld == d.v_ld:
+        first = min(q.data_ptr(), k.data_ptr(), v.data_ptr())
+        offs = [(t.data_ptr() - first) // 2 for t in (q, k, v)]
+        end = 0
+        for o, t in sorted(zip(offs, (q, k, v)), key=lambda x: x[0]):
+            if o < end:
+                break
+            end = o + t.shape[2] * t.shape[3]
+        else:
+            if end <= ld:
+                buf = torch.empty(rows * ld, dtype=q.dtype, device=q.device)
+                return [buf.as_strided(t.shape, (d.T * ld, ld, t.shape[3], 1), o) for o, t in zip(offs, (q, k, v))]
+    return [torch.empty(rows * n, dtype=q.dtype, device=q.device).as_strided(t.shape, (d.T * n, n, t.shape[3], 1))
+            for t, n in ((q, ld), (k, d.k_ld), (v, d.v_ld))]
+
+
+def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=None, grads=None, workspace=None):
+    """(dq, dk, dv) of attention_train, bf16 with the strides of q, k, v (parts
+    of one buffer where q, k, v are; `grads` gives them). out and lse are the
+    forward's; dout has out's shape and strides. workspace: a uint8 tensor of
+    glt_attention_bwd_workspace_size bytes to use instead of a new one."""
+    d = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
+    B, T, dev = d.B, d.T, q.device
+    _need(_heads_ld("dout", dout, B, T, dev) == d.o_ld and dout.shape == out.shape, "dout: out's shape and strides")
+    if lse.dtype != torch.float32 or lse.shape != (B, d.n_q_heads, T) or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError(f"lse: contiguous f32 [{B}, {d.n_q_heads}, {T}] on {dev}")
+    if grads is None:
+        grads = _attn_grad_buffers(q, k, v, d)
+    else:
+        for n, t, x, ld in zip(("dq", "dk", "dv"), grads, (q, k, v), (d.q_ld, d.k_ld, d.v_ld)):
+            _need(t.shape == x.shape and _heads_ld(n, t, B, T, dev) == ld, "dq, dk, dv: the shapes and strides of q, k, v")
+    nb = F.load().glt_attention_bwd_workspace_size(ctypes.byref(d))
+    workspace = _workspace(workspace, nb, dev)
+    dq, dk, dv = grads
+    _call_on(q, "glt_attention_bwd", ctypes.byref(d), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(dout), _p(dq), _p(dk),
+             _p(dv), _p(workspace), workspace.numel())
+    return dq, dk, dv
+
+
 def adamw_step(w, g, m, v, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, clip_norm=0.0,
                mirror=None):
     """One AdamW step (reference adamw_fused_kernel + optional global clip)."""

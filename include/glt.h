@@ -319,6 +319,46 @@ glt_status glt_attention_fwd(const void* q, const void* k, const void* v, void* 
                              int32_t head_dim, float scale, int32_t causal, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* Attention of a training step: the forward that keeps each row's log-sum-exp
+ * and the backward that recomputes the probabilities from it (the reference
+ * re-runs its forward under autograd, src/attention_autograd_impl.inc:1-39).
+ * Tensors as in glt_attention_fwd, with a stride: token (b, t) of q starts at
+ * element (b * T + t) * q_ld, head h at + h * 128 (k, v, out alike), so q, k, v
+ * may be parts of one projection output of (n_q_heads + 2 n_kv_heads) * 128
+ * columns. Strides are multiples of 8 and at least the heads' columns;
+ * T + 256 rows of each stay under 2 GiB.
+ * seq_lens (device [B], NULL = all T; values outside [0, T] are clamped): the
+ * sequences of a padded batch. Keys at or past a sequence's length take no
+ * part, whatever the buffers hold there, NaN included; its rows past it get
+ * zero output, lse -inf and zero gradients.
+ * scale is positive and finite. head_dim must be 128; tensors 16-byte aligned. */
+typedef struct {
+  int32_t B, T, n_q_heads, n_kv_heads, head_dim;
+  float scale;
+  int32_t causal;
+  int64_t q_ld, k_ld, v_ld, o_ld; /* elements between a sequence's tokens */
+  const int32_t* seq_lens;
+} glt_attn_desc;
+/* out = softmax(scale q . k^T + mask) . v (bf16), lse [B, n_q_heads, T] f32 =
+ * log(sum exp) of each row's scaled scores. Statistics, sums and products in
+ * f32; probabilities rounded to bf16 for the product with v. No workspace. */
+glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
+                                   void* out, float* lse, void* stream);
+
+/* dq, dk, dv (bf16, with the strides of q, k, v) from dout (out's stride) and
+ * the forward's out and lse: D = rowsum(dout * out), p = exp(scale q.k - lse),
+ * ds = p (dout.v - D), dq = scale ds . k, dk = scale ds^T . q, dv = p^T . dout,
+ * k and v gradients summed over the query heads of their group. p and ds are
+ * rounded to bf16 for the products, sums are f32 in one fixed order (a sequence's
+ * gradients do not depend on the others of the call, nor on the run). Rows past a
+ * sequence's length are zero. The gradients overlap no input. workspace:
+ * glt_attention_bwd_workspace_size bytes, 256-byte aligned, nothing kept in
+ * it between calls. */
+size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d);
+glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
+                             const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                             void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------- decoder layer */
 /* One decoder layer forward with the grafted MLP (reference forward_layer,
  * src/layer_forward_impl.inc:15-290):
