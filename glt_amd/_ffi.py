@@ -170,6 +170,10 @@ SIGNATURES = {
     "glt_masked_ce_workspace_size": (_sz, [_i32, _i32]),
     "glt_masked_ce": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, ctypes.c_float, _vp, _i64, _vp, _vp, _vp, _sz,
                              _vp]),
+    "glt_token_logprobs_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
+    "glt_token_logprobs": (_i32, [_vp, _i32, _i64, _i32, _i32, _f32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                  _vp]),
+    "glt_token_logprobs_bwd": (_i32, [_vp, _i32, _i64, _i32, _i32, _f32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "glt_silence_energy": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _vp]),
     "glt_silence_blend": (_i32, [_vp, _vp, _vp, _i32, _i32, ctypes.c_float, _vp]),
     "glt_silence_blend_energy": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, ctypes.c_float, _vp]),

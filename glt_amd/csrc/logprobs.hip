@@ -1,0 +1,668 @@
+// Log probabilities of given tokens, entropy and top alternatives of rows of
+// logits, and the gradient of the first two.
+//
+//   z = x / temperature, lse = log sum exp z, logp_v = z_v - lse, p = exp logp
+//   entropy H = -sum p logp = lse - sum p z
+//   d logp_id / dz_v = [v = id] - p_v,  dH / dz_v = -p_v (logp_v + H)
+//
+// Everything is read once and bound by HBM: 2 or 4 bytes a logit forward, twice
+// that backward, against about ten vector instructions.
+//
+// Forward: one workgroup of four wavefronts per piece of a row (32 KB, held in
+// registers: eight 16-byte chunks a thread, chunk k of thread t being chunk
+// 256 k + t), each wavefront leaving its maximum, sum exp and sum z exp, and the
+// workgroup its k largest logits; one wavefront per row then joins the row's
+// parts in their order, in 64 bits. The cut depends on V alone, so a row has the
+// same bits in every call, and a single row still spreads over V / 16384
+// workgroups (bf16; half as many logits a piece in f32).
+//
+// In log2 units c = log2(e) / temperature: a wavefront's shift is the rounded
+// product m c of its maximum, the terms exp2(fma(x, c, -shift)); the shift is
+// exactly what the joined sum is told, so its rounding does not enter.
+#include <cmath>
+
+#include "common.hpp"
+
+namespace glt {
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kChunks = 8;                       // 16-byte chunks a thread holds
+constexpr int kMaxTop = 64;                      // alternatives at most: one per lane of the selecting wavefront
+constexpr int kMaxIds = 64;
+constexpr int kMaxV = 1 << 20;
+constexpr int kCap = 1024;                       // candidates of a piece held in LDS
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453094;
+
+// 16 bytes of logits at any element address (gfx950 loads and stores
+// unaligned vectors; rows of an odd vocabulary start anywhere)
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+template <typename T>
+struct Elems;
+template <>
+struct Elems<uint16_t> {
+  static constexpr int n = 8;
+  static __device__ __forceinline__ float get(const u32x4& c, int e) {
+    return (e & 1) ? __uint_as_float(c[e >> 1] & 0xFFFF0000u) : __uint_as_float(c[e >> 1] << 16);
+  }
+  static constexpr uint32_t neg_inf = 0xFF80u;
+  static __device__ __forceinline__ void put(u32x4& c, int e, uint32_t bits) { c[e >> 1] |= bits << (16 * (e & 1)); }
+};
+template <>
+struct Elems<float> {
+  static constexpr int n = 4;
+  static __device__ __forceinline__ float get(const u32x4& c, int e) { return __uint_as_float(c[e]); }
+  static constexpr uint32_t neg_inf = 0xFF800000u;
+  static __device__ __forceinline__ void put(u32x4& c, int e, uint32_t bits) { c[e] = bits; }
+};
+template <typename T>
+constexpr int kPiece = kThreads * kChunks * Elems<T>::n;  // logits per workgroup
+
+__device__ __forceinline__ uint32_t bits_of(uint16_t v) { return v; }
+__device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ float value_of(uint16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ float value_of(float v) { return v; }
+
+// Chunk of a row from element e; elements at or past V are -inf.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* row, int e, int V) {
+  using E = Elems<T>;
+  if (e + E::n <= V) return *reinterpret_cast<const u32x4_any*>(row + e);
+  u32x4 c = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < E::n; ++j) E::put(c, j, e + j < V ? bits_of(row[e + j]) : E::neg_inf);
+  return c;
+}
+
+// Order-preserving integer of a float's bits (NaN beyond the infinities; both
+// zeros are one value).
+__device__ __forceinline__ uint32_t ord(float f) {
+  const uint32_t u = __float_as_uint(f + 0.0f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_ord(uint32_t o) {
+  return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu));
+}
+// Key of a candidate: larger is better, the lower index among equal values.
+__device__ __forceinline__ uint64_t make_key(uint32_t o, uint32_t index) { return (uint64_t)o << 32 | (0xFFFFFFFFu - index); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// A wavefront's part of a row: sum of exp2(a - shift) and of (a - shift)
+// exp2(a - shift) over its logits, a = x c.
+struct Part {
+  double shift;
+  float s, t;
+};
+
+struct TopLds {
+  uint32_t group[kWaves][64];
+  uint32_t tau, count, bad;
+  uint32_t sums[kWaves];
+  uint64_t cand[kCap];
+};
+
+// Appends the lanes' keys where `hit`: one LDS atomic per wavefront.
+__device__ __forceinline__ void append(TopLds& L, bool hit, uint64_t key) {
+  const uint64_t mask = __ballot(hit);
+  if (!mask) return;
+  const int lane = threadIdx.x & 63;
+  uint32_t base = 0;
+  if (lane == __ffsll((unsigned long long)mask) - 1) base = atomicAdd(&L.count, (uint32_t)__popcll(mask));
+  base = __shfl(base, __ffsll((unsigned long long)mask) - 1);
+  const uint32_t at = base + __popcll(mask & ((1ull << lane) - 1));
+  if (hit && at < kCap) L.cand[at] = key;
+}
+
+// Sum over the workgroup of a per-thread count (all threads get it).
+__device__ __forceinline__ uint32_t block_count(TopLds& L, uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) L.sums[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return L.sums[0] + L.sums[1] + L.sums[2] + L.sums[3];
+}
+
+// The k largest logits of the piece, in order, as keys to out[0, k).
+// c: the thread's chunks, cm: their maxima, nan: the thread saw one (or +inf).
+//
+// A bound first: the k-th largest of the 64 lanes' maxima (over the four
+// wavefronts) is at most the k-th largest logit; found by bisection over the
+// bits on one wavefront. The logits that reach it (some k more than k) are
+// collected and ranked by counting. Where they are more than kCap, they are
+// either mostly equal to the bound (a masked vocabulary, a constant row): those
+// above it are collected, then equal ones by index; or they are not, or NaNs
+// have spoilt the maxima: the exact k-th key by bisection over all logits. Those
+// two read the piece again, a chunk at a time, so that the ordinary one keeps
+// its registers.
+template <typename T>
+__device__ __forceinline__ void piece_top(const T* x, const u32x4* c, const float* cm, bool nan, int e0, int V, int k,
+                                          uint64_t* out, TopLds& L) {
+  using E = Elems<T>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto elem0 = [&](int q) { return e0 + (q * kThreads + tid) * E::n; };
+  float m = cm[0];
+#pragma unroll
+  for (int q = 1; q < kChunks; ++q) m = fmaxf(m, cm[q]);
+  L.group[wave][lane] = ord(m);
+  if (tid == 0) L.count = L.bad = 0;
+  __syncthreads();
+  if (nan) L.bad = 1;
+  if (wave == 0) {
+    uint32_t g = L.group[0][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) g = max(g, L.group[w][lane]);
+    // the largest value that at least k lanes reach
+    constexpr int low = sizeof(T) == 2 ? 16 : 0;
+    uint32_t tau = 0;
+#pragma unroll 1
+    for (int b = 31; b >= low; --b) {
+      const uint32_t y = tau | (1u << b);
+      if (__popcll(__ballot(g >= y)) >= k) tau = y;
+    }
+    // bf16: the low half of ord() follows from the sign
+    if (low && !(tau & 0x80000000u)) tau |= 0xFFFFu;
+    if (lane == 0) L.tau = max(tau, 0x007FFFFFu);  // -inf
+  }
+  __syncthreads();
+  const float tf = from_ord(L.tau);
+  bool exact = L.bad != 0;
+  if (!exact) {
+#pragma unroll
+    for (int q = 0; q < kChunks; ++q)
+      if (__ballot(cm[q] >= tf))
+#pragma unroll
+        for (int j = 0; j < E::n; ++j) {
+          const float v = E::get(c[q], j);
+          append(L, v >= tf && elem0(q) + j < V, make_key(ord(v), elem0(q) + j));
+        }
+    __syncthreads();
+  }
+  uint32_t n = L.count;
+  if (!exact && n > kCap) {
+    __syncthreads();
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int q = 0; q < kChunks; ++q) {
+      const int e = elem0(q);
+      const u32x4 y = load_chunk(x, e, V);
+#pragma unroll
+      for (int j = 0; j < E::n; ++j) append(L, E::get(y, j) > tf && e + j < V, make_key(ord(E::get(y, j)), e + j));
+    }
+    __syncthreads();
+    n = L.count;
+    if (n > kCap - kMaxTop) {
+      exact = true;
+    } else {
+      // equal ones in index order: chunk by chunk, a thread's behind those of
+      // the threads before it
+      uint32_t have = n;
+#pragma unroll 1
+      for (int q = 0; q < kChunks && have < (uint32_t)k; ++q) {
+        const int e = elem0(q);
+        const u32x4 y = load_chunk(x, e, V);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < E::n; ++j) mine += E::get(y, j) == tf && e + j < V;
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint32_t z = __shfl_up(upto, o);
+          if (lane >= o) upto += z;
+        }
+        __syncthreads();
+        if (lane == 63) L.sums[wave] = upto;
+        __syncthreads();
+        uint32_t at = have + upto - mine;
+        for (int w = 0; w < wave; ++w) at += L.sums[w];
+#pragma unroll
+        for (int j = 0; j < E::n; ++j)
+          if (E::get(y, j) == tf && e + j < V) {
+            if (at < (uint32_t)k) L.cand[at] = make_key(ord(tf), e + j);
+            ++at;
+          }
+        have += L.sums[0] + L.sums[1] + L.sums[2] + L.sums[3];
+      }
+      n = min(have, max((uint32_t)k, n));
+      __syncthreads();
+    }
+  }
+  if (exact) {
+    // the k-th largest key (or the piece's last), bit by bit
+    const uint32_t want = min(k, min(V - e0, kPiece<T>));
+    uint64_t best = 0;
+#pragma unroll 1
+    for (int b = 63; b >= 0; --b) {
+      const uint64_t key = best | (1ull << b);
+      if (b < 32 && b >= 20) {  // 0xFFFFFFFF - index, index < 2^20
+        best = key;
+        continue;
+      }
+      uint32_t v = 0;
+#pragma unroll 1
+      for (int q = 0; q < kChunks; ++q) {
+        const int e = elem0(q);
+        const u32x4 y = load_chunk(x, e, V);
+#pragma unroll
+        for (int j = 0; j < E::n; ++j) v += e + j < V && make_key(ord(E::get(y, j)), e + j) >= key;
+      }
+      if (block_count(L, v) >= want) best = key;
+    }
+    __syncthreads();
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int q = 0; q < kChunks; ++q) {
+      const int e = elem0(q);
+      const u32x4 y = load_chunk(x, e, V);
+#pragma unroll
+      for (int j = 0; j < E::n; ++j) {
+        const uint64_t key = make_key(ord(E::get(y, j)), e + j);
+        append(L, e + j < V && key >= best, key);
+      }
+    }
+    __syncthreads();
+    n = L.count;
+  }
+  // rank by counting; a piece of fewer than k logits leaves zeros, which are
+  // below every key
+  for (uint32_t i = tid; i < n; i += kThreads) {
+    const uint64_t key = L.cand[i];
+    uint32_t r = 0;
+    for (uint32_t j = 0; j < n; ++j) r += L.cand[j] > key;
+    if (r < (uint32_t)k) out[r] = key;
+  }
+  for (int i = (int)n + tid; i < k; i += kThreads) out[i] = 0;
+}
+
+struct FwdArgs {
+  const void* logits;
+  int64_t ld;
+  int rows, V, np, n_ids, k;
+  float c;        // log2(e) / temperature
+  const int32_t* ids;
+  Part* parts;    // [rows, np, kWaves]
+  uint64_t* top;  // [rows, np, k]
+  float* logprobs;
+  float* entropy;
+  float* lse;
+  int32_t* top_ids;
+  float* top_logprobs;
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads, 4) logprobs_piece_kernel(const FwdArgs a) {
+  using E = Elems<T>;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.np;
+  const int piece = blockIdx.x - (int)row * a.np, e0 = piece * kPiece<T>;
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  u32x4 ch[kChunks];
+#pragma unroll
+  for (int q = 0; q < kChunks; ++q) ch[q] = load_chunk(x, e0 + (q * kThreads + tid) * E::n, a.V);
+  float cm[kChunks], mn = INFINITY;
+#pragma unroll
+  for (int q = 0; q < kChunks; ++q) {
+    cm[q] = E::get(ch[q], 0);
+    mn = fminf(mn, cm[q]);
+#pragma unroll
+    for (int j = 1; j < E::n; ++j) {
+      cm[q] = fmaxf(cm[q], E::get(ch[q], j));
+      mn = fminf(mn, E::get(ch[q], j));
+    }
+  }
+  float m = cm[0];
+#pragma unroll
+  for (int q = 1; q < kChunks; ++q) m = fmaxf(m, cm[q]);
+  m = wave_max(m);
+  Part p;
+  p.s = p.t = 0.f;
+  // terms so small that 0 * -inf or an overflow of x c could come up are
+  // rare enough for a loop of their own: masked logits, and the row's end
+  if (__any(!(mn * a.c > -1e37f)) || !(fabsf(m * a.c) < 1e37f)) {
+    // m = -inf: nothing is allowed, and nothing is added
+    p.shift = (double)m * (double)a.c;
+    if (m != -INFINITY) {
+#pragma unroll
+      for (int q = 0; q < kChunks; ++q)
+#pragma unroll
+        for (int j = 0; j < E::n; ++j) {
+          const float d = (E::get(ch[q], j) - m) * a.c;
+          const float arg = d < -200.f ? -200.f : d;  // exp2 of it is 0; NaN stays
+          const float e = __builtin_amdgcn_exp2f(arg);
+          p.s += e;
+          p.t = fmaf(e, arg, p.t);
+        }
+    }
+  } else {
+    const float shift = m * a.c;
+    p.shift = (double)shift;
+    float s0 = 0.f, t0 = 0.f;
+#pragma unroll
+    for (int q = 0; q < kChunks; ++q)
+#pragma unroll
+      for (int j = 0; j < E::n; j += 2) {
+        const float a0 = fmaf(E::get(ch[q], j), a.c, -shift), a1 = fmaf(E::get(ch[q], j + 1), a.c, -shift);
+        const float e0_ = __builtin_amdgcn_exp2f(a0), e1_ = __builtin_amdgcn_exp2f(a1);
+        p.s += e0_;
+        s0 += e1_;
+        p.t = fmaf(e0_, a0, p.t);
+        t0 = fmaf(e1_, a1, t0);
+      }
+    p.s += s0;
+    p.t += t0;
+  }
+  const bool nan = TOP && !(p.s < INFINITY);
+  p.s = wave_sum(p.s);
+  p.t = wave_sum(p.t);
+  if ((tid & 63) == 0) a.parts[(row * a.np + piece) * kWaves + (tid >> 6)] = p;
+  if constexpr (TOP) {
+    __shared__ TopLds L;
+    piece_top<T>(x, ch, cm, nan, e0, a.V, a.k, a.top + (row * a.np + piece) * a.k, L);
+  }
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// One wavefront per row: its parts joined in 64 bits, the given tokens' log
+// probabilities, and the pieces' alternatives merged (each list is sorted, so
+// a candidate's rank is a sum of searches). LDS: np * k keys.
+template <typename T>
+__global__ void __launch_bounds__(64) logprobs_row_kernel(const FwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint64_t keys[];
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const Part* parts = a.parts + row * a.np * kWaves;
+  const int n = a.np * kWaves;
+  double M = -INFINITY;
+  for (int i = lane; i < n; i += 64) M = fmax(M, parts[i].shift);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmax(M, __shfl_xor(M, o));
+  double s = 0.0, t = 0.0;
+  for (int i = lane; i < n; i += 64) {
+    const Part p = parts[i];
+    if (p.shift == -INFINITY && p.s == 0.f) continue;  // nothing allowed in it
+    const double d = p.shift - M, f = d < -1000.0 ? 0.0 : exp2(d);  // (a NaN part stays one)
+    s += p.s * f;
+    t += (p.t + p.s * d) * f;
+  }
+  s = wave_sum64(s);
+  t = wave_sum64(t);
+  const bool none = M == -INFINITY && s == 0.0;  // no token is allowed
+  const double l2 = none ? -INFINITY : M + log2(s);
+  if (lane == 0) {
+    if (a.lse) a.lse[row] = (float)(l2 * kLn2);
+    if (a.entropy) a.entropy[row] = none ? 0.f : (float)((log2(s) - t / s) * kLn2);
+  }
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  // z - lse in log2 units, where both carry c's rounding alike
+  auto logp = [&](float v) {
+    if (v == -INFINITY) return s == s ? -INFINITY : NAN;
+    return (float)(((double)v * (double)a.c - l2) * kLn2);
+  };
+  for (int j = lane; j < a.n_ids; j += 64) {
+    const int id = a.ids[row * a.n_ids + j];
+    a.logprobs[row * a.n_ids + j] = id < 0 ? 0.f : id >= a.V ? NAN : logp(value_of(x[id]));
+  }
+  if (a.k == 0) return;
+  const int nk = a.np * a.k;
+  const uint64_t* top = a.top + row * nk;
+  for (int i = lane; i < nk; i += 64) keys[i] = top[i];
+  __syncthreads();
+  for (int i = lane; i < nk; i += 64) {
+    const uint64_t key = keys[i];
+    if (!key) continue;
+    int r = 0;
+    for (int p = 0; p < a.np && r < a.k; ++p) {
+      int lo = 0, hi = a.k;  // keys of the list that are larger
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (keys[p * a.k + mid] > key) lo = mid + 1;
+        else hi = mid;
+      }
+      r += lo;
+    }
+    if (r < a.k) {
+      a.top_ids[row * a.k + r] = (int32_t)(0xFFFFFFFFu - (uint32_t)key);
+      a.top_logprobs[row * a.k + r] = logp(from_ord((uint32_t)(key >> 32)));
+    }
+  }
+}
+
+// ------------------------------------------------------------- backward
+struct BwdArgs {
+  const void* logits;
+  void* grad;
+  int64_t ld, ld_grad;
+  int rows, V, np, n_ids;
+  float inv_temp;
+  const int32_t* ids;
+  const float* g_logp;
+  const float* lse;
+  const float* entropy;
+  const float* g_ent;
+};
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* row, int e, int V, const float* v) {
+  using E = Elems<T>;
+  if (e + E::n <= V) {
+    u32x4 o;
+    if constexpr (sizeof(T) == 2) {
+      typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)v[2 * j], (__bf16)v[2 * j + 1]});
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = __float_as_uint(v[j]);
+    }
+    *reinterpret_cast<u32x4_any*>(row + e) = o;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < E::n; ++j)
+    if (e + j < V) {
+      if constexpr (sizeof(T) == 2) row[e + j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+      else row[e + j] = v[j];
+    }
+}
+
+// One workgroup per piece of a row, as in the forward. dx = (sum_j g_j [v =
+// id_j] - p (G + g_ent (logp + H))) / temperature, G = sum g_j. grad may be
+// logits: a workgroup reads its piece before it writes it, and the given
+// tokens' logits before any of it is written.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a) {
+  using E = Elems<T>;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.np;
+  const int piece = blockIdx.x - (int)row * a.np, e0 = piece * kPiece<T>;
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  T* out = static_cast<T*>(a.grad) + row * a.ld_grad;
+  const int32_t* ids = a.ids + row * a.n_ids;
+  const float* gl = a.g_logp + row * a.n_ids;
+  float G = 0.f;
+  bool any = false;  // an upstream gradient that is not zero
+  for (int j = 0; j < a.n_ids; ++j) {
+    const int id = ids[j];
+    if (id < 0) continue;
+    G += id < a.V ? gl[j] : NAN;
+    any = any || id >= a.V || !(gl[j] == 0.f);
+  }
+  const float gh = a.g_ent ? a.g_ent[row] : 0.f;
+  any = any || !(gh == 0.f);
+  const float lse = a.lse[row], H = a.g_ent ? a.entropy[row] : 0.f;
+  if (!any || lse == -INFINITY) {  // nothing flows, or nothing is allowed: zeros, whatever the logits hold
+    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < kChunks; ++q) {
+      const int e = e0 + (q * kThreads + tid) * E::n;
+      if (e < a.V) store_chunk(out, e, a.V, z);
+    }
+    return;
+  }
+  // without the given tokens' own terms
+  auto base = [&](float v) {
+    float d = fmaf(v, a.inv_temp, -lse);
+    d = d < -1e4f ? -1e4f : d;  // p = 0 there: no 0 * inf; NaN stays
+    return -__builtin_amdgcn_exp2f(d * kLog2e) * fmaf(gh, d + H, G);
+  };
+  u32x4 ch[kChunks];
+#pragma unroll
+  for (int q = 0; q < kChunks; ++q) ch[q] = load_chunk(x, e0 + (q * kThreads + tid) * E::n, a.V);
+  // thread j: the j-th given token where it lies in this piece and has not
+  // been given before
+  int mine = -1;
+  float mine_g = 0.f;
+  if (tid < a.n_ids) {
+    const int id = ids[tid];
+    if (id >= e0 && id < min(a.V, e0 + kPiece<T>)) {
+      mine = id;
+      float g = 0.f;
+      for (int j = 0; j < a.n_ids; ++j)
+        if (ids[j] == id) {
+          if (j < tid) mine = -1;
+          g += gl[j];
+        }
+      mine_g = (base(value_of(x[id])) + g) * a.inv_temp;
+    }
+  }
+  if (a.n_ids) __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kChunks; ++q) {
+    const int e = e0 + (q * kThreads + tid) * E::n;
+    float v[E::n];
+#pragma unroll
+    for (int j = 0; j < E::n; ++j) v[j] = base(E::get(ch[q], j)) * a.inv_temp;
+    if (e < a.V) store_chunk(out, e, a.V, v);
+  }
+  if (a.n_ids) {
+    __syncthreads();
+    if (mine >= 0) {
+      if constexpr (sizeof(T) == 2) out[mine] = __builtin_bit_cast(uint16_t, (__bf16)mine_g);
+      else out[mine] = mine_g;
+    }
+  }
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+int pieces(int V, int dtype) {
+  const int p = dtype == GLT_DTYPE_BF16 ? kPiece<uint16_t> : kPiece<float>;
+  return (V + p - 1) / p;
+}
+size_t parts_bytes(int rows, int V, int dtype) { return round256((size_t)rows * pieces(V, dtype) * kWaves * sizeof(Part)); }
+
+glt_status check_rows(const char* who, int32_t dtype, int64_t ld, int32_t rows, int32_t V, float temperature, int32_t n_ids) {
+  GLT_CHECK(dtype == GLT_DTYPE_BF16 || dtype == GLT_DTYPE_F32, GLT_ERR_DTYPE, "%s: dtype %d", who, dtype);
+  GLT_CHECK(rows >= 0 && V > 0 && ld >= V, GLT_ERR_SHAPE, "%s: rows=%d V=%d ld=%lld", who, rows, V, (long long)ld);
+  GLT_CHECK(V <= kMaxV, GLT_ERR_UNSUPPORTED, "%s: V=%d (at most %d)", who, V, kMaxV);
+  GLT_CHECK(n_ids >= 0 && n_ids <= kMaxIds, GLT_ERR_UNSUPPORTED, "%s: %d given tokens a row (at most %d)", who, n_ids, kMaxIds);
+  // 1 / temperature and log2(e) / temperature are finite and not zero
+  GLT_CHECK(temperature > 1e-30f && temperature < 1e30f, GLT_ERR_INVALID_ARG, "%s: temperature %g", who, (double)temperature);
+  GLT_CHECK((int64_t)rows * pieces(V, dtype) < INT32_MAX, GLT_ERR_SHAPE, "%s: rows=%d V=%d", who, rows, V);
+  return GLT_OK;
+}
+
+template <typename T>
+glt_status launch_fwd(const FwdArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.rows * a.np));
+  if (a.k > 0) GLT_LAUNCH("logprobs", (logprobs_piece_kernel<T, true>), grid, dim3(kThreads), 0, st, a);
+  else GLT_LAUNCH("logprobs", (logprobs_piece_kernel<T, false>), grid, dim3(kThreads), 0, st, a);
+  GLT_LAUNCH_CHECK("logprobs");
+  GLT_LAUNCH("logprobs_row", logprobs_row_kernel<T>, dim3((unsigned)a.rows), dim3(64), (size_t)a.np * a.k * 8, st, a);
+  GLT_LAUNCH_CHECK("logprobs_row");
+  return GLT_OK;
+}
+
+}  // namespace
+
+}  // namespace glt
+
+using namespace glt;
+
+extern "C" {
+
+size_t glt_token_logprobs_workspace_size(int32_t rows, int32_t V, int32_t dtype, int32_t top_k) {
+  if (rows <= 0 || V <= 0 || top_k < 0 || (dtype != GLT_DTYPE_BF16 && dtype != GLT_DTYPE_F32)) return 256;
+  return parts_bytes(rows, V, dtype) + round256((size_t)rows * pieces(V, dtype) * top_k * 8);
+}
+
+glt_status glt_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V, float temperature,
+                              const int32_t* ids, int32_t n_ids, int32_t top_k, float* logprobs, float* entropy,
+                              float* lse, int32_t* top_ids, float* top_logprobs, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  const char* who = "glt_token_logprobs";
+  const glt_status s = check_rows(who, dtype, ld, rows, V, temperature, n_ids);
+  if (s != GLT_OK) return s;
+  GLT_CHECK(top_k >= 0 && top_k <= kMaxTop && top_k <= V, GLT_ERR_UNSUPPORTED, "%s: top_k %d (at most %d, and V=%d)", who,
+            top_k, kMaxTop, V);
+  if (rows == 0) return GLT_OK;
+  GLT_CHECK(logits && (n_ids == 0 || (ids && logprobs)) && (top_k == 0 || (top_ids && top_logprobs)),
+            GLT_ERR_INVALID_ARG, "%s: null pointer", who);
+  const int es = dtype == GLT_DTYPE_BF16 ? 2 : 4;
+  GLT_CHECK((uintptr_t)logits % es == 0 && ((uintptr_t)ids | (uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)lse |
+                                            (uintptr_t)top_ids | (uintptr_t)top_logprobs) % 4 == 0,
+            GLT_ERR_ALIGNMENT, "%s: pointers must be aligned to their elements", who);
+  const size_t need = glt_token_logprobs_workspace_size(rows, V, dtype, top_k);
+  GLT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, GLT_ERR_WORKSPACE,
+            "%s: needs %zu workspace bytes, 256-byte aligned", who, need);
+  FwdArgs a{};
+  a.logits = logits;
+  a.ld = ld;
+  a.rows = rows; a.V = V; a.np = pieces(V, dtype); a.n_ids = n_ids; a.k = top_k;
+  a.c = (float)(1.4426950408889634074 / (double)temperature);
+  a.ids = ids;
+  a.parts = static_cast<Part*>(workspace);
+  a.top = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + parts_bytes(rows, V, dtype));
+  a.logprobs = logprobs; a.entropy = entropy; a.lse = lse; a.top_ids = top_ids; a.top_logprobs = top_logprobs;
+  return dtype == GLT_DTYPE_BF16 ? launch_fwd<uint16_t>(a, as_stream(stream)) : launch_fwd<float>(a, as_stream(stream));
+}
+
+glt_status glt_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V,
+                                  float temperature, const int32_t* ids, int32_t n_ids, const float* grad_logprobs,
+                                  const float* lse, const float* entropy, const float* grad_entropy, void* grad,
+                                  int64_t ld_grad, void* stream) {
+  const char* who = "glt_token_logprobs_bwd";
+  const glt_status s = check_rows(who, dtype, ld, rows, V, temperature, n_ids);
+  if (s != GLT_OK) return s;
+  GLT_CHECK(ld_grad >= V, GLT_ERR_SHAPE, "%s: ld_grad=%lld V=%d", who, (long long)ld_grad, V);
+  if (rows == 0) return GLT_OK;
+  GLT_CHECK(logits && grad && lse && (n_ids == 0 || (ids && grad_logprobs)) && (!grad_entropy || entropy),
+            GLT_ERR_INVALID_ARG, "%s: null pointer", who);
+  GLT_CHECK(grad != logits || ld_grad == ld, GLT_ERR_SHAPE, "%s: in place with strides %lld and %lld", who, (long long)ld,
+            (long long)ld_grad);
+  const int es = dtype == GLT_DTYPE_BF16 ? 2 : 4;
+  GLT_CHECK(((uintptr_t)logits | (uintptr_t)grad) % es == 0 &&
+                ((uintptr_t)ids | (uintptr_t)grad_logprobs | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)grad_entropy) % 4 == 0,
+            GLT_ERR_ALIGNMENT, "%s: pointers must be aligned to their elements", who);
+  const BwdArgs a{logits, grad, ld, ld_grad, rows, V, pieces(V, dtype), n_ids, (float)(1.0 / (double)temperature), ids,
+                  grad_logprobs, lse, entropy, grad_entropy};
+  const dim3 grid((unsigned)(rows * a.np));
+  if (dtype == GLT_DTYPE_BF16)
+    GLT_LAUNCH("logprobs_bwd", logprobs_bwd_kernel<uint16_t>, grid, dim3(kThreads), 0, as_stream(stream), a);
+  else
+    GLT_LAUNCH("logprobs_bwd", logprobs_bwd_kernel<float>, grid, dim3(kThreads), 0, as_stream(stream), a);
+  GLT_LAUNCH_CHECK("logprobs_bwd");
+  return GLT_OK;
+}
+
+}  // extern "C"

@@ -476,6 +476,70 @@ def masked_ce(logits, ids, ood=None, scale=1.0, grad=None, want_grad=True, ce_pe
     return stats, (grad if want_grad else None), ce
 
 
+def _logit_rows(logits, ids):
+    """(rows, V, row stride, dtype code) of logits [rows, V], bf16 or f32;
+    checks ids [rows, n] int32."""
+    _need(logits.dim() == 2 and logits.is_cuda, "logits: [rows, V] on a GPU")
+    rows, V = logits.shape
+    dt = _dtype_code(logits.dtype)
+    ld = logits.stride(0) if rows > 1 else V
+    if (V > 1 and logits.stride(1) != 1) or ld < V:
+        raise ValueError(f"logits: strides {logits.stride()} (rows contiguous, not overlapping)")
+    if ids is not None and not (ids.dim() == 2 and ids.shape[0] == rows and ids.dtype == torch.int32
+                                and ids.device == logits.device and ids.is_contiguous()):
+        raise ValueError(f"ids: contiguous int32 [{rows}, n] on {logits.device}")
+    return rows, V, ld, dt
+
+
+def _row_values(name, t, shape, device):
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous f32 {list(shape)} on {device}")
+
+
+def token_logprobs(logits, ids=None, top_k=0, temperature=1.0, workspace=None):
+    """Log probabilities under softmax(logits / temperature) of the given
+    tokens ids [rows, n] int32 (below 0 = padding, 0), with what else an answer
+    shows of each row: dict(logprobs [rows, n], entropy [rows], lse [rows]) and,
+    with top_k, top_ids int32 and top_logprobs [rows, top_k]. logits [rows, V]
+    bf16 or f32."""
+    rows, V, ld, dt = _logit_rows(logits, ids)
+    dev = logits.device
+    n = ids.shape[1] if ids is not None else 0
+    new = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=dev)
+    r = dict(logprobs=new((rows, n)), entropy=new(rows), lse=new(rows))
+    if top_k > 0:
+        r["top_ids"], r["top_logprobs"] = new((rows, top_k), torch.int32), new((rows, top_k))
+    nb = F.load().glt_token_logprobs_workspace_size(rows, V, dt, top_k)
+    ws = _workspace(workspace, nb, dev)
+    _call_on(logits, "glt_token_logprobs", _p(logits), dt, ld, rows, V, temperature, _p(ids), n, top_k, _p(r["logprobs"]),
+             _p(r["entropy"]), _p(r["lse"]), _p(r.get("top_ids")), _p(r.get("top_logprobs")), _p(ws), ws.numel())
+    return r
+
+
+def token_logprobs_bwd(logits, ids, lse, grad_logprobs, entropy=None, grad_entropy=None, temperature=1.0, grad=None):
+    """Gradient on the logits (their dtype) of sum(grad_logprobs * logprobs) +
+    sum(grad_entropy * entropy), from token_logprobs' lse and entropy. Pass
+    grad=logits to overwrite the logits with it."""
+    rows, V, ld, dt = _logit_rows(logits, ids)
+    dev = logits.device
+    n = ids.shape[1] if ids is not None else 0
+    _row_values("lse", lse, (rows,), dev)
+    if n:
+        _row_values("grad_logprobs", grad_logprobs, (rows, n), dev)
+    if grad_entropy is not None:
+        _need(entropy is not None, "grad_entropy needs the forward's entropy")
+        _row_values("grad_entropy", grad_entropy, (rows,), dev)
+        _row_values("entropy", entropy, (rows,), dev)
+    if grad is None:
+        grad = torch.empty((rows, V), dtype=logits.dtype, device=dev)
+    _need(grad.shape == logits.shape and grad.dtype == logits.dtype and grad.device == dev
+          and (V == 1 or grad.stride(1) == 1), "grad: the logits' shape, dtype and device, rows contiguous")
+    _call_on(logits, "glt_token_logprobs_bwd", _p(logits), dt, ld, rows, V, temperature, _p(ids), n,
+             _p(grad_logprobs if n else None), _p(lse), _p(entropy if grad_entropy is not None else None),
+             _p(grad_entropy), _p(grad), grad.stride(0) if rows > 1 else V)
+    return grad
+
+
 def silence_energy(delta, ld=None):
     """Per-token energy ||delta_t|| / sqrt(slice) of [tokens, slice] f32 or
     bf16 rows (reference compute_energy_kernel)."""

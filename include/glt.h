@@ -651,6 +651,39 @@ glt_status glt_masked_ce(const uint16_t* logits, int64_t ld, const int32_t* ids,
                          float* ce_per_token, float* stats, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* Log probabilities of given tokens, entropy and top alternatives of rows of
+ * logits, z = logits / temperature: scoring of answers, and the objective of
+ * training on them (the reference scores one label a row and keeps its mean,
+ * grafting.hip:1027-1050). logits: `rows` rows of V <= 2^20 values of `dtype`
+ * (GLT_DTYPE_BF16 or GLT_DTYPE_F32) at row stride ld, aligned to their element.
+ * ids [rows, n_ids] int32, n_ids <= 64: logprobs[r, j] = z[id] - lse; an id
+ * below 0 is padding (0), one at or past V gives NaN. entropy and lse [rows]
+ * (NULL = not wanted): -sum p log p and log sum exp z. top_ids and top_logprobs
+ * [rows, top_k], top_k <= min(64, V): the largest logits in falling order, the
+ * lower index first among equal ones. A logit of -inf has probability 0; a row
+ * of nothing else has lse -inf, log probabilities -inf, entropy 0. NaN or +inf
+ * make the row's statistics NaN (NaN logits rank by their bits). f32 sums, joined
+ * in 64 bits in an order that V alone fixes. workspace:
+ * glt_token_logprobs_workspace_size bytes, 256-byte aligned. */
+size_t glt_token_logprobs_workspace_size(int32_t rows, int32_t V, int32_t dtype, int32_t top_k);
+glt_status glt_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V,
+                              float temperature, const int32_t* ids, int32_t n_ids, int32_t top_k,
+                              float* logprobs, float* entropy, float* lse, int32_t* top_ids,
+                              float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradient on the logits of sum(grad_logprobs * logprobs) + sum(grad_entropy *
+ * entropy), from the forward's lse and entropy (grad_entropy and entropy NULL =
+ * no entropy term):
+ *   grad[r, v] = (sum_j g_j [v = id_j] - p_v (sum_j g_j + g_ent (log p_v + H))) / temperature
+ * in the logits' dtype at row stride ld_grad, rounded once; may be the logits
+ * themselves (ld_grad = ld). Padding ids add nothing, the same id twice adds
+ * twice, an id at or past V makes the row NaN. Rows whose upstream gradients are
+ * all zero get zeros whatever their logits hold, and so do rows without an
+ * allowed token (lse -inf). */
+glt_status glt_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V,
+                                  float temperature, const int32_t* ids, int32_t n_ids,
+                                  const float* grad_logprobs, const float* lse, const float* entropy,
+                                  const float* grad_entropy, void* grad, int64_t ld_grad, void* stream);
+
 /* OOD silence terms on per-token graft outputs delta [tokens, slice]
  * (row stride ld): energy[t] = sqrt(sum delta^2 + 1e-8) / sqrt(slice)
  * (compute_energy_kernel, src/kernels_elementwise_impl.inc:222-275;

@@ -1,21 +1,18 @@
 """Attention for training on the GPU: the forward with log-sum-exp and the
 backward, against the formulas in 64 bits on the same inputs.
 
-Tolerances. Rows have unit-variance v and dout; relative to an output's 2-norm:
-  out  rounded once (half a step, 2^-9 relative at most, 2^-8 the step) and
-       summed over probabilities rounded to bf16 (2^-9 each): below 2 * 2^-9
-       in the 2-norm for any cancellation-free sum, 3 * 2^-9 with the
-       cancelling ones of mean-zero v.
-  dv   as out. dq, dk: ds rounded to bf16, D from f32 or from the rounded out
-       (2^-9 relative of each product of its sum) and the output's rounding:
-       below 4 * 2^-9.
+Tolerances. A rounding to bf16 is off by at most 2^-8 of the value, and in the
+2-norm over values whose mantissas are spread by about 2^-8 / sqrt(3) * 0.72 =
+1.7e-3, less than 2^-9. Relative to an output's 2-norm:
+  out, dv  two such roundings (of p, and of the result): 2 * 2^-9 if they add
+       outright, 3 * 2^-9 with half as much again for sums that cancel.
+  dq, dk  ds and the result, and D's share of out's rounding: 4 * 2^-9.
   lse  off by no more than the scores are, and roundings of its own. A score is
        an f32 sum of 128 products (exact in f32: 8 x 8 bits): in any order at
        most 127 roundings of half a step of a partial sum, 127 * 2^-24 *
        sum |q k|, times scale. The shift, the logarithm and the last sum round
        values of at most max |lse| + 8: four times 2^-24 of that.
-Every element: within 8 times the 2-norm bound of max(|value|, rms), the
-roundings of one element being bounded by the same steps."""
+Every element: within 8 times the 2-norm bound of max(|value|, rms)."""
 import math
 
 import pytest
