@@ -18,7 +18,7 @@ STATUS_NAMES = {
     11: "GLT_ERR_FORMAT", 12: "GLT_ERR_NOT_FOUND",
 }
 DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
-MLP_EXPLICIT, MLP_RECOMPUTE, MLP_RESIDUAL, MLP_DY_F32 = 1, 2, 4, 8
+MLP_EXPLICIT, MLP_RECOMPUTE, MLP_RESIDUAL, MLP_DY_F32, MLP_SAVED_CKPT8 = 1, 2, 4, 8, 16
 FNV_BASIS = 1469598103934665603
 EVAL_HASH_REFERENCE, EVAL_HASH_ROWS = 0, 1
 BAKE_IN_PLACE, BAKE_MATERIALIZE = 0, 1
@@ -122,6 +122,10 @@ SIGNATURES = {
                                    _vp, ctypes.POINTER(GraftGrads), _vp, _sz, _vp, _vp, _vp, _f32, _vp, _vp]),
     "glt_silu_mul": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "glt_gate_up_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "glt_ckpt8_size": (_sz, [_i64, _i32]),
+    "glt_ckpt8_save": (_i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp]),
+    "glt_ckpt8_load": (_i32, [_vp, _i64, _i32, _vp, _i32, _i64, _vp]),
+    "glt_ckpt8_swiglu": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
     "glt_rmsnorm_fwd": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
     "glt_rmsnorm_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
     "glt_rope_fwd": (_i32, [_vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _i32, _vp]),

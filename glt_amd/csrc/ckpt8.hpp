@@ -1,0 +1,13 @@
+// 8-bit checkpoints inside the library.
+#pragma once
+
+#include "common.hpp"
+
+namespace glt {
+
+// glt_ckpt8_swiglu with inter written only where the 16-column pieces meet
+// [lo, hi).
+glt_status ckpt8_swiglu(const void* gate8, const void* up8, int64_t rows, int32_t cols, uint16_t* gate, uint16_t* up,
+                        uint16_t* inter, int lo, int hi, hipStream_t st);
+
+}  // namespace glt

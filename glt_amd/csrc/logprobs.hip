@@ -73,7 +73,10 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int e, int V) {
   if (e + E::n <= V) return *reinterpret_cast<const u32x4_any*>(row + e);
   u32x4 c = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int j = 0; j < E::n; ++j) E::put(c, j, e + j < V ? bits_of(row[e + j]) : E::neg_inf);
+  for (int j = 0; j < E::n; ++j) {
+    const uint32_t b = bits_of(row[min(e + j, V - 1)]);  // in place of what lies past the row
+    E::put(c, j, e + j < V ? b : E::neg_inf);
+  }
   return c;
 }
 

@@ -5,6 +5,7 @@
 #include <atomic>
 #include <mutex>
 
+#include "ckpt8.hpp"
 #include "gemm.hpp"
 #include "layout.hpp"
 #include "norm_rope.hpp"
@@ -200,7 +201,7 @@ static BwdLayout bwd_layout(const glt_mlp_desc* d) {
     L.dyb = off;
     off += align256((size_t)d->M * d->D * 2);
   }
-  if (d->flags & GLT_MLP_RECOMPUTE) {
+  if (d->flags & (GLT_MLP_RECOMPUTE | GLT_MLP_SAVED_CKPT8)) {
     L.g = off; off += align256(MN);
     L.u = off; off += align256(MN);
     L.inter = off; off += align256(MN);
@@ -350,8 +351,13 @@ static glt_status mlp_bwd_impl(const glt_mlp_desc* d, const glt_base_weights* w,
   if (s != GLT_OK) return s;
   GLT_CHECK(!(d->state && d->state->baked), GLT_ERR_BAKED_NO_BACKWARD,
             "glt_mlp_bwd: backward on a shadow-baked model is forbidden");
-  const bool recompute = d->flags & GLT_MLP_RECOMPUTE;
-  GLT_CHECK(d->M == 0 || (x && dy && (recompute || (gate_pre && up_pre && inter))), GLT_ERR_INVALID_ARG,
+  const bool recompute = d->flags & GLT_MLP_RECOMPUTE, ckpt8 = d->flags & GLT_MLP_SAVED_CKPT8;
+  GLT_CHECK(!ckpt8 || !recompute, GLT_ERR_INVALID_ARG,
+            "glt_mlp_bwd: GLT_MLP_RECOMPUTE and GLT_MLP_SAVED_CKPT8 exclude each other");
+  GLT_CHECK(!ckpt8 || d->dtype == GLT_DTYPE_BF16, GLT_ERR_DTYPE, "glt_mlp_bwd: 8-bit checkpoints on the bf16 path only");
+  GLT_CHECK(!ckpt8 || ((reinterpret_cast<uintptr_t>(gate_pre) | reinterpret_cast<uintptr_t>(up_pre)) & 255) == 0,
+            GLT_ERR_ALIGNMENT, "glt_mlp_bwd: checkpoints must be 256-byte aligned");
+  GLT_CHECK(d->M == 0 || (x && dy && (recompute || (gate_pre && up_pre && (ckpt8 || inter)))), GLT_ERR_INVALID_ARG,
             "glt_mlp_bwd: null x/dy or saved activations (set GLT_MLP_RECOMPUTE to recompute them)");
   const bool explicit_graft = d->flags & GLT_MLP_EXPLICIT;
   GLT_CHECK(!explicit_graft || d->n_slices == 0 || grads, GLT_ERR_INVALID_ARG, "glt_mlp_bwd: null grads");
@@ -370,7 +376,7 @@ static glt_status mlp_bwd_impl(const glt_mlp_desc* d, const glt_base_weights* w,
 
   const bool grads_wanted = explicit_graft && d->n_slices > 0;
   const bool wgrad_mfma =
-      grads_wanted && L.wgrad_mfma && wgrad_aligned(d, recompute ? W + L.inter : inter, grads);
+      grads_wanted && L.wgrad_mfma && wgrad_aligned(d, recompute || ckpt8 ? W + L.inter : inter, grads);
   bool operands_laid_out = false;  // x and dy already in the weight-gradient fragment layout
   if (L.dy_f32) {
     // The reference multiplies its f32 upstream gradient by the f32 copy of
@@ -399,6 +405,23 @@ static glt_status mlp_bwd_impl(const glt_mlp_desc* d, const glt_base_weights* w,
     up_pre = W + L.u;
     inter = W + L.inter;
     if ((s = gate_up_forward(d, w, x, W + L.g, W + L.u, W + L.inter, st)) != GLT_OK) return s;
+  }
+  if (ckpt8) {
+    // inter is read by the down projection's weight gradients alone: the
+    // columns of the slices that have one
+    int lo = N, hi = 0;
+    for (int j = 0; grads_wanted && j < d->n_slices; ++j)
+      if (d->slices[j].master_down && grads[j].down) {
+        lo = std::min(lo, d->slices[j].i_start);
+        hi = std::max(hi, d->slices[j].i_start + d->slices[j].s);
+      }
+    uint16_t* g16 = reinterpret_cast<uint16_t*>(W + L.g);
+    uint16_t* u16 = reinterpret_cast<uint16_t*>(W + L.u);
+    uint16_t* i16 = reinterpret_cast<uint16_t*>(W + L.inter);
+    if ((s = ckpt8_swiglu(gate_pre, up_pre, M, N, g16, u16, hi > lo ? i16 : nullptr, lo, hi, st)) != GLT_OK) return s;
+    gate_pre = g16;
+    up_pre = u16;
+    inter = i16;
   }
 
   // 1) dInter = dy . [W_down | grafts] with the SiLU*up derivative epilogue

@@ -99,10 +99,11 @@ class BaseMLP:
         return F.BaseWeights(_p(self.gate), _p(self.up), _p(self.down), _p(self.prepared))
 
 
-def _desc(base, slices, M, N, explicit, recompute=False, state=None, residual=False, dy_f32=False):
+def _desc(base, slices, M, N, explicit, recompute=False, state=None, residual=False, dy_f32=False, ckpt8=False):
     arr = _slices_array(slices)
     flags = ((F.MLP_EXPLICIT if explicit else 0) | (F.MLP_RECOMPUTE if recompute else 0)
-             | (F.MLP_RESIDUAL if residual else 0) | (F.MLP_DY_F32 if dy_f32 else 0))
+             | (F.MLP_RESIDUAL if residual else 0) | (F.MLP_DY_F32 if dy_f32 else 0)
+             | (F.MLP_SAVED_CKPT8 if ckpt8 else 0))
     d = F.MlpDesc(M, base.D, base.I, N, _dtype_code(base.dtype), flags, len(slices), arr,
                   ctypes.pointer(state) if state is not None else None)
     return d, arr
@@ -125,8 +126,8 @@ def mlp_forward(base, slices, x, N, explicit=True, save=True, residual=None):
     return y, g, u, inter
 
 
-def mlp_backward_workspace(base, slices, M, N, explicit=True, recompute=False):
-    d, keep = _desc(base, slices, M, N, explicit, recompute)
+def mlp_backward_workspace(base, slices, M, N, explicit=True, recompute=False, ckpt8=False):
+    d, keep = _desc(base, slices, M, N, explicit, recompute, ckpt8=ckpt8)
     return F.load().glt_mlp_bwd_workspace_size(ctypes.byref(d))
 
 
@@ -136,7 +137,8 @@ def mlp_backward(base, slices, x, dy, N, gate_pre=None, up_pre=None, inter=None,
     src/layer_backward_impl.inc:10-361). dy is [M,D] in the path dtype or
     f32 (the reference's upstream gradient, rounded once inside on the bf16
     path). Returns dx (f32) and per-slice [gate, up, down] f32 gradients in
-    [S,H] storage.
+    [S,H] storage. gate_pre and up_pre may be 8-bit checkpoints (ckpt8_save of
+    the forward's); inter is then formed from them.
 
     norm = (norm_x, norm_w, var, eps): x is the output of that RMSNorm
     (reference rms_norm of the FFN input); the call then also runs its
@@ -146,7 +148,12 @@ def mlp_backward(base, slices, x, dy, N, gate_pre=None, up_pre=None, inter=None,
     M = x.shape[0]
     if norm is not None:
         want_dx = True
-    d, keep = _desc(base, slices, M, N, explicit, recompute, state, dy_f32=dy.dtype == torch.float32)
+    ckpt8 = isinstance(gate_pre, Ckpt8)
+    if ckpt8:
+        _need(isinstance(up_pre, Ckpt8) and (gate_pre.rows, gate_pre.cols) == (up_pre.rows, up_pre.cols) == (M, N),
+              f"gate_pre and up_pre: checkpoints of [{M}, {N}]")
+        gate_pre, up_pre = gate_pre.buf, up_pre.buf
+    d, keep = _desc(base, slices, M, N, explicit, recompute, state, dy_f32=dy.dtype == torch.float32, ckpt8=ckpt8)
     nbytes = F.load().glt_mlp_bwd_workspace_size(ctypes.byref(d))
     if workspace is None or workspace.numel() < nbytes:
         workspace = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
@@ -169,6 +176,55 @@ def mlp_backward(base, slices, x, dy, N, gate_pre=None, up_pre=None, inter=None,
     F.call("glt_mlp_bwd", ctypes.byref(d), ctypes.byref(b), _p(x), _p(dy), _p(gate_pre), _p(up_pre), _p(inter),
            _p(dx), garr, _p(workspace), nbytes, _stream())
     return dx, grads
+
+
+class Ckpt8:
+    """An activation [rows, cols] held in 8 bits for the backward: codes and an
+    exponent per 32 columns in buf. Made by ckpt8_save."""
+
+    def __init__(self, buf, rows, cols, dtype):
+        self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
+
+    def load(self, dtype=None, out=None):
+        """The values, bf16 or f32 (by default what was saved), into out where
+        it is given."""
+        if out is None:
+            out = torch.empty((self.rows, self.cols), dtype=dtype or self.dtype, device=self.buf.device)
+        _need(dtype in (None, out.dtype) and out.shape == (self.rows, self.cols) and out.device == self.buf.device,
+              f"out: [{self.rows}, {self.cols}] on {self.buf.device}")
+        dt, ld = _rows_ld("out", out)
+        _call_on(self.buf, "glt_ckpt8_load", _p(self.buf), self.rows, self.cols, _p(out), dt, ld)
+        return out
+
+
+def _rows_ld(name, t):
+    """(dtype code, row stride) of t [rows, cols] with contiguous rows."""
+    rows, cols = t.shape
+    ld = t.stride(0) if rows > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise ValueError(f"{name}: strides {t.stride()} (rows contiguous, not overlapping)")
+    return _dtype_code(t.dtype), ld
+
+
+def ckpt8_save(x, buf=None):
+    """x [rows, cols] bf16 or f32 as an 8-bit checkpoint, in buf (uint8,
+    glt_ckpt8_size bytes) where it is given."""
+    _need(x.dim() == 2 and x.is_cuda, "x: [rows, cols] on a GPU")
+    rows, cols = x.shape
+    dt, ld = _rows_ld("x", x)
+    buf = _workspace(buf, F.load().glt_ckpt8_size(rows, cols), x.device)
+    _call_on(x, "glt_ckpt8_save", _p(x), dt, ld, rows, cols, _p(buf))
+    return Ckpt8(buf, rows, cols, x.dtype)
+
+
+def ckpt8_swiglu(gate8, up8):
+    """(gate, up, silu(gate) * up) bf16 [rows, cols] from checkpoints of the
+    MLP's gate_pre and up_pre."""
+    rows, cols, dev = gate8.rows, gate8.cols, gate8.buf.device
+    _need((rows, cols) == (up8.rows, up8.cols) and up8.buf.device == dev, "gate8 and up8: checkpoints of one shape")
+    out = [torch.empty((rows, cols), dtype=torch.bfloat16, device=dev) for _ in range(3)]
+    _call_on(gate8.buf, "glt_ckpt8_swiglu", _p(gate8.buf), _p(up8.buf), rows, cols, _p(out[0]), _p(out[1]), _p(out[2]))
+    return tuple(out)
 
 
 def graft_gemm(kind, M, S, H, out, a=None, lda=0, delta=None, dy=None, ldo=None, alpha=1.0, beta=0.0):
@@ -226,7 +282,7 @@ def _need(cond, msg):
 
 
 def _workspace(ws, nbytes, device):
-    """ws where it is given (uint8, on the device, at least nbytes), else new."""
+    """ws where it is given (uint8, on the device, at least nbytes), else a new one."""
     if ws is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     if ws.dtype != torch.uint8 or ws.device != device or not ws.is_contiguous() or ws.numel() < nbytes:

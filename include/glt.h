@@ -135,6 +135,12 @@ typedef struct {
  * It is rounded once (RNE) to the bf16 MFMA operand inside the call; without
  * the flag dy is in the path dtype. No effect on the f32 path (dy is f32). */
 #define GLT_MLP_DY_F32 8
+/* GLT_MLP_SAVED_CKPT8: gate_pre and up_pre of glt_mlp_bwd are 8-bit checkpoints
+ * [M,N] (glt_ckpt8_save); they are restored in the workspace and inter =
+ * silu(gate_pre) * up_pre is formed from them (the inter argument is not
+ * read). bf16 path only, not together with GLT_MLP_RECOMPUTE. No effect on the
+ * forward, which writes bf16. */
+#define GLT_MLP_SAVED_CKPT8 16
 typedef struct {
   int32_t M, D, I, N;
   int32_t dtype;   /* GLT_DTYPE_BF16 or GLT_DTYPE_F32 */
@@ -273,6 +279,27 @@ glt_status glt_silu_mul(const uint16_t* g, const uint16_t* u, uint16_t* out, int
                         void* stream);
 glt_status glt_gate_up_bwd(const float* gi, const uint16_t* g, const uint16_t* u,
                            float* dg, float* du, int64_t n, void* stream);
+
+/* ------------------------------------------------- 8-bit checkpoints
+ * An activation [rows, cols] held for the backward in 1 + 1/32 bytes a value
+ * (the reference saves bf16 or recomputes, src/layer_recompute_impl.inc:8-91).
+ * A block of 32 consecutive columns shares a power of two, the smallest step
+ * for which its largest magnitude rounds to at most 127 steps; a value is held
+ * as rint(x / step) and restored exactly as that many steps: at most half a
+ * step off, 1/127.5 of the block's largest magnitude. A block with NaN or infinity
+ * is restored as NaN. x: dtype GLT_DTYPE_BF16 or GLT_DTYPE_F32 at row stride
+ * ld. ckpt: glt_ckpt8_size bytes, 256-byte aligned; a checkpoint of either
+ * dtype is restored to either (the values are exact in both). */
+size_t glt_ckpt8_size(int64_t rows, int32_t cols);
+glt_status glt_ckpt8_save(const void* x, int32_t dtype, int64_t ld, int64_t rows, int32_t cols,
+                          void* ckpt, void* stream);
+glt_status glt_ckpt8_load(const void* ckpt, int64_t rows, int32_t cols, void* x, int32_t dtype,
+                          int64_t ld, void* stream);
+/* The MLP's saved activations from checkpoints of gate_pre and up_pre [rows,
+ * cols]: gate, up (restored) and inter = bf16(silu(gate) * up), dense bf16
+ * [rows, cols] each (NULL = not wanted). */
+glt_status glt_ckpt8_swiglu(const void* gate8, const void* up8, int64_t rows, int32_t cols,
+                            uint16_t* gate, uint16_t* up, uint16_t* inter, void* stream);
 
 /* --------------------------------------------------------------- RMSNorm */
 /* y = bf16(x * rsqrt(var+eps) * w), var[m] = mean(x^2) (mean-square, as the
