@@ -193,7 +193,7 @@ class Ckpt8:
         _need(dtype in (None, out.dtype) and out.shape == (self.rows, self.cols) and out.device == self.buf.device,
               f"out: [{self.rows}, {self.cols}] on {self.buf.device}")
         dt, ld = _rows_ld("out", out)
-        _call_on(self.buf, "glt_ckpt8_load", _p(self.buf), self.rows, self.cols, _p(out), dt, ld)
+        _call_on(self.buf, "glt_ckpt8_load", _a(self.buf), self.rows, self.cols, _a(out), dt, ld)
         return out
 
 
@@ -213,7 +213,7 @@ def ckpt8_save(x, buf=None):
     rows, cols = x.shape
     dt, ld = _rows_ld("x", x)
     buf = _workspace(buf, F.load().glt_ckpt8_size(rows, cols), x.device)
-    _call_on(x, "glt_ckpt8_save", _p(x), dt, ld, rows, cols, _p(buf))
+    _call_on(x, "glt_ckpt8_save", _a(x), dt, ld, rows, cols, _a(buf))
     return Ckpt8(buf, rows, cols, x.dtype)
 
 
@@ -223,7 +223,7 @@ def ckpt8_swiglu(gate8, up8):
     rows, cols, dev = gate8.rows, gate8.cols, gate8.buf.device
     _need((rows, cols) == (up8.rows, up8.cols) and up8.buf.device == dev, "gate8 and up8: checkpoints of one shape")
     out = [torch.empty((rows, cols), dtype=torch.bfloat16, device=dev) for _ in range(3)]
-    _call_on(gate8.buf, "glt_ckpt8_swiglu", _p(gate8.buf), _p(up8.buf), rows, cols, _p(out[0]), _p(out[1]), _p(out[2]))
+    _call_on(gate8.buf, "glt_ckpt8_swiglu", _a(gate8.buf), _a(up8.buf), rows, cols, _a(out[0]), _a(out[1]), _a(out[2]))
     return tuple(out)
 
 
@@ -290,14 +290,26 @@ def _workspace(ws, nbytes, device):
     return ws
 
 
+def _a(t):
+    """A tensor's address (ctypes takes it for a pointer as it is)."""
+    return None if t is None else t.data_ptr()
+
+
+# the current stream's handle by device index (the Stream object that the public
+# function makes first costs 2 us of a small call's 12)
+_stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call_on(t, name, *args):
     """The entry point on t's device and that device's current stream, which
     is passed last."""
-    if t.device.index == torch.cuda.current_device():
-        F.call(name, *args, _stream())
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        F.call(name, *args, _stream_handle(index))
     else:
-        with torch.cuda.device(t.device):
-            F.call(name, *args, _stream())
+        with torch.cuda.device(index):
+            F.call(name, *args, _stream_handle(index))
 
 
 def _heads_ld(name, t, B, T, device):
@@ -328,7 +340,7 @@ def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
                                      and seq_lens.device == dev and seq_lens.is_contiguous()):
         raise ValueError(f"seq_lens: contiguous int32 [{B}] on {dev}")
     return F.AttnDesc(B, T, Hq, k.shape[2], hd, hd ** -0.5 if scale is None else scale, 1 if causal else 0, *lds,
-                      _p(seq_lens))
+                      _a(seq_lens))
 
 
 def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
@@ -339,7 +351,7 @@ def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     d = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
     lse = torch.empty((d.B, d.n_q_heads, d.T), dtype=torch.float32, device=q.device)
-    _call_on(q, "glt_attention_train_fwd", ctypes.byref(d), _p(q), _p(k), _p(v), _p(out), _p(lse))
+    _call_on(q, "glt_attention_train_fwd", ctypes.byref(d), _a(q), _a(k), _a(v), _a(out), _a(lse))
     return out, lse
 
 
@@ -381,8 +393,8 @@ def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=Non
     nb = F.load().glt_attention_bwd_workspace_size(ctypes.byref(d))
     workspace = _workspace(workspace, nb, dev)
     dq, dk, dv = grads
-    _call_on(q, "glt_attention_bwd", ctypes.byref(d), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(dout), _p(dq), _p(dk),
-             _p(dv), _p(workspace), workspace.numel())
+    _call_on(q, "glt_attention_bwd", ctypes.byref(d), _a(q), _a(k), _a(v), _a(out), _a(lse), _a(dout), _a(dq), _a(dk),
+             _a(dv), _a(workspace), workspace.numel())
     return dq, dk, dv
 
 
@@ -567,8 +579,8 @@ def token_logprobs(logits, ids=None, top_k=0, temperature=1.0, workspace=None):
         r["top_ids"], r["top_logprobs"] = new((rows, top_k), torch.int32), new((rows, top_k))
     nb = F.load().glt_token_logprobs_workspace_size(rows, V, dt, top_k)
     ws = _workspace(workspace, nb, dev)
-    _call_on(logits, "glt_token_logprobs", _p(logits), dt, ld, rows, V, temperature, _p(ids), n, top_k, _p(r["logprobs"]),
-             _p(r["entropy"]), _p(r["lse"]), _p(r.get("top_ids")), _p(r.get("top_logprobs")), _p(ws), ws.numel())
+    _call_on(logits, "glt_token_logprobs", _a(logits), dt, ld, rows, V, temperature, _a(ids), n, top_k, _a(r["logprobs"]),
+             _a(r["entropy"]), _a(r["lse"]), _a(r.get("top_ids")), _a(r.get("top_logprobs")), _a(ws), ws.numel())
     return r
 
 
@@ -590,9 +602,9 @@ def token_logprobs_bwd(logits, ids, lse, grad_logprobs, entropy=None, grad_entro
         grad = torch.empty((rows, V), dtype=logits.dtype, device=dev)
     _need(grad.shape == logits.shape and grad.dtype == logits.dtype and grad.device == dev
           and (V == 1 or grad.stride(1) == 1), "grad: the logits' shape, dtype and device, rows contiguous")
-    _call_on(logits, "glt_token_logprobs_bwd", _p(logits), dt, ld, rows, V, temperature, _p(ids), n,
-             _p(grad_logprobs if n else None), _p(lse), _p(entropy if grad_entropy is not None else None),
-             _p(grad_entropy), _p(grad), grad.stride(0) if rows > 1 else V)
+    _call_on(logits, "glt_token_logprobs_bwd", _a(logits), dt, ld, rows, V, temperature, _a(ids), n,
+             _a(grad_logprobs if n else None), _a(lse), _a(entropy if grad_entropy is not None else None),
+             _a(grad_entropy), _a(grad), grad.stride(0) if rows > 1 else V)
     return grad
 
 
