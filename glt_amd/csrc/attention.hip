@@ -102,24 +102,9 @@ __global__ void __launch_bounds__(256) vt_pack_kernel(const uint16_t* __restrict
   }
 }
 
-// What the training form takes beside the inference form's arguments.
-struct TrainArgs {
-  const int32_t* seq_lens;  // [B] or null
-  float* lse;               // [B, Hq, T]
-  int64_t q_ld, k_ld, v_ld, o_ld;
-};
-
-// TRAIN (glt_attention_train_fwd): row strides, sequence lengths (keys past a
-// sequence's end are masked and read as zeros, its rows past the end give zero
-// output and lse -inf), and lse = log(sum exp) of each row. V^T fragments come
-// from the V tile itself by transposed LDS reads (`vt` is v, the v tile laid
-// out as attention_dev.hpp describes), whose key order is the accumulators'
-// own: no transposed copy of v and no lane exchange for P^T.
-template <bool TRAIN>
 __global__ void __launch_bounds__(512, 1)
 attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ vt,
-                uint16_t* __restrict__ out, int B, int T, int Tpad, int Hq, int Hkv, float scale_log2, int causal,
-                TrainArgs ta) {
+                uint16_t* __restrict__ out, int B, int T, int Tpad, int Hq, int Hkv, float scale_log2, int causal) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -139,11 +124,9 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
   const int myq = wq0 + lq;                          // this lane's query
   // key tiles up to the workgroup's last row's limit (every wavefront runs
   // every tile; a tile past a wavefront's causal limit is masked whole)
-  const int len = TRAIN && ta.seq_lens ? min(max(ta.seq_lens[b], 0), T) : T;
-  const int kv_end = TRAIN && q0 >= len ? 0 : causal ? min(len, q0 + kQBlock) : len;
+  const int kv_end = causal ? min(T, q0 + kQBlock) : T;
   const int ntiles = (kv_end + kKvTile - 1) / kKvTile;
-  const int64_t q_ld = TRAIN ? ta.q_ld : (int64_t)Hq * kHd, kv_ld = TRAIN ? ta.k_ld : (int64_t)Hkv * kHd;
-  const int64_t o_ld = TRAIN ? ta.o_ld : q_ld;
+  const int64_t q_ld = (int64_t)Hq * kHd, kv_ld = (int64_t)Hkv * kHd;
 
   // ---- Q fragments (B operand of S^T): lane holds query lq, d = 16s + 8lh .. +7
   bf16x8 qf[8];
@@ -151,19 +134,15 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
     const uint16_t* qp = q + ((int64_t)b * T + min(myq, T - 1)) * q_ld + (int64_t)h * kHd + 8 * lh;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const u32x4 x = myq < len ? *reinterpret_cast<const u32x4*>(qp + 16 * s) : u32x4{0, 0, 0, 0};
+      const u32x4 x = myq < T ? *reinterpret_cast<const u32x4*>(qp + 16 * s) : u32x4{0, 0, 0, 0};
       qf[s] = __builtin_bit_cast(bf16x8, x);
     }
   }
 
-  // TRAIN: descriptors of this sequence's rows of this head alone, so that
-  // rows at or past len read as zeros
-  const __amdgpu_buffer_rsrc_t rk = TRAIN ? uni_rsrc_a(k + (int64_t)b * T * kv_ld + (int64_t)g * kHd, rows_extent(len, kv_ld))
-                                          : uni_rsrc_a(k, kExtentA);
-  const __amdgpu_buffer_rsrc_t rv = TRAIN ? uni_rsrc_a(vt + (int64_t)b * T * ta.v_ld + (int64_t)g * kHd, rows_extent(len, ta.v_ld))
-                                          : uni_rsrc_a(vt, kExtentA);
+  const __amdgpu_buffer_rsrc_t rk = uni_rsrc_a(k, kExtentA);
+  const __amdgpu_buffer_rsrc_t rv = uni_rsrc_a(vt, kExtentA);
   const uint32_t row_bytes = (uint32_t)(kv_ld * 2);
-  const uint32_t kv_base = TRAIN ? 0u : (uint32_t)(((int64_t)b * T * kv_ld + (int64_t)g * kHd) * 2);
+  const uint32_t kv_base = (uint32_t)(((int64_t)b * T * kv_ld + (int64_t)g * kHd) * 2);
   // ---- K tile (by one group of four wavefronts: group A in its
   // arithmetic phases, K(1) by group B in the prologue): 16 direct-to-LDS
   // loads of 1 KB, four per wavefront; load i of the group's wavefront w
@@ -181,7 +160,7 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
   auto load_k = [&](int tile, int slot) {
     char* dst = smem + slot * kTileBytes;
     const uint32_t tile_off = (uint32_t)tile * kKvTile * row_bytes;
-    if ((tile + 1) * kKvTile <= len) {
+    if ((tile + 1) * kKvTile <= T) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(dst + (4 * i + wig) * 1024), 16, kof[i], tile_off, 0,
@@ -190,7 +169,7 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = tile * kKvTile + 4 * (4 * i + wig) + (lane >> 4);
-        const uint32_t off = key < len ? kof[i] + tile_off : kOob;
+        const uint32_t off = key < T ? kof[i] + tile_off : kOob;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(dst + (4 * i + wig) * 1024), 16, off, 0, 0, 0);
       }
     }
@@ -202,13 +181,7 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
   // logical row R = r ^ ((r>>3)&1) and logical chunk (L&7) ^ ((r>>1)&7)
   // (the layout vt_off reads). The tile's part of the offset is scalar.
   uint32_t vof[4];
-  if constexpr (TRAIN) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * (4 * i + wig) + (lane >> 4);
-      vof[i] = (uint32_t)(((lane & 15) ^ tile_key(row)) * 16) + (uint32_t)row * (uint32_t)(ta.v_ld * 2);
-    }
-  } else {
+  {
     const uint32_t vt_base = (uint32_t)(((int64_t)b * Hkv + g) * kHd * Tpad * 2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -219,14 +192,6 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
   }
   auto load_vt = [&](int tile, int slot) {
     char* dst = smem + kVtBase + slot * kTileBytes;
-    if constexpr (TRAIN) {
-      const uint32_t tile_off = (uint32_t)tile * kKvTile * (uint32_t)(ta.v_ld * 2);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (4 * i + wig) * 1024), 16, vof[i] + tile_off, 0,
-                                                 0, 0);
-      return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(dst + (4 * i + wig) * 1024), 16, vof[i],
@@ -240,7 +205,6 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
   for (int s = 0; s < 8; ++s) kfa[s] = (uint32_t)(lq * 256 + (((2 * s + lh) ^ (lq & 15)) << 4));
 #pragma unroll
   for (int s2 = 0; s2 < 4; ++s2) vfa[s2] = vt_off(lq, 2 * s2 + lh, 0);
-  const uint32_t vca = TRAIN ? lds_addr(smem) + kVtBase + col_frag_off(lane) : 0u;
 
   // ---- state
   f32x16 o[4];
@@ -251,24 +215,19 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
 #pragma unroll
   for (int i = 0; i < 4; ++i) pb[i] = bf16x8{};
   float m_run = kMaskVal, l_run = 0.f;
-  float l_exact = 0.f;  // TRAIN: row sum of the unrounded probabilities, for lse
 
   // MFMA phase m: S^T(m) = K(m) . Q^T (K slot m % 3) and O^T += V^T(m-1) .
   // P^T(m-1) (V^T slot (m-1)&1), the two products' MFMAs interleaved.
   auto mfma_phase = [&](int m) {
     const char* kt = smem + (m % 3) * kTileBytes;
     const char* vt = smem + kVtBase + ((m + 1) & 1) * kTileBytes;
-    const uint32_t vcol = vca + ((m + 1) & 1) * kTileBytes;
     sacc[0] = f32x16{};
     sacc[1] = f32x16{};
     // MFMA pair i: S^T step (key block i & 1, d step i >> 1) and PV step
     // (16-key step i >> 2, d block i & 3); each fragment is read three
     // pairs ahead (a fence per pair keeps the reads from all being hoisted).
     auto kread = [&](int i) { return *reinterpret_cast<const bf16x8*>(kt + (i & 1) * 8192 + kfa[i >> 1]); };
-    auto vread = [&](int i) {
-      if constexpr (TRAIN) return col_frag(vcol, i & 3, i >> 2);
-      else return *reinterpret_cast<const bf16x8*>(vt + (i & 3) * 4096 + vfa[i >> 2]);
-    };
+    auto vread = [&](int i) { return *reinterpret_cast<const bf16x8*>(vt + (i & 3) * 4096 + vfa[i >> 2]); };
     bf16x8 kq[3], vq[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -297,16 +256,13 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
   // adds exactly nothing (p = 0, no rescale).
   auto softmax = [&](int m) {
     const int key0 = m * kKvTile;
-    // TRAIN masks with -inf, which no scale lifts (a live row's first tile
-    // holds a key that it may read, so the running maximum stays finite).
-    if (key0 + kKvTile > len || (causal && key0 + kKvTile - 1 > wq0)) {
-      const float masked = TRAIN ? -INFINITY : kMaskVal;
-      const int lim = (causal ? min(len, myq + 1) : len) - (key0 + 4 * lh);
+    if (key0 + kKvTile > T || (causal && key0 + kKvTile - 1 > wq0)) {
+      const int lim = (causal ? min(T, myq + 1) : T) - (key0 + 4 * lh);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          sacc[kb][e] = (32 * kb + 8 * (e >> 2) + (e & 3)) < lim ? sacc[kb][e] : masked;
+          sacc[kb][e] = (32 * kb + 8 * (e >> 2) + (e & 3)) < lim ? sacc[kb][e] : kMaskVal;
     }
     // two independent chains of three-input maxima, one per key block
     float m2[2];
@@ -322,7 +278,6 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
-      if constexpr (TRAIN) l_exact *= alpha;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] *= alpha;
     }
@@ -335,7 +290,6 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           p4[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kb][4 * gi + e], scale_log2, -m_run));
-        if constexpr (TRAIN) l_exact += (p4[0] + p4[1]) + (p4[2] + p4[3]);
         pk[kb][gi][0] = pack2_rne(p4[0], p4[1]);
         pk[kb][gi][1] = pack2_rne(p4[2], p4[3]);
       }
@@ -361,10 +315,6 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
 #pragma unroll
     for (int s2 = 0; s2 < 4; ++s2) {
       const int kb = s2 >> 1, g0 = 2 * (s2 & 1), g1 = g0 + 1;
-      if constexpr (TRAIN) {
-        pb[s2] = __builtin_bit_cast(bf16x8, u32x4{pk[kb][g0][0], pk[kb][g0][1], pk[kb][g1][0], pk[kb][g1][1]});
-        continue;
-      }
       const auto s0 = __builtin_amdgcn_permlane32_swap(pk[kb][g0][0], pk[kb][g1][0], false, false);
       const auto s1 = __builtin_amdgcn_permlane32_swap(pk[kb][g0][1], pk[kb][g1][1], false, false);
       pb[s2] = __builtin_bit_cast(bf16x8, u32x4{s0[0], s1[0], s0[1], s1[1]});
@@ -426,20 +376,9 @@ attn_fwd_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, 
 
   // ---- normalise and store: lane holds d = 32hb + 8(e>>2) + 4lh + (e&3)
   const float l_tot = pair_sum(l_run);
-  // (a NaN sum gives NaN)
-  const float inv = TRAIN ? (l_tot == 0.f || myq >= len ? 0.f : 1.0f / l_tot) : l_tot > 0.f ? 1.0f / l_tot : 0.f;
-  if constexpr (TRAIN) {
-    const float le = pair_sum(l_exact);
-    if (lh == 0 && myq < T)
-      ta.lse[((int64_t)b * Hq + h) * T + myq] =
-          myq < len ? (m_run + __builtin_amdgcn_logf(le)) * 0.6931471805599453f : -INFINITY;
-    // dead rows: zeros, whatever the lanes hold
-    if (myq >= len)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = f32x16{};
-  }
+  const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
   if (myq < T) {
-    uint16_t* op = out + ((int64_t)b * T + myq) * o_ld + (int64_t)h * kHd + 4 * lh;
+    uint16_t* op = out + ((int64_t)b * T + myq) * q_ld + (int64_t)h * kHd + 4 * lh;
 #pragma unroll
     for (int hb = 0; hb < 4; ++hb)
 #pragma unroll
@@ -486,7 +425,7 @@ extern "C" glt_status glt_attention_fwd(const void* q, const void* k, const void
   GLT_TRY_HIP(hipGetDevice(&dev));
   GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_attention_fwd: device index %d out of range", dev);
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_fwd_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, kAttnLds));
+    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_fwd_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kAttnLds));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const float scale_log2 = scale * 1.4426950408889634f;
@@ -499,65 +438,9 @@ extern "C" glt_status glt_attention_fwd(const void* q, const void* k, const void
   const int64_t nblk = (int64_t)((T + kQBlock - 1) / kQBlock) * Hq * B;
   GLT_CHECK(nblk < INT32_MAX, GLT_ERR_SHAPE, "glt_attention_fwd: %lld workgroups", (long long)nblk);
   dim3 grid((unsigned)nblk, 1, 1);
-  GLT_LAUNCH("attention", attn_fwd_kernel<false>, grid, dim3(512), kAttnLds, as_stream(stream),
+  GLT_LAUNCH("attention", attn_fwd_kernel, grid, dim3(512), kAttnLds, as_stream(stream),
              static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), vt, static_cast<uint16_t*>(out), B, T,
-             Tpad, Hq, Hkv, scale_log2, causal, TrainArgs{});
+             Tpad, Hq, Hkv, scale_log2, causal);
   GLT_LAUNCH_CHECK("attention");
-  return GLT_OK;
-}
-
-namespace glt {
-
-glt_status check_attn_desc(const glt_attn_desc* d, const char* who) {
-  GLT_CHECK(d, GLT_ERR_INVALID_ARG, "%s: null descriptor", who);
-  GLT_CHECK(d->B >= 0 && d->T >= 0 && d->n_q_heads > 0 && d->n_kv_heads > 0 && d->n_q_heads % d->n_kv_heads == 0,
-            GLT_ERR_SHAPE, "%s: B=%d T=%d n_q_heads=%d n_kv_heads=%d (n_q_heads must be a multiple of n_kv_heads)", who,
-            d->B, d->T, d->n_q_heads, d->n_kv_heads);
-  GLT_CHECK(d->head_dim == kHd, GLT_ERR_UNSUPPORTED, "%s: head_dim %d (only %d)", who, d->head_dim, kHd);
-  GLT_CHECK(d->scale > 0.f && d->scale <= 3.4028234e38f, GLT_ERR_INVALID_ARG, "%s: scale %g must be positive and finite",
-            who, (double)d->scale);
-  const int64_t lds[4] = {d->q_ld, d->k_ld, d->v_ld, d->o_ld};
-  const int heads[4] = {d->n_q_heads, d->n_kv_heads, d->n_kv_heads, d->n_q_heads};
-  for (int i = 0; i < 4; ++i) {
-    GLT_CHECK(lds[i] >= (int64_t)heads[i] * kHd && lds[i] % 8 == 0, GLT_ERR_SHAPE,
-              "%s: %c_ld %lld (at least %d heads of %d, a multiple of 8)", who, "qkvo"[i], (long long)lds[i], heads[i],
-              kHd);
-    // one sequence's rows, and the last tiles' past its end, are addressed
-    // through 31-bit offsets
-    GLT_CHECK(lds[i] < (int64_t)kOob && ((int64_t)d->T + 256) * lds[i] * 2 < (int64_t)kOob, GLT_ERR_SHAPE,
-              "%s: T=%d rows of %c_ld %lld pass 2 GiB", who, d->T, "qkvo"[i], (long long)lds[i]);
-  }
-  GLT_CHECK(((int64_t)d->T + 255) / 256 * d->B < INT32_MAX / d->n_q_heads / 8, GLT_ERR_SHAPE, "%s: B=%d T=%d n_q_heads=%d",
-            who, d->B, d->T, d->n_q_heads);
-  return GLT_OK;
-}
-
-}  // namespace glt
-
-extern "C" glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
-                                              void* out, float* lse, void* stream) {
-  const glt_status s = check_attn_desc(d, "glt_attention_train_fwd");
-  if (s != GLT_OK) return s;
-  if (d->B == 0 || d->T == 0) return GLT_OK;
-  GLT_CHECK(q && k && v && out && lse, GLT_ERR_INVALID_ARG, "glt_attention_train_fwd: null pointer");
-  GLT_CHECK(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0 && (uintptr_t)lse % 4 == 0 &&
-                (uintptr_t)d->seq_lens % 4 == 0,
-            GLT_ERR_ALIGNMENT, "glt_attention_train_fwd: tensors must be 16-byte aligned");
-  static std::atomic<bool> attr_set[64];
-  int dev = 0;
-  GLT_TRY_HIP(hipGetDevice(&dev));
-  GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_attention_train_fwd: device index %d out of range", dev);
-  if (!attr_set[dev].load(std::memory_order_acquire)) {
-    GLT_TRY_HIP(
-        hipFuncSetAttribute((const void*)attn_fwd_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, kAttnLds));
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-  const int64_t nblk = (int64_t)((d->T + kQBlock - 1) / kQBlock) * d->n_q_heads * d->B;
-  const TrainArgs ta{d->seq_lens, lse, d->q_ld, d->k_ld, d->v_ld, d->o_ld};
-  GLT_LAUNCH("attention_train", attn_fwd_kernel<true>, dim3((unsigned)nblk), dim3(512), kAttnLds, as_stream(stream),
-             static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
-             static_cast<uint16_t*>(out), d->B, d->T, 0, d->n_q_heads, d->n_kv_heads, d->scale * 1.4426950408889634f,
-             d->causal, ta);
-  GLT_LAUNCH_CHECK("attention_train");
   return GLT_OK;
 }

@@ -18,6 +18,19 @@
 // directions that the products need (attention_dev.hpp). The score products
 // are formed so that a lane holds one OWNED row: the packed p or ds is then the
 // next product's operand as it stands in the accumulator's layout.
+//
+// Bound by the matrix instructions and the arithmetic between them: the rows in
+// registers leave room for two wavefronts per SIMD, and a wavefront's own
+// products depend on its exponentials, so one wavefront's arithmetic has to run
+// beside the other's products. The two come from two workgroups of four, which
+// nothing keeps in step. With one workgroup of eight instead (half the loads
+// into LDS) they wait at the same barrier, and short rows leave more of them
+// idle; dq + dkdv in us, 32 query and 8 kv heads, eight against four:
+//   6 x 777 causal 217, 190; 1 x 1024 causal 98, 76;
+//   2 x 4096 causal 911, 891; 2 x 4096 full 1672, 1698.
+// At 2 x 4096 causal the two kernels and the sum of parts take 393, 498 and 49
+// us: 0.96 * 10^15 operations a second of the seven products, the matrix units
+// busy half of the time (a large library product: 1.24 * 10^15).
 #include <algorithm>
 #include <atomic>
 
@@ -27,9 +40,6 @@ namespace glt {
 
 namespace {
 
-constexpr int kTile = 64;                     // walked rows per tile
-constexpr int kTileB = kTile * kHd * 2;       // 16 KB
-constexpr float kLog2e = 1.4426950408889634f;
 // Key tiles up to which a block of rows takes D from its own probabilities.
 constexpr int kExactTiles = 8;
 
@@ -40,7 +50,7 @@ struct BwdArgs {
   const uint16_t* out;
   const uint16_t* dout;
   const float* lse;    // [B, Hq, T]
-  float* delta;        // [B, Hq, T]: D, written by the dq kernel
+  float* stats;        // [2][B, Hq, T]: lse log2(e) and D, written by the dq kernel
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
@@ -51,105 +61,47 @@ struct BwdArgs {
   float scale;
 };
 
-__device__ __forceinline__ int seq_len(const BwdArgs& a, int b) {
-  return a.seq_lens ? min(max(a.seq_lens[b], 0), a.T) : a.T;
+// D of the lane's row: the diagonal of out . dout^T. The matrix product sums it
+// in the order in which it sums dp, so a row whose output is one key's value (a
+// single key) gets ds = 0 exactly.
+__device__ __forceinline__ float row_delta(const uint16_t* out_row, bool live, const bf16x8* dof, int lane) {
+  const int lq = lane & 31, lh = lane >> 5;
+  bf16x8 of[8];
+  load_rows(of, out_row, live, lh);
+  f32x16 x{};
+#pragma unroll
+  for (int s = 0; s < 8; ++s) x = mfma(of[s], dof[s], x);
+  // row lq = 8 (lq >> 3) + 4 ((lq >> 2) & 1) + (lq & 3) of column lq
+  const int e = 4 * (lq >> 3) + (lq & 3);
+  float y = x[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) y = e == i ? x[i] : y;
+  return pair_sum(((lq >> 2) & 1) == lh ? y : 0.f);
 }
 
-// One tile (64 rows of a head, from byte row0_bytes) into LDS, by this
-// wavefront's share of the 16 loads of 1 KB (four rows each). off: this lane's
-// byte offset of its first load (tile_lane_off); a further load lies 4 WAVES
-// rows on, a multiple of 16, where tile_key is the same. Rows past the
-// descriptor are zeros.
-template <int WAVES>
-__device__ __forceinline__ void load_tile(__amdgpu_buffer_rsrc_t r, char* dst, int wave, uint32_t off, uint32_t row_bytes,
-                                          uint32_t row0_bytes) {
-#pragma unroll
-  for (int i = 0; i < 16 / WAVES; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + (WAVES * i + wave) * 1024), 16,
-                                             off + (row0_bytes + 4 * WAVES * i * row_bytes), 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t tile_lane_off(int wave, int lane, uint32_t row_bytes) {
-  const int row = 4 * wave + (lane >> 4);
-  return (uint32_t)row * row_bytes + (uint32_t)(((lane & 15) ^ tile_key(row)) << 4);
-}
+constexpr int kWaves = 4;
+constexpr int kRows = 32 * kWaves;  // rows that a workgroup owns
 
-// A wavefront's 32 rows of 128 as MFMA operands: lane row (lane & 31),
-// elements 16 s + 8 (lane >> 5) .. +7; rows at or past the end are zeros.
-__device__ __forceinline__ void load_rows(bf16x8* f, const uint16_t* row, bool live, int lh) {
-#pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    const u32x4 x = live ? *reinterpret_cast<const u32x4*>(row + 16 * s + 8 * lh) : u32x4{0u, 0u, 0u, 0u};
-    f[s] = __builtin_bit_cast(bf16x8, x);
-  }
-}
-
-__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-// elements 8 s2 .. +7 of an accumulator, rounded: the operand of 16 contracted
-// rows in the order that col_frag() reads them
-__device__ __forceinline__ bf16x8 pack_frag(const f32x16& x, int s2) {
-  const int o = 8 * s2;
-  return __builtin_bit_cast(bf16x8, u32x4{pack2_rne(x[o], x[o + 1]), pack2_rne(x[o + 2], x[o + 3]),
-                                          pack2_rne(x[o + 4], x[o + 5]), pack2_rne(x[o + 6], x[o + 7])});
-}
-
-// Score product of 32 walked rows: x += X . f^T over the 128 columns, the
-// fragments read kAhead steps ahead; between(i) is arithmetic that the
-// scheduler may put beside step i's matrix instruction. (The fence per step
-// keeps the reads from all being hoisted, which needs more registers than
-// there are.)
-constexpr int kAhead = 2;
-template <typename F>
-__device__ __forceinline__ void score_product(uint32_t X, const bf16x8* f, f32x16& x, F between) {
-  bf16x8 xa[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) xa[i] = row_frag(X, i);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x = mfma(xa[i % kAhead], f[i], x);
-    if (i + kAhead < 8) xa[i % kAhead] = row_frag(X, i + kAhead);
-    between(i);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-}
-// an address that is worked out where it is used, not kept in a register for
-// every offset
-__device__ __forceinline__ uint32_t opaque(uint32_t x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
-// Accumulator of a transposed product (lane: owned row, elements: d = 32 db +
-// 8 g + 4 lh + e) times `scale`, rounded once, to this lane's output row.
-__device__ __forceinline__ void store_rows(uint16_t* row, const f32x16* acc, float scale, int lh) {
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const u32x2a w = {pack2_rne(acc[db][4 * g] * scale, acc[db][4 * g + 1] * scale),
-                        pack2_rne(acc[db][4 * g + 2] * scale, acc[db][4 * g + 3] * scale)};
-      *reinterpret_cast<u32x2a*>(row + 32 * db + 8 * g + 4 * lh) = w;
-    }
-}
+// Steps that fragments are read ahead of their matrix instructions: what the
+// registers of each loop allow (dkdv holds two more sets of accumulators).
+constexpr int kDqAhead = 4, kDkdvAhead = 2, kGradAhead = 2;
 
 // ------------------------------------------------------------------- dq
-// One workgroup per (batch, query head, block of 32 WAVES queries), longest
-// rows first. LDS: two buffers of a K and a V tile (64 KB).
-template <int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a) {
+// One workgroup per (batch, query head, block of 128 queries), longest rows
+// first. LDS: two buffers of a K and a V tile (65 KB).
+__global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nqb = (a.T + 32 * WAVES - 1) / (32 * WAVES);
+  const int nqb = (a.T + kRows - 1) / kRows;
   const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
   const int id = blockIdx.x, hb = id % nhb;
   const int qb = nqb - 1 - id / nhb;
   const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
-  const int q0 = qb * 32 * WAVES, wq0 = q0 + 32 * wave, myq = wq0 + lq;
-  const int len = seq_len(a, b);
+  const int q0 = qb * kRows, wq0 = q0 + 32 * wave, myq = wq0 + lq;
+  const int len = seq_len(a.seq_lens, b, a.T);
   const bool live = myq < len;
-  const int kv_end = q0 >= len ? 0 : a.causal ? min(len, q0 + 32 * WAVES) : len;
+  const int kv_end = q0 >= len ? 0 : a.causal ? min(len, q0 + kRows) : len;
   const int ntiles = (kv_end + kTile - 1) / kTile;
   const int64_t tok = (int64_t)b * a.T + min(myq, a.T - 1);
   const int64_t stat = ((int64_t)b * a.Hq + h) * a.T + min(myq, a.T - 1);
@@ -160,8 +112,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a)
   const uint32_t kof = tile_lane_off(wave, lane, kb_ld), vof = tile_lane_off(wave, lane, vb_ld);
   auto load = [&](int t, int buf) {
     char* dst = smem + buf * 2 * kTileB;
-    load_tile<WAVES>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
-    load_tile<WAVES>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
+    load_tile<kWaves>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
+    load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
   };
   if (ntiles > 0) load(0, 0);
 
@@ -169,23 +121,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a)
   load_rows(qf, a.q + tok * a.q_ld + (int64_t)h * kHd, live, lh);
   load_rows(dof, a.dout + tok * a.o_ld + (int64_t)h * kHd, live, lh);
   const float lse2 = live ? a.lse[stat] * kLog2e : 0.f;
-  // D of the lane's row: the diagonal of out . dout^T. The matrix product sums
-  // it in the order in which it sums dp, so a row whose output is one key's
-  // value (a single key) gets ds = 0 exactly.
-  float D;
-  {
-    bf16x8 of[8];
-    load_rows(of, a.out + tok * a.o_ld + (int64_t)h * kHd, live, lh);
-    f32x16 x{};
-#pragma unroll
-    for (int s = 0; s < 8; ++s) x = mfma(of[s], dof[s], x);
-    // row lq = 8 (lq >> 3) + 4 ((lq >> 2) & 1) + (lq & 3) of column lq
-    const int e = 4 * (lq >> 3) + (lq & 3);
-    float y = x[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) y = e == i ? x[i] : y;
-    D = pair_sum(((lq >> 2) & 1) == lh ? y : 0.f);
-  }
+  float D = row_delta(a.out + tok * a.o_ld + (int64_t)h * kHd, live, dof, lane);
 
   const uint32_t ro = lds_addr(smem) + row_frag_off(lane), co = lds_addr(smem) + col_frag_off(lane);
   const float scale_log2 = a.scale * kLog2e;
@@ -193,14 +129,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a)
   // Score products of key block kb (32 keys) of tile t: p in s, dp.
   auto probs = [&](int t, int kb, uint32_t row, f32x16& s, f32x16& dp) {
     const int key0 = t * kTile + 32 * kb;
-    score_product(row, qf, s, [](int) {});
+    score_product<kDqAhead>(row, qf, s, [](int) {});
     if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {
       const int lim = (a.causal ? min(len, myq + 1) : len) - (key0 + 4 * lh);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < lim ? s[e] : -INFINITY;
     }
     // the exponentials beside the other product
-    score_product(row + kTileB, dof, dp, [&](int i) {
+    score_product<kDqAhead>(row + kTileB, dof, dp, [&](int i) {
 #pragma unroll
       for (int e = 2 * i; e < 2 * i + 2; ++e)
         s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale_log2, -lse2));
@@ -220,7 +156,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a)
       for (int kb = 0; kb < 2; ++kb) {
         const int key0 = t * kTile + 32 * kb;
         if (key0 >= kv_end || (a.causal && key0 > wq0 + 31)) continue;
-        block(t, kb, opaque(ro + buf + kb * 8192), opaque(co + buf + kb * 8192));
+        block(t, kb, opaque(ro + buf + kb * 8 * kGroupB), opaque(co + buf + kb * 8 * kGroupB));
       }
     }
   };
@@ -239,7 +175,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a)
     });
     D += pair_sum(d);
   }
-  if (lh == 0 && myq < a.T) a.delta[stat] = live ? D : 0.f;
+  if (lh == 0 && myq < a.T) {
+    a.stats[stat] = lse2;
+    a.stats[(int64_t)a.B * a.Hq * a.T + stat] = live ? D : 0.f;
+  }
 
   f32x16 dq[4];
 #pragma unroll
@@ -265,25 +204,25 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dq_kernel(const BwdArgs a)
 }
 
 // ---------------------------------------------------------------- dk, dv
-// One workgroup per (batch, query head, block of 32 WAVES keys), the blocks
-// with the most queries first. LDS: two buffers of a Q and a dout tile and their
-// 64 lse and D values. Where query heads share a kv head, each writes its f32
-// part and attn_dkdv_sum_kernel adds the parts in head order: a workgroup that
-// walked the group's heads one after the other would leave too few workgroups
-// for the chip (2 x 4096 tokens, 8 kv heads: 256 of very different length),
-// and a cut that depends on the batch would make the sums' order depend on it.
+// One workgroup per (batch, query head, block of 128 keys), the blocks with the
+// most queries first. LDS: two buffers of a Q and a dout tile and their 64 lse
+// (times log2 e) and D values. Where query heads share a kv head, each writes its
+// f32 part and attn_dkdv_sum_kernel adds the parts in head order: a workgroup
+// that walked the group's heads one after the other would leave too few
+// workgroups for the chip (2 x 4096 tokens, 8 kv heads: 512 of very different
+// length), and a cut that depends on the batch would make the sums' order depend
+// on it. The parts cost 49 of 940 us at 2 x 4096 (268 MB written and read).
 constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
 
-template <int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 2) attn_dkdv_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
   const int id = blockIdx.x, hb = id % nhb, kb = id / nhb;
   const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
-  const int k0 = kb * 32 * WAVES, wk0 = k0 + 32 * wave;
-  const int len = seq_len(a, b);
+  const int k0 = kb * kRows, wk0 = k0 + 32 * wave;
+  const int len = seq_len(a.seq_lens, b, a.T);
 
   bf16x8 kf[8], vf[8];
   {
@@ -300,12 +239,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dkdv_kernel(const BwdArgs 
   // and dout = 0, so they add nothing
   const __amdgpu_buffer_rsrc_t rq = uni_rsrc_a(a.q + (int64_t)b * a.T * a.q_ld + (int64_t)h * kHd, rows_extent(len, a.q_ld));
   const __amdgpu_buffer_rsrc_t rdo = uni_rsrc_a(a.dout + (int64_t)b * a.T * a.o_ld + (int64_t)h * kHd, rows_extent(len, a.o_ld));
-  const __amdgpu_buffer_rsrc_t rs = uni_rsrc_a((wave & 1 ? a.delta : a.lse) + ((int64_t)b * a.Hq + h) * a.T, (uint32_t)len * 4);
+  const __amdgpu_buffer_rsrc_t rs = uni_rsrc_a(a.stats + ((wave & 1) * (int64_t)a.B * a.Hq + (int64_t)b * a.Hq + h) * a.T, (uint32_t)len * 4);
   auto load = [&](int qt, int buf) {
     char* dst = smem + buf * kDkdvBuf;
     const int l = opaque(threadIdx.x) & 63;
-    load_tile<WAVES>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld);
-    load_tile<WAVES>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld);
+    load_tile<kWaves>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld);
+    load_tile<kWaves>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld);
     if (wave < 2)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + 2 * kTileB + wave * kTile * 4), 4,
                                                (uint32_t)(qt * kTile + l) * 4, 0, 0, 0);
@@ -329,8 +268,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dkdv_kernel(const BwdArgs 
       const int q0 = q0t + 32 * qb;
       if (q0 >= len || (a.causal && q0 + 31 < wk0)) continue;
       f32x16 s{}, dp{};
-      const uint32_t row = opaque(ro + buf + qb * 8192);
-      score_product(row, kf, s, [](int) {});
+      const uint32_t row = opaque(ro + buf + qb * 8 * kGroupB);
+      score_product<kDkdvAhead>(row, kf, s, [](int) {});
       if (a.causal && q0 < wk0 + 31) {  // row q0 + 8 (e >> 2) + 4 lh + (e & 3) reads keys up to itself
         const int l = opaque(threadIdx.x) & 63;
         const int lim = wk0 + (l & 31) - (q0 + 4 * (l >> 5));
@@ -340,11 +279,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dkdv_kernel(const BwdArgs 
       // the exponentials beside the other product; elements 4 i .. + 3 are
       // query rows 8 i + 4 lh .. + 3
       const uint32_t st = opaque(lds_addr(smem) + buf + 2 * kTileB + 128 * qb + 16 * (lane >> 5));
-      score_product(row + kTileB, vf, dp, [&](int i) {
+      score_product<kDkdvAhead>(row + kTileB, vf, dp, [&](int i) {
         const f32x2 l = *reinterpret_cast<const lds_f32x2*>((uintptr_t)(st + 32 * (i >> 1) + 8 * (i & 1)));
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          s[2 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + e], scale_log2, -l[e] * kLog2e));
+          s[2 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + e], scale_log2, -l[e]));
       });
       u32x4 pw[2], dw[2];  // packed p and ds
 #pragma unroll
@@ -358,23 +297,25 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attn_dkdv_kernel(const BwdArgs 
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      const uint32_t col = opaque(co + buf + qb * 8192);
-      bf16x8 oa[kAhead], qa[kAhead];  // step i: 16 query rows i >> 2, d block i & 3
+      const uint32_t col = opaque(co + buf + qb * 8 * kGroupB);
+      __builtin_amdgcn_s_setprio(1);
+      bf16x8 oa[kGradAhead], qa[kGradAhead];  // step i: 16 query rows i >> 2, d block i & 3
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+      for (int i = 0; i < kGradAhead; ++i) {
         oa[i] = col_frag(col + kTileB, i & 3, i >> 2);
         qa[i] = col_frag(col, i & 3, i >> 2);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        dv[i & 3] = mfma(oa[i % kAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), dv[i & 3]);
-        dk[i & 3] = mfma(qa[i % kAhead], __builtin_bit_cast(bf16x8, dw[i >> 2]), dk[i & 3]);
-        if (i + kAhead < 8) {
-          oa[i % kAhead] = col_frag(col + kTileB, (i + kAhead) & 3, (i + kAhead) >> 2);
-          qa[i % kAhead] = col_frag(col, (i + kAhead) & 3, (i + kAhead) >> 2);
+        dv[i & 3] = mfma(oa[i % kGradAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), dv[i & 3]);
+        dk[i & 3] = mfma(qa[i % kGradAhead], __builtin_bit_cast(bf16x8, dw[i >> 2]), dk[i & 3]);
+        if (i + kGradAhead < 8) {
+          oa[i % kGradAhead] = col_frag(col + kTileB, (i + kGradAhead) & 3, (i + kGradAhead) >> 2);
+          qa[i % kGradAhead] = col_frag(col, (i + kGradAhead) & 3, (i + kGradAhead) >> 2);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   // the output rows' addresses are worked out again here: kept across the
@@ -424,12 +365,11 @@ __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-size_t delta_bytes(const glt_attn_desc* d) { return round256((size_t)d->B * d->n_q_heads * d->T * sizeof(float)); }
+size_t stats_bytes(const glt_attn_desc* d) { return round256((size_t)2 * d->B * d->n_q_heads * d->T * sizeof(float)); }
 size_t part_bytes(const glt_attn_desc* d) {
   return d->n_q_heads > d->n_kv_heads ? (size_t)2 * d->B * d->T * d->n_q_heads * kHd * sizeof(float) : 0;
 }
 
-template <int WAVES>
 glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   constexpr int kDqLds = 4 * kTileB, kDkdvLds = 2 * kDkdvBuf;
   // the dynamic-LDS limit is a per-device attribute of the kernels
@@ -438,15 +378,15 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   GLT_TRY_HIP(hipGetDevice(&dev));
   GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_attention_bwd: device index %d out of range", dev);
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_dq_kernel<WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, kDqLds));
+    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_dq_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kDqLds));
     GLT_TRY_HIP(
-        hipFuncSetAttribute((const void*)attn_dkdv_kernel<WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
+        hipFuncSetAttribute((const void*)attn_dkdv_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
     attr_set[dev].store(true, std::memory_order_release);
   }
-  const unsigned nb = (unsigned)cdiv(a.T, 32 * WAVES);
-  GLT_LAUNCH("attn_dq", attn_dq_kernel<WAVES>, dim3(nb * a.Hq * a.B), dim3(WAVES * 64), kDqLds, st, a);
+  const unsigned nb = (unsigned)cdiv(a.T, kRows);
+  GLT_LAUNCH("attn_dq", attn_dq_kernel, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDqLds, st, a);
   GLT_LAUNCH_CHECK("attn_dq");
-  GLT_LAUNCH("attn_dkdv", attn_dkdv_kernel<WAVES>, dim3(nb * a.Hq * a.B), dim3(WAVES * 64), kDkdvLds, st, a);
+  GLT_LAUNCH("attn_dkdv", attn_dkdv_kernel, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDkdvLds, st, a);
   GLT_LAUNCH_CHECK("attn_dkdv");
   if (a.Hq > a.Hkv) {
     const int64_t chunks = (int64_t)a.B * a.T * a.Hkv * (kHd / 8);
@@ -464,7 +404,7 @@ using namespace glt;
 
 extern "C" size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d) {
   if (!d || d->B <= 0 || d->T <= 0 || d->n_q_heads <= 0 || d->n_kv_heads <= 0) return 256;
-  return delta_bytes(d) + part_bytes(d);
+  return stats_bytes(d) + part_bytes(d);
 }
 
 extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
@@ -488,14 +428,14 @@ extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, c
   a.out = static_cast<const uint16_t*>(out);
   a.dout = static_cast<const uint16_t*>(dout);
   a.lse = lse;
-  a.delta = static_cast<float*>(workspace);
+  a.stats = static_cast<float*>(workspace);
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);
   a.dv = static_cast<uint16_t*>(dv);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(d));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(d));
   a.seq_lens = d->seq_lens;
   a.q_ld = d->q_ld; a.k_ld = d->k_ld; a.v_ld = d->v_ld; a.o_ld = d->o_ld;
   a.B = d->B; a.T = d->T; a.Hq = d->n_q_heads; a.Hkv = d->n_kv_heads;
   a.causal = d->causal; a.scale = d->scale;
-  return launch_bwd<8>(a, as_stream(stream));
+  return launch_bwd(a, as_stream(stream));
 }

@@ -74,10 +74,10 @@ def test_empty_batches_need_nothing():
 
 
 def test_workspace_holds_row_sums_and_partials():
-    """At least D of every row, and whatever partial sums a call needs."""
+    """lse and D of every row, and f32 dk and dv by query head where heads share a kv head."""
     lib = F.load()
     for B, T, Hq, Hkv in ((1, 1, 8, 1), (2, 61, 16, 4), (3, 777, 32, 8), (2, 4096, 32, 8), (1, 300, 6, 2)):
         d = desc(B=B, T=T, n_q_heads=Hq, n_kv_heads=Hkv, q_ld=Hq * 128, o_ld=Hq * 128, k_ld=Hkv * 128, v_ld=Hkv * 128)
         n = lib.glt_attention_bwd_workspace_size(ctypes.byref(d))
-        assert n % 256 == 0 and n >= 4 * B * T * Hq
-        assert n <= 4 * B * T * Hq + 256 + 8 * B * T * Hq * 128
+        assert n % 256 == 0 and n >= 8 * B * T * Hq
+        assert n <= 8 * B * T * Hq + 256 + 8 * B * T * Hq * 128
