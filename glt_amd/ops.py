@@ -188,12 +188,13 @@ class Ckpt8:
     def load(self, dtype=None, out=None):
         """The values, bf16 or f32 (by default what was saved), into out where
         it is given."""
+        buf, rows, cols = self.buf, self.rows, self.cols
         if out is None:
-            out = torch.empty((self.rows, self.cols), dtype=dtype or self.dtype, device=self.buf.device)
-        _need(dtype in (None, out.dtype) and out.shape == (self.rows, self.cols) and out.device == self.buf.device,
-              f"out: [{self.rows}, {self.cols}] on {self.buf.device}")
+            out = torch.empty(rows, cols, dtype=dtype or self.dtype, device=buf.device)
+        elif dtype not in (None, out.dtype) or out.shape != (rows, cols) or out.device != buf.device:
+            raise ValueError(f"out: [{rows}, {cols}] on {buf.device}")
         dt, ld = _rows_ld("out", out)
-        _call_on(self.buf, "glt_ckpt8_load", _a(self.buf), self.rows, self.cols, _a(out), dt, ld)
+        _call_on(buf, "glt_ckpt8_load", buf.data_ptr(), rows, cols, out.data_ptr(), dt, ld)
         return out
 
 
@@ -222,9 +223,10 @@ def ckpt8_swiglu(gate8, up8):
     MLP's gate_pre and up_pre."""
     rows, cols, dev = gate8.rows, gate8.cols, gate8.buf.device
     _need((rows, cols) == (up8.rows, up8.cols) and up8.buf.device == dev, "gate8 and up8: checkpoints of one shape")
-    out = [torch.empty((rows, cols), dtype=torch.bfloat16, device=dev) for _ in range(3)]
-    _call_on(gate8.buf, "glt_ckpt8_swiglu", _a(gate8.buf), _a(up8.buf), rows, cols, _a(out[0]), _a(out[1]), _a(out[2]))
-    return tuple(out)
+    gate, up, inter = (torch.empty(rows, cols, dtype=torch.bfloat16, device=dev) for _ in range(3))
+    _call_on(gate8.buf, "glt_ckpt8_swiglu", gate8.buf.data_ptr(), up8.buf.data_ptr(), rows, cols, gate.data_ptr(),
+             up.data_ptr(), inter.data_ptr())
+    return gate, up, inter
 
 
 def graft_gemm(kind, M, S, H, out, a=None, lda=0, delta=None, dy=None, ldo=None, alpha=1.0, beta=0.0):
@@ -304,7 +306,7 @@ _stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 def _call_on(t, name, *args):
     """The entry point on t's device and that device's current stream, which
     is passed last."""
-    index = t.device.index
+    index = t.get_device()
     if index == torch.cuda.current_device():
         F.call(name, *args, _stream_handle(index))
     else:
@@ -320,9 +322,11 @@ def _heads_ld(name, t, B, T, device):
         raise ValueError(f"{name}: bf16 [{B}, {T}, heads, head_dim] on {device}, not {t.dtype} {tuple(shape)} on "
                          f"{t.device}")
     H, hd = shape[2], shape[3]
+    sb, st, sh, se = t.stride()
+    if se == 1 and sh == hd and st >= H * hd > 0 and sb == T * st:  # as they mostly come
+        return st
     if B * T == 0:
         return H * hd
-    sb, st, sh, se = t.stride()
     ld = st if T > 1 else sb if B > 1 else H * hd
     if (hd > 1 and se != 1) or (H > 1 and sh != hd) or (B > 1 and sb != T * ld):
         raise ValueError(f"{name}: strides {t.stride()} (a token's heads contiguous, tokens evenly spaced)")
@@ -330,16 +334,18 @@ def _heads_ld(name, t, B, T, device):
 
 
 def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
-    _need(q.dim() == 4 and q.is_cuda, "q: [B, T, heads, head_dim] on a GPU")
-    B, T, Hq, hd = q.shape
+    shape = q.shape
+    _need(len(shape) == 4 and q.is_cuda, "q: [B, T, heads, head_dim] on a GPU")
+    B, T, Hq, hd = shape
     dev = q.device
     lds = (_heads_ld("q", q, B, T, dev), _heads_ld("k", k, B, T, dev), _heads_ld("v", v, B, T, dev),
            _heads_ld("out", out, B, T, dev))
-    _need(k.shape == v.shape and k.shape[3] == hd and out.shape == q.shape, "k, v and out do not fit q")
-    if seq_lens is not None and not (seq_lens.dtype == torch.int32 and tuple(seq_lens.shape) == (B,)
+    kshape = k.shape
+    _need(kshape == v.shape and kshape[3] == hd and out.shape == shape, "k, v and out do not fit q")
+    if seq_lens is not None and not (seq_lens.dtype == torch.int32 and seq_lens.shape == (B,)
                                      and seq_lens.device == dev and seq_lens.is_contiguous()):
         raise ValueError(f"seq_lens: contiguous int32 [{B}] on {dev}")
-    return F.AttnDesc(B, T, Hq, k.shape[2], hd, hd ** -0.5 if scale is None else scale, 1 if causal else 0, *lds,
+    return F.AttnDesc(B, T, Hq, kshape[2], hd, hd ** -0.5 if scale is None else scale, 1 if causal else 0, *lds,
                       _a(seq_lens))
 
 
@@ -358,20 +364,16 @@ def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
 def _attn_grad_buffers(q, k, v, d):
     """Gradients with the strides of q, k, v: parts of one buffer where q, k, v
     are parts of one (that do not overlap)."""
-    ld, rows = d.q_ld, d.B * d.T
+    T, ld, hd, rows = d.T, d.q_ld, d.head_dim, d.B * d.T
+    nq, nk = 2 * hd * d.n_q_heads, 2 * hd * d.n_kv_heads  # bytes of a token's heads
     if ld == d.k_ld == d.v_ld:
-        first = min(q.data_ptr(), k.data_ptr(), v.data_ptr())
-        offs = [(t.data_ptr() - first) // 2 for t in (q, k, v)]
-        end = 0
-        for o, t in sorted(zip(offs, (q, k, v)), key=lambda x: x[0]):
-            if o < end:
-                break
-            end = o + t.shape[2] * t.shape[3]
-        else:
-            if end <= ld:
-                buf = torch.empty(rows * ld, dtype=q.dtype, device=q.device)
-                return [buf.as_strided(t.shape, (d.T * ld, ld, t.shape[3], 1), o) for o, t in zip(offs, (q, k, v))]
-    return [torch.empty(rows * n, dtype=q.dtype, device=q.device).as_strided(t.shape, (d.T * n, n, t.shape[3], 1))
+        pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        (p0, n0), (p1, n1), (p2, n2) = sorted(((pq, nq), (pk, nk), (pv, nk)))
+        if p0 + n0 <= p1 and p1 + n1 <= p2 and p2 + n2 <= p0 + 2 * ld:
+            buf = torch.empty(rows * ld, dtype=q.dtype, device=q.device)
+            strides = (T * ld, ld, hd, 1)
+            return [buf.as_strided(t.shape, strides, (p - p0) // 2) for p, t in ((pq, q), (pk, k), (pv, v))]
+    return [torch.empty(rows * n, dtype=q.dtype, device=q.device).as_strided(t.shape, (T * n, n, hd, 1))
             for t, n in ((q, ld), (k, d.k_ld), (v, d.v_ld))]
 
 
@@ -393,8 +395,9 @@ def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=Non
     nb = F.load().glt_attention_bwd_workspace_size(ctypes.byref(d))
     workspace = _workspace(workspace, nb, dev)
     dq, dk, dv = grads
-    _call_on(q, "glt_attention_bwd", ctypes.byref(d), _a(q), _a(k), _a(v), _a(out), _a(lse), _a(dout), _a(dq), _a(dk),
-             _a(dv), _a(workspace), workspace.numel())
+    _call_on(q, "glt_attention_bwd", ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+             lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(),
+             workspace.numel())
     return dq, dk, dv
 
 
@@ -573,14 +576,19 @@ def token_logprobs(logits, ids=None, top_k=0, temperature=1.0, workspace=None):
     rows, V, ld, dt = _logit_rows(logits, ids)
     dev = logits.device
     n = ids.shape[1] if ids is not None else 0
-    new = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=dev)
-    r = dict(logprobs=new((rows, n)), entropy=new(rows), lse=new(rows))
+    f32, empty = torch.float32, torch.empty
+    logprobs = empty(rows, n, dtype=f32, device=dev)
+    entropy, lse = empty(rows, dtype=f32, device=dev), empty(rows, dtype=f32, device=dev)
+    r = dict(logprobs=logprobs, entropy=entropy, lse=lse)
+    top_ids = top_logprobs = None
     if top_k > 0:
-        r["top_ids"], r["top_logprobs"] = new((rows, top_k), torch.int32), new((rows, top_k))
+        r["top_ids"] = top_ids = empty(rows, top_k, dtype=torch.int32, device=dev)
+        r["top_logprobs"] = top_logprobs = empty(rows, top_k, dtype=f32, device=dev)
     nb = F.load().glt_token_logprobs_workspace_size(rows, V, dt, top_k)
     ws = _workspace(workspace, nb, dev)
-    _call_on(logits, "glt_token_logprobs", _a(logits), dt, ld, rows, V, temperature, _a(ids), n, top_k, _a(r["logprobs"]),
-             _a(r["entropy"]), _a(r["lse"]), _a(r.get("top_ids")), _a(r.get("top_logprobs")), _a(ws), ws.numel())
+    _call_on(logits, "glt_token_logprobs", _a(logits), dt, ld, rows, V, temperature, _a(ids), n, top_k,
+             logprobs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), _a(top_ids), _a(top_logprobs), ws.data_ptr(),
+             ws.numel())
     return r
 
 
