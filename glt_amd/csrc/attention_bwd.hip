@@ -110,12 +110,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const __amdgpu_buffer_rsrc_t rv = uni_rsrc_a(a.v + (int64_t)b * a.T * a.v_ld + (int64_t)g * kHd, rows_extent(len, a.v_ld));
   const uint32_t kb_ld = (uint32_t)(a.k_ld * 2), vb_ld = (uint32_t)(a.v_ld * 2);  // bytes
   const uint32_t kof = tile_lane_off(wave, lane, kb_ld), vof = tile_lane_off(wave, lane, vb_ld);
-  auto load = [&](int t, int buf) {
-    char* dst = smem + buf * 2 * kTileB;
+  lds_char* const lds = (lds_char*)smem;
+  auto load = [&](int t, lds_char* dst) {
     load_tile<kWaves>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
     load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
   };
-  if (ntiles > 0) load(0, 0);
+  if (ntiles > 0) load(0, lds);
 
   bf16x8 qf[8], dof[8];
   load_rows(qf, a.q + tok * a.q_ld + (int64_t)h * kHd, live, lh);
@@ -123,11 +123,11 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const float lse2 = live ? a.lse[stat] * kLog2e : 0.f;
   float D = row_delta(a.out + tok * a.o_ld + (int64_t)h * kHd, live, dof, lane);
 
-  const uint32_t ro = lds_addr(smem) + row_frag_off(lane), co = lds_addr(smem) + col_frag_off(lane);
+  const uint32_t ro = row_frag_off(lane), co = col_frag_off(lane);
   const float scale_log2 = a.scale * kLog2e;
 
   // Score products of key block kb (32 keys) of tile t: p in s, dp.
-  auto probs = [&](int t, int kb, uint32_t row, f32x16& s, f32x16& dp) {
+  auto probs = [&](int t, int kb, const lds_char* row, f32x16& s, f32x16& dp) {
     const int key0 = t * kTile + 32 * kb;
     score_product<kDqAhead>(row, qf, s, [](int) {});
     if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {
@@ -144,20 +144,28 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   };
   // Walks the tiles; step u of the workgroup uses buffer u & 1. block(t, kb,
   // row, col) gets each 32-key block that this wavefront's rows read.
+  const int mine = a.causal ? min(ntiles, (wq0 + 31) / kTile + 1) : ntiles;
   auto walk = [&](int u0, bool last, auto block) {
-    for (int t = 0; t < ntiles; ++t) {
-      __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
-      phase_barrier();  // this step's tiles are whole, and every wavefront is done with the step before
-      const int u = u0 + t;
-      if (t + 1 < ntiles) load(t + 1, (u + 1) & 1);
-      else if (!last) load(0, (u + 1) & 1);
-      const uint32_t buf = (u & 1) * 2 * kTileB;  // K tile, V tile
+    auto next = [&](int t, lds_char* wr) {
+      if (t + 1 < ntiles) load(t + 1, wr);
+      else if (!last) load(0, wr);
+    };
+    auto step = [&](int t, const lds_char* __restrict__ rd, lds_char* __restrict__ wr) {  // K and V tile in rd
+      next(t, wr);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         const int key0 = t * kTile + 32 * kb;
         if (key0 >= kv_end || (a.causal && key0 > wq0 + 31)) continue;
-        block(t, kb, opaque(ro + buf + kb * 8 * kGroupB), opaque(co + buf + kb * 8 * kGroupB));
+        block(t, kb, rd + opaque(ro + kb * 8 * kGroupB), rd + opaque(co + kb * 8 * kGroupB));
       }
+    };
+    for (int t = 0; t < ntiles; ++t) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
+      phase_barrier();  // this step's tiles are whole, and every wavefront is done with the step before
+      const int u = u0 + t;
+      lds_char *x = lds + (u & 1) * 2 * kTileB, *y = lds + (~u & 1) * 2 * kTileB;
+      if (t < mine) step(t, x, y);
+      else next(t, y);
     }
   };
 
@@ -167,7 +175,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const bool exact = ntiles <= kExactTiles;
   if (exact) {
     float d = 0.f;
-    walk(0, false, [&](int t, int kb, uint32_t row, uint32_t) {
+    walk(0, false, [&](int t, int kb, const lds_char* row, const lds_char*) {
       f32x16 s{}, dp{};
       probs(t, kb, row, s, dp);
 #pragma unroll
@@ -183,7 +191,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   f32x16 dq[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
-  walk(exact ? ntiles : 0, true, [&](int t, int kb, uint32_t row, uint32_t col) {
+  walk(exact ? ntiles : 0, true, [&](int t, int kb, const lds_char* row, const lds_char* col) {
     f32x16 s{}, dp{};
     probs(t, kb, row, s, dp);
 #pragma unroll
@@ -240,8 +248,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
   const __amdgpu_buffer_rsrc_t rq = uni_rsrc_a(a.q + (int64_t)b * a.T * a.q_ld + (int64_t)h * kHd, rows_extent(len, a.q_ld));
   const __amdgpu_buffer_rsrc_t rdo = uni_rsrc_a(a.dout + (int64_t)b * a.T * a.o_ld + (int64_t)h * kHd, rows_extent(len, a.o_ld));
   const __amdgpu_buffer_rsrc_t rs = uni_rsrc_a(a.stats + ((wave & 1) * (int64_t)a.B * a.Hq + (int64_t)b * a.Hq + h) * a.T, (uint32_t)len * 4);
-  auto load = [&](int qt, int buf) {
-    char* dst = smem + buf * kDkdvBuf;
+  lds_char* const lds = (lds_char*)smem;
+  auto load = [&](int qt, lds_char* dst) {
     const int l = opaque(threadIdx.x) & 63;
     load_tile<kWaves>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld);
     load_tile<kWaves>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld);
@@ -249,26 +257,24 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + 2 * kTileB + wave * kTile * 4), 4,
                                                (uint32_t)(qt * kTile + l) * 4, 0, 0, 0);
   };
-  if (qt0 < qt1) load(qt0, 0);
+  if (qt0 < qt1) load(qt0, lds);
 
-  const uint32_t ro = lds_addr(smem) + row_frag_off(lane), co = lds_addr(smem) + col_frag_off(lane);
+  const uint32_t ro = row_frag_off(lane), co = col_frag_off(lane);
   f32x16 dk[4], dv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) dk[i] = dv[i] = f32x16{};
   const float scale_log2 = a.scale * kLog2e;
 
-  for (int qt = qt0; qt < qt1; ++qt) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
-    phase_barrier();  // tile qt is whole, and every wavefront is done with tile qt - 1
-    const int q0t = qt * kTile, cur = (qt - qt0) & 1;
-    if (qt + 1 < qt1) load(qt + 1, cur ^ 1);
-    const uint32_t buf = cur * kDkdvBuf;  // Q tile, dout tile, lse, D
+  // tile qt, in rd (Q, dout, lse, D); tile qt + 1 into wr
+  auto step = [&](int qt, const lds_char* __restrict__ rd, lds_char* __restrict__ wr) {
+    if (qt + 1 < qt1) load(qt + 1, wr);
+    const int q0t = qt * kTile;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       const int q0 = q0t + 32 * qb;
       if (q0 >= len || (a.causal && q0 + 31 < wk0)) continue;
       f32x16 s{}, dp{};
-      const uint32_t row = opaque(ro + buf + qb * 8 * kGroupB);
+      const lds_char* row = rd + opaque(ro + qb * 8 * kGroupB);
       score_product<kDkdvAhead>(row, kf, s, [](int) {});
       if (a.causal && q0 < wk0 + 31) {  // row q0 + 8 (e >> 2) + 4 lh + (e & 3) reads keys up to itself
         const int l = opaque(threadIdx.x) & 63;
@@ -278,9 +284,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       }
       // the exponentials beside the other product; elements 4 i .. + 3 are
       // query rows 8 i + 4 lh .. + 3
-      const uint32_t st = opaque(lds_addr(smem) + buf + 2 * kTileB + 128 * qb + 16 * (lane >> 5));
+      const lds_char* st = rd + opaque(2 * kTileB + 128 * qb + 16 * (lane >> 5));
       score_product<kDkdvAhead>(row + kTileB, vf, dp, [&](int i) {
-        const f32x2 l = *reinterpret_cast<const lds_f32x2*>((uintptr_t)(st + 32 * (i >> 1) + 8 * (i & 1)));
+        const f32x2 l = *(const lds_f32x2*)(st + 32 * (i >> 1) + 8 * (i & 1));
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           s[2 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + e], scale_log2, -l[e]));
@@ -288,7 +294,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       u32x4 pw[2], dw[2];  // packed p and ds
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 D = *reinterpret_cast<const lds_f32x4*>((uintptr_t)(st + 32 * i + kTile * 4));
+        const f32x4 D = *(const lds_f32x4*)(st + 32 * i + kTile * 4);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           const int x = 4 * i + e, w = 2 * (i & 1) + e / 2;
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      const uint32_t col = opaque(co + buf + qb * 8 * kGroupB);
+      const lds_char* col = rd + opaque(co + qb * 8 * kGroupB);
       __builtin_amdgcn_s_setprio(1);
       bf16x8 oa[kGradAhead], qa[kGradAhead];  // step i: 16 query rows i >> 2, d block i & 3
 #pragma unroll
@@ -317,6 +323,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       }
       __builtin_amdgcn_s_setprio(0);
     }
+  };
+  for (int qt = qt0; qt < qt1; ++qt) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
+    phase_barrier();  // tile qt is whole, and every wavefront is done with tile qt - 1
+    const int cur = (qt - qt0) & 1;
+    step(qt, lds + cur * kDkdvBuf, lds + (cur ^ 1) * kDkdvBuf);
   }
   // the output rows' addresses are worked out again here: kept across the
   // loop they cost registers that it does not have

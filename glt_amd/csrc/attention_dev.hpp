@@ -98,8 +98,8 @@ __device__ __forceinline__ uint32_t row_frag_off(int lane) {
   const int r = lane & 31;
   return (uint32_t)((r >> 2) * kGroupB + (r & 3) * 64 + (lane >> 5) * 16);
 }
-__device__ __forceinline__ bf16x8 row_frag(uint32_t addr, int s) {
-  return *reinterpret_cast<const lds_bf16x8*>((uintptr_t)(addr + (uint32_t)((s >> 1) * 256 + (s & 1) * 32)));
+__device__ __forceinline__ bf16x8 row_frag(const lds_char* p, int s) {
+  return *(const lds_bf16x8*)(p + (s >> 1) * 256 + (s & 1) * 32);
 }
 
 // Fragment with rows as the contracted index, 32 columns from 32 db and 16 rows
@@ -113,12 +113,12 @@ __device__ __forceinline__ uint32_t col_frag_off(int lane) {
   const int s = lane & 15;
   return (uint32_t)((lane >> 5) * kGroupB + (s >> 2) * 64 + ((lane >> 4) & 1) * 32 + (s & 3) * 8);
 }
-__device__ __forceinline__ bf16x8 col_frag(uint32_t addr, int db, int s2) {
-  struct Pair { s16x4 a, b; } p;
-  const uint32_t x = addr + (uint32_t)(256 * db + 4 * s2 * kGroupB);
-  p.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)x);
-  p.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(x + 2 * kGroupB));
-  return __builtin_bit_cast(bf16x8, p);
+__device__ __forceinline__ bf16x8 col_frag(const lds_char* p, int db, int s2) {
+  struct Pair { s16x4 a, b; } f;
+  lds_char* x = const_cast<lds_char*>(p) + 256 * db + 4 * s2 * kGroupB;
+  f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)x);
+  f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + 2 * kGroupB));
+  return __builtin_bit_cast(bf16x8, f);
 }
 
 // ------------------------------------------------------ training kernels
@@ -136,7 +136,7 @@ __device__ __forceinline__ int seq_len(const int32_t* seq_lens, int b, int T) {
 // this lane's byte offset of its first load (tile_lane_off). Rows past the
 // descriptor are zeros.
 template <int WAVES>
-__device__ __forceinline__ void load_tile(__amdgpu_buffer_rsrc_t r, char* dst, int wave, uint32_t off, uint32_t row_bytes,
+__device__ __forceinline__ void load_tile(__amdgpu_buffer_rsrc_t r, lds_char* dst, int wave, uint32_t off, uint32_t row_bytes,
                                           uint32_t row0_bytes) {
 #pragma unroll
   for (int i = 0; i < 16 / WAVES; ++i)
@@ -174,7 +174,7 @@ __device__ __forceinline__ bf16x8 pack_frag(const f32x16& x, int s2) {
 // keeps the reads from all being hoisted, which needs more registers than
 // there are.)
 template <int AHEAD, typename F>
-__device__ __forceinline__ void score_product(uint32_t X, const bf16x8* f, f32x16& x, F between) {
+__device__ __forceinline__ void score_product(const lds_char* X, const bf16x8* f, f32x16& x, F between) {
   bf16x8 xa[AHEAD];
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) xa[i] = row_frag(X, i);

@@ -71,16 +71,16 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
   const __amdgpu_buffer_rsrc_t rv = uni_rsrc_a(a.v + (int64_t)b * a.T * a.v_ld + (int64_t)g * kHd, rows_extent(len, a.v_ld));
   const uint32_t kb_ld = (uint32_t)(a.k_ld * 2), vb_ld = (uint32_t)(a.v_ld * 2);  // bytes
   const uint32_t kof = tile_lane_off(wave, lane, kb_ld), vof = tile_lane_off(wave, lane, vb_ld);
-  auto load = [&](int t) {
-    char* dst = smem + (t & 1) * 2 * kTileB;
+  lds_char* const lds = (lds_char*)smem;
+  auto load = [&](int t, lds_char* dst) {
     load_tile<kWaves>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
     load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
   };
-  if (ntiles > 0) load(0);
+  if (ntiles > 0) load(0, lds);
 
   bf16x8 qf[8];
   load_rows(qf, a.q + tok * a.q_ld + (int64_t)h * kHd, live, lh);
-  const uint32_t ro = lds_addr(smem) + row_frag_off(lane), co = lds_addr(smem) + col_frag_off(lane);
+  const uint32_t ro = row_frag_off(lane), co = col_frag_off(lane) + kTileB;
 
   f32x16 o[4];
 #pragma unroll
@@ -89,14 +89,11 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
   // output's product uses (its divisor), sum of the unrounded ones (lse's)
   float m_run = -3.0e38f, l_run = 0.f, l_exact = 0.f;
 
-  for (int t = 0; t < ntiles; ++t) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
-    phase_barrier();  // tile t is whole, and every wavefront is done with tile t - 1
-    if (t + 1 < ntiles) load(t + 1);
+  // tile t, in rd (K, V); tile t + 1 into wr
+  auto step = [&](int t, const lds_char* __restrict__ rd, lds_char* __restrict__ wr) {
+    if (t + 1 < ntiles) load(t + 1, wr);
     const int key0 = t * kTile;
-    if (a.causal && key0 > wq0 + 31) continue;
-    const uint32_t buf = (t & 1) * 2 * kTileB;  // K tile, V tile
-    const uint32_t row = opaque(ro + buf), col = opaque(co + buf + kTileB);
+    const lds_char *row = rd + opaque(ro), *col = rd + opaque(co);
     f32x16 s[2] = {f32x16{}, f32x16{}};  // key blocks 0, 1
     {
       constexpr int kAhead = 4;
@@ -169,6 +166,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
       }
       __builtin_amdgcn_s_setprio(0);
     }
+  };
+  const int mine = a.causal ? min(ntiles, (wq0 + 31) / kTile + 1) : ntiles;  // tiles that this wavefront's rows read
+  for (int t = 0; t < ntiles; ++t) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
+    phase_barrier();  // tile t is whole, and every wavefront is done with tile t - 1
+    lds_char *x = lds + (t & 1) * 2 * kTileB, *y = lds + (~t & 1) * 2 * kTileB;
+    if (t < mine) step(t, x, y);
+    else if (t + 1 < ntiles) load(t + 1, y);
   }
 
   const float l_tot = pair_sum(l_run), le = pair_sum(l_exact);
