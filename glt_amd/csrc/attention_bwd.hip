@@ -19,18 +19,17 @@
 // are formed so that a lane holds one OWNED row: the packed p or ds is then the
 // next product's operand as it stands in the accumulator's layout.
 //
-// Bound by the matrix instructions and the arithmetic between them: the rows in
-// registers leave room for two wavefronts per SIMD, and a wavefront's own
-// products depend on its exponentials, so one wavefront's arithmetic has to run
-// beside the other's products. The two come from two workgroups of four, which
-// nothing keeps in step. With one workgroup of eight instead (half the loads
-// into LDS) they wait at the same barrier, and short rows leave more of them
-// idle; dq + dkdv in us, 32 query and 8 kv heads, eight against four:
-//   6 x 777 causal 217, 190; 1 x 1024 causal 98, 76;
-//   2 x 4096 causal 911, 891; 2 x 4096 full 1672, 1698.
-// At 2 x 4096 causal the two kernels and the sum of parts take 393, 498 and 49
-// us: 0.96 * 10^15 operations a second of the seven products, the matrix units
-// busy half of the time (a large library product: 1.24 * 10^15).
+// Bound by the matrix instructions. The rows in registers leave room for two
+// wavefronts per SIMD, and a wavefront's own products depend on its
+// exponentials, so one wavefront's arithmetic has to run beside the other's
+// products. The two come from two workgroups of four, which nothing keeps in
+// step. With one workgroup of eight instead (half the loads into LDS) they wait
+// at the same barrier, and short rows leave more of them idle; dq + dkdv in us,
+// 32 query and 8 kv heads, eight against four:
+//   1 x 512 causal 73, 56;  6 x 777 causal 213, 184;  1 x 1024 causal 97, 75;
+//   4 x 2048 causal 521, 489;  2 x 4096 causal 872, 858;  full 1571, 1600.
+// At 2 x 4096 causal dq and dkdv run at 1.11 and 1.13 * 10^15 operations a second
+// of the unmasked part (a large library product: 1.24 * 10^15).
 #include <algorithm>
 #include <atomic>
 
@@ -219,7 +218,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
 // that walked the group's heads one after the other would leave too few
 // workgroups for the chip (2 x 4096 tokens, 8 kv heads: 512 of very different
 // length), and a cut that depends on the batch would make the sums' order depend
-// on it. The parts cost 49 of 940 us at 2 x 4096 (268 MB written and read).
+// on it. The parts cost 49 of 907 us at 2 x 4096 (268 MB written and read).
 constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
 
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs a) {

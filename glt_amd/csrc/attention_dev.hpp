@@ -89,7 +89,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 typedef __attribute__((address_space(3))) char lds_char;
-__device__ __forceinline__ uint32_t lds_addr(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
 
 // Fragment with rows as outer index: row lane & 31, elements 16 s + 8 (lane >>
 // 5) .. +7, from the tile's address + row_frag_off(lane). 32 rows further are

@@ -12,17 +12,20 @@
 // stand. Two workgroups fit a CU, one wavefront of each per SIMD; as nothing
 // keeps the two in step, one's arithmetic runs beside the other's products.
 //
-// Bound by the matrix instructions and the softmax between them, which a SIMD
-// has two wavefronts to overlap. us with 32 query and 8 kv heads, against eight
-// wavefronts in halves held half a tile apart (attention.hip's schedule, which
-// serves long single sequences; here with strides, lengths and lse):
-//   1 x 512 causal 18.6, 24.2;  6 x 777 causal 60, 78;  1 x 1024 causal 27, 33;
-//   4 x 2048 causal 166, 177;  2 x 4096 causal 296, 289;  2 x 4096 full 564, 519.
-// A training batch pays for what its short rows leave idle, so this one serves
-// all. 2 x 4096 causal is 0.93 * 10^15 operations a second of the unmasked part
-// (a large library product: 1.24 * 10^15). Running the next tile's scores under
-// this tile's softmax in one wavefront, and tiles of 32 keys with three
-// wavefronts per SIMD, both need more registers than there are.
+// The reads of a tile and the loads of the next go through distinct restrict
+// pointers (step's rd and wr): without that the compiler lets every transposing
+// read wait for all loads to LDS, the next tile's too (2 x 4096 causal 296 us).
+//
+// Bound by the matrix instructions: 2 x 4096 causal with 32 query and 8 kv heads
+// runs at 1.06 * 10^15 operations a second of the unmasked part, full at 1.13 *
+// 10^15 (a large library product: 1.24 * 10^15). us, against one workgroup of
+// eight wavefronts (half the loads into LDS, but they wait at the same barrier):
+//   1 x 512 causal 15, 19;  6 x 777 causal 55, 65;  1 x 1024 causal 24, 31;
+//   4 x 2048 causal 148, 160;  2 x 4096 causal 260, 265;  2 x 4096 full 486, 484.
+// Tiles of 32 keys let three wavefronts share a SIMD and measure the same within
+// 5 % (6 x 777 52, 2 x 4096 full 497); longer read-ahead of the fragments
+// changes nothing, without the raised priority of the second product 2 x 4096
+// full takes 511.
 #include <atomic>
 
 #include "attention_dev.hpp"
