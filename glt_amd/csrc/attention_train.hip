@@ -212,8 +212,11 @@ glt_status check_attn_desc(const glt_attn_desc* d, const char* who) {
     GLT_CHECK(lds[i] < (int64_t)kOob && ((int64_t)d->T + 256) * lds[i] * 2 < (int64_t)kOob, GLT_ERR_SHAPE,
               "%s: T=%d rows of %c_ld %lld pass 2 GiB", who, d->T, "qkvo"[i], (long long)lds[i]);
   }
-  GLT_CHECK(((int64_t)d->T + 127) / 128 * d->B < INT32_MAX / d->n_q_heads / 8, GLT_ERR_SHAPE, "%s: B=%d T=%d n_q_heads=%d",
-            who, d->B, d->T, d->n_q_heads);
+  // a launch holds less than 2^32 threads, 256 for 128 rows of a head or (the
+  // sum of parts) 16 for a token's kv head
+  GLT_CHECK(((int64_t)d->T + kRows - 1) / kRows * d->B < (1 << 24) / d->n_q_heads &&
+                (int64_t)d->T * d->B < (1 << 28) / d->n_kv_heads,
+            GLT_ERR_SHAPE, "%s: B=%d T=%d n_q_heads=%d n_kv_heads=%d", who, d->B, d->T, d->n_q_heads, d->n_kv_heads);
   return GLT_OK;
 }
 

@@ -23,6 +23,7 @@
 // In log2 units c = log2(e) / temperature: a wavefront's shift is the rounded
 // product m c of its maximum, the terms exp2(fma(x, c, -shift)); the shift is
 // exactly what the joined sum is told, so its rounding does not enter.
+#include <atomic>
 #include <cmath>
 
 #include "common.hpp"
@@ -37,6 +38,7 @@ constexpr int kMaxTop = 64;                      // alternatives at most: one pe
 constexpr int kMaxIds = 64;
 constexpr int kMaxV = 1 << 20;
 constexpr int kCap = 1024;                       // candidates of a piece held in LDS
+constexpr int kLdsFree = 60 * 1024;              // dynamic LDS that needs no leave, beside RowList
 constexpr int kHitCap = 128;                     // chunks of a piece that hold candidates
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453094;
@@ -389,11 +391,11 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_piece_kernel(const FwdAr
 #pragma unroll
   for (int q = 0; q < kChunks; ++q) {
     float c = E::get(ch[q], 0);
-    mn = fminf(mn, c);
+    mn = __builtin_elementwise_minimum(mn, c);  // of NaN and anything: NaN
 #pragma unroll
     for (int j = 1; j < E::n; ++j) {
       c = fmaxf(c, E::get(ch[q], j));
-      mn = fminf(mn, E::get(ch[q], j));
+      mn = __builtin_elementwise_minimum(mn, E::get(ch[q], j));
     }
     m = fmaxf(m, c);
     if constexpr (TOP) cm.set(q, c);
@@ -404,11 +406,12 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_piece_kernel(const FwdAr
   Part p;
   p.s = p.t = 0.f;
   // terms so small that 0 * -inf or an overflow of x c could come up are
-  // rare enough for a loop of their own: masked logits, and the row's end
+  // rare enough for a loop of their own: masked logits, NaN, and the row's end
   if (__any(!(mn * a.c > -1e37f)) || !(fabsf(m * a.c) < 1e37f)) {
-    // m = -inf: nothing is allowed, and nothing is added
     p.shift = (double)m * (double)a.c;
-    if (m != -INFINITY) {
+    if (m == -INFINITY) {  // nothing is allowed, and nothing is added but a NaN, which the maximum passed over
+      p.s = mn == mn ? 0.f : mn;
+    } else {
 #pragma unroll
       for (int q = 0; q < kChunks; ++q)
 #pragma unroll
@@ -680,7 +683,8 @@ glt_status check_rows(const char* who, int32_t dtype, int64_t ld, int32_t rows, 
   GLT_CHECK(n_ids >= 0 && n_ids <= kMaxIds, GLT_ERR_UNSUPPORTED, "%s: %d given tokens a row (at most %d)", who, n_ids, kMaxIds);
   // 1 / temperature and log2(e) / temperature are finite and not zero
   GLT_CHECK(temperature > 1e-30f && temperature < 1e30f, GLT_ERR_INVALID_ARG, "%s: temperature %g", who, (double)temperature);
-  GLT_CHECK((int64_t)rows * pieces(V, dtype) < INT32_MAX, GLT_ERR_SHAPE, "%s: rows=%d V=%d", who, rows, V);
+  // a launch holds less than 2^32 threads
+  GLT_CHECK((int64_t)rows * pieces(V, dtype) < (1ll << 32) / kThreads, GLT_ERR_SHAPE, "%s: rows=%d V=%d", who, rows, V);
   return GLT_OK;
 }
 
@@ -691,6 +695,18 @@ glt_status launch_fwd(const FwdArgs& a, hipStream_t st) {
   else GLT_LAUNCH("logprobs", (logprobs_piece_kernel<T, false>), grid, dim3(kThreads), 0, st, a);
   GLT_LAUNCH_CHECK("logprobs");
   const int nk = a.np * a.k;
+  if (nk * 8 > kLdsFree) {
+    // the dynamic-LDS limit is a per-device attribute of the kernel
+    static std::atomic<bool> attr_set[64];
+    int dev = 0;
+    GLT_TRY_HIP(hipGetDevice(&dev));
+    GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_token_logprobs: device index %d out of range", dev);
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+      GLT_TRY_HIP(hipFuncSetAttribute((const void*)logprobs_row_kernel<T, kThreads>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      kMaxV / kPiece<T> * kMaxTop * 8));
+      attr_set[dev].store(true, std::memory_order_release);
+    }
+  }
   if (nk <= 64)
     GLT_LAUNCH("logprobs_row", (logprobs_row_kernel<T, 64>), dim3((unsigned)a.rows), dim3(64), (size_t)nk * 8, st, a);
   else

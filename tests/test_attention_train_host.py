@@ -43,6 +43,8 @@ def bwd(d, ws=P, nbytes=1 << 40, **kw):
     (dict(k_ld=1 << 40), 2),
     (dict(T=1 << 22), 2),               # 4M rows of 512 columns pass 2 GiB
     (dict(B=1 << 30, n_q_heads=4), 2),  # more workgroups than a launch has
+    (dict(B=1 << 22, T=1), 2),
+    (dict(B=1 << 15, T=1 << 12), 2),    # more kv rows than the sum of parts can launch for
 ])
 def test_descriptor_refusals(kw, code):
     assert fwd(desc(**kw)) == code

@@ -171,6 +171,38 @@ def test_nan_and_inf_rows(dev, dtype):
     assert int(got["top_ids"][2, 0]) == 19999
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_nan_among_masked_logits(dev, dtype):
+    """A NaN counts where all logits near it are -inf or NaN too, wherever it
+    stands in its row; a row of NaN alone is no row without tokens."""
+    from glt_amd import ops
+    V = 50001
+    x = torch.full((9, V), -math.inf, dtype=dtype, device="cuda")
+    for r, at in enumerate((0, 1, 7777, 16384, 40000, V - 1)):
+        x[r, at] = math.nan
+    x[6] = math.nan
+    x[7] = make(1, V, dtype, 3)[0]
+    x[7, 30000:40000] = -math.inf
+    x[7, 35000] = math.nan
+    x[8] = make(1, V, dtype, 4)[0]
+    x[8, 16384:32768] = math.nan
+    got = ops.token_logprobs(x, ids_for(9, V, 2, 1), top_k=20)
+    for name in ("lse", "entropy", "logprobs"):
+        assert bool(torch.isnan(got[name]).all()), name
+    for r in range(9):
+        ids = got["top_ids"][r].cpu().numpy()
+        assert len(set(ids)) == 20 and ids.min() >= 0 and ids.max() < V
+    grad = ops.token_logprobs_bwd(x, ids_for(9, V, 2, 1), got["lse"], torch.ones(9, 2, device="cuda"))
+    assert bool(torch.isnan(grad.float()).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_the_largest_vocabulary(dev, dtype):
+    """2^20 tokens and 64 alternatives: the most that a row's workgroup holds."""
+    x = make(2, 1 << 20, dtype, 21)
+    check(x, ids_for(2, 1 << 20, 64, 5), 64)
+
+
 def test_padding_and_foreign_ids(dev):
     from glt_amd import ops
     V = 1000

@@ -23,6 +23,7 @@ def bwd(logits=P, dtype=0, ld=100, rows=3, V=100, temp=1.0, ids=P, n=1, gl=P, ls
     (dict(n=-1), 9), (dict(n=65), 9),
     (dict(temp=0.0), 1), (dict(temp=-1.0), 1), (dict(temp=float("nan")), 1), (dict(temp=float("inf")), 1),
     (dict(rows=2 ** 31 - 1, V=20000, ld=20000, ldg=20000), 2),   # more workgroups than a launch has
+    (dict(rows=1 << 24), 2),
     (dict(logits=None), 1), (dict(ids=None), 1),
     (dict(logits=P + 1), 4), (dict(logits=P + 2, dtype=1), 4), (dict(ids=P + 2), 4), (dict(lse=P + 1), 4),
 ])
