@@ -105,7 +105,10 @@ CASES = [
     (1, 33, 6, 2, True, None, True),
     (2, 64, 4, 4, True, None, False),             # a tile
     (2, 65, 8, 1, False, None, True),
-    (1, 255, 2, 1, True, None, False),            # a workgroup's 256 rows
+    (2, 127, 2, 1, False, None, False),           # a workgroup's 128 rows
+    (1, 128, 4, 1, True, None, False),
+    (1, 129, 3, 3, True, None, True),
+    (1, 255, 2, 1, True, None, False),
     (1, 256, 4, 2, True, None, True),
     (1, 257, 3, 1, False, None, False),
     (2, 513, 4, 2, True, None, False),            # either side of the rows that take D from p
@@ -113,6 +116,7 @@ CASES = [
     (5, 130, 4, 2, True, (130, 0, 1, 64, 65), True),
     (4, 300, 2, 2, False, (0, 300, 33, 256), False),
     (3, 600, 8, 2, True, (599, 600, 17), False),
+    (1, 5003, 2, 1, True, None, False),           # a long sequence
 ]
 
 
@@ -323,3 +327,30 @@ def test_python_refusals(dev):
     from glt_amd import _ffi as F
     with pytest.raises(F.GltError):
         ops.attention_train(q, k, v, scale=0.0)
+
+
+def test_offsets_past_32_bits(dev):
+    """Sequences of nearly 2 GiB of strided rows each, 6 GB in all: the same
+    bits as from dense tensors."""
+    B, T, ld = 3, 20000, 49152
+    q, k, v, dout = make(B, T, 1, 1, 9)
+    big = torch.empty((B, T, ld // HD, HD), dtype=BF, device=dev)
+    Q, K, V, O = (big[:, :, i:i + 1] for i in (0, 100, 382, 383))
+    Q.copy_(q)
+    K.copy_(k)
+    V.copy_(v)
+    lens = torch.tensor([17, 300, T], dtype=torch.int32, device=dev)
+    want, got = run(q, k, v, dout, seq_lens=lens), run(Q, K, V, dout, seq_lens=lens)
+    for name, w in want.items():
+        assert torch.equal(got[name], w), name
+    assert got["dq"].stride() == Q.stride()
+    # out and dout at the same stride, through the entry points
+    from glt_amd import _ffi as F
+    import ctypes
+    d = F.AttnDesc(B, T, 1, 1, HD, HD ** -0.5, 1, ld, ld, ld, ld, lens.data_ptr())
+    lse = torch.empty((B, 1, T), device=dev)
+    st = torch.cuda.current_stream().cuda_stream
+    F.call("glt_attention_train_fwd", ctypes.byref(d), Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(),
+           lse.data_ptr(), st)
+    assert torch.equal(O, want["out"]) and torch.equal(lse, want["lse"])
+    assert torch.equal(Q, q) and torch.equal(V, v)

@@ -231,3 +231,20 @@ def test_python_refusals(dev):
             pytest.fail(f"call {i} was taken")
     with pytest.raises(TypeError):
         ops.ckpt8_save(x.half())
+
+
+def test_offsets_past_32_bits(dev):
+    """4.5 * 10^9 values, 9 GB: the last rows as on their own, and what lies
+    before them."""
+    from glt_amd import ops
+    rows, cols = 275000, 16384
+    x = torch.full((rows, cols), 0.75, dtype=BF, device=dev)
+    tail = make(5, cols, BF, 77)
+    x[-5:] = tail
+    y = ops.ckpt8_save(x).load()
+    assert torch.equal(y[-5:], ops.ckpt8_save(tail).load())
+    assert torch.equal(y[:-5], x[:-5])          # 0.75 is 96 steps of 2^-7
+    gate, up, inter = ops.ckpt8_swiglu(ops.ckpt8_save(x), ops.ckpt8_save(x))
+    w = ops.ckpt8_swiglu(ops.ckpt8_save(tail), ops.ckpt8_save(tail))
+    for a, b in zip((gate, up, inter), w):
+        assert torch.equal(a[-5:], b)

@@ -402,3 +402,24 @@ def test_python_refusals(dev):
     for f in (lambda: ops.token_logprobs(x, ids, top_k=51), lambda: ops.token_logprobs(x, ids, temperature=0.0)):
         with pytest.raises(F.GltError):
             f()
+
+
+def test_offsets_past_32_bits(dev):
+    """20000 rows of 128256 logits (5.1 GB): the last rows as on their own, the
+    gradient in place."""
+    from glt_amd import ops
+    rows, V = 20000, 128256
+    x = torch.zeros((rows, V), dtype=BF, device=dev)
+    tail = make(3, V, BF, 31)
+    x[-3:] = tail
+    ids, few = torch.full((rows, 1), 5, dtype=torch.int32, device=dev), ids_for(3, V, 1, 2)
+    ids[-3:] = few
+    got, want = ops.token_logprobs(x, ids, top_k=3), ops.token_logprobs(tail, few, top_k=3)
+    for name, w in want.items():
+        assert torch.equal(got[name][-3:], w), name
+    assert float((got["lse"][:-3] - math.log(V)).abs().max()) <= U * (80 + 4 * math.log(V))
+    g = torch.ones((rows, 1), device=dev)
+    w = ops.token_logprobs_bwd(tail, few, want["lse"], g[-3:])
+    grad = ops.token_logprobs_bwd(x, ids, got["lse"], g, grad=x)
+    assert grad.data_ptr() == x.data_ptr() and torch.equal(x[-3:], w)
+    assert bool((x[:-3, 5] > 0.99).all()) and bool((x[:-3, 6] < 0).all())
