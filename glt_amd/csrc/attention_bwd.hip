@@ -26,10 +26,11 @@
 // step. With one workgroup of eight instead (half the loads into LDS) they wait
 // at the same barrier, and short rows leave more of them idle; dq + dkdv in us,
 // 32 query and 8 kv heads, eight against four:
-//   1 x 512 causal 73, 56;  6 x 777 causal 213, 184;  1 x 1024 causal 97, 75;
-//   4 x 2048 causal 521, 489;  2 x 4096 causal 872, 858;  full 1571, 1600.
-// At 2 x 4096 causal dq and dkdv run at 1.11 and 1.13 * 10^15 operations a second
-// of the unmasked part (a large library product: 1.24 * 10^15).
+//   1 x 512 causal 73, 55;  6 x 777 causal 213, 188;  1 x 1024 causal 99, 74;
+//   4 x 2048 causal 515, 498;  2 x 4096 causal 864, 849;  full 1568, 1579.
+// At 2 x 4096 causal dq and dkdv take 385 and 464 us: 1.07 and 1.18 * 10^15
+// operations a second of the unmasked part (a large library product: 1.24 *
+// 10^15); 25 of dq's go into watching D's error (kOff).
 #include <algorithm>
 #include <atomic>
 
@@ -41,6 +42,11 @@ namespace {
 
 // Key tiles up to which a block of rows takes D from its own probabilities.
 constexpr int kExactTiles = 8;
+// Error of a longer row's D, relative to the 2-norm of its ds, that is put right:
+// 2 roundings of p and out and the one of ds leave 2^-8.5 in flat rows. Without
+// the second walk rows of one heavy key (T 700, scores of deviation 16) bring
+// dq's error to 3.0 * 2^-9, with it to 2.0 * 2^-9.
+constexpr float kOff = 0x1p-5f;
 
 struct BwdArgs {
   const uint16_t* q;
@@ -49,7 +55,7 @@ struct BwdArgs {
   const uint16_t* out;
   const uint16_t* dout;
   const float* lse;    // [B, Hq, T]
-  float* stats;        // [2][B, Hq, T]: lse log2(e) and D, written by the dq kernel
+  float* stats;        // [2][B, Hq, T]: lse log2(e) and -D, written by the dq kernel
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
@@ -60,9 +66,7 @@ struct BwdArgs {
   float scale;
 };
 
-// D of the lane's row: the diagonal of out . dout^T. The matrix product sums it
-// in the order in which it sums dp, so a row whose output is one key's value (a
-// single key) gets ds = 0 exactly.
+// D of the lane's row: the diagonal of out . dout^T.
 __device__ __forceinline__ float row_delta(const uint16_t* out_row, bool live, const bf16x8* dof, int lane) {
   const int lq = lane & 31, lh = lane >> 5;
   bf16x8 of[8];
@@ -169,9 +173,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   };
 
   // D from out carries out's rounding, which counts where few keys share a
-  // row's weight: dp - D nearly cancels there. Such rows take it from the
-  // probabilities, as D + sum p (dp - D), in a walk of their own.
+  // row's weight: dp - D nearly cancels there. Blocks of few keys take it from
+  // the probabilities, as D + sum p (dp - D), in a walk of their own.
   const bool exact = ntiles <= kExactTiles;
+  int u = 0;
   if (exact) {
     float d = 0.f;
     walk(0, false, [&](int t, int kb, const lds_char* row, const lds_char*) {
@@ -181,44 +186,85 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
       for (int e = 0; e < 16; ++e) d = __builtin_fmaf(s[e], dp[e] - D, d);
     });
     D += pair_sum(d);
-  }
-  if (lh == 0 && myq < a.T) {
-    a.stats[stat] = lse2;
-    a.stats[(int64_t)a.B * a.Hq * a.T + stat] = live ? D : 0.f;
+    u = ntiles;
   }
 
   f32x16 dq[4];
+  float D_sum = 0.f;
+  for (;;) {
+    float sums = 0.f, squares = 0.f;  // of the row's ds
+    f32x16 nD;  // where dp starts (16 subtractions less in each block)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
-  walk(exact ? ntiles : 0, true, [&](int t, int kb, const lds_char* row, const lds_char* col) {
-    f32x16 s{}, dp{};
-    probs(t, kb, row, s, dp);
+    for (int e = 0; e < 16; ++e) nD[e] = -D;
+    asm volatile("" : "+v"(nD));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] *= dp[e] - D;
+    for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
+    walk(u, true, [&](int t, int kb, const lds_char* row, const lds_char* col) {
+      f32x16 s{}, dp = nD;
+      probs(t, kb, row, s, dp);
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const bf16x8 f = pack_frag(s, s2);
+      for (int e = 0; e < 16; ++e) s[e] *= dp[e];
 #pragma unroll
-      for (int db = 0; db < 4; ++db) dq[db] = mfma(col_frag(col, db, s2), f, dq[db]);
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const bf16x8 f = pack_frag(s, s2);
+#pragma unroll
+        for (int db = 0; db < 4; ++db) dq[db] = mfma(col_frag(col, db, s2), f, dq[db]);
+        const u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t pair = w[i];  // (a bit_cast of the vector's element itself reads element 0)
+          const bf16x2_t x = __builtin_bit_cast(bf16x2_t, pair);
+          sums = __builtin_amdgcn_fdot2_f32_bf16(x, kOnes2, sums, false);
+          squares = __builtin_amdgcn_fdot2_f32_bf16(x, x, squares, false);
+        }
+      }
+    });
+    if (exact) {
+      D_sum = D;
+      break;
     }
-  });
+    // With more keys the row's ds tell: their sum is what D is off by (dkdv gets
+    // it without). Where that is more than kOff of their 2-norm the workgroup
+    // walks once more with this row's D put right: rows of which one key has
+    // some 0.95 of the weight (of flat ones it is 2^-8.5).
+    if (u > 0) break;
+    const float sum = pair_sum(sums);
+    const bool off = live && sum * sum > kOff * kOff * pair_sum(squares);
+    D_sum = D + sum;
+    uint32_t* any = reinterpret_cast<uint32_t*>(smem + 4 * kTileB);
+    const uint64_t offs = __ballot(off);
+    if (lane == 0) any[wave] = offs != 0;
+    phase_barrier();
+    static_assert(kWaves == 4, "one flag a wavefront");
+    if (!(any[0] | any[1] | any[2] | any[3])) break;
+    D = off ? D_sum : D;
+    u = ntiles;
+    load(0, lds + (u & 1) * 2 * kTileB);
+  }
+  if (lh == 0 && myq < a.T) {
+    a.stats[stat] = lse2;
+    a.stats[(int64_t)a.B * a.Hq * a.T + stat] = live ? -D_sum : 0.f;
+  }
   if (myq < a.T) {
     if (!live)
 #pragma unroll
       for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
-    store_rows(a.dq + tok * a.q_ld + (int64_t)h * kHd, dq, a.scale, lh);
+    // a row that reads one key has no gradient on its score: not the rounding
+    // that the product's order leaves (NaN stays)
+    const bool one = myq == 0 && (a.causal || len == 1);
+    store_rows(a.dq + tok * a.q_ld + (int64_t)h * kHd, dq, one ? 0.f : a.scale, lh);
   }
 }
 
 // ---------------------------------------------------------------- dk, dv
 // One workgroup per (batch, query head, block of 128 keys), the blocks with the
 // most queries first. LDS: two buffers of a Q and a dout tile and their 64 lse
-// (times log2 e) and D values. Where query heads share a kv head, each writes its
+// (times log2 e) and -D values. Where query heads share a kv head, each writes its
 // f32 part and attn_dkdv_sum_kernel adds the parts in head order: a workgroup
 // that walked the group's heads one after the other would leave too few
 // workgroups for the chip (2 x 4096 tokens, 8 kv heads: 512 of very different
 // length), and a cut that depends on the batch would make the sums' order depend
-// on it. The parts cost 49 of 907 us at 2 x 4096 (268 MB written and read).
+// on it. The parts cost 49 of 898 us at 2 x 4096 (268 MB written and read).
 constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
 
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs a) {
@@ -272,7 +318,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
     for (int qb = 0; qb < 2; ++qb) {
       const int q0 = q0t + 32 * qb;
       if (q0 >= len || (a.causal && q0 + 31 < wk0)) continue;
-      f32x16 s{}, dp{};
+      f32x16 s{}, dp;
       const lds_char* row = rd + opaque(ro + qb * 8 * kGroupB);
       score_product<kDkdvAhead>(row, kf, s, [](int) {});
       if (a.causal && q0 < wk0 + 31) {  // row q0 + 8 (e >> 2) + 4 lh + (e & 3) reads keys up to itself
@@ -284,21 +330,30 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       // the exponentials beside the other product; elements 4 i .. + 3 are
       // query rows 8 i + 4 lh .. + 3
       const lds_char* st = rd + opaque(2 * kTileB + 128 * qb + 16 * (lane >> 5));
+      // the product starts at -D (16 subtractions less)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 D = *(const lds_f32x4*)(st + 32 * i + kTile * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * i + e] = D[e];
+      }
       score_product<kDkdvAhead>(row + kTileB, vf, dp, [&](int i) {
         const f32x2 l = *(const lds_f32x2*)(st + 32 * (i >> 1) + 8 * (i & 1));
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           s[2 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + e], scale_log2, -l[e]));
       });
+      // a row that reads one key has no gradient on its score: not the rounding
+      // that the product's order leaves (NaN stays)
+      if (q0 == 0 && (a.causal || len == 1)) dp[0] = (opaque(threadIdx.x) & 32) || dp[0] != dp[0] ? dp[0] : 0.f;
       u32x4 pw[2], dw[2];  // packed p and ds
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 D = *(const lds_f32x4*)(st + 32 * i + kTile * 4);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           const int x = 4 * i + e, w = 2 * (i & 1) + e / 2;
           pw[i >> 1][w] = pack2_rne(s[x], s[x + 1]);
-          dw[i >> 1][w] = pack2_rne(s[x] * (dp[x] - D[e]), s[x + 1] * (dp[x + 1] - D[e + 1]));
+          dw[i >> 1][w] = pack2_rne(s[x] * dp[x], s[x + 1] * dp[x + 1]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -382,7 +437,7 @@ size_t part_bytes(const glt_attn_desc* d) {
 }
 
 glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
-  constexpr int kDqLds = 4 * kTileB, kDkdvLds = 2 * kDkdvBuf;
+  constexpr int kDqLds = 4 * kTileB + 4 * kWaves, kDkdvLds = 2 * kDkdvBuf;
   // the dynamic-LDS limit is a per-device attribute of the kernels
   static std::atomic<bool> attr_set[64];
   int dev = 0;

@@ -375,7 +375,9 @@ glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const 
 /* dq, dk, dv (bf16, with the strides of q, k, v) from dout (out's stride) and
  * the forward's out and lse: D = rowsum(dout * out), p = exp(scale q.k - lse),
  * ds = p (dout.v - D), dq = scale ds . k, dk = scale ds^T . q, dv = p^T . dout,
- * k and v gradients summed over the query heads of their group. p and ds are
+ * k and v gradients summed over the query heads of their group. (D is put
+ * right from the probabilities where out's rounding would show: in rows of
+ * few keys, or of one that has nearly all the weight.) p and ds are
  * rounded to bf16 for the products, sums are f32 in one fixed order (a sequence's
  * gradients do not depend on the others of the call, nor on the run). Rows past a
  * sequence's length are zero. The gradients overlap no input. workspace:

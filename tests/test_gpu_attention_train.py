@@ -225,6 +225,20 @@ def test_scale_and_peaked_rows(dev):
         check(name, got[name], want[name], lse_bound(q, k, 1.5, want["lse"]))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("T,sharpness", [(700, 4), (700, 16), (1500, 8), (1500, 16)])
+def test_peaked_rows_of_many_keys(dev, T, sharpness, causal):
+    """Rows of more than 512 keys of which one has nearly all the weight: dp - D
+    cancels, and out's rounding in D would show (twice the bounds' elements
+    without the second walk of such rows)."""
+    q, k, v, dout = make(1, T, 2, 1, 5)
+    scale = sharpness * HD ** -0.5
+    got = run(q, k, v, dout, scale=scale, causal=causal)
+    want = formula(q, k, v, dout, scale, causal, [T])
+    for name in want:
+        check(name, got[name], want[name], lse_bound(q, k, scale, want["lse"]))
+
+
 def test_captured_in_a_graph_with_two_workspaces(dev):
     """Forward and backward captured twice, each with a workspace of its own,
     replayed several times with eager work between on new inputs in the
