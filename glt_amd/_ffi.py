@@ -213,10 +213,13 @@ def load(path=LIB_PATH):
 
 def call(name, *args):
     """Calls an entry point and raises GltError on a non-OK status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    return check(getattr(load(), name)(*args), name)
+
+
+def check(rc, name):
+    """Raises GltError where an entry point's status is not OK."""
     if rc != GLT_OK:
-        raise GltError(rc, name, lib.glt_last_error_string().decode(errors="replace"))
+        raise GltError(rc, name, load().glt_last_error_string().decode(errors="replace"))
     return rc
 
 

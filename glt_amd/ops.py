@@ -8,6 +8,7 @@ back as glt_amd._ffi.GltError (the reference throws std::runtime_error,
 src/checks.hpp:10-18).
 """
 import ctypes
+import functools
 
 import torch
 
@@ -201,20 +202,28 @@ class Ckpt8:
 def _rows_ld(name, t):
     """(dtype code, row stride) of t [rows, cols] with contiguous rows."""
     rows, cols = t.shape
-    ld = t.stride(0) if rows > 1 else cols
-    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+    ld, step = t.stride()
+    if rows <= 1:
+        ld = cols
+    if (cols > 1 and step != 1) or ld < cols:
         raise ValueError(f"{name}: strides {t.stride()} (rows contiguous, not overlapping)")
     return _dtype_code(t.dtype), ld
+
+
+@functools.lru_cache(maxsize=256)
+def _ckpt8_size(rows, cols):
+    return F.load().glt_ckpt8_size(rows, cols)
 
 
 def ckpt8_save(x, buf=None):
     """x [rows, cols] bf16 or f32 as an 8-bit checkpoint, in buf (uint8,
     glt_ckpt8_size bytes) where it is given."""
-    _need(x.dim() == 2 and x.is_cuda, "x: [rows, cols] on a GPU")
-    rows, cols = x.shape
+    shape = x.shape
+    _need(len(shape) == 2 and x.is_cuda, "x: [rows, cols] on a GPU")
+    rows, cols = shape
     dt, ld = _rows_ld("x", x)
-    buf = _workspace(buf, F.load().glt_ckpt8_size(rows, cols), x.device)
-    _call_on(x, "glt_ckpt8_save", _a(x), dt, ld, rows, cols, _a(buf))
+    buf = _workspace(buf, _ckpt8_size(rows, cols), x.device)
+    _call_on(x, "glt_ckpt8_save", x.data_ptr(), dt, ld, rows, cols, buf.data_ptr())
     return Ckpt8(buf, rows, cols, x.dtype)
 
 
@@ -308,7 +317,7 @@ def _call_on(t, name, *args):
     is passed last."""
     index = t.get_device()
     if index == torch.cuda.current_device():
-        F.call(name, *args, _stream_handle(index))
+        F.check(getattr(F.load(), name)(*args, _stream_handle(index)), name)
     else:
         with torch.cuda.device(index):
             F.call(name, *args, _stream_handle(index))
@@ -345,8 +354,9 @@ def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
     if seq_lens is not None and not (seq_lens.dtype == torch.int32 and seq_lens.shape == (B,)
                                      and seq_lens.device == dev and seq_lens.is_contiguous()):
         raise ValueError(f"seq_lens: contiguous int32 [{B}] on {dev}")
-    return F.AttnDesc(B, T, Hq, kshape[2], hd, hd ** -0.5 if scale is None else scale, 1 if causal else 0, *lds,
-                      _a(seq_lens))
+    d = F.AttnDesc(B, T, Hq, kshape[2], hd, hd ** -0.5 if scale is None else scale, 1 if causal else 0, *lds,
+                   _a(seq_lens))
+    return d, (B, T, Hq, kshape[2], hd), lds
 
 
 def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
@@ -355,18 +365,25 @@ def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
     as views of one projection output [B,T,(Hq+2Hkv)*hd]. seq_lens int32 [B]:
     the lengths of a padded batch (rows past them: zero output, lse -inf)."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    d = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
-    lse = torch.empty((d.B, d.n_q_heads, d.T), dtype=torch.float32, device=q.device)
-    _call_on(q, "glt_attention_train_fwd", ctypes.byref(d), _a(q), _a(k), _a(v), _a(out), _a(lse))
+    d, (B, T, Hq, _, _), _ = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
+    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device)
+    _call_on(q, "glt_attention_train_fwd", ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+             lse.data_ptr())
     return out, lse
 
 
-def _attn_grad_buffers(q, k, v, d):
+@functools.lru_cache(maxsize=256)
+def _attention_bwd_size(B, T, Hq, Hkv, hd):
+    return F.load().glt_attention_bwd_workspace_size(ctypes.byref(F.AttnDesc(B, T, Hq, Hkv, hd)))
+
+
+def _attn_grad_buffers(q, k, v, shape, lds):
     """Gradients with the strides of q, k, v: parts of one buffer where q, k, v
     are parts of one (that do not overlap)."""
-    T, ld, hd, rows = d.T, d.q_ld, d.head_dim, d.B * d.T
-    nq, nk = 2 * hd * d.n_q_heads, 2 * hd * d.n_kv_heads  # bytes of a token's heads
-    if ld == d.k_ld == d.v_ld:
+    B, T, Hq, Hkv, hd = shape
+    ld, k_ld, v_ld, _ = lds
+    rows, nq, nk = B * T, 2 * hd * Hq, 2 * hd * Hkv  # nq, nk: bytes of a token's heads
+    if ld == k_ld == v_ld:
         pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
         (p0, n0), (p1, n1), (p2, n2) = sorted(((pq, nq), (pk, nk), (pv, nk)))
         if p0 + n0 <= p1 and p1 + n1 <= p2 and p2 + n2 <= p0 + 2 * ld:
@@ -374,7 +391,7 @@ def _attn_grad_buffers(q, k, v, d):
             strides = (T * ld, ld, hd, 1)
             return [buf.as_strided(t.shape, strides, (p - p0) // 2) for p, t in ((pq, q), (pk, k), (pv, v))]
     return [torch.empty(rows * n, dtype=q.dtype, device=q.device).as_strided(t.shape, (T * n, n, hd, 1))
-            for t, n in ((q, ld), (k, d.k_ld), (v, d.v_ld))]
+            for t, n in ((q, ld), (k, k_ld), (v, v_ld))]
 
 
 def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=None, grads=None, workspace=None):
@@ -382,18 +399,18 @@ def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=Non
     of one buffer where q, k, v are; `grads` gives them). out and lse are the
     forward's; dout has out's shape and strides. workspace: a uint8 tensor of
     glt_attention_bwd_workspace_size bytes to use instead of a new one."""
-    d = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
-    B, T, dev = d.B, d.T, q.device
-    _need(_heads_ld("dout", dout, B, T, dev) == d.o_ld and dout.shape == out.shape, "dout: out's shape and strides")
-    if lse.dtype != torch.float32 or lse.shape != (B, d.n_q_heads, T) or not lse.is_contiguous() or lse.device != dev:
-        raise ValueError(f"lse: contiguous f32 [{B}, {d.n_q_heads}, {T}] on {dev}")
+    d, shape, lds = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
+    B, T, Hq, _, _ = shape
+    dev = q.device
+    _need(_heads_ld("dout", dout, B, T, dev) == lds[3] and dout.shape == out.shape, "dout: out's shape and strides")
+    if lse.dtype != torch.float32 or lse.shape != (B, Hq, T) or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError(f"lse: contiguous f32 [{B}, {Hq}, {T}] on {dev}")
     if grads is None:
-        grads = _attn_grad_buffers(q, k, v, d)
+        grads = _attn_grad_buffers(q, k, v, shape, lds)
     else:
-        for n, t, x, ld in zip(("dq", "dk", "dv"), grads, (q, k, v), (d.q_ld, d.k_ld, d.v_ld)):
+        for n, t, x, ld in zip(("dq", "dk", "dv"), grads, (q, k, v), lds):
             _need(t.shape == x.shape and _heads_ld(n, t, B, T, dev) == ld, "dq, dk, dv: the shapes and strides of q, k, v")
-    nb = F.load().glt_attention_bwd_workspace_size(ctypes.byref(d))
-    workspace = _workspace(workspace, nb, dev)
+    workspace = _workspace(workspace, _attention_bwd_size(*shape), dev)
     dq, dk, dv = grads
     _call_on(q, "glt_attention_bwd", ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
              lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(),
@@ -567,6 +584,11 @@ def _row_values(name, t, shape, device):
         raise ValueError(f"{name}: contiguous f32 {list(shape)} on {device}")
 
 
+@functools.lru_cache(maxsize=256)
+def _logprobs_size(rows, V, dt, top_k):
+    return F.load().glt_token_logprobs_workspace_size(rows, V, dt, top_k)
+
+
 def token_logprobs(logits, ids=None, top_k=0, temperature=1.0, workspace=None):
     """Log probabilities under softmax(logits / temperature) of the given
     tokens ids [rows, n] int32 (below 0 = padding, 0), with what else an answer
@@ -584,8 +606,7 @@ def token_logprobs(logits, ids=None, top_k=0, temperature=1.0, workspace=None):
     if top_k > 0:
         r["top_ids"] = top_ids = empty(rows, top_k, dtype=torch.int32, device=dev)
         r["top_logprobs"] = top_logprobs = empty(rows, top_k, dtype=f32, device=dev)
-    nb = F.load().glt_token_logprobs_workspace_size(rows, V, dt, top_k)
-    ws = _workspace(workspace, nb, dev)
+    ws = _workspace(workspace, _logprobs_size(rows, V, dt, top_k), dev)
     _call_on(logits, "glt_token_logprobs", _a(logits), dt, ld, rows, V, temperature, _a(ids), n, top_k,
              logprobs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), _a(top_ids), _a(top_logprobs), ws.data_ptr(),
              ws.numel())
