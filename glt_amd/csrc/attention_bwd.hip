@@ -30,7 +30,7 @@
 //   4 x 2048 causal 515, 498;  2 x 4096 causal 864, 849;  full 1568, 1579.
 // At 2 x 4096 causal dq and dkdv take 385 and 464 us: 1.07 and 1.18 * 10^15
 // operations a second of the unmasked part (a large library product: 1.24 *
-// 10^15); 25 of dq's go into watching D's error (kOff).
+// 10^15); 22 of dq's go into watching D's error (kOff).
 #include <algorithm>
 #include <atomic>
 
@@ -42,10 +42,10 @@ namespace {
 
 // Key tiles up to which a block of rows takes D from its own probabilities.
 constexpr int kExactTiles = 8;
-// Error of a longer row's D, relative to the 2-norm of its ds, that is put right:
-// 2 roundings of p and out and the one of ds leave 2^-8.5 in flat rows. Without
-// the second walk rows of one heavy key (T 700, scores of deviation 16) bring
-// dq's error to 3.0 * 2^-9, with it to 2.0 * 2^-9.
+// Error of a longer row's D, relative to the 2-norm of its ds, that is put right
+// in dq: the roundings of p and out leave 2^-9 in flat rows. Without the second
+// walk rows of one heavy key (T 700, scores of deviation 16) bring dq's error to
+// 3.0 * 2^-9 and dk's to 2.9 * 2^-9, with it to 2.0 and 1.2.
 constexpr float kOff = 0x1p-5f;
 
 struct BwdArgs {
@@ -203,20 +203,16 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
       f32x16 s{}, dp = nD;
       probs(t, kb, row, s, dp);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] *= dp[e];
+      for (int e = 0; e < 16; ++e) {
+        s[e] *= dp[e];
+        sums += s[e];
+        squares = __builtin_fmaf(s[e], s[e], squares);
+      }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const bf16x8 f = pack_frag(s, s2);
 #pragma unroll
         for (int db = 0; db < 4; ++db) dq[db] = mfma(col_frag(col, db, s2), f, dq[db]);
-        const u32x4 w = __builtin_bit_cast(u32x4, f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t pair = w[i];  // (a bit_cast of the vector's element itself reads element 0)
-          const bf16x2_t x = __builtin_bit_cast(bf16x2_t, pair);
-          sums = __builtin_amdgcn_fdot2_f32_bf16(x, kOnes2, sums, false);
-          squares = __builtin_amdgcn_fdot2_f32_bf16(x, x, squares, false);
-        }
       }
     });
     if (exact) {
@@ -226,7 +222,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
     // With more keys the row's ds tell: their sum is what D is off by (dkdv gets
     // it without). Where that is more than kOff of their 2-norm the workgroup
     // walks once more with this row's D put right: rows of which one key has
-    // some 0.95 of the weight (of flat ones it is 2^-8.5).
+    // some 0.95 of the weight (of flat ones it is 2^-9).
     if (u > 0) break;
     const float sum = pair_sum(sums);
     const bool off = live && sum * sum > kOff * kOff * pair_sum(squares);
