@@ -157,6 +157,24 @@ def test_nan_and_inf_past_the_end_take_no_part(dev):
             assert torch.equal(r[name], res[0][name]), name
 
 
+def test_rows_of_a_single_key_have_no_score_gradient(dev):
+    """The first row under the causal mask and sequences of one token: exact
+    zeros, in dk too; a NaN of theirs is passed on."""
+    q, k, v, dout = make(3, 90, 4, 2, 6)
+    got = run(q, k, v, dout)
+    assert not got["dq"][:, 0].any() and got["dq"][:, 1:].any()
+    one = torch.tensor([1, 90, 1], dtype=torch.int32, device=dev)
+    for causal in (True, False):
+        got = run(q, k, v, dout, seq_lens=one, causal=causal)
+        for name in ("dq", "dk"):
+            assert not got[name][[0, 2]].any() and got[name][1].any(), (name, causal)
+        assert torch.equal(got["dv"][0, 0].float(), dout[0, 0].float().view(2, 2, HD).sum(1).to(BF).float())
+    dout[0, 0, 3, 5] = math.nan
+    got = run(q, k, v, dout, seq_lens=one)
+    for name in ("dq", "dk", "dv"):
+        assert bool(torch.isnan(got[name][0, 0].float()).any()) and not bool(torch.isnan(got[name][1:].float()).any())
+
+
 def test_lengths_outside_the_batch_are_clamped(dev):
     q, k, v, dout = make(3, 90, 2, 1, 8)
     a = run(q, k, v, dout, seq_lens=torch.tensor((-5, 90, 40), dtype=torch.int32, device=dev))
