@@ -19,7 +19,15 @@
 //
 // Layout of a checkpoint [rows, cols]: rows of codes, padded to whole blocks
 // (code 128, zero), then from the next multiple of 256 bytes the exponents, row
-// by row. All kernels stream: a thread takes half a block, 16 values.
+// by row.
+//
+// All kernels stream and are bound by HBM: a thread takes a part of 8 columns, a
+// quarter of a block, so that each of a wavefront's bf16 loads and stores covers
+// whole lines (with 16 columns a thread each store wrote every other 16 bytes:
+// gate, up and inter of 8192 x 15360 207 us against 155, which is 6.5 TB/s).
+// 16384 x 4096 bf16: save 39 us, load 30 (5.2 and 6.8 TB/s, the codes partly from
+// cache). Two or four parts a thread are no faster (save 39, 44), nor are
+// non-temporal stores, which the reader of small activations would pay for.
 #include "common.hpp"
 #include "ckpt8.hpp"
 
@@ -28,13 +36,14 @@ namespace glt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHalf = 16;  // values per thread
+constexpr int kVals = 8;   // values per thread
 
 // 16 bytes at any element address (rows of an odd width start anywhere)
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct Shape8 {
-  uint32_t halves;  // half blocks per row, even
+  uint32_t parts;   // of 8 columns per row, a multiple of four
   uint32_t total;   // of all rows
   int cols;
   int64_t ld;       // of the activation
@@ -42,11 +51,11 @@ struct Shape8 {
 };
 
 template <typename T>
-__device__ __forceinline__ void load16(const T* row, int c, int cols, float* v) {
+__device__ __forceinline__ void load8(const T* row, int c, int cols, float* v) {
   constexpr int n = 16 / sizeof(T);
-  if (c + kHalf <= cols) {
+  if (c + kVals <= cols) {
 #pragma unroll
-    for (int q = 0; q < kHalf / n; ++q) {
+    for (int q = 0; q < kVals / n; ++q) {
       const u32x4 x = *reinterpret_cast<const u32x4_any*>(row + c + q * n);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -62,7 +71,7 @@ __device__ __forceinline__ void load16(const T* row, int c, int cols, float* v) 
   }
   // the row's end: the last element in the place of those past it, then zero
 #pragma unroll
-  for (int j = 0; j < kHalf; ++j) {
+  for (int j = 0; j < kVals; ++j) {
     const T t = row[min(c + j, cols - 1)];
     float y;
     if constexpr (sizeof(T) == 2) y = bf16_to_f32(t);
@@ -77,17 +86,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store16(T* row, int c, int cols, const float* v) {
-  if (c + kHalf <= cols) {
+__device__ __forceinline__ void store8(T* row, int c, int cols, const float* v) {
+  if (c + kVals <= cols) {
     if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        *reinterpret_cast<u32x4_any*>(row + c + 8 * q) =
-            u32x4{pack2(v[8 * q], v[8 * q + 1]), pack2(v[8 * q + 2], v[8 * q + 3]), pack2(v[8 * q + 4], v[8 * q + 5]),
-                  pack2(v[8 * q + 6], v[8 * q + 7])};
+      *reinterpret_cast<u32x4_any*>(row + c) = u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
     } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < 2; ++q)
         *reinterpret_cast<u32x4_any*>(row + c + 4 * q) =
             u32x4{__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
                   __float_as_uint(v[4 * q + 3])};
@@ -95,7 +100,7 @@ __device__ __forceinline__ void store16(T* row, int c, int cols, const float* v)
     return;
   }
 #pragma unroll
-  for (int j = 0; j < kHalf; ++j)
+  for (int j = 0; j < kVals; ++j)
     if (c + j < cols) {
       if constexpr (sizeof(T) == 2) row[c + j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
       else row[c + j] = v[j];
@@ -105,19 +110,20 @@ __device__ __forceinline__ void store16(T* row, int c, int cols, const float* v)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) ckpt8_save_kernel(const T* __restrict__ x, uint8_t* __restrict__ ck, const Shape8 s) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-  if (i >= s.total) return;  // a block's two halves leave together: total is even
-  const uint32_t row = i / s.halves, h = i - row * s.halves;
-  float v[kHalf];
-  load16(x + (int64_t)row * s.ld, (int)h * kHalf, s.cols, v);
+  if (i >= s.total) return;  // a block's four parts leave together
+  const uint32_t row = i / s.parts, h = i - row * s.parts;
+  float v[kVals];
+  load8(x + (int64_t)row * s.ld, (int)h * kVals, s.cols, v);
   uint32_t top = 0;  // the largest magnitude's bits; NaN and infinity are larger than any number's
 #pragma unroll
-  for (int j = 0; j < kHalf; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  for (int j = 0; j < kVals; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
   top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 2));
   // 127.5 steps and more, mantissa 0x7F0000, carry into the exponent
   const uint32_t E = top >= 0x7F800000u ? 255u : min((top + 0x10000u) >> 23, 254u);
-  uint32_t w[4];
+  uint32_t w[2];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < 2; ++q) {
     uint32_t b[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -128,17 +134,17 @@ __global__ void __launch_bounds__(kThreads) ckpt8_save_kernel(const T* __restric
     const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000C0Cu);
     w[q] = E == 255u ? 0x80808080u : lo | hi;
   }
-  *reinterpret_cast<u32x4*>(ck + (uint64_t)i * kHalf) = u32x4{w[0], w[1], w[2], w[3]};
-  if (!(h & 1)) ck[s.exp_off + (i >> 1)] = (uint8_t)E;
+  *reinterpret_cast<u32x2*>(ck + (uint64_t)i * kVals) = u32x2{w[0], w[1]};
+  if (!(h & 3)) ck[s.exp_off + (i >> 2)] = (uint8_t)E;
 }
 
-// The 16 values of half block i.
-__device__ __forceinline__ void restore16(const uint8_t* ck, const Shape8& s, uint32_t i, float* v) {
-  const u32x4 w = *reinterpret_cast<const u32x4*>(ck + (uint64_t)i * kHalf);
-  const uint32_t E = ck[s.exp_off + (i >> 1)];
+// The 8 values of part i.
+__device__ __forceinline__ void restore8(const uint8_t* ck, const Shape8& s, uint32_t i, float* v) {
+  const u32x2 w = *reinterpret_cast<const u32x2*>(ck + (uint64_t)i * kVals);
+  const uint32_t E = ck[s.exp_off + (i >> 2)];
   const float step = E == 255u ? NAN : __builtin_amdgcn_ldexpf(1.0f, (int)E - 133);
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
+  for (int q = 0; q < 2; ++q)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[4 * q + j] = ((float)((w[q] >> (8 * j)) & 0xFFu) - 128.f) * step;
 }
@@ -147,10 +153,10 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) ckpt8_load_kernel(const uint8_t* __restrict__ ck, T* __restrict__ x, const Shape8 s) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
   if (i >= s.total) return;
-  const uint32_t row = i / s.halves, h = i - row * s.halves;
-  float v[kHalf];
-  restore16(ck, s, i, v);
-  store16(x + (int64_t)row * s.ld, (int)h * kHalf, s.cols, v);
+  const uint32_t row = i / s.parts, h = i - row * s.parts;
+  float v[kVals];
+  restore8(ck, s, i, v);
+  store8(x + (int64_t)row * s.ld, (int)h * kVals, s.cols, v);
 }
 
 // gate, up and silu(gate) * up (in the order and with the sigmoid of the MLP's
@@ -161,34 +167,34 @@ __global__ void __launch_bounds__(kThreads) ckpt8_swiglu_kernel(const uint8_t* _
                                                                 uint16_t* __restrict__ inter, int lo, int hi, const Shape8 s) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
   if (i >= s.total) return;
-  const uint32_t row = i / s.halves;
-  const int c = (int)(i - row * s.halves) * kHalf;
+  const uint32_t row = i / s.parts;
+  const int c = (int)(i - row * s.parts) * kVals;
   const int64_t at = (int64_t)row * s.ld;
-  float g[kHalf], u[kHalf];
-  restore16(g8, s, i, g);
-  restore16(u8, s, i, u);
-  if (gate) store16(gate + at, c, s.cols, g);
-  if (up) store16(up + at, c, s.cols, u);
-  if (inter && c + kHalf > lo && c < hi) {
+  float g[kVals], u[kVals];
+  restore8(g8, s, i, g);
+  restore8(u8, s, i, u);
+  if (gate) store8(gate + at, c, s.cols, g);
+  if (up) store8(up + at, c, s.cols, u);
+  if (inter && c + kVals > lo && c < hi) {
 #pragma unroll
-    for (int j = 0; j < kHalf; ++j) {
+    for (int j = 0; j < kVals; ++j) {
       const float sg = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g[j] * 1.4426950408889634f));
       u[j] = g[j] * sg * u[j];
     }
-    store16(inter + at, c, s.cols, u);
+    store8(inter + at, c, s.cols, u);
   }
 }
 
-uint64_t halves_of(int32_t cols) { return 2 * (uint64_t)(((int64_t)cols + 31) / 32); }
-uint64_t code_bytes(int64_t rows, int32_t cols) { return (rows * halves_of(cols) * kHalf + 255) / 256 * 256; }
+uint64_t parts_of(int32_t cols) { return 4 * (uint64_t)(((int64_t)cols + 31) / 32); }
+uint64_t code_bytes(int64_t rows, int32_t cols) { return (rows * parts_of(cols) * kVals + 255) / 256 * 256; }
 
 glt_status check_shape(const char* who, int64_t rows, int32_t cols, int64_t ld, Shape8& s) {
   GLT_CHECK(rows >= 0 && cols > 0 && ld >= cols, GLT_ERR_SHAPE, "%s: rows=%lld cols=%d ld=%lld", who, (long long)rows, cols,
             (long long)ld);
-  GLT_CHECK(rows < INT32_MAX && rows * (int64_t)halves_of(cols) < INT32_MAX - kThreads, GLT_ERR_SHAPE,
-            "%s: %lld rows of %d columns (at most 2^31 half blocks of 16)", who, (long long)rows, cols);
-  s.halves = (uint32_t)halves_of(cols);
-  s.total = (uint32_t)(rows * s.halves);
+  GLT_CHECK(rows < INT32_MAX && rows * (int64_t)parts_of(cols) < (1ll << 32) - kThreads, GLT_ERR_SHAPE,
+            "%s: %lld rows of %d columns (at most 2^32 parts of 8)", who, (long long)rows, cols);
+  s.parts = (uint32_t)parts_of(cols);
+  s.total = (uint32_t)(rows * s.parts);
   s.cols = cols;
   s.ld = ld;
   s.exp_off = code_bytes(rows, cols);
@@ -226,7 +232,7 @@ extern "C" {
 
 size_t glt_ckpt8_size(int64_t rows, int32_t cols) {
   if (rows <= 0 || cols <= 0 || rows >= INT32_MAX) return 256;
-  return code_bytes(rows, cols) + (rows * halves_of(cols) / 2 + 255) / 256 * 256;
+  return code_bytes(rows, cols) + (rows * parts_of(cols) / 4 + 255) / 256 * 256;
 }
 
 glt_status glt_ckpt8_save(const void* x, int32_t dtype, int64_t ld, int64_t rows, int32_t cols, void* ckpt, void* stream) {

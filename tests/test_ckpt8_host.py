@@ -19,7 +19,7 @@ def load(ck=P, rows=3, cols=64, x=P, dtype=0, ld=64):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=2), 3), (dict(rows=-1), 2), (dict(cols=0), 2), (dict(cols=-3), 2), (dict(ld=63), 2),
-    (dict(rows=1 << 31), 2), (dict(rows=1 << 28, cols=256, ld=256), 2),  # half blocks past 31 bits
+    (dict(rows=1 << 31), 2), (dict(rows=1 << 28, cols=256, ld=256), 2),  # parts of 8 columns past 32 bits
     (dict(x=None), 1), (dict(ck=None), 1),
     (dict(ck=P + 16), 4), (dict(x=P + 1), 4), (dict(x=P + 2, dtype=1), 4),
 ])
