@@ -589,18 +589,24 @@ __device__ __forceinline__ void store_chunk(T* row, int e, int V, const float* v
     }
 }
 
-// One workgroup per piece of a row, as in the forward (4096 x 128256 bf16: 405 us,
-// 5.2 TB/s read and written). dx = (sum_j g_j [v =
-// id_j] - p (G + g_ent (logp + H))) / temperature, G = sum g_j. grad may be
-// logits: a workgroup reads its piece before it writes it, and the given
-// tokens' logits before any of it is written.
+// One workgroup per piece of a row, 8 KB (two chunks a thread: a workgroup
+// reads all of its piece before it writes, and the shorter it is the better the
+// two mix over the chip: 4096 x 128256 bf16 362 us, 5.8 TB/s read and written;
+// with eight, four and one chunks a thread 404, 402 and 445).
+// dx = (sum_j g_j [v = id_j] - p (G + g_ent (logp + H))) / temperature, G = sum
+// g_j. grad may be logits: a workgroup reads its piece before it writes it, and
+// the given tokens' logits before any of it is written.
+constexpr int kBwdChunks = 2;
+template <typename T>
+constexpr int kBwdPiece = kThreads * kBwdChunks * Elems<T>::n;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a) {
   using E = Elems<T>;
   const int tid = threadIdx.x;
   const uint32_t at = piece_index(blockIdx.x, gridDim.x);
   const int64_t row = at / a.np;
-  const int piece = (int)(at % a.np), e0 = piece * kPiece<T>;
+  const int piece = (int)(at % a.np), e0 = piece * kBwdPiece<T>;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   T* out = static_cast<T*>(a.grad) + row * a.ld_grad;
   const int32_t* ids = a.ids + row * a.n_ids;
@@ -619,7 +625,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   if (!any || lse == -INFINITY) {  // nothing flows, or nothing is allowed: zeros, whatever the logits hold
     const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < kChunks; ++q) {
+    for (int q = 0; q < kBwdChunks; ++q) {
       const int e = e0 + (q * kThreads + tid) * E::n;
       if (e < a.V) store_chunk(out, e, a.V, z);
     }
@@ -631,16 +637,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
     d = d < -1e4f ? -1e4f : d;  // p = 0 there: no 0 * inf; NaN stays
     return -__builtin_amdgcn_exp2f(d * kLog2e) * fmaf(gh, d + H, G);
   };
-  u32x4 ch[kChunks];
+  u32x4 ch[kBwdChunks];
 #pragma unroll
-  for (int q = 0; q < kChunks; ++q) ch[q] = load_chunk(x, e0 + (q * kThreads + tid) * E::n, a.V);
+  for (int q = 0; q < kBwdChunks; ++q) ch[q] = load_chunk(x, e0 + (q * kThreads + tid) * E::n, a.V);
   // thread j: the j-th given token where it lies in this piece and has not
   // been given before
   int mine = -1;
   float mine_g = 0.f;
   if (tid < a.n_ids) {
     const int id = ids[tid];
-    if (id >= e0 && id < min(a.V, e0 + kPiece<T>)) {
+    if (id >= e0 && id < min(a.V, e0 + kBwdPiece<T>)) {
       mine = id;
       float g = 0.f;
       for (int j = 0; j < a.n_ids; ++j)
@@ -653,7 +659,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   }
   if (a.n_ids) __syncthreads();
 #pragma unroll
-  for (int q = 0; q < kChunks; ++q) {
+  for (int q = 0; q < kBwdChunks; ++q) {
     const int e = e0 + (q * kThreads + tid) * E::n;
     float v[E::n];
 #pragma unroll
@@ -675,6 +681,11 @@ int pieces(int V, int dtype) {
   return (V + p - 1) / p;
 }
 size_t parts_bytes(int rows, int V, int dtype) { return round256((size_t)rows * pieces(V, dtype) * kWaves * sizeof(Part)); }
+
+int bwd_pieces(int V, int dtype) {
+  const int p = dtype == GLT_DTYPE_BF16 ? kBwdPiece<uint16_t> : kBwdPiece<float>;
+  return (V + p - 1) / p;
+}
 
 glt_status check_rows(const char* who, int32_t dtype, int64_t ld, int32_t rows, int32_t V, float temperature, int32_t n_ids) {
   GLT_CHECK(dtype == GLT_DTYPE_BF16 || dtype == GLT_DTYPE_F32, GLT_ERR_DTYPE, "%s: dtype %d", who, dtype);
@@ -767,6 +778,8 @@ glt_status glt_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld,
   const glt_status s = check_rows(who, dtype, ld, rows, V, temperature, n_ids);
   if (s != GLT_OK) return s;
   GLT_CHECK(ld_grad >= V, GLT_ERR_SHAPE, "%s: ld_grad=%lld V=%d", who, (long long)ld_grad, V);
+  GLT_CHECK((int64_t)rows * bwd_pieces(V, dtype) < (1ll << 32) / kThreads, GLT_ERR_SHAPE,
+            "%s: rows=%d V=%d are more workgroups than a launch holds", who, rows, V);
   if (rows == 0) return GLT_OK;
   GLT_CHECK(logits && grad && lse && (n_ids == 0 || (ids && grad_logprobs)) && (!grad_entropy || entropy),
             GLT_ERR_INVALID_ARG, "%s: null pointer", who);
@@ -776,7 +789,7 @@ glt_status glt_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld,
   GLT_CHECK(((uintptr_t)logits | (uintptr_t)grad) % es == 0 &&
                 ((uintptr_t)ids | (uintptr_t)grad_logprobs | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)grad_entropy) % 4 == 0,
             GLT_ERR_ALIGNMENT, "%s: pointers must be aligned to their elements", who);
-  const BwdArgs a{logits, grad, ld, ld_grad, rows, V, pieces(V, dtype), n_ids, (float)(1.0 / (double)temperature), ids,
+  const BwdArgs a{logits, grad, ld, ld_grad, rows, V, bwd_pieces(V, dtype), n_ids, (float)(1.0 / (double)temperature), ids,
                   grad_logprobs, lse, entropy, grad_entropy};
   const dim3 grid((unsigned)(rows * a.np));
   if (dtype == GLT_DTYPE_BF16)
