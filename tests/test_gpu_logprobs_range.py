@@ -1,0 +1,96 @@
+"""Token log probabilities and their gradient over the whole range of finite
+logits, on the GPU: tokens masked with a large negative number, rows far from
+zero, rows of one certain token.
+
+The definition takes a row's maximum m off before it scales, so that it is exact
+in 64 bits at any size: d = (x - m) / temperature, log p = d - log sum exp d.
+
+Tolerances, u = 2^-24 (half a step of f32, relative). The temperature, its
+reciprocal's product and the result are rounded to f32, u of |log p| (of |lse|)
+each; the sum of exponentials is off by less than 80 u (64 terms a lane in two
+chains, a tree of 6, exponentials and their arguments).
+  logprobs u (80 + 4 |log p|), lse u (80 + 4 |lse|)
+  entropy  u (80 (2 + H) + 4 sum p (|d| + d^2)): a term p d is off by what its
+           exponential's argument is, 3 u |d|, and by its own roundings
+No log probability is above 0 and no entropy below: the largest term is exactly 1,
+so the sum is at least 1, and every other step keeps the sign."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_logprobs import BF, F32, U, ids_for, make
+
+pytestmark = pytest.mark.gpu
+
+V, ROWS, K = 40000, 3, 20
+MASKS = [-1e9, -1e10, -1e20, -1e30]
+
+
+def exact(logits, temp):
+    x = logits.detach().float().cpu().double().numpy()
+    m = x.max(1, keepdims=True)
+    d = (x - m) / temp
+    ls = np.log(np.exp(d).sum(1, keepdims=True))
+    logp = d - ls
+    p = np.exp(logp)
+    H = -(p * np.where(p > 0, logp, 0)).sum(1)
+    return dict(d=d, logp=logp, p=p, H=H, lse=(m / temp + ls)[:, 0])
+
+
+def rows_of(name, value, dtype):
+    x = make(ROWS, V, dtype, 41)
+    if name == "part":       # whole wavefronts and pieces are masked, parts of others
+        x[:, 9000:31000] = value
+    elif name == "most":     # five tokens are allowed
+        keep = x[:, 7::8000].clone()
+        x[:] = value
+        x[:, 7::8000] = keep
+    elif name == "row":      # a row whose mask leaves nothing, between ordinary ones
+        x[1] = value
+    elif name == "offset":   # ordinary rows far from zero
+        x = (x.float() * 1000 + value).to(dtype)
+    return x
+
+
+CASES = [(n, v) for n in ("part", "most", "row") for v in MASKS] + [("offset", s * v) for v in (1e10, 1e20) for s in (1, -1)]
+
+
+def check_forward(logits, ids, temp, k):
+    from glt_amd import ops
+    got = ops.token_logprobs(logits, ids, top_k=k, temperature=temp)
+    torch.cuda.synchronize()
+    w = exact(logits, temp)
+    i = ids.cpu().numpy()
+    order = np.argsort(-logits.float().cpu().numpy(), 1, kind="stable")[:, :k]
+    assert np.array_equal(got["top_ids"].cpu().numpy(), order)
+    tol_h = U * (80 * (2 + w["H"]) + 4 * (w["p"] * (np.abs(w["d"]) + w["d"] ** 2)).sum(1))
+    for name, want, tol in [
+            ("lse", w["lse"], U * (80 + 4 * np.abs(w["lse"]))), ("entropy", w["H"], tol_h),
+            ("logprobs", np.take_along_axis(w["logp"], i, 1), None),
+            ("top_logprobs", np.take_along_axis(w["logp"], order, 1), None)]:
+        g = got[name].double().cpu().numpy()
+        tol = U * (80 + 4 * np.abs(want)) if tol is None else tol
+        assert np.isfinite(g).all() and (np.abs(g - want) <= tol).all(), (name, g, want)
+    assert bool((got["logprobs"] <= 0).all()) and bool((got["top_logprobs"] <= 0).all())
+    assert bool((got["entropy"] >= 0).all())
+    return got, w
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("temp", [0.7, 1.0, 1.3])
+@pytest.mark.parametrize("name,value", CASES)
+def test_statistics_of_large_logits(dev, dtype, temp, name, value):
+    check_forward(rows_of(name, value, dtype), ids_for(ROWS, V, 4, 42), temp, K)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("temp", [0.7, 1.0])
+def test_certain_tokens_have_no_positive_log_probability(dev, dtype, temp):
+    """One token has all the weight: its logit 14 to 86 temperatures above the
+    rest."""
+    rows, v = 300, 9000
+    x = make(rows, v, dtype, 43, std=0.5).float()
+    at = ids_for(rows, v, 1, 44)
+    x.scatter_(1, at.long(), temp * torch.linspace(14, 86, rows, device="cuda")[:, None])
+    x = x.to(dtype)
+    check_forward(x, at, temp, 5)
