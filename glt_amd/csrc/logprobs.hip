@@ -606,11 +606,17 @@ __device__ __forceinline__ void store_chunk(T* row, int e, int V, const float* v
 
 // One workgroup per piece of a row, 8 KB (two chunks a thread: a workgroup
 // reads all of its piece before it writes, and the shorter it is the better the
-// two mix over the chip: 4096 x 128256 bf16 362 us, 5.8 TB/s read and written;
-// with eight, four and one chunks a thread 404, 402 and 445).
+// two mix over the chip: 4096 x 128256 bf16 350 us, 6.0 TB/s read and written;
+// with eight, four and one chunks a thread 404, 402 and 445 where it took 362).
 // dx = (sum_j g_j [v = id_j] - p (G + g_ent (logp + H))) / temperature, G = sum
 // g_j. grad may be logits: a workgroup reads its piece before it writes it, and
 // the given tokens' logits before any of it is written.
+//
+// p comes from the f32 lse, whose rounding is |lse| 2^-24 of it: at most 2^-12
+// below kLseMax. At 1e8 log V is lost and past 3e38 lse is infinite; rows from
+// kLseMax on are one workgroup's, which forms their maximum and sum again
+// (4096 x 128256 bf16, every row such: 1460 us against 350; 4 rows 57 against 9).
+constexpr float kLseMax = 4096.f;
 constexpr int kBwdChunks = 2;
 template <typename T>
 constexpr int kBwdPiece = kThreads * kBwdChunks * Elems<T>::n;
@@ -637,57 +643,106 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   const float gh = a.g_ent ? a.g_ent[row] : 0.f;
   any = any || !(gh == 0.f);
   const float lse = a.lse[row], H = a.g_ent ? a.entropy[row] : 0.f;
-  if (!any || lse == -INFINITY) {  // nothing flows, or nothing is allowed: zeros, whatever the logits hold
+  auto zeros = [&](int from, int to) {
     const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int q = 0; q < kBwdChunks; ++q) {
-      const int e = e0 + (q * kThreads + tid) * E::n;
-      if (e < a.V) store_chunk(out, e, a.V, z);
-    }
+    for (int e = from + tid * E::n; e < to; e += kThreads * E::n) store_chunk(out, e, a.V, z);
+  };
+  if (!any) {  // nothing flows: zeros, whatever the logits hold
+    zeros(e0, min(a.V, e0 + kBwdPiece<T>));
     return;
   }
-  // without the given tokens' own terms
-  auto base = [&](float v) {
-    float d = fmaf(v, a.inv_temp, -lse);
+  // log p in, without the given tokens' own terms
+  auto base = [&](float d) {
     d = d < -1e4f ? -1e4f : d;  // p = 0 there: no 0 * inf; NaN stays
     return -__builtin_amdgcn_exp2f(d * kLog2e) * fmaf(gh, d + H, G);
   };
-  u32x4 ch[kBwdChunks];
-#pragma unroll
-  for (int q = 0; q < kBwdChunks; ++q) ch[q] = load_chunk(x, e0 + (q * kThreads + tid) * E::n, a.V);
-  // thread j: the j-th given token where it lies in this piece and has not
-  // been given before
+  // thread j: the j-th given token where it lies in [from, to) and has not been
+  // given before, and its gradient
   int mine = -1;
   float mine_g = 0.f;
-  if (tid < a.n_ids) {
-    const int id = ids[tid];
-    if (id >= e0 && id < min(a.V, e0 + kBwdPiece<T>)) {
-      mine = id;
-      float g = 0.f;
-      for (int j = 0; j < a.n_ids; ++j)
-        if (ids[j] == id) {
-          if (j < tid) mine = -1;
-          g += gl[j];
-        }
-      mine_g = (base(value_of(x[id])) + g) * a.inv_temp;
+  auto given = [&](int from, int to, auto logp) {
+    if (tid < a.n_ids) {
+      const int id = ids[tid];
+      if (id >= from && id < to) {
+        mine = id;
+        float g = 0.f;
+        for (int j = 0; j < a.n_ids; ++j)
+          if (ids[j] == id) {
+            if (j < tid) mine = -1;
+            g += gl[j];
+          }
+        mine_g = (base(logp(value_of(x[id]))) + g) * a.inv_temp;
+      }
     }
-  }
-  if (a.n_ids) __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kBwdChunks; ++q) {
-    const int e = e0 + (q * kThreads + tid) * E::n;
-    float v[E::n];
-#pragma unroll
-    for (int j = 0; j < E::n; ++j) v[j] = base(E::get(ch[q], j)) * a.inv_temp;
-    if (e < a.V) store_chunk(out, e, a.V, v);
-  }
-  if (a.n_ids) {
+    if (a.n_ids) __syncthreads();
+  };
+  auto put_given = [&]() {
+    if (!a.n_ids) return;
     __syncthreads();
     if (mine >= 0) {
       if constexpr (sizeof(T) == 2) out[mine] = __builtin_bit_cast(uint16_t, (__bf16)mine_g);
       else out[mine] = mine_g;
     }
+  };
+  if (!(fabsf(lse) < kLseMax) && lse == lse) {
+    // The first piece's workgroup alone, as it reads all of the row before it
+    // writes any: log p from the row's own maximum and sum.
+    if (piece) return;
+    __shared__ float s_m[kWaves];
+    __shared__ double s_s[kWaves];
+    float m = -INFINITY;
+#pragma unroll 1
+    for (int e = tid * E::n; e < a.V; e += kThreads * E::n) {
+      const u32x4 c = load_chunk(x, e, a.V);
+#pragma unroll
+      for (int j = 0; j < E::n; ++j) m = fmaxf(m, E::get(c, j));
+    }
+    m = wave_max(m);
+    if ((tid & 63) == 0) s_m[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    if (m == -INFINITY) {  // nothing is allowed
+      zeros(0, a.V);
+      return;
+    }
+    double sum = 0.0;
+#pragma unroll 1
+    for (int e = tid * E::n; e < a.V; e += kThreads * E::n) {
+      const u32x4 c = load_chunk(x, e, a.V);
+#pragma unroll
+      for (int j = 0; j < E::n; ++j) sum += __builtin_amdgcn_exp2f((E::get(c, j) - m) * a.inv_temp * kLog2e);
+    }
+    sum = wave_sum64(sum);
+    if ((tid & 63) == 0) s_s[tid >> 6] = sum;
+    __syncthreads();
+    const float log_sum = (float)(log2(s_s[0] + s_s[1] + s_s[2] + s_s[3]) * kLn2);
+    auto logp = [&](float v) { return fmaf(v - m, a.inv_temp, -log_sum); };
+    given(0, a.V, logp);
+#pragma unroll 1
+    for (int e = tid * E::n; e < a.V; e += kThreads * E::n) {
+      const u32x4 c = load_chunk(x, e, a.V);
+      float v[E::n];
+#pragma unroll
+      for (int j = 0; j < E::n; ++j) v[j] = base(logp(E::get(c, j))) * a.inv_temp;
+      store_chunk(out, e, a.V, v);
+    }
+    put_given();
+    return;
   }
+  u32x4 ch[kBwdChunks];
+#pragma unroll
+  for (int q = 0; q < kBwdChunks; ++q) ch[q] = load_chunk(x, e0 + (q * kThreads + tid) * E::n, a.V);
+  auto logp = [&](float v) { return fmaf(v, a.inv_temp, -lse); };
+  given(e0, min(a.V, e0 + kBwdPiece<T>), logp);
+#pragma unroll
+  for (int q = 0; q < kBwdChunks; ++q) {
+    const int e = e0 + (q * kThreads + tid) * E::n;
+    float v[E::n];
+#pragma unroll
+    for (int j = 0; j < E::n; ++j) v[j] = base(logp(E::get(ch[q], j))) * a.inv_temp;
+    if (e < a.V) store_chunk(out, e, a.V, v);
+  }
+  put_given();
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }

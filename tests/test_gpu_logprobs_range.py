@@ -94,3 +94,91 @@ def test_certain_tokens_have_no_positive_log_probability(dev, dtype, temp):
     x.scatter_(1, at.long(), temp * torch.linspace(14, 86, rows, device="cuda")[:, None])
     x = x.to(dtype)
     check_forward(x, at, temp, 5)
+
+
+def check_gradient(logits, ids, temp, ent, place=False):
+    """Against the formula. p is off by u (100 + 8 min(|d|, 110)) relative where
+    it is formed from d (past 110 it is 0), and by 8 u |lse| more where from z and
+    the rounded lse, which rows of |lse| of 4096 and more do not use."""
+    from glt_amd import ops
+    n = ids.shape[1]
+    g = torch.randn((ROWS, n), generator=torch.Generator().manual_seed(1)).cuda()
+    ge = torch.randn((ROWS,), generator=torch.Generator().manual_seed(2)).cuda() if ent else None
+    r = ops.token_logprobs(logits, ids, temperature=temp)
+    w = exact(logits, temp)
+    got = ops.token_logprobs_bwd(logits, ids, r["lse"], g, r["entropy"], ge, temp, grad=logits if place else None)
+    torch.cuda.synchronize()
+    gn = g.cpu().double().numpy()
+    gh = ge.cpu().double().numpy()[:, None] if ent else np.zeros((ROWS, 1))
+    p, H = w["p"], w["H"][:, None]
+    lp_h = np.where(p > 0, w["logp"] + H, 0)
+    want = -p * (gn.sum(1, keepdims=True) + gh * lp_h)
+    size = p * (np.abs(gn).sum(1, keepdims=True) + np.abs(gh) * (np.abs(lp_h) + H))
+    i = ids.cpu().numpy()
+    for j in range(n):
+        np.add.at(want, (np.arange(ROWS), i[:, j]), gn[:, j])
+        np.add.at(size, (np.arange(ROWS), i[:, j]), np.abs(gn[:, j]))
+    want, size = want / temp, size / temp
+    near = 8 * np.minimum(np.abs(w["d"]), 110) + np.where(np.abs(w["lse"]) < 4096, 8 * np.abs(w["lse"]), 0)[:, None]
+    half = 2.0 ** -8 if logits.dtype == BF else 2.0 ** -24
+    tol = U * (100 + near) * size + half * np.abs(want) + 2.0 ** -133
+    d = np.abs(got.double().cpu().numpy() - want)
+    assert np.isfinite(d).all() and (d <= tol).all(), (d.max(), (d / tol).max())
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("temp", [0.7, 1.0, 1.3])
+@pytest.mark.parametrize("name,value", CASES)
+def test_gradient_of_large_logits(dev, dtype, temp, name, value):
+    ids = ids_for(ROWS, V, 4, 45)
+    ids[:, 1] = ids[:, 0]    # the same token twice
+    x = rows_of(name, value, dtype)
+    got = check_gradient(x, ids, temp, True)
+    y = x.clone()
+    assert torch.equal(check_gradient(y, ids, temp, True, place=True), got) and torch.equal(y, got)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradient_where_lse_passes_the_range(dev, dtype):
+    """Rows masked with the type's lowest value, whose scaled lse is -inf in f32:
+    every token has its share. A row of -inf has none, and no other row's
+    gradient changes."""
+    x = rows_of("row", torch.finfo(dtype).min, dtype)
+    ids = ids_for(ROWS, V, 2, 46)
+    got = check_gradient(x, ids, 0.7, True)
+    assert bool(got[1].any())
+    from glt_amd import ops
+    x[1] = -np.inf
+    g = torch.ones((ROWS, 2), device="cuda")
+    r = ops.token_logprobs(x, ids, temperature=0.7)
+    a = ops.token_logprobs_bwd(x, ids, r["lse"], g, temperature=0.7)
+    b = ops.token_logprobs_bwd(x[::2], ids[::2].contiguous(), r["lse"][::2].contiguous(), g[::2].contiguous(), temperature=0.7)
+    assert not a[1].any() and torch.equal(a[::2], b)
+
+
+@pytest.mark.parametrize("v,n", [(1, 1), (37, 3), (4097, 64), (1 << 20, 2)])
+def test_gradient_far_from_zero_of_any_width(dev, v, n):
+    """One logit to the largest vocabulary, rows of large lse beside one of
+    ordinary lse, with padding and foreign ids."""
+    from glt_amd import ops
+    x = make(3, v, F32, 47)
+    x[1] += 30000
+    x[2] -= 30000
+    ids = ids_for(3, v, n, 48)
+    r = ops.token_logprobs(x, ids)
+    g = torch.full((3, n), 0.25, device="cuda")
+    got = ops.token_logprobs_bwd(x, ids, r["lse"], g)
+    for i in range(3):
+        w = exact(x[i:i + 1], 1.0)
+        want = -w["p"][0] * 0.25 * n
+        np.add.at(want, ids[i].cpu().numpy(), 0.25)
+        size = w["p"][0] * 0.25 * n
+        np.add.at(size, ids[i].cpu().numpy(), 0.25)
+        tol = U * (100 + 8 * np.minimum(np.abs(w["d"][0]), 110) + 60) * size + U * np.abs(want) + 2.0 ** -133
+        assert (np.abs(got[i].double().cpu().numpy() - want) <= tol).all(), i
+    ids[:, 0] = -1
+    a = ops.token_logprobs_bwd(x, ids, r["lse"], g)
+    assert bool(torch.isfinite(a).all()) and a.any() == (n > 1 and v > 1)
+    ids[:, 0] = v
+    assert bool(torch.isnan(ops.token_logprobs_bwd(x, ids, r["lse"], g)).all())
