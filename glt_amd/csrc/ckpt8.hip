@@ -7,9 +7,10 @@
 // step), step = 2^(E - 133), so
 //   * every step and every restored value is exact in f32 and bf16 (seven bits
 //     and a power of two), the only rounding is to the nearest step (ties to
-//     even): at most half a step, 1/127.5 of the block's largest magnitude;
+//     even): at most half a step, 1/127.5 of the block's largest magnitude
+//     or, where that is more, 2^-134: steps end at 2^-133, E = 0;
 //   * zero stays zero, and saving a restored block gives the same bytes (its
-//     largest code is 64 or more, so its exponent is the same).
+//     largest code is 64 or more, or E is 0, so its exponent is the same).
 // E = 255: the block holds NaN or infinity and is restored as NaN. E = 254 is
 // the last finite exponent; codes end at +-127 there. An integer code serves
 // activations better than an 8-bit float of the same block: its error is
@@ -119,8 +120,9 @@ __global__ void __launch_bounds__(kThreads) ckpt8_save_kernel(const T* __restric
   for (int j = 0; j < kVals; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
   top = max(top, (uint32_t)__shfl_xor((int)top, 1));
   top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-  // 127.5 steps and more, mantissa 0x7F0000, carry into the exponent
-  const uint32_t E = top >= 0x7F800000u ? 255u : min((top + 0x10000u) >> 23, 254u);
+  // 127.5 steps and more carry into the exponent: mantissa 0x7F0000, below the
+  // normal range, where no 1 stands before it, 0x7F8000
+  const uint32_t E = top >= 0x7F800000u ? 255u : min((top + (top < 0x800000u ? 0x8000u : 0x10000u)) >> 23, 254u);
   uint32_t w[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {

@@ -283,11 +283,12 @@ glt_status glt_gate_up_bwd(const float* gi, const uint16_t* g, const uint16_t* u
 /* ------------------------------------------------- 8-bit checkpoints
  * An activation [rows, cols] held for the backward in 1 + 1/32 bytes a value
  * (the reference saves bf16 or recomputes, src/layer_recompute_impl.inc:8-91).
- * A block of 32 consecutive columns shares a power of two, the smallest step
- * for which its largest magnitude rounds to at most 127 steps; a value is held
- * as rint(x / step) and restored exactly as that many steps: at most half a
- * step off, 1/127.5 of the block's largest magnitude. A block with NaN or infinity
- * is restored as NaN. x: dtype GLT_DTYPE_BF16 or GLT_DTYPE_F32 at row stride
+ * A block of 32 consecutive columns shares a power of two, the smallest step, not
+ * below 2^-133, for which its largest magnitude rounds to at most 127 steps; a
+ * value is held as rint(x / step) and restored exactly as that many steps: at
+ * most half a step off (a whole one for magnitudes from 127.5 * 2^121 on, where
+ * exponents end), 1/127.5 of the block's largest magnitude or, where that is
+ * more, 2^-134. A block with NaN or infinity is restored as NaN. x: dtype GLT_DTYPE_BF16 or GLT_DTYPE_F32 at row stride
  * ld. ckpt: glt_ckpt8_size bytes, 256-byte aligned; a checkpoint of either
  * dtype is restored to either (the values are exact in both). */
 size_t glt_ckpt8_size(int64_t rows, int32_t cols);
