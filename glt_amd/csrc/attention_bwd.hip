@@ -35,6 +35,7 @@
 #include <atomic>
 
 #include "attention_dev.hpp"
+#include "overlap.hpp"
 
 namespace glt {
 
@@ -483,6 +484,18 @@ extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, c
   const size_t need = glt_attention_bwd_workspace_size(d);
   GLT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, GLT_ERR_WORKSPACE,
             "glt_attention_bwd: needs %zu workspace bytes, 256-byte aligned", need);
+  // every kernel reads inputs after others have written gradients
+  const int64_t tokens = (int64_t)d->B * d->T, nq = 2 * kHd * d->n_q_heads, nk = 2 * kHd * d->n_kv_heads;
+  const ByteRows in[] = {{q, tokens, nq, 2 * d->q_ld},   {k, tokens, nk, 2 * d->k_ld},    {v, tokens, nk, 2 * d->v_ld},
+                         {out, tokens, nq, 2 * d->o_ld}, {dout, tokens, nq, 2 * d->o_ld}, dense_bytes(lse, tokens * d->n_q_heads * 4)};
+  const ByteRows to[] = {{dq, tokens, nq, 2 * d->q_ld}, {dk, tokens, nk, 2 * d->k_ld}, {dv, tokens, nk, 2 * d->v_ld},
+                         dense_bytes(workspace, (int64_t)need)};
+  for (int i = 0; i < 4; ++i) {
+    for (const ByteRows& x : in)
+      GLT_CHECK(!overlap(to[i], x), GLT_ERR_INVALID_ARG, "glt_attention_bwd: gradients and workspace must overlap no input");
+    for (int j = 0; j < i; ++j)
+      GLT_CHECK(!overlap(to[i], to[j]), GLT_ERR_INVALID_ARG, "glt_attention_bwd: gradients and workspace must not overlap");
+  }
   BwdArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);

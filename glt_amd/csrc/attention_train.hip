@@ -29,6 +29,7 @@
 #include <atomic>
 
 #include "attention_dev.hpp"
+#include "overlap.hpp"
 
 namespace glt {
 
@@ -233,6 +234,15 @@ extern "C" glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void
   GLT_CHECK(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0 && (uintptr_t)lse % 4 == 0 &&
                 (uintptr_t)d->seq_lens % 4 == 0,
             GLT_ERR_ALIGNMENT, "glt_attention_train_fwd: tensors must be 16-byte aligned");
+  // workgroups read keys and values that others' rows are written beside; a
+  // query row is read by its own workgroup alone, before it writes
+  const int64_t tokens = (int64_t)d->B * d->T, nq = 2 * kHd * d->n_q_heads, nk = 2 * kHd * d->n_kv_heads;
+  const ByteRows rq{q, tokens, nq, 2 * d->q_ld}, rk{k, tokens, nk, 2 * d->k_ld}, rv{v, tokens, nk, 2 * d->v_ld},
+      ro{out, tokens, nq, 2 * d->o_ld}, rl = dense_bytes(lse, tokens * d->n_q_heads * 4);
+  GLT_CHECK(!overlap(ro, rk) && !overlap(ro, rv) && ((out == q && d->o_ld == d->q_ld) || !overlap(ro, rq)),
+            GLT_ERR_INVALID_ARG, "glt_attention_train_fwd: out must overlap no input (but q itself)");
+  GLT_CHECK(!overlap(rl, rq) && !overlap(rl, rk) && !overlap(rl, rv) && !overlap(rl, ro), GLT_ERR_INVALID_ARG,
+            "glt_attention_train_fwd: lse must overlap no other tensor");
   // the dynamic-LDS limit is a per-device attribute of the kernel
   static std::atomic<bool> attr_set[64];
   int dev = 0;

@@ -396,8 +396,8 @@ def _attn_grad_buffers(q, k, v, shape, lds):
 
 def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=None, grads=None, workspace=None):
     """(dq, dk, dv) of attention_train, bf16 with the strides of q, k, v (parts
-    of one buffer where q, k, v are; `grads` gives them). out and lse are the
-    forward's; dout has out's shape and strides. workspace: a uint8 tensor of
+    of one buffer where q, k, v are; `grads` gives them, overlapping no input).
+    out and lse are the forward's; dout has out's shape and strides. workspace: a uint8 tensor of
     glt_attention_bwd_workspace_size bytes to use instead of a new one."""
     d, shape, lds = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
     B, T, Hq, _, _ = shape

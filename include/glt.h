@@ -34,7 +34,7 @@ extern "C" {
 /* ------------------------------------------------------------------ status */
 typedef int32_t glt_status;
 #define GLT_OK                     0
-#define GLT_ERR_INVALID_ARG        1  /* null pointer / bad enum / bad flag        */
+#define GLT_ERR_INVALID_ARG        1  /* null pointer / bad enum / bad flag / overlapping operands */
 #define GLT_ERR_SHAPE              2  /* inconsistent or out-of-range dimensions   */
 #define GLT_ERR_DTYPE              3  /* unsupported dtype combination             */
 #define GLT_ERR_ALIGNMENT          4  /* pointer or stride alignment not met       */
@@ -369,7 +369,9 @@ typedef struct {
 } glt_attn_desc;
 /* out = softmax(scale q . k^T + mask) . v (bf16), lse [B, n_q_heads, T] f32 =
  * log(sum exp) of each row's scaled scores. Statistics, sums and products in
- * f32; probabilities rounded to bf16 for the product with v. No workspace. */
+ * f32; probabilities rounded to bf16 for the product with v. out may be q itself
+ * (the same pointer and stride), otherwise it overlaps no input, and lse no other
+ * tensor (GLT_ERR_INVALID_ARG). No workspace. */
 glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
                                    void* out, float* lse, void* stream);
 
@@ -381,7 +383,8 @@ glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const 
  * few keys, or of one that has nearly all the weight.) p and ds are
  * rounded to bf16 for the products, sums are f32 in one fixed order (a sequence's
  * gradients do not depend on the others of the call, nor on the run). Rows past a
- * sequence's length are zero. The gradients overlap no input. workspace:
+ * sequence's length are zero. The gradients overlap no input and each other
+ * nowhere (GLT_ERR_INVALID_ARG; columns of one buffer do not overlap). workspace:
  * glt_attention_bwd_workspace_size bytes, 256-byte aligned, nothing kept in
  * it between calls. */
 size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d);

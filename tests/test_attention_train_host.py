@@ -83,3 +83,43 @@ def test_workspace_holds_row_sums_and_partials():
         n = lib.glt_attention_bwd_workspace_size(ctypes.byref(d))
         assert n % 256 == 0 and n >= 8 * B * T * Hq
         assert n <= 8 * B * T * Hq + 256 + 8 * B * T * Hq * 128
+
+
+def spread(**at):
+    """Operands far apart, but for those given."""
+    a = {n: (i + 1) << 32 for i, n in enumerate(("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "ws"))}
+    a.update(at)
+    return a
+
+
+@pytest.mark.parametrize("at", [
+    dict(dq=1 << 32), dict(dk=2 << 32), dict(dv=3 << 32),       # over what it is the gradient of
+    dict(dv=1 << 32), dict(dq=6 << 32), dict(dk=4 << 32),
+    dict(dq=(1 << 32) + 79 * 1024 + 512),                       # the last row's second half
+    dict(dq=(1 << 32) - 79 * 1024 - 512),                       # the other way round
+    dict(dk=(1 << 32) + 1024 * 30 + 512 - 16),                  # rows of another stride
+    dict(dv=(5 << 32) + 16), dict(dk=7 << 32), dict(dv=8 << 32),
+    dict(ws=(1 << 32) + 256), dict(ws=9 << 32), dict(ws=5 << 32),
+])
+def test_overlapping_gradients_are_refused(at):
+    """The queries' gradient is written before the keys' kernel reads the
+    queries: nothing that a call writes may lie over what it reads."""
+    a = spread(**at)
+    ws = a.pop("ws")
+    assert bwd(desc(), ws=ws, **a) == 1
+    assert b"overlap" in F.load().glt_last_error_string()
+
+
+@pytest.mark.parametrize("at", [
+    dict(out=2 << 32), dict(out=3 << 32), dict(out=(1 << 32) + 16), dict(out=(1 << 32) - 1024), dict(lse=1 << 32),
+    dict(lse=2 << 32), dict(lse=3 << 32), dict(lse=(4 << 32) + 8),
+])
+def test_overlapping_outputs_are_refused(at):
+    a = {n: v for n, v in spread(**at).items() if n in ("q", "k", "v", "out", "lse")}
+    assert fwd(desc(), **a) == 1
+    assert b"overlap" in F.load().glt_last_error_string()
+
+
+def test_an_output_over_the_queries_has_their_stride():
+    a = {n: v for n, v in spread(out=1 << 32).items() if n in ("q", "k", "v", "out", "lse")}
+    assert fwd(desc(o_ld=520), **a) == 1

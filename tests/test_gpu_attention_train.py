@@ -386,3 +386,42 @@ def test_offsets_past_32_bits(dev):
            lse.data_ptr(), st)
     assert torch.equal(O, want["out"]) and torch.equal(lse, want["lse"])
     assert torch.equal(Q, q) and torch.equal(V, v)
+
+
+def test_gradients_beside_their_inputs_in_one_buffer(dev):
+    """q, k, v, dout and dq, dk, dv as columns of one buffer, which do not overlap;
+    gradients over their inputs are refused and leave them alone."""
+    from glt_amd import _ffi as F
+    from glt_amd import ops
+    B, T, Hq, Hkv = 2, 70, 4, 2
+    heads = Hq + 2 * Hkv
+    buf = torch.full((B, T, 2 * heads + Hq, HD), 7.0, dtype=BF, device=dev)
+    cut = lambda t: (t[:, :, :Hq], t[:, :, Hq:Hq + Hkv], t[:, :, Hq + Hkv:heads])
+    x, grads, dout = cut(buf), cut(buf[:, :, heads:]), buf[:, :, 2 * heads:]
+    for t, src in zip(x + (dout,), make(B, T, Hq, Hkv, 23)):
+        t.copy_(src)
+    dense = dout.contiguous()
+    out, lse = ops.attention_train(*x)
+    want = run(*(t.contiguous() for t in x), dense)
+    for t, n in zip(ops.attention_bwd(*x, out, lse, dense, grads=grads), ("dq", "dk", "dv")):
+        assert torch.equal(t, want[n]), n
+    keep = buf.clone()
+    for bad in (x, (grads[0], x[1], grads[2]), (grads[0], grads[1], grads[1])):
+        with pytest.raises(F.GltError, match="overlap"):
+            ops.attention_bwd(*x, out, lse, dense, grads=bad)
+    assert torch.equal(buf, keep)
+
+
+def test_output_over_the_queries(dev):
+    """out may be q itself: the same bits as apart from it."""
+    import ctypes
+
+    from glt_amd import _ffi as F
+    q, k, v, dout = make(3, 300, 4, 2, 24)
+    lens = torch.tensor((300, 130, 1), dtype=torch.int32, device=dev)
+    want = run(q, k, v, dout, seq_lens=lens)
+    d = F.AttnDesc(3, 300, 4, 2, HD, HD ** -0.5, 1, 4 * HD, 2 * HD, 2 * HD, 4 * HD, lens.data_ptr())
+    lse = torch.empty((3, 4, 300), device=dev)
+    F.call("glt_attention_train_fwd", ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), q.data_ptr(),
+           lse.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(q, want["out"]) and torch.equal(lse, want["lse"])
