@@ -31,6 +31,7 @@
 #include <cmath>
 
 #include "common.hpp"
+#include "overlap.hpp"
 
 namespace glt {
 
@@ -859,6 +860,15 @@ glt_status glt_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld,
   GLT_CHECK(((uintptr_t)logits | (uintptr_t)grad) % es == 0 &&
                 ((uintptr_t)ids | (uintptr_t)grad_logprobs | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)grad_entropy) % 4 == 0,
             GLT_ERR_ALIGNMENT, "%s: pointers must be aligned to their elements", who);
+  // a workgroup writes its piece while others still read theirs and their row's values
+  const ByteRows to{grad, rows, (int64_t)V * es, ld_grad * es};
+  GLT_CHECK(grad == logits || !overlap(to, {logits, rows, (int64_t)V * es, ld * es}), GLT_ERR_INVALID_ARG,
+            "%s: grad overlaps the logits without being them", who);
+  for (const void* x : {static_cast<const void*>(lse), static_cast<const void*>(entropy), static_cast<const void*>(grad_entropy)})
+    GLT_CHECK(!x || !overlap(to, dense_bytes(x, (int64_t)rows * 4)), GLT_ERR_INVALID_ARG, "%s: grad overlaps an input", who);
+  for (const void* x : {static_cast<const void*>(ids), static_cast<const void*>(grad_logprobs)})
+    GLT_CHECK(n_ids == 0 || !overlap(to, dense_bytes(x, (int64_t)rows * n_ids * 4)), GLT_ERR_INVALID_ARG,
+              "%s: grad overlaps an input", who);
   const BwdArgs a{logits, grad, ld, ld_grad, rows, V, bwd_pieces(V, dtype), n_ids, (float)(1.0 / (double)temperature), ids,
                   grad_logprobs, lse, entropy, grad_entropy};
   const dim3 grid((unsigned)(rows * a.np));

@@ -708,7 +708,8 @@ glt_status glt_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int
  * no entropy term):
  *   grad[r, v] = (sum_j g_j [v = id_j] - p_v (sum_j g_j + g_ent (log p_v + H))) / temperature
  * in the logits' dtype at row stride ld_grad, rounded once; may be the logits
- * themselves (ld_grad = ld). Padding ids add nothing, the same id twice adds
+ * themselves (ld_grad = ld), otherwise it overlaps no input
+ * (GLT_ERR_INVALID_ARG). Padding ids add nothing, the same id twice adds
  * twice, an id at or past V makes the row NaN. Rows whose upstream gradients are
  * all zero get zeros whatever their logits hold, and so do rows without an
  * allowed token (lse -inf). */

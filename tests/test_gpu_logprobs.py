@@ -423,3 +423,22 @@ def test_offsets_past_32_bits(dev):
     grad = ops.token_logprobs_bwd(x, ids, got["lse"], g, grad=x)
     assert grad.data_ptr() == x.data_ptr() and torch.equal(x[-3:], w)
     assert bool((x[:-3, 5] > 0.99).all()) and bool((x[:-3, 6] < 0).all())
+
+
+def test_gradient_beside_the_logits_in_one_buffer(dev):
+    """Gradients in the columns behind the logits do not overlap them; one that is
+    shifted over them is refused and leaves them alone."""
+    from glt_amd import _ffi as F
+    from glt_amd import ops
+    buf = torch.full((4, 207), 3.0, dtype=BF, device="cuda")
+    x, ids = buf[:, :100], ids_for(4, 100, 1, 16)
+    x.copy_(make(4, 100, BF, 15))
+    r = ops.token_logprobs(x, ids)
+    g = torch.ones((4, 1), device="cuda")
+    want = ops.token_logprobs_bwd(x, ids, r["lse"], g)
+    assert torch.equal(ops.token_logprobs_bwd(x, ids, r["lse"], g, grad=buf[:, 101:201]), want)
+    keep = buf.clone()
+    for at in (1, 99):
+        with pytest.raises(F.GltError, match="overlap"):
+            ops.token_logprobs_bwd(x, ids, r["lse"], g, grad=buf[:, at:at + 100])
+    assert torch.equal(buf, keep)

@@ -66,3 +66,18 @@ def test_workspace_sizes():
         # eight pieces of four 16-byte parts and 20 keys of 8 bytes
         assert n >= rows * 8 * (4 * 16 + 20 * 8) and n > last and n % 256 == 0
         last = n
+
+
+@pytest.mark.parametrize("kw", [
+    dict(grad=P + 2), dict(grad=P + 200), dict(grad=P - 200),            # a step or a row off, the same stride
+    dict(grad=P + 600 - 2), dict(grad=P + 400, ldg=164),                 # the last logit; rows of another stride
+    dict(ld=200, ldg=200, grad=P + 198), dict(ld=200, ldg=200, grad=P - 200 + 2),
+    dict(lse=3 * P, grad=3 * P), dict(ent=3 * P, grad=3 * P + 8), dict(ge=3 * P, grad=3 * P - 598),
+    dict(ids=3 * P, grad=3 * P + 10), dict(gl=3 * P, grad=3 * P - 200),
+])
+def test_a_gradient_partly_over_an_input_is_refused(kw):
+    """Workgroups write their pieces while others read."""
+    far = dict(logits=P, ids=16 * P, gl=17 * P, lse=18 * P, ent=19 * P, ge=20 * P)
+    far.update(kw)
+    assert bwd(**far) == 1
+    assert b"overlap" in F.load().glt_last_error_string()
