@@ -264,8 +264,11 @@ def rms_norm_bwd(dy, x, w, var, eps, out=None):
 
 
 def apply_rope(q, k, theta, pos_offset=0):
-    """In-place RoPE on q [B,T,nq,hd] and k [B,T,nk,hd] (reference apply_rope,
-    src/rope_impl.inc:8-39)."""
+    """In-place RoPE on q [B,T,nq,hd] and k [B,T,nk,hd], dense bf16 (reference
+    apply_rope, src/rope_impl.inc:8-39). It has no backward: the gradients of
+    attention_bwd are those on the rotated q and k."""
+    for name, t in (("q", q), ("k", k)):
+        _need(t is None or t.is_contiguous(), f"{name}: contiguous (parts of a fused projection are not)")
     B, T, nq, hd = q.shape
     nk = k.shape[2] if k is not None else 0
     F.call("glt_rope_fwd", _p(q), nq, _p(k), nk, B, T, hd, theta, pos_offset, _stream())
@@ -274,7 +277,10 @@ def apply_rope(q, k, theta, pos_offset=0):
 def attention(q, k, v, causal=True, scale=None):
     """Causal GQA attention forward (the reference's SDPA call in
     forward_layer, src/layer_forward_impl.inc:41-49). q [B,T,Hq,hd],
-    k/v [B,T,Hkv,hd] bf16; returns [B,T,Hq,hd]."""
+    k/v [B,T,Hkv,hd] dense bf16; returns [B,T,Hq,hd]. (attention_train takes
+    parts of a fused projection.)"""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _need(t.is_contiguous(), f"{name}: contiguous (parts of a fused projection are not)")
     B, T, Hq, hd = q.shape
     Hkv = k.shape[2]
     if scale is None:
