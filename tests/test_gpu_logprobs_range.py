@@ -182,3 +182,22 @@ def test_gradient_far_from_zero_of_any_width(dev, v, n):
     assert bool(torch.isfinite(a).all()) and a.any() == (n > 1 and v > 1)
     ids[:, 0] = v
     assert bool(torch.isnan(ops.token_logprobs_bwd(x, ids, r["lse"], g)).all())
+
+
+def test_entropy_gradient_without_tokens_far_from_zero(dev):
+    """No given tokens: the entropy's gradient alone, of rows either side of zero
+    and of the lse from which a row is formed again."""
+    from glt_amd import ops
+    x = make(4, V, F32, 49)
+    x += torch.tensor([0.0, 4000.0, 4100.0, -1e6], device="cuda")[:, None]
+    r = ops.token_logprobs(x, temperature=1.0)
+    ge = torch.tensor([1.0, -2.0, 0.5, 3.0], device="cuda")
+    got = ops.token_logprobs_bwd(x, None, r["lse"], None, r["entropy"], ge)
+    w = exact(x, 1.0)
+    gh, H = ge.cpu().double().numpy()[:, None], w["H"][:, None]
+    lp_h = np.where(w["p"] > 0, w["logp"] + H, 0)
+    want, size = -w["p"] * gh * lp_h, w["p"] * np.abs(gh) * (np.abs(lp_h) + H)
+    assert (np.abs(w["lse"])[:2] < 4096).all() and (np.abs(w["lse"])[2:] > 4096).all()
+    far = np.where(np.abs(w["lse"]) < 4096, 8 * np.abs(w["lse"]), 0)[:, None]
+    tol = U * (100 + 8 * np.minimum(np.abs(w["d"]), 110) + far) * (size + w["p"] * np.abs(gh)) + U * np.abs(want) + 2.0 ** -133
+    assert (np.abs(got.double().cpu().numpy() - want) <= tol).all()
