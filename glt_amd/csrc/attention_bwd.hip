@@ -19,8 +19,13 @@
 // are formed so that a lane holds one OWNED row: the packed p or ds is then the
 // next product's operand as it stands in the accumulator's layout.
 //
-// Bound by the matrix instructions. The rows in registers leave room for two
-// wavefronts per SIMD, and a wavefront's own products depend on its
+// p and ds are rounded to bf16, as the matrix instructions take them, all sums are
+// f32: the gradients are off by 2.4 * 10^-3 in the 2-norm, of which their own
+// rounding is 1.6.
+//
+// Long rows: matrix instructions run 0.52 (dq) and 0.59 (dkdv) of the time, at the
+// power limit's 1.8 GHz. The rows in registers leave room for two wavefronts per
+// SIMD, and a wavefront's own products depend on its
 // exponentials, so one wavefront's arithmetic has to run beside the other's
 // products. The two come from two workgroups of four, which nothing keeps in
 // step. With one workgroup of eight instead (half the loads into LDS) they wait
@@ -28,9 +33,12 @@
 // 32 query and 8 kv heads, eight against four:
 //   1 x 512 causal 73, 55;  6 x 777 causal 213, 188;  1 x 1024 causal 99, 74;
 //   4 x 2048 causal 515, 498;  2 x 4096 causal 864, 849;  full 1568, 1579.
-// At 2 x 4096 causal dq and dkdv take 385 and 464 us: 1.07 and 1.18 * 10^15
+// At 2 x 4096 causal dq and dkdv take 385 and 464 us at best, 1.07 and 1.18 * 10^15
 // operations a second of the unmasked part (a large library product: 1.24 *
-// 10^15); 22 of dq's go into watching D's error (kOff).
+// 10^15), and the whole backward 926 to 963 from machine to machine; 22 of dq's go
+// into watching D's error (kOff). With few tokens the chip is not full (1 x 512
+// launches 128 workgroups), and blocks of at most 512 keys are walked twice: the
+// whole of 1 x 512 59 us, 1 x 1024 78, 4 x 2048 563.
 #include <algorithm>
 #include <atomic>
 

@@ -16,10 +16,17 @@
 // pointers (step's rd and wr): without that the compiler lets every transposing
 // read wait for all loads to LDS, the next tile's too (2 x 4096 causal 296 us).
 //
-// Bound by the matrix instructions: 2 x 4096 causal with 32 query and 8 kv heads
-// runs at 1.06 * 10^15 operations a second of the unmasked part, full at 1.13 *
-// 10^15 (a large library product: 1.24 * 10^15). us, against one workgroup of
-// eight wavefronts (half the loads into LDS, but they wait at the same barrier):
+// p is rounded to bf16, as the matrix instructions take it, the sums that divide
+// and give lse are f32: out is off by 2.1 * 10^-3 in the 2-norm, of which its own
+// rounding is 1.6.
+//
+// Long rows: matrix instructions run 0.54 of the time and vector ones 0.53, at the
+// power limit's 1.8 GHz. 2 x 4096 causal with 32 query and 8 kv heads takes 260 to 277 us
+// from machine to machine, 0.99 to 1.06 * 10^15 operations a second of the
+// unmasked part, full 1.13 * 10^15 at best (a large library product: 1.24 * 10^15).
+// Short ones: the longest rows' chain of tiles, 1.3 us each (1 x 512 15 us, 1 x
+// 1024 24). us, against one workgroup of eight wavefronts (half the loads into
+// LDS, but they wait at the same barrier):
 //   1 x 512 causal 15, 19;  6 x 777 causal 55, 65;  1 x 1024 causal 24, 31;
 //   4 x 2048 causal 148, 160;  2 x 4096 causal 260, 265;  2 x 4096 full 486, 484.
 // Tiles of 32 keys let three wavefronts share a SIMD and measure the same within

@@ -16,9 +16,13 @@
 // parts in their order, in 64 bits, and merges the lists. The cut depends on V
 // alone, so a row has the same bits in every call, and a single row still spreads
 // over V / 16384 workgroups (bf16; half as many logits a piece in f32).
-// 4096 x 128256 bf16: 191 us without alternatives (5.5 TB/s), 205 with 5, 217
-// with 20, 260 with 64; 2048 x 128256 f32: 179 us (5.9 TB/s), 183 with 20. Seven
-// rows of f32 with 20: 8 + 6 us, the latency of its steps.
+// 4096 x 128256 bf16: 176 to 190 us without alternatives (5.5 to 6.0 TB/s), 200
+// with 5, 216 with 20, 260 with 64; 2048 x 128256 f32: 178 us (5.9 TB/s), 189 with
+// 20. Seven rows of f32 with 20: 8 + 6 us, the latency of its steps.
+// Not fast: alternatives of rows in which nearly all logits are equal, masked ones
+// too. Their pieces are left to the row's one workgroup (piece_top_any): with
+// 100 allowed tokens and 20 alternatives 4096 rows of bf16 take 2780 us, seven of
+// f32 1190 (183 and 17 without alternatives).
 //
 // In log2 units c = log2(e) / temperature: a wavefront's terms are exp2((x - m)
 // c) of its maximum m, and the joined sum is told m c in 64 bits, where the

@@ -288,9 +288,10 @@ glt_status glt_gate_up_bwd(const float* gi, const uint16_t* g, const uint16_t* u
  * value is held as rint(x / step) and restored exactly as that many steps: at
  * most half a step off (a whole one for magnitudes from 127.5 * 2^121 on, where
  * exponents end), 1/127.5 of the block's largest magnitude or, where that is
- * more, 2^-134. A block with NaN or infinity is restored as NaN. x: dtype GLT_DTYPE_BF16 or GLT_DTYPE_F32 at row stride
- * ld. ckpt: glt_ckpt8_size bytes, 256-byte aligned; a checkpoint of either
- * dtype is restored to either (the values are exact in both). */
+ * more, 2^-134. A block with NaN or infinity is restored as NaN.
+ * x: dtype GLT_DTYPE_BF16 or GLT_DTYPE_F32 at row stride ld. ckpt: glt_ckpt8_size
+ * bytes, 256-byte aligned; a checkpoint of either dtype is restored to either
+ * (the values are exact in both). */
 size_t glt_ckpt8_size(int64_t rows, int32_t cols);
 glt_status glt_ckpt8_save(const void* x, int32_t dtype, int64_t ld, int64_t rows, int32_t cols,
                           void* ckpt, void* stream);
@@ -359,7 +360,13 @@ glt_status glt_attention_fwd(const void* q, const void* k, const void* v, void* 
  * sequences of a padded batch. Keys at or past a sequence's length take no
  * part, whatever the buffers hold there, NaN included; its rows past it get
  * zero output, lse -inf and zero gradients.
- * scale is positive and finite. head_dim must be 128; tensors 16-byte aligned. */
+ * scale is positive and finite. head_dim must be 128; tensors 16-byte aligned.
+ * Scores and lse are f32, so probabilities are off by some 2^-23 of a scaled score's
+ * magnitude: 10^4 costs 10^-3, and past 10^9 nothing is left of them (NaN). A NaN or
+ * infinity in a token reaches the causal rows before it that share its tile of
+ * 64 keys or queries (0 * NaN in the products), as in the formula.
+ * The gradients are those on q and k as they are passed: glt_rope_fwd has no
+ * backward here. */
 typedef struct {
   int32_t B, T, n_q_heads, n_kv_heads, head_dim;
   float scale;
@@ -695,8 +702,10 @@ glt_status glt_masked_ce(const uint16_t* logits, int64_t ld, const int32_t* ids,
  * [rows, top_k], top_k <= min(64, V): the largest logits in falling order, the
  * lower index first among equal ones. A logit of -inf has probability 0; a row
  * of nothing else has lse -inf, log probabilities -inf, entropy 0. NaN or +inf
- * make the row's statistics NaN (NaN logits rank by their bits). f32 sums, joined
- * in 64 bits in an order that V alone fixes. workspace:
+ * make the row's statistics NaN (NaN logits rank by their bits). Finite logits may
+ * have any size (lse is infinite where it passes f32's range, the others are not);
+ * no log probability is above 0, no entropy below. f32 sums, joined in 64 bits in
+ * an order that V alone fixes. workspace:
  * glt_token_logprobs_workspace_size bytes, 256-byte aligned. */
 size_t glt_token_logprobs_workspace_size(int32_t rows, int32_t V, int32_t dtype, int32_t top_k);
 glt_status glt_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V,
@@ -712,7 +721,8 @@ glt_status glt_token_logprobs(const void* logits, int32_t dtype, int64_t ld, int
  * (GLT_ERR_INVALID_ARG). Padding ids add nothing, the same id twice adds
  * twice, an id at or past V makes the row NaN. Rows whose upstream gradients are
  * all zero get zeros whatever their logits hold, and so do rows without an
- * allowed token (lse -inf). */
+ * allowed token. p is off by 2^-24 |lse| from lse's rounding; rows of |lse| of 4096
+ * and more form it from their logits again, in one workgroup each. */
 glt_status glt_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ld, int32_t rows, int32_t V,
                                   float temperature, const int32_t* ids, int32_t n_ids,
                                   const float* grad_logprobs, const float* lse, const float* entropy,
