@@ -85,7 +85,7 @@ def draw(rng):
     if kind == "decode":
         B, T = _log_int(rng, 1, 64), rng.choice([1, 1, 1, 2, 5, _log_int(rng, 1, 512)])
         B = max(1, min(B, 1024 * 32 // (T * Hq)))
-        hi = max(T + 1, _log_int(rng, 1, max(2, min(32768, 32 * 16384 * 8 // (B * Hkv), 2 * 512 * 32 * 7000 // (B * T * Hq)))))
+        hi = max(T + 1, _log_int(rng, 1, max(2, min(32768, 32 * 13000 * 8 // (B * Hkv), 2 * 512 * 32 * 7000 // (B * T * Hq)))))
         c = dict(kind=kind, B=B, T=T, Hq=Hq, Hkv=Hkv, lo=rng.randint(T, hi), hi=hi, ragged=rng.random() < 0.4, group=0,
                  plo=0, phi=0, window=0, sinks=0)
         if rng.random() < 0.4:
