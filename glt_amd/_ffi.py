@@ -71,6 +71,20 @@ class AttnDesc(ctypes.Structure):
                 ("seq_lens", _vp)]
 
 
+class Kv8Cache(ctypes.Structure):
+    _fields_ = [("data", _vp), ("n_pages", _i64), ("n_kv_heads", _i32), ("head_dim", _i32)]
+
+
+class Kv8Seqs(ctypes.Structure):
+    _fields_ = [("B", _i32), ("T", _i32), ("pages", _vp), ("pages_ld", _i64), ("n_table", _i32), ("lens", _vp),
+                ("new_lens", _vp)]
+
+
+class Kv8Attn(ctypes.Structure):
+    _fields_ = [("n_q_heads", _i32), ("scale", _f32), ("window", _i32), ("sinks", _i32), ("n_groups", _i32),
+                ("prefix_pages", _vp), ("prefix_ld", _i64), ("n_prefix_table", _i32), ("prefix_lens", _vp)]
+
+
 class LayerDesc(ctypes.Structure):
     _fields_ = [("B", _i32), ("T", _i32), ("n_q_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
                 ("rope_theta", _f32), ("rms_eps", _f32), ("mlp", MlpDesc)]
@@ -134,6 +148,13 @@ SIGNATURES = {
     "glt_attention_train_fwd": (_i32, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
     "glt_attention_bwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc)]),
     "glt_attention_bwd": (_i32, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "glt_kv8_size": (_sz, [_i64, _i32, _i32]),
+    "glt_kv8_write": (_i32, [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Seqs), _vp, _i64, _vp, _i64, _vp]),
+    "glt_kv8_read": (_i32, [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Seqs), _vp, _i64, _vp, _i64, _vp]),
+    "glt_kv8_attention_workspace_size": (_sz, [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Seqs),
+                                               ctypes.POINTER(Kv8Attn)]),
+    "glt_kv8_attention": (_i32, [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Seqs), ctypes.POINTER(Kv8Attn), _vp, _i64,
+                                 _vp, _i64, _vp, _vp, _sz, _vp]),
     "glt_grft_save": (_i32, [ctypes.c_char_p, ctypes.POINTER(GrftInfo), _vp, _i32, _vp]),
     "glt_grft_load": (_i32, [ctypes.c_char_p, ctypes.POINTER(GrftInfo), _vp, _i32, _vp]),
     "glt_grft_load_raw_f32": (_i32, [ctypes.c_char_p, ctypes.POINTER(GrftInfo), _vp, _i32, _vp]),

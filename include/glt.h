@@ -399,6 +399,79 @@ glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* 
                              const void* out, const float* lse, const void* dout, void* dq, void* dk,
                              void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------ keys and values in 8 bits */
+/* The cache of one layer's keys and values for generation: a pool of pages of 64
+ * tokens, glt_kv8_size bytes (260 a token and kv head, of 512 in bf16), 16-byte
+ * aligned, laid out as the kernels read it. A token's head is held as
+ *   step = bf16(max |x| / 127), in [2^-100, 2^121];  value = step * round(x / step)
+ * (nearest, ties to even; NaN throughout where x holds NaN or infinity), so that
+ * a value is within half a step of x, and a row of zeros stays one. head_dim is 128. The
+ * pool needs no clearing: what no call has written is never looked at. */
+typedef struct {
+  void* data;
+  int64_t n_pages;
+  int32_t n_kv_heads, head_dim;
+} glt_kv8_cache;
+size_t glt_kv8_size(int64_t n_pages, int32_t n_kv_heads, int32_t head_dim);
+
+/* B sequences (at most 8192) in the pool. Token i of sequence b lies in page
+ * pages[b * pages_ld + i / 64] (device, n_table entries a row, in any order;
+ * sequences may share pages that no call writes). lens[b] (device) is the number of
+ * tokens that it holds, the call's new ones counted; the new ones are its last new_lens[b]
+ * (device, NULL = T), padded to T in the call's tensors: new token t is token
+ * lens[b] - new_lens[b] + t. Lengths are clamped: lens to [0, 64 n_table], new_lens to [0,
+ * min(T, lens)]. A page id outside the pool is never followed: what would be written
+ * there is dropped, what would be read is NaN. */
+typedef struct {
+  int32_t B, T;
+  const int32_t* pages;
+  int64_t pages_ld;
+  int32_t n_table;
+  const int32_t* lens;
+  const int32_t* new_lens;
+} glt_kv8_seqs;
+
+/* The new tokens' k and v [B, T, n_kv_heads, 128] bf16 (strides and alignment as
+ * in glt_attn_desc) into the cache. Tokens t >= new_lens[b] are not read, and no other
+ * byte of the pool is touched. Two sequences that write the same token leave
+ * either's codes. */
+glt_status glt_kv8_write(const glt_kv8_cache* c, const glt_kv8_seqs* s, const void* k, int64_t k_ld, const void* v,
+                         int64_t v_ld, void* stream);
+/* The values that the cache holds of the new tokens, rounded to bf16 once; rows t
+ * >= new_lens[b] get zeros. (new_lens = lens and T = the longest read everything.) */
+glt_status glt_kv8_read(const glt_kv8_cache* c, const glt_kv8_seqs* s, void* k, int64_t k_ld, void* v, int64_t v_ld,
+                        void* stream);
+
+/* Attention of the new tokens over the cache, into which they have been written:
+ * the new token at position p (the prefix's tokens counted) reads the keys at positions
+ *   j <= p  and  (window == 0  or  j > p - window  or  j < sinks).
+ * n_groups > 0: the B sequences come in n_groups groups of B / n_groups, and each
+ * group's share a prefix: prefix_lens[g] (device; clamped to the table) tokens in pages
+ * prefix_pages[g * prefix_ld ..] of the same pool, before their own ones. It is read once
+ * for its group. */
+typedef struct {
+  int32_t n_q_heads;
+  float scale;
+  int32_t window, sinks;
+  int32_t n_groups;
+  const int32_t* prefix_pages;
+  int64_t prefix_ld;
+  int32_t n_prefix_table;
+  const int32_t* prefix_lens;
+} glt_kv8_attn;
+/* out = softmax(scale q . k^T) . v over the visible keys, [B, T, n_q_heads, 128]
+ * bf16 (strides as in glt_attn_desc), lse [B, n_q_heads, T] f32. Scores are products of q
+ * and the codes, scaled in f32; probabilities times the value's step are rounded to bf16 for
+ * the second product; all sums and statistics are f32, in one fixed order. Rows t >=
+ * new_lens[b] get zeros and -inf. |q| < 2^112 (the codes' products stay in f32). q
+ * overlaps neither out, lse nor the workspace, nor any of them each other or the
+ * cache. workspace: glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing
+ * kept in it between calls. */
+size_t glt_kv8_attention_workspace_size(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d);
+glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d, const void* q,
+                             int64_t q_ld, void* out, int64_t o_ld, float* lse, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------- decoder layer */
 /* One decoder layer forward with the grafted MLP (reference forward_layer,
  * src/layer_forward_impl.inc:15-290):
