@@ -148,6 +148,10 @@ SIGNATURES = {
     "glt_attention_train_fwd": (_i32, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
     "glt_attention_bwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc)]),
     "glt_attention_bwd": (_i32, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "glt_attention_window_fwd": (_i32, [ctypes.POINTER(AttnDesc), _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "glt_attention_window_bwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc), _i32, _i32]),
+    "glt_attention_window_bwd": (_i32, [ctypes.POINTER(AttnDesc), _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                        _vp, _vp, _sz, _vp]),
     "glt_kv8_size": (_sz, [_i64, _i32, _i32]),
     "glt_kv8_write": (_i32, [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Seqs), _vp, _i64, _vp, _i64, _vp]),
     "glt_kv8_read": (_i32, [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Seqs), _vp, _i64, _vp, _i64, _vp]),

@@ -73,6 +73,10 @@ struct BwdArgs {
   int64_t q_ld, k_ld, v_ld, o_ld;
   int B, T, Hq, Hkv, causal;
   float scale;
+  // WIN: causal, and of the keys before it a row reads those less than `window`
+  // back and the first `sinks`, which lie in sink_blocks blocks of keys
+  int window, sinks, sink_blocks, sink_cuts;
+  float* sink_part;  // dk, dv of these blocks by query head and cut, [B, Hq, block, cut][2][128][128]
 };
 
 // D of the lane's row: the diagonal of out . dout^T.
@@ -101,6 +105,7 @@ constexpr int kDqAhead = 4, kDkdvAhead = 2, kGradAhead = 2;
 // ------------------------------------------------------------------- dq
 // One workgroup per (batch, query head, block of 128 queries), longest rows
 // first. LDS: two buffers of a K and a V tile (65 KB).
+template <bool WIN>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31, lh = lane >> 5;
@@ -114,7 +119,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const int len = seq_len(a.seq_lens, b, a.T);
   const bool live = myq < len;
   const int kv_end = q0 >= len ? 0 : a.causal ? min(len, q0 + kRows) : len;
-  const int ntiles = (kv_end + kTile - 1) / kTile;
+  const TileWalk<WIN> tiles(q0, (kv_end + kTile - 1) / kTile, a.window, a.sinks);
+  const int ntiles = tiles.n;
   const int64_t tok = (int64_t)b * a.T + min(myq, a.T - 1);
   const int64_t stat = ((int64_t)b * a.Hq + h) * a.T + min(myq, a.T - 1);
 
@@ -124,8 +130,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const uint32_t kof = tile_lane_off(wave, lane, kb_ld), vof = tile_lane_off(wave, lane, vb_ld);
   lds_char* const lds = (lds_char*)smem;
   auto load = [&](int t, lds_char* dst) {
-    load_tile<kWaves>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
-    load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
+    const uint32_t row0 = (uint32_t)tiles.tile(t) * kTile;
+    load_tile<kWaves>(rk, dst, wave, kof, kb_ld, row0 * kb_ld);
+    load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, row0 * vb_ld);
   };
   if (ntiles > 0) load(0, lds);
 
@@ -138,11 +145,21 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const uint32_t ro = row_frag_off(lane), co = col_frag_off(lane);
   const float scale_log2 = a.scale * kLog2e;
 
-  // Score products of key block kb (32 keys) of tile t: p in s, dp.
+  // Score products of key block kb (32 keys) of the walk's tile t: p in s, dp.
   auto probs = [&](int t, int kb, const lds_char* row, f32x16& s, f32x16& dp) {
-    const int key0 = t * kTile + 32 * kb;
+    const int key0 = tiles.tile(t) * kTile + 32 * kb;
     score_product<kDqAhead>(row, qf, s, [](int) {});
-    if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {
+    if (WIN) {
+      if (key0 + 32 > len || key0 + 31 > wq0 || (key0 <= wq0 + 31 - a.window && key0 + 32 > a.sinks)) {
+        const int base = key0 + 4 * lh;
+        const int hi = min(len, myq + 1) - base, lo = myq - a.window + 1 - base, sunk = a.sinks - base;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = 8 * (e >> 2) + (e & 3);
+          s[e] = i < hi && (i >= lo || i < sunk) ? s[e] : -INFINITY;
+        }
+      }
+    } else if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {
       const int lim = (a.causal ? min(len, myq + 1) : len) - (key0 + 4 * lh);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < lim ? s[e] : -INFINITY;
@@ -156,7 +173,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   };
   // Walks the tiles; step u of the workgroup uses buffer u & 1. block(t, kb,
   // row, col) gets each 32-key block that this wavefront's rows read.
-  const int mine = a.causal ? min(ntiles, (wq0 + 31) / kTile + 1) : ntiles;
+  const int mine = !WIN && a.causal ? min(ntiles, (wq0 + 31) / kTile + 1) : ntiles;
   auto walk = [&](int u0, bool last, auto block) {
     auto next = [&](int t, lds_char* wr) {
       if (t + 1 < ntiles) load(t + 1, wr);
@@ -166,8 +183,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
       next(t, wr);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const int key0 = t * kTile + 32 * kb;
-        if (key0 >= kv_end || (a.causal && key0 > wq0 + 31)) continue;
+        const int key0 = tiles.tile(t) * kTile + 32 * kb;
+        if (key0 >= kv_end || (a.causal && key0 > wq0 + 31) || !tiles.wanted(t, wq0, 32, 32 * kb)) continue;
         block(t, kb, rd + opaque(ro + kb * 8 * kGroupB), rd + opaque(co + kb * 8 * kGroupB));
       }
     };
@@ -256,7 +273,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
       for (int i = 0; i < 4; ++i) dq[i] = f32x16{};
     // a row that reads one key has no gradient on its score: not the rounding
     // that the product's order leaves (NaN stays)
-    const bool one = myq == 0 && (a.causal || len == 1);
+    const bool one = (myq == 0 && (a.causal || len == 1)) || (WIN && a.window == 1 && a.sinks == 0);
     store_rows(a.dq + tok * a.q_ld + (int64_t)h * kHd, dq, one ? 0.f : a.scale, lh);
   }
 }
@@ -272,12 +289,36 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
 // on it. The parts cost 49 of 898 us at 2 x 4096 (268 MB written and read).
 constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
 
+//
+// WIN: a block's queries end with its last key's window. A block that holds sinks
+// is read by all queries after that too: they are cut into runs of kSinkTiles
+// tiles, each with a workgroup of its own (launched first) that leaves an f32
+// part, the block's own window being cut 0; attn_sink_sum_kernel adds these parts by
+// head and cut. (Walked by the block's one workgroup they would be the longest
+// chain by far.)
+constexpr int kSinkTiles = 16;
+// Query tiles that the window of the key block from k0 reaches, of `tiles` in all.
+__device__ __forceinline__ int window_tiles(int k0, int window, int tiles) {
+  return min((k0 + kRows - 1 + window + kTile - 1) / kTile, tiles);
+}
+
+template <bool WIN>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
-  const int id = blockIdx.x, hb = id % nhb, kb = id / nhb;
+  const int id = blockIdx.x, hb = id % nhb;
+  int kb = id / nhb, cut = 0;
+  if (WIN && a.sink_blocks) {
+    const int extra = a.sink_blocks * (a.sink_cuts - 1);
+    if (kb < extra) {
+      cut = 1 + kb / a.sink_blocks;
+      kb = kb % a.sink_blocks;
+    } else {
+      kb -= extra;
+    }
+  }
   const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
   const int k0 = kb * kRows, wk0 = k0 + 32 * wave;
   const int len = seq_len(a.seq_lens, b, a.T);
@@ -290,8 +331,20 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
   }
 
   // query tiles of this workgroup
-  const int qt0 = a.causal ? k0 / kTile : 0;
-  const int qt1 = k0 < len ? (len + kTile - 1) / kTile : qt0;
+  int qt0 = a.causal ? k0 / kTile : 0;
+  int qt1 = k0 < len ? (len + kTile - 1) / kTile : qt0;
+  if (WIN && k0 < len) {
+    const int all = qt1, in = window_tiles(k0, a.window, all);
+    if (cut > 0) {
+      qt0 = in + (cut - 1) * kSinkTiles;
+      if (qt0 >= all) return;
+      qt1 = min(qt0 + kSinkTiles, all);
+    } else {
+      qt1 = in;
+    }
+  } else if (WIN && cut > 0) {
+    return;
+  }
   const uint32_t qb_ld = (uint32_t)(a.q_ld * 2), ob_ld = (uint32_t)(a.o_ld * 2);  // bytes
   // rows at or past len read as zeros, lse and D too: p = 1 there, dp - D = 0
   // and dout = 0, so they add nothing
@@ -323,9 +376,16 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
     for (int qb = 0; qb < 2; ++qb) {
       const int q0 = q0t + 32 * qb;
       if (q0 >= len || (a.causal && q0 + 31 < wk0)) continue;
+      if (WIN && q0 >= wk0 + 31 + a.window && wk0 >= a.sinks) continue;
       f32x16 s{}, dp;
       const lds_char* row = rd + opaque(ro + qb * 8 * kGroupB);
       score_product<kDkdvAhead>(row, kf, s, [](int) {});
+      if (WIN && q0 + 31 >= wk0 + a.window && wk0 + 32 > a.sinks) {  // and those that its window leaves
+        const int l = opaque(threadIdx.x) & 63, key = wk0 + (l & 31);
+        const int lim = key < a.sinks ? INT32_MAX : key + a.window - (q0 + 4 * (l >> 5));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < lim ? s[e] : -INFINITY;
+      }
       if (a.causal && q0 < wk0 + 31) {  // row q0 + 8 (e >> 2) + 4 lh + (e & 3) reads keys up to itself
         const int l = opaque(threadIdx.x) & 63;
         const int lim = wk0 + (l & 31) - (q0 + 4 * (l >> 5));
@@ -398,13 +458,21 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
   if (myk >= len)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dk[i] = dv[i] = f32x16{};
-  if (rep == 1) {
+  if (WIN && a.window == 1 && a.sinks == 0)  // rows of a single key, as above
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dk[i] *= 0.f;
+  float *pk, *pv;
+  if (WIN && kb < a.sink_blocks) {
+    pk = a.sink_part + (((((int64_t)b * a.Hq + h) * a.sink_blocks + kb) * a.sink_cuts + cut) * 2 * kRows + (myk - k0)) * kHd + 4 * lh;
+    pv = pk + kRows * kHd;
+  } else if (rep == 1) {
     store_rows(a.dk + tok * a.k_ld + (int64_t)g * kHd, dk, a.scale, lh);
     store_rows(a.dv + tok * a.v_ld + (int64_t)g * kHd, dv, 1.0f, lh);
     return;
+  } else {
+    pk = a.part + (tok * a.Hq + h) * kHd + 4 * lh;
+    pv = pk + (int64_t)a.B * a.T * a.Hq * kHd;
   }
-  float* pk = a.part + (tok * a.Hq + h) * kHd + 4 * lh;
-  float* pv = pk + (int64_t)a.B * a.T * a.Hq * kHd;
 #pragma unroll
   for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -421,6 +489,7 @@ __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
   const int rep = a.Hq / a.Hkv, cols = a.Hkv * (kHd / 8);
   if (i >= (int64_t)a.B * a.T * cols) return;
   const int64_t row = i / cols;
+  if (a.sink_blocks && row % a.T < a.sink_blocks * kRows) return;  // attn_sink_sum_kernel's
   const int c = (int)(i - row * cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
   const float* p = a.part + ((blockIdx.y ? (int64_t)a.B * a.T : 0) + row) * a.Hq * kHd + (int64_t)g * rep * kHd + e;
   f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
@@ -435,12 +504,54 @@ __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
             pack2_rne(y[2] * f, y[3] * f)};
 }
 
+// The keys of the sink blocks: parts added by query head, then by cut.
+__global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
+  const int cols = a.Hkv * (kHd / 8), rows = min(a.sink_blocks * kRows, a.T);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.B * rows * cols) return;
+  const int c = (int)(i % cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
+  const int t = (int)(i / cols % rows), b = (int)(i / cols / rows), kb = t / kRows, rep = a.Hq / a.Hkv;
+  const int len = seq_len(a.seq_lens, b, a.T), k0 = kb * kRows;
+  int cuts = 1;
+  if (k0 < len) {
+    const int all = (len + kTile - 1) / kTile;
+    cuts += (all - window_tiles(k0, a.window, all) + kSinkTiles - 1) / kSinkTiles;
+  }
+  f32x4 x{}, y{};
+  for (int s = 0; s < rep; ++s)
+    for (int cut = 0; cut < cuts; ++cut) {
+      const float* p = a.sink_part +
+                       (((((int64_t)b * a.Hq + g * rep + s) * a.sink_blocks + kb) * a.sink_cuts + cut) * 2 * kRows +
+                        (blockIdx.y ? kRows : 0) + t - k0) * kHd + e;
+      x += *reinterpret_cast<const f32x4*>(p);
+      y += *reinterpret_cast<const f32x4*>(p + 4);
+    }
+  const int64_t row = (int64_t)b * a.T + t;
+  const float f = blockIdx.y ? 1.0f : a.scale;
+  uint16_t* dst = blockIdx.y ? a.dv + row * a.v_ld : a.dk + row * a.k_ld;
+  *reinterpret_cast<u32x4*>(dst + g * kHd + e) =
+      u32x4{pack2_rne(x[0] * f, x[1] * f), pack2_rne(x[2] * f, x[3] * f), pack2_rne(y[0] * f, y[1] * f),
+            pack2_rne(y[2] * f, y[3] * f)};
+}
+
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t stats_bytes(const glt_attn_desc* d) { return round256((size_t)2 * d->B * d->n_q_heads * d->T * sizeof(float)); }
 size_t part_bytes(const glt_attn_desc* d) {
   return d->n_q_heads > d->n_kv_heads ? (size_t)2 * d->B * d->T * d->n_q_heads * kHd * sizeof(float) : 0;
 }
 
+// Blocks of keys that hold sinks, and the cuts that their queries come in at most.
+struct SinkCut { int blocks, cuts; };
+SinkCut sink_cut(const glt_attn_desc* d, int32_t window, int32_t sinks) {
+  if (window <= 0 || sinks <= 0) return {0, 0};
+  const int64_t tiles = cdiv(d->T, kTile), in = std::min<int64_t>(cdiv((int64_t)kRows - 1 + window, kTile), tiles);
+  return {(int)cdiv(std::min(sinks, d->T), kRows), 1 + (int)cdiv(tiles - in, kSinkTiles)};
+}
+size_t sink_bytes(const glt_attn_desc* d, SinkCut c) {
+  return (size_t)d->B * d->n_q_heads * c.blocks * c.cuts * 2 * kRows * kHd * sizeof(float);
+}
+
+template <bool WIN>
 glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   constexpr int kDqLds = 4 * kTileB + 4 * kWaves, kDkdvLds = 2 * kDkdvBuf;
   // the dynamic-LDS limit is a per-device attribute of the kernels
@@ -449,49 +560,48 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   GLT_TRY_HIP(hipGetDevice(&dev));
   GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_attention_bwd: device index %d out of range", dev);
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_dq_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kDqLds));
+    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_dq_kernel<WIN>, hipFuncAttributeMaxDynamicSharedMemorySize, kDqLds));
     GLT_TRY_HIP(
-        hipFuncSetAttribute((const void*)attn_dkdv_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
+        hipFuncSetAttribute((const void*)attn_dkdv_kernel<WIN>, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const unsigned nb = (unsigned)cdiv(a.T, kRows);
-  GLT_LAUNCH("attn_dq", attn_dq_kernel, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDqLds, st, a);
+  GLT_LAUNCH(WIN ? "attn_window_dq" : "attn_dq", attn_dq_kernel<WIN>, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDqLds, st, a);
   GLT_LAUNCH_CHECK("attn_dq");
-  GLT_LAUNCH("attn_dkdv", attn_dkdv_kernel, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDkdvLds, st, a);
+  const unsigned blocks = nb + (WIN && a.sink_blocks ? (unsigned)(a.sink_blocks * (a.sink_cuts - 1)) : 0u);
+  GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", attn_dkdv_kernel<WIN>, dim3(blocks * a.Hq * a.B), dim3(kWaves * 64),
+             kDkdvLds, st, a);
   GLT_LAUNCH_CHECK("attn_dkdv");
   if (a.Hq > a.Hkv) {
     const int64_t chunks = (int64_t)a.B * a.T * a.Hkv * (kHd / 8);
     GLT_LAUNCH("attn_dkdv_sum", attn_dkdv_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
     GLT_LAUNCH_CHECK("attn_dkdv_sum");
   }
+  if (WIN && a.sink_blocks) {
+    const int64_t chunks = (int64_t)a.B * std::min(a.sink_blocks * kRows, a.T) * a.Hkv * (kHd / 8);
+    GLT_LAUNCH("attn_sink_sum", attn_sink_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
+    GLT_LAUNCH_CHECK("attn_sink_sum");
+  }
   return GLT_OK;
 }
 
-}  // namespace
+size_t bwd_bytes(const glt_attn_desc* d, SinkCut c) { return stats_bytes(d) + part_bytes(d) + sink_bytes(d, c); }
 
-}  // namespace glt
-
-using namespace glt;
-
-extern "C" size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d) {
-  if (!d || d->B <= 0 || d->T <= 0 || d->n_q_heads <= 0 || d->n_kv_heads <= 0) return 256;
-  return stats_bytes(d) + part_bytes(d);
-}
-
-extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
-                                        const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                                        void* dv, void* workspace, size_t workspace_bytes, void* stream) {
-  const glt_status s = check_attn_desc(d, "glt_attention_bwd");
-  if (s != GLT_OK) return s;
+glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q, const void* k, const void* v,
+                     const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                     size_t workspace_bytes, void* stream, const char* who) {
   if (d->B == 0 || d->T == 0) return GLT_OK;
-  GLT_CHECK(q && k && v && out && lse && dout && dq && dk && dv, GLT_ERR_INVALID_ARG, "glt_attention_bwd: null pointer");
+  GLT_CHECK(q && k && v && out && lse && dout && dq && dk && dv, GLT_ERR_INVALID_ARG, "%s: null pointer", who);
   const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq |
                         (uintptr_t)dk | (uintptr_t)dv;
   GLT_CHECK(all % 16 == 0 && (uintptr_t)lse % 4 == 0 && (uintptr_t)d->seq_lens % 4 == 0, GLT_ERR_ALIGNMENT,
-            "glt_attention_bwd: tensors must be 16-byte aligned");
-  const size_t need = glt_attention_bwd_workspace_size(d);
+            "%s: tensors must be 16-byte aligned", who);
+  const SinkCut cut = sink_cut(d, window, sinks);
+  GLT_CHECK((cdiv(d->T, kRows) + (int64_t)cut.blocks * cut.cuts) * d->B < (1 << 24) / d->n_q_heads, GLT_ERR_SHAPE,
+            "%s: B=%d T=%d n_q_heads=%d sinks=%d", who, d->B, d->T, d->n_q_heads, sinks);
+  const size_t need = bwd_bytes(d, cut);
   GLT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, GLT_ERR_WORKSPACE,
-            "glt_attention_bwd: needs %zu workspace bytes, 256-byte aligned", need);
+            "%s: needs %zu workspace bytes, 256-byte aligned", who, need);
   // every kernel reads inputs after others have written gradients
   const int64_t tokens = (int64_t)d->B * d->T, nq = 2 * kHd * d->n_q_heads, nk = 2 * kHd * d->n_kv_heads;
   const ByteRows in[] = {{q, tokens, nq, 2 * d->q_ld},   {k, tokens, nk, 2 * d->k_ld},    {v, tokens, nk, 2 * d->v_ld},
@@ -500,9 +610,9 @@ extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, c
                          dense_bytes(workspace, (int64_t)need)};
   for (int i = 0; i < 4; ++i) {
     for (const ByteRows& x : in)
-      GLT_CHECK(!overlap(to[i], x), GLT_ERR_INVALID_ARG, "glt_attention_bwd: gradients and workspace must overlap no input");
+      GLT_CHECK(!overlap(to[i], x), GLT_ERR_INVALID_ARG, "%s: gradients and workspace must overlap no input", who);
     for (int j = 0; j < i; ++j)
-      GLT_CHECK(!overlap(to[i], to[j]), GLT_ERR_INVALID_ARG, "glt_attention_bwd: gradients and workspace must not overlap");
+      GLT_CHECK(!overlap(to[i], to[j]), GLT_ERR_INVALID_ARG, "%s: gradients and workspace must not overlap", who);
   }
   BwdArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -520,5 +630,45 @@ extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, c
   a.q_ld = d->q_ld; a.k_ld = d->k_ld; a.v_ld = d->v_ld; a.o_ld = d->o_ld;
   a.B = d->B; a.T = d->T; a.Hq = d->n_q_heads; a.Hkv = d->n_kv_heads;
   a.causal = d->causal; a.scale = d->scale;
-  return launch_bwd(a, as_stream(stream));
+  a.window = window;
+  a.sinks = sinks;
+  a.sink_blocks = cut.blocks;
+  a.sink_cuts = cut.cuts;
+  a.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(d) + part_bytes(d));
+  return window > 0 ? launch_bwd<true>(a, as_stream(stream)) : launch_bwd<false>(a, as_stream(stream));
+}
+
+}  // namespace
+
+}  // namespace glt
+
+using namespace glt;
+
+extern "C" size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d) {
+  return glt_attention_window_bwd_workspace_size(d, 0, 0);
+}
+
+extern "C" size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks) {
+  if (!d || d->B <= 0 || d->T <= 0 || d->n_q_heads <= 0 || d->n_kv_heads <= 0) return 256;
+  return bwd_bytes(d, window < d->T && sinks <= kMaxSinks ? sink_cut(d, window, sinks) : SinkCut{0, 0});
+}
+
+extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
+                                        const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                        void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  const glt_status s = check_attn_desc(d, "glt_attention_bwd");
+  return s != GLT_OK ? s
+                     : train_bwd(d, 0, 0, q, k, v, out, lse, dout, dq, dk, dv, workspace, workspace_bytes, stream,
+                                 "glt_attention_bwd");
+}
+
+extern "C" glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
+                                               const void* k, const void* v, const void* out, const float* lse,
+                                               const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                               size_t workspace_bytes, void* stream) {
+  glt_status s = check_attn_desc(d, "glt_attention_window_bwd");
+  if (s == GLT_OK) s = check_window(d, &window, &sinks, "glt_attention_window_bwd");
+  return s != GLT_OK ? s
+                     : train_bwd(d, window, sinks, q, k, v, out, lse, dout, dq, dk, dv, workspace, workspace_bytes,
+                                 stream, "glt_attention_window_bwd");
 }

@@ -10,6 +10,9 @@ constexpr int kHd = 128;          // head dimension
 
 // Refuses what no attention training entry point serves (attention_train.hip).
 glt_status check_attn_desc(const glt_attn_desc* d, const char* who);
+// Refuses windows, and sets one that hides nothing to 0 (attention_train.hip).
+constexpr int kMaxSinks = 1024;
+glt_status check_window(const glt_attn_desc* d, int32_t* window, int32_t* sinks, const char* who);
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef uint32_t u32x2a __attribute__((ext_vector_type(2)));
@@ -129,6 +132,30 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ int seq_len(const int32_t* seq_lens, int b, int T) {
   return seq_lens ? min(max(seq_lens[b], 0), T) : T;
 }
+
+// The key tiles that a block of query rows from q0 walks, of `tiles` in all: with a
+// window those that hold sinks and then those from the first row's window on.
+template <bool WIN>
+struct TileWalk {
+  int n, sink_tiles = 0, skipped = 0, window = 0, sinks = 0;
+  __device__ __forceinline__ TileWalk(int q0, int tiles, int w, int s) : n(tiles) {
+    if (!WIN || tiles == 0) return;
+    const int first = max(q0 - w + 1, 0) / kTile;
+    sink_tiles = min((s + kTile - 1) / kTile, first);
+    skipped = first - sink_tiles;
+    n = tiles - skipped;
+    window = w;
+    sinks = s;
+  }
+  __device__ __forceinline__ int tile(int i) const { return WIN && i >= sink_tiles ? i + skipped : i; }
+  // Whether any of the 32 rows from wq0 reads a key of the `keys` ones from the walk's
+  // tile i on (and `from` keys further).
+  __device__ __forceinline__ bool wanted(int i, int wq0, int keys, int from = 0) const {
+    if (!WIN) return true;
+    const int key0 = tile(i) * kTile + from;
+    return key0 <= wq0 + 31 && (key0 + keys > wq0 - window + 1 || key0 < sinks);
+  }
+};
 
 // One tile (64 rows of a head, from byte row0_bytes) into LDS, by this
 // wavefront's share of the 16 loads of 1 KB (a group of four rows each). off:

@@ -57,8 +57,12 @@ struct FwdArgs {
   int64_t q_ld, k_ld, v_ld, o_ld;
   int B, T, Hq, Hkv, causal;
   float scale_log2;
+  int window, sinks;  // WIN
 };
 
+// WIN: causal, and of the keys before it a row reads those less than `window`
+// back and the first `sinks`.
+template <bool WIN>
 __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31, lh = lane >> 5;
@@ -74,7 +78,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
   const int len = seq_len(a.seq_lens, b, a.T);
   const bool live = myq < len;
   const int kv_end = q0 >= len ? 0 : a.causal ? min(len, q0 + kRows) : len;
-  const int ntiles = (kv_end + kTile - 1) / kTile;
+  const TileWalk<WIN> walk(q0, (kv_end + kTile - 1) / kTile, a.window, a.sinks);
+  const int ntiles = walk.n;
   const int64_t tok = (int64_t)b * a.T + min(myq, a.T - 1);
 
   // keys at or past len read as zeros
@@ -84,8 +89,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
   const uint32_t kof = tile_lane_off(wave, lane, kb_ld), vof = tile_lane_off(wave, lane, vb_ld);
   lds_char* const lds = (lds_char*)smem;
   auto load = [&](int t, lds_char* dst) {
-    load_tile<kWaves>(rk, dst, wave, kof, kb_ld, (uint32_t)t * kTile * kb_ld);
-    load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, (uint32_t)t * kTile * vb_ld);
+    const uint32_t row0 = (uint32_t)walk.tile(t) * kTile;
+    load_tile<kWaves>(rk, dst, wave, kof, kb_ld, row0 * kb_ld);
+    load_tile<kWaves>(rv, dst + kTileB, wave, vof, vb_ld, row0 * vb_ld);
   };
   if (ntiles > 0) load(0, lds);
 
@@ -100,10 +106,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
   // output's product uses (its divisor), sum of the unrounded ones (lse's)
   float m_run = -3.0e38f, l_run = 0.f, l_exact = 0.f;
 
-  // tile t, in rd (K, V); tile t + 1 into wr
+  // the walk's tile t, in rd (K, V); tile t + 1 into wr
   auto step = [&](int t, const lds_char* __restrict__ rd, lds_char* __restrict__ wr) {
     if (t + 1 < ntiles) load(t + 1, wr);
-    const int key0 = t * kTile;
+    const int key0 = walk.tile(t) * kTile;
     const lds_char *row = rd + opaque(ro), *col = rd + opaque(co);
     f32x16 s[2] = {f32x16{}, f32x16{}};  // key blocks 0, 1
     {
@@ -120,8 +126,22 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
       }
     }
     // Masked with -inf, which no scale lifts; a live row's first tile holds a
-    // key that it may read, so its running maximum is finite from then on.
-    if (key0 + kTile > len || (a.causal && key0 + kTile - 1 > wq0)) {
+    // key that it may read, so its running maximum is finite from then on. (With
+    // a window it may not: the maximum stays where it starts and the
+    // probabilities are zeros.)
+    if (WIN) {
+      if (key0 + kTile > len || key0 + kTile - 1 > wq0 || (key0 <= wq0 + 31 - a.window && key0 + kTile > a.sinks)) {
+        const int base = key0 + 4 * lh;
+        const int hi = min(len, myq + 1) - base, lo = myq - a.window + 1 - base, sunk = a.sinks - base;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i = 32 * kb + 8 * (e >> 2) + (e & 3);
+            s[kb][e] = i < hi && (i >= lo || i < sunk) ? s[kb][e] : -INFINITY;
+          }
+      }
+    } else if (key0 + kTile > len || (a.causal && key0 + kTile - 1 > wq0)) {
       const int lim = (a.causal ? min(len, myq + 1) : len) - (key0 + 4 * lh);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -178,12 +198,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
       __builtin_amdgcn_s_setprio(0);
     }
   };
-  const int mine = a.causal ? min(ntiles, (wq0 + 31) / kTile + 1) : ntiles;  // tiles that this wavefront's rows read
+  const int mine = !WIN && a.causal ? min(ntiles, (wq0 + 31) / kTile + 1) : ntiles;  // tiles that this wavefront's rows read
   for (int t = 0; t < ntiles; ++t) {
     __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
     phase_barrier();  // tile t is whole, and every wavefront is done with tile t - 1
     lds_char *x = lds + (t & 1) * 2 * kTileB, *y = lds + (~t & 1) * 2 * kTileB;
-    if (t < mine) step(t, x, y);
+    if (t < mine && walk.wanted(t, wq0, kTile)) step(t, x, y);
     else if (t + 1 < ntiles) load(t + 1, y);
   }
 
@@ -228,35 +248,41 @@ glt_status check_attn_desc(const glt_attn_desc* d, const char* who) {
   return GLT_OK;
 }
 
-}  // namespace glt
+// Windows and sinks within a sequence of T; window 0 where it hides nothing.
+glt_status check_window(const glt_attn_desc* d, int32_t* window, int32_t* sinks, const char* who) {
+  GLT_CHECK(*window >= 1 && *sinks >= 0 && *sinks <= kMaxSinks, GLT_ERR_INVALID_ARG,
+            "%s: window %d (at least 1), sinks %d (0 to %d)", who, *window, *sinks, kMaxSinks);
+  GLT_CHECK(d->causal, GLT_ERR_UNSUPPORTED, "%s: a window is causal", who);
+  if (*window >= d->T) *window = *sinks = 0;
+  return GLT_OK;
+}
 
-using namespace glt;
+namespace {
 
-extern "C" glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
-                                              void* out, float* lse, void* stream) {
-  const glt_status s = check_attn_desc(d, "glt_attention_train_fwd");
-  if (s != GLT_OK) return s;
+glt_status train_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q, const void* k, const void* v,
+                     void* out, float* lse, void* stream, const char* who) {
   if (d->B == 0 || d->T == 0) return GLT_OK;
-  GLT_CHECK(q && k && v && out && lse, GLT_ERR_INVALID_ARG, "glt_attention_train_fwd: null pointer");
+  GLT_CHECK(q && k && v && out && lse, GLT_ERR_INVALID_ARG, "%s: null pointer", who);
   GLT_CHECK(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0 && (uintptr_t)lse % 4 == 0 &&
                 (uintptr_t)d->seq_lens % 4 == 0,
-            GLT_ERR_ALIGNMENT, "glt_attention_train_fwd: tensors must be 16-byte aligned");
+            GLT_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", who);
   // workgroups read keys and values that others' rows are written beside; a
   // query row is read by its own workgroup alone, before it writes
   const int64_t tokens = (int64_t)d->B * d->T, nq = 2 * kHd * d->n_q_heads, nk = 2 * kHd * d->n_kv_heads;
   const ByteRows rq{q, tokens, nq, 2 * d->q_ld}, rk{k, tokens, nk, 2 * d->k_ld}, rv{v, tokens, nk, 2 * d->v_ld},
       ro{out, tokens, nq, 2 * d->o_ld}, rl = dense_bytes(lse, tokens * d->n_q_heads * 4);
   GLT_CHECK(!overlap(ro, rk) && !overlap(ro, rv) && ((out == q && d->o_ld == d->q_ld) || !overlap(ro, rq)),
-            GLT_ERR_INVALID_ARG, "glt_attention_train_fwd: out must overlap no input (but q itself)");
+            GLT_ERR_INVALID_ARG, "%s: out must overlap no input (but q itself)", who);
   GLT_CHECK(!overlap(rl, rq) && !overlap(rl, rk) && !overlap(rl, rv) && !overlap(rl, ro), GLT_ERR_INVALID_ARG,
-            "glt_attention_train_fwd: lse must overlap no other tensor");
+            "%s: lse must overlap no other tensor", who);
   // the dynamic-LDS limit is a per-device attribute of the kernel
   static std::atomic<bool> attr_set[64];
   int dev = 0;
   GLT_TRY_HIP(hipGetDevice(&dev));
-  GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "glt_attention_train_fwd: device index %d out of range", dev);
+  GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "%s: device index %d out of range", who, dev);
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_train_fwd_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+    for (const void* f : {(const void*)attn_train_fwd_kernel<false>, (const void*)attn_train_fwd_kernel<true>})
+      GLT_TRY_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
     attr_set[dev].store(true, std::memory_order_release);
   }
   FwdArgs a{};
@@ -269,8 +295,34 @@ extern "C" glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void
   a.q_ld = d->q_ld; a.k_ld = d->k_ld; a.v_ld = d->v_ld; a.o_ld = d->o_ld;
   a.B = d->B; a.T = d->T; a.Hq = d->n_q_heads; a.Hkv = d->n_kv_heads; a.causal = d->causal;
   a.scale_log2 = d->scale * kLog2e;
+  a.window = window;
+  a.sinks = sinks;
   const int64_t nblk = cdiv(d->T, kRows) * d->n_q_heads * d->B;
-  GLT_LAUNCH("attention_train", attn_train_fwd_kernel, dim3((unsigned)nblk), dim3(kWaves * 64), kLds, as_stream(stream), a);
+  if (window > 0)
+    GLT_LAUNCH("attention_window", attn_train_fwd_kernel<true>, dim3((unsigned)nblk), dim3(kWaves * 64), kLds,
+               as_stream(stream), a);
+  else
+    GLT_LAUNCH("attention_train", attn_train_fwd_kernel<false>, dim3((unsigned)nblk), dim3(kWaves * 64), kLds,
+               as_stream(stream), a);
   GLT_LAUNCH_CHECK("attention_train");
   return GLT_OK;
+}
+
+}  // namespace
+
+}  // namespace glt
+
+using namespace glt;
+
+extern "C" glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
+                                              void* out, float* lse, void* stream) {
+  const glt_status s = check_attn_desc(d, "glt_attention_train_fwd");
+  return s != GLT_OK ? s : train_fwd(d, 0, 0, q, k, v, out, lse, stream, "glt_attention_train_fwd");
+}
+
+extern "C" glt_status glt_attention_window_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
+                                               const void* k, const void* v, void* out, float* lse, void* stream) {
+  glt_status s = check_attn_desc(d, "glt_attention_window_fwd");
+  if (s == GLT_OK) s = check_window(d, &window, &sinks, "glt_attention_window_fwd");
+  return s != GLT_OK ? s : train_fwd(d, window, sinks, q, k, v, out, lse, stream, "glt_attention_window_fwd");
 }

@@ -365,22 +365,25 @@ def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
     return d, (B, T, Hq, kshape[2], hd), lds
 
 
-def attention_train(q, k, v, causal=True, scale=None, seq_lens=None):
+def attention_train(q, k, v, causal=True, scale=None, seq_lens=None, window=None, sinks=0):
     """GQA attention forward of a training step: (out [B,T,Hq,hd] bf16, lse
     [B,Hq,T] f32) for attention_bwd. q [B,T,Hq,hd], k/v [B,T,Hkv,hd] bf16, also
     as views of one projection output [B,T,(Hq+2Hkv)*hd]. seq_lens int32 [B]:
-    the lengths of a padded batch (rows past them: zero output, lse -inf)."""
+    the lengths of a padded batch (rows past them: zero output, lse -inf).
+    window=W: of the keys up to itself a row reads the last W (its own among
+    them) and the first `sinks` of its sequence."""
+    _need(sinks == 0 or window is not None, "sinks: with a window")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     d, (B, T, Hq, _, _), _ = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
     lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device)
-    _call_on(q, "glt_attention_train_fwd", ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-             lse.data_ptr())
+    name, sight = ("glt_attention_train_fwd", ()) if window is None else ("glt_attention_window_fwd", (window, sinks))
+    _call_on(q, name, ctypes.byref(d), *sight, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
     return out, lse
 
 
 @functools.lru_cache(maxsize=256)
-def _attention_bwd_size(B, T, Hq, Hkv, hd):
-    return F.load().glt_attention_bwd_workspace_size(ctypes.byref(F.AttnDesc(B, T, Hq, Hkv, hd)))
+def _attention_bwd_size(B, T, Hq, Hkv, hd, window=0, sinks=0):
+    return F.load().glt_attention_window_bwd_workspace_size(ctypes.byref(F.AttnDesc(B, T, Hq, Hkv, hd)), window, sinks)
 
 
 def _attn_grad_buffers(q, k, v, shape, lds):
@@ -400,11 +403,13 @@ def _attn_grad_buffers(q, k, v, shape, lds):
             for t, n in ((q, ld), (k, k_ld), (v, v_ld))]
 
 
-def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=None, grads=None, workspace=None):
-    """(dq, dk, dv) of attention_train, bf16 with the strides of q, k, v (parts
+def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=None, grads=None, workspace=None, window=None,
+                  sinks=0):
+    """(dq, dk, dv) of attention_train (with its window and sinks), bf16 with the strides of q, k, v (parts
     of one buffer where q, k, v are; `grads` gives them, overlapping no input).
     out and lse are the forward's; dout has out's shape and strides. workspace: a uint8 tensor of
-    glt_attention_bwd_workspace_size bytes to use instead of a new one."""
+    glt_attention_bwd_workspace_size (glt_attention_window_bwd_workspace_size) bytes to use instead of a new one."""
+    _need(sinks == 0 or window is not None, "sinks: with a window")
     d, shape, lds = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
     B, T, Hq, _, _ = shape
     dev = q.device
@@ -416,9 +421,10 @@ def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=Non
     else:
         for n, t, x, ld in zip(("dq", "dk", "dv"), grads, (q, k, v), lds):
             _need(t.shape == x.shape and _heads_ld(n, t, B, T, dev) == ld, "dq, dk, dv: the shapes and strides of q, k, v")
-    workspace = _workspace(workspace, _attention_bwd_size(*shape), dev)
+    name, sight = ("glt_attention_bwd", ()) if window is None else ("glt_attention_window_bwd", (window, sinks))
+    workspace = _workspace(workspace, _attention_bwd_size(*shape, *sight), dev)
     dq, dk, dv = grads
-    _call_on(q, "glt_attention_bwd", ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+    _call_on(q, name, ctypes.byref(d), *sight, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
              lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(),
              workspace.numel())
     return dq, dk, dv

@@ -399,6 +399,20 @@ glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* 
                              const void* out, const float* lse, const void* dout, void* dq, void* dk,
                              void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same with a window: row t reads, of the keys up to itself, those less than
+ * `window` (at least 1) back and the first `sinks` (0 to 1024) of its sequence; d->causal
+ * is 1. A window of T or more gives glt_attention_train_fwd's results. Tiles of 64 keys
+ * that no row of a block reads are not visited: the work is T * (window + sinks), not T^2. */
+glt_status glt_attention_window_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
+                                    const void* k, const void* v, void* out, float* lse, void* stream);
+/* Its backward, as glt_attention_bwd. The gradients of the sinks' keys are added from
+ * every row of their sequence, in one fixed order. */
+size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks);
+glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
+                                    const void* k, const void* v, const void* out, const float* lse,
+                                    const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------ keys and values in 8 bits */
 /* The cache of one layer's keys and values for generation: a pool of pages of 64
  * tokens, glt_kv8_size bytes (260 a token and kv head, of 512 in bf16), 16-byte

@@ -1,0 +1,57 @@
+"""Refusals and sizes of attention for training with a window (CPU)."""
+import ctypes
+
+import pytest
+
+from glt_amd import _ffi as F
+from test_attention_train_host import P, desc, spread
+
+
+def fwd(d, window=8, sinks=2, **at):
+    a = {n: v for n, v in spread(**at).items() if n in ("q", "k", "v", "out", "lse")}
+    return F.load().glt_attention_window_fwd(ctypes.byref(d) if d else None, window, sinks, *a.values(), None)
+
+
+def bwd(d, window=8, sinks=2, nbytes=1 << 31, **at):
+    a = spread(**at)
+    ws = a.pop("ws")
+    return F.load().glt_attention_window_bwd(ctypes.byref(d) if d else None, window, sinks, *a.values(), ws, nbytes, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(window=0), 1), (dict(window=-5), 1), (dict(sinks=-1), 1), (dict(sinks=1025), 1),
+    (dict(d=desc(causal=0)), 9), (dict(d=desc(head_dim=64)), 9), (dict(d=desc(n_q_heads=5)), 2),
+    (dict(d=desc(q_ld=504)), 2), (dict(d=None), 1), (dict(q=None), 1), (dict(out=(1 << 32) + 8), 4),
+])
+def test_refusals(kw, code):
+    kw = {"d": desc(), **kw}
+    assert fwd(**kw) == code
+    assert bwd(**kw) == code
+
+
+def test_overlaps_are_refused():
+    assert fwd(desc(), out=2 << 32) == 1 and fwd(desc(), lse=1 << 32) == 1
+    assert bwd(desc(), dq=2 << 32) == 1 and bwd(desc(), ws=9 << 32) == 1
+
+
+def test_workspace():
+    lib = F.load()
+
+    def size(d, window, sinks):
+        return lib.glt_attention_window_bwd_workspace_size(ctypes.byref(d), window, sinks)
+    d = desc(T=2000)
+    plain = lib.glt_attention_bwd_workspace_size(ctypes.byref(d))
+    assert size(d, 100, 0) == size(d, 2000, 9) == size(d, 0, 0) == plain
+    # the parts of a block of 128 keys by head, its window and the queries after it 1024 by 1024
+    one = 2 * 4 * 2 * 128 * 128 * 4
+    assert size(d, 100, 1) == size(d, 100, 128) == plain + 3 * one
+    assert size(d, 100, 129) == plain + 6 * one
+    assert bwd(d, 100, 1, nbytes=plain + 3 * one - 1) == 5
+    assert bwd(d, 100, 1, ws=None) == 5
+    assert lib.glt_attention_window_bwd_workspace_size(None, 1, 1) == 256
+
+
+def test_empty_batches_need_nothing():
+    for kw in (dict(B=0), dict(T=0)):
+        assert fwd(desc(**kw), q=None, k=None, v=None, out=None, lse=None) == 0
+        assert bwd(desc(**kw), ws=None, nbytes=0) == 0
