@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int i = 8 * (e >> 2) + (e & 3);
-          s[e] = i < hi && (i >= lo || i < sunk) ? s[e] : -INFINITY;
+          s[e] = (i < hi) & ((i >= lo) | (i < sunk)) ? s[e] : -INFINITY;
         }
       }
     } else if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int i = 32 * kb + 8 * (e >> 2) + (e & 3);
-            s[kb][e] = i < hi && (i >= lo || i < sunk) ? s[kb][e] : -INFINITY;
+            s[kb][e] = (i < hi) & ((i >= lo) | (i < sunk)) ? s[kb][e] : -INFINITY;
           }
       }
     } else if (key0 + kTile > len || (a.causal && key0 + kTile - 1 > wq0)) {

@@ -7,13 +7,10 @@
 //   s = (q . code_k) step_k scale,   o += (p step_v) . code_v
 // need one rounding, of p step_v, and no value of k or v is formed.
 //
-// Segments are cut into pieces of a fixed number of pages, which depends on the
-// sizes of the call alone; a piece's output, maximum and sum go into the workspace
-// and a last kernel joins each row's pieces in order: results do not depend on the
-// other sequences of the call, nor on the run.
-//
-// Few rows a segment (new tokens x query heads of a kv head: kv8_few_kernel) or
-// many (kv8_many_kernel); the comments are at the kernels.
+// A segment's keys are cut into pieces; a piece's output, maximum and sum go into the
+// workspace, and a last kernel joins each row's pieces in order. Few rows a segment
+// (new tokens x query heads of a kv head: kv8_few_kernel) or many
+// (kv8_many_kernel); how each is cut stands there.
 #include <algorithm>
 #include <atomic>
 
@@ -42,12 +39,14 @@ struct DecArgs {
   uint16_t* out;
   float* lse;
   int64_t q_ld, o_ld;
-  // [0] the sequences' own tokens, [1] prefixes: pages of a piece, pieces that a
-  // segment has at most, rows of a segment and head, and the pieces' results
-  // [segment][head][piece][row]
-  int chunk[2], n_max[2], rows[2];
-  float* part_o[2];  // 128 each
-  float* part_m[2];  // maximum (log2 units) and sum
+  // [0] the sequences' own tokens, [1] prefixes: rows of a segment and head, pages
+  // of a piece (1: kv8_few_kernel cuts by itself), pieces that a segment has at most,
+  // and the pieces' results by slot and row
+  int rows[2], chunk[2], n_max[2];
+  int workers[2];      // wavefronts of kv8_few_kernel, 0 where kv8_many_kernel runs
+  int* first[2];       // its pages before each segment, and in all
+  float* part_o[2];    // 128 each
+  float* part_m[2];    // maximum (log2 units) and sum
 };
 
 __device__ __forceinline__ int prefix_len(const DecArgs& a, int b) {
@@ -64,14 +63,14 @@ template <bool PRE>
 __device__ __forceinline__ Sight sight(const DecArgs& a, int seg) {
   int hi, lo = 0, sunk = 0;
   if (PRE) {
-    const int P = min(max(a.plens[seg], 0), a.n_prefix_table * kPage);
-    int from = INT32_MAX;  // the earliest new token of the group
-    for (int b = seg * a.gs; b < (seg + 1) * a.gs; ++b) {
-      const Kv8Len n = kv8_len(a.s, b);
-      if (n.fresh > 0) from = min(from, P + n.len - n.fresh);
-    }
-    hi = from == INT32_MAX ? 0 : P;
-    if (a.W && hi) {
+    hi = min(max(a.plens[seg], 0), a.n_prefix_table * kPage);
+    if (a.W) {
+      int from = INT32_MAX;  // the earliest new token of the group
+      for (int b = seg * a.gs; b < (seg + 1) * a.gs; ++b) {
+        const Kv8Len n = kv8_len(a.s, b);
+        if (n.fresh > 0) from = min(from, hi + n.len - n.fresh);
+      }
+      if (from == INT32_MAX) hi = 0;
       lo = max(from - a.W + 1, 0);
       sunk = min(a.S, hi);
     }
@@ -143,28 +142,30 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
 }
 
 // -------------------------------------------------------------- few rows
-// Up to 16 NB rows a segment and head. A wavefront takes whole pages of a piece: it
-// loads a page's codes with 16-byte loads straight into the operands of
+// Up to 16 NB rows a segment and head. The pages that the segments' rows see, of all
+// heads, are one list, of which each wavefront takes an equal run whatever the
+// lengths; where a run enters another segment or head, a piece ends. A wavefront loads a
+// page's codes with 16-byte loads straight into the operands of
 //   S^T[key][row] = K . Q^T,  O^T[channel][row] += V^T . P^T
-// (16 x 16 x 32), with the softmax between: no LDS, and every code is converted once.
-// The four wavefronts' results meet in LDS at the piece's end.
+// (16 x 16 x 32), with the softmax between: no LDS, no barrier, and every code is
+// converted once.
 //
 // Lane l: row l & 15 of a block of 16, g = l >> 4. The keys of score block (beta, a) are
 // numbered so that the accumulators are the second product's operand as they stand:
 // element e of lane group g is key 16 g + 8 a + 4 beta + e of the page.
 constexpr int kFewWaves = 4;
-constexpr int few_lds(int nb) { return 2 * nb * (16 * kKv8Hd * 4 + 128); }
+
+// Pages of a wavefront's run.
+__device__ __forceinline__ int run_pages(int total, int workers) { return max((total + workers - 1) / workers, 1); }
 
 template <int NB, bool PRE>
-__global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // few_lds(NB), then the segments' first pieces
-  int* const first = reinterpret_cast<int*>(smem + few_lds(NB));
+__global__ void __launch_bounds__(kFewWaves * 64, NB == 1 ? 3 : 2) kv8_few_kernel(const DecArgs a) {
+  extern __shared__ int first[];  // pages before each segment, and in all
   __shared__ int wave_sum[kFewWaves];
   const int tid = threadIdx.x, lane = tid & 63, r15 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n_seg = PRE ? a.n_groups : a.s.B, R = a.rows[PRE];
 
-  // pieces before each segment
   int total = 0;
   for (int s0 = 0; s0 < n_seg; s0 += kFewWaves * 64) {
     const int s = s0 + tid, n = s < n_seg ? sight<PRE>(a, s).n : 0;
@@ -185,26 +186,37 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArg
     if (s < n_seg) first[s] = before + x - n;
     __syncthreads();
   }
+  total = __builtin_amdgcn_readfirstlane(total);
+  if (blockIdx.x == 0) {  // for the join
+    for (int s = tid; s < n_seg; s += kFewWaves * 64) a.first[PRE][s] = first[s];
+    if (tid == 0) a.first[PRE][n_seg] = total;
+  }
 
-  for (int unit = blockIdx.x; unit < total * a.Hkv; unit += gridDim.x) {
-    const int h = unit % a.Hkv, at = unit / a.Hkv;
-    int seg = 0;  // the last segment that starts at or before `at`
+  const int worker = blockIdx.x * kFewWaves + wave, all = total * a.Hkv, run = run_pages(all, a.workers[PRE]);
+  int at = worker * run;  // workers * run stays below all + workers
+  const int stop = min(at + run, all);
+  while (at < stop) {
+    const int h = at / total, pos = at - h * total;
+    int seg = 0;  // the last segment that starts at or before pos
     for (int end = n_seg; end - seg > 1;) {
       const int mid = (seg + end) >> 1;
-      if (first[mid] <= at) seg = mid;
+      if (__builtin_amdgcn_readfirstlane(first[mid]) <= pos) seg = mid;
       else end = mid;
     }
     const Sight si = sight<PRE>(a, seg);
-    const int piece = at - first[seg], chunk = si.chunk_at(piece);
-    const int p_end = min((chunk + 1) * a.chunk[PRE], (si.hi + kPage - 1) / kPage);
+    const int i0 = pos - __builtin_amdgcn_readfirstlane(first[seg]), i1 = min(si.n, i0 + stop - at);  // of the segment's list
+    at += i1 - i0;
 
+    // (what depends on the lane is worked out for each run: kept, it costs registers
+    // that there are not)
+    const int l1 = (int)opaque(threadIdx.x) & 63;
     Row row[NB];
     bf16x8 qf[NB][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int r = 16 * nb + r15;
+      const int r = 16 * nb + (l1 & 15);
       row[nb] = row_of<PRE>(a, seg, h, min(r, R - 1), si.hi);
-      const uint16_t* qp = a.q + row[nb].q_row * a.q_ld + (int64_t)row[nb].head * kKv8Hd + 16 * g;
+      const uint16_t* qp = a.q + row[nb].q_row * a.q_ld + (int64_t)row[nb].head * kKv8Hd + 16 * (l1 >> 4);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         qf[nb][s] = __builtin_bit_cast(bf16x8, row[nb].hi > 0 ? *reinterpret_cast<const u32x4*>(qp + 64 * (s >> 1) + 8 * (s & 1))
@@ -220,22 +232,29 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArg
       for (int i = 0; i < 8; ++i) o[nb][i] = f32x4{};
     }
 
-    for (int p = chunk * a.chunk[PRE] + wave; p < p_end; p += kFewWaves) {
-      int64_t id = __builtin_amdgcn_readfirstlane((int)page_id<PRE>(a, seg, p));
+    int ids = 0;  // lane x: the id of the run's page i0 + x, 64 at a time
+    for (int i = i0; i < i1; ++i) {
+      const int x = (i - i0) & 63;
+      if (x == 0) ids = i + lane < i1 ? (int)page_id<PRE>(a, seg, si.chunk_at(i + lane)) : 0;
+      const int64_t id = __builtin_amdgcn_readlane(ids, x);
+      const int p = si.chunk_at(i);
       const bool ok = id >= 0 && id < a.n_pages;
       const uint8_t* pg = a.cache + ((ok ? id : 0) * a.Hkv + h) * kHeadB;
       u32x4 kx[8], vx[8], kst[2], vst[2];
-      const uint8_t* kp = pg + (16 * (r15 >> 2) + (r15 & 3)) * kKv8Hd + 16 * g;
+      const uint8_t* kp = pg + (uint32_t)((16 * (r15 >> 2) + (r15 & 3)) * kKv8Hd + 16 * g);
 #pragma unroll
       for (int i = 0; i < 8; ++i)  // block (beta = i >> 2, a = (i >> 1) & 1), channels 64 (i & 1) + 16 g ..
         kx[i] = *reinterpret_cast<const u32x4*>(kp + (8 * ((i >> 1) & 1) + 4 * (i >> 2)) * kKv8Hd + 64 * (i & 1));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        kst[i] = *reinterpret_cast<const u32x4*>(pg + kKStepOff + 32 * g + 16 * i);
-        vst[i] = *reinterpret_cast<const u32x4*>(pg + kVStepOff + 32 * g + 16 * i);
+        kst[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kKStepOff + 32 * g + 16 * i));
+        vst[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVStepOff + 32 * g + 16 * i));
       }
+      auto load_v = [&](int from, int to) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) vx[i] = *reinterpret_cast<const u32x4*>(pg + kVOff + (16 * i + r15) * kPage + 16 * g);
+        for (int i = from; i < to; ++i) vx[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + (16 * i + r15) * kPage + 16 * g));
+      };
+      if (NB == 1) load_v(0, 8);
       if (!ok)
 #pragma unroll
         for (int i = 0; i < 2; ++i) kst[i] = vst[i] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
@@ -257,6 +276,11 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArg
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) s[nb][blk] = mfma16(ka, qf[nb][st], s[nb][blk]);
         }
+        if (NB > 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (NB > 1) {  // no registers for both, nor for all of v
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(0, 4);
       }
       bf16x8 pf[NB][2];
 #pragma unroll
@@ -269,19 +293,15 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArg
         for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nb][blk][e] *= step(kst, 8 * (blk & 1) + 4 * (blk >> 1) + e) * a.scale_log2;
-        uint32_t seen = 0xffff;
-        if (!whole) {
-          seen = 0;
+        if (!whole)
 #pragma unroll
           for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = key0 + 8 * (blk & 1) + 4 * (blk >> 1) + e;
-              const bool in = j < w.hi && (j >= w.lo || j < w.sunk);
+              const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
               s[nb][blk][e] = in ? s[nb][blk][e] : -INFINITY;
-              seen |= in ? 1u << (4 * blk + e) : 0u;
             }
-        }
         float mt = s[nb][0][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mt = fmax_nc(mt, s[nb][i >> 2][i & 3]);
@@ -303,7 +323,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArg
         }
         if (!whole)  // an unseen key's step may be anything
 #pragma unroll
-          for (int i = 0; i < 16; ++i) pv[i] = seen >> i & 1 ? pv[i] : 0.f;
+          for (int i = 0; i < 16; ++i) pv[i] = s[nb][i >> 2][i & 3] == -INFINITY ? 0.f : pv[i];
 #pragma unroll
         for (int beta = 0; beta < 2; ++beta) {
           const float* x = pv + 8 * beta;
@@ -312,70 +332,30 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) kv8_few_kernel(const DecArg
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        if (NB > 1 && i == 0) load_v(4, 8);
 #pragma unroll
         for (int beta = 0; beta < 2; ++beta) {
           const bf16x8 va = codes8(vx[i][2 * beta], vx[i][2 * beta + 1]);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) o[nb][i] = mfma16(va, pf[nb][beta], o[nb][i]);
         }
+      }
     }
 
-    // join the wavefronts: 2 and 3 into 0 and 1, 1 into 0
-    float l[NB];
+    const int l2 = (int)opaque(threadIdx.x) & 63, c15 = l2 & 15, cg = l2 >> 4;
+    const int64_t slot = (int64_t)worker + (int64_t)h * n_seg + seg;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) l[nb] = quad_sum(l_run[nb]);
-    char* const buf = smem + (wave & 1) * NB * (16 * kKv8Hd * 4 + 128);
-    auto put = [&] {
+    for (int nb = 0; nb < NB; ++nb) {
+      const float l = quad_sum(l_run[nb]);
+      const int r = 16 * nb + c15;
+      if (r < R) {
+        float* to = a.part_o[PRE] + (slot * R + r) * kKv8Hd + 4 * cg;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float* to = reinterpret_cast<float*>(buf) + nb * 16 * kKv8Hd + lane * 4;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<f32x4*>(to + 256 * i) = o[nb][i];
-        if (g < 2) reinterpret_cast<float*>(buf + NB * 16 * kKv8Hd * 4)[nb * 32 + lane] = g ? l[nb] : m_run[nb];
-      }
-    };
-    auto take = [&] {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float* from = reinterpret_cast<const float*>(buf) + nb * 16 * kKv8Hd + lane * 4;
-        const float* ml = reinterpret_cast<const float*>(buf + NB * 16 * kKv8Hd * 4) + nb * 32 + r15;
-        const float m2 = ml[0], m = fmax_nc(m_run[nb], m2);
-        const float f1 = __builtin_amdgcn_exp2f(m_run[nb] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
-        l[nb] = l[nb] * f1 + ml[16] * f2;
-        m_run[nb] = m;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[nb][i] = o[nb][i] * f1 + *reinterpret_cast<const f32x4*>(from + 256 * i) * f2;
-      }
-    };
-    __syncthreads();  // the unit before is done with the buffers
-    if (wave >= 2) put();
-    __syncthreads();
-    if (wave < 2) take();
-    __syncthreads();
-    if (wave == 1) put();
-    __syncthreads();
-    if (wave == 0) {
-      // wave 1's buffer
-      const char* b1 = smem + NB * (16 * kKv8Hd * 4 + 128);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float* from = reinterpret_cast<const float*>(b1) + nb * 16 * kKv8Hd + lane * 4;
-        const float* ml = reinterpret_cast<const float*>(b1 + NB * 16 * kKv8Hd * 4) + nb * 32 + r15;
-        const float m2 = ml[0], m = fmax_nc(m_run[nb], m2);
-        const float f1 = __builtin_amdgcn_exp2f(m_run[nb] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
-        const float lt = l[nb] * f1 + ml[16] * f2;
-        const int r = 16 * nb + r15;
-        if (r < R) {
-          const int64_t slot = (((int64_t)seg * a.Hkv + h) * a.n_max[PRE] + piece) * R + r;
-          float* to = a.part_o[PRE] + slot * kKv8Hd + 4 * g;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<f32x4*>(to + 16 * i) = o[nb][i] * f1 + *reinterpret_cast<const f32x4*>(from + 256 * i) * f2;
-          if (g == 0) {
-            a.part_m[PRE][2 * slot] = m;
-            a.part_m[PRE][2 * slot + 1] = lt;
-          }
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<f32x4*>(to + 16 * i) = o[nb][i];
+        if (cg == 0) {
+          a.part_m[PRE][2 * (slot * R + r)] = m_run[nb];
+          a.part_m[PRE][2 * (slot * R + r) + 1] = l;
         }
       }
     }
@@ -491,19 +471,15 @@ __global__ void __launch_bounds__(kManyWaves * 64, 2) kv8_many_kernel(const DecA
         for (int e = 0; e < 4; ++e) s[kb][4 * i + e] *= f[e];
       }
     const bool whole = __all(!live || (key0 + kPage <= w.hi && (key0 >= w.lo || key0 + kPage <= w.sunk)));
-    uint32_t seen = 0xffffffffu;
-    if (!whole) {
-      seen = 0;
+    if (!whole)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int j = key0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
-          const bool in = j < w.hi && (j >= w.lo || j < w.sunk);
+          const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
           s[kb][e] = in ? s[kb][e] : -INFINITY;
-          seen |= in ? 1u << (16 * kb + e) : 0u;
         }
-    }
     float m2[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -535,7 +511,7 @@ __global__ void __launch_bounds__(kManyWaves * 64, 2) kv8_many_kernel(const DecA
         }
         if (!whole)  // an unseen key's step may be anything
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = seen >> (16 * kb + 4 * i + e) & 1 ? x[e] : 0.f;
+          for (int e = 0; e < 4; ++e) x[e] = s[kb][4 * i + e] == -INFINITY ? 0.f : x[e];
         pw[2 * kb + (i >> 1)][2 * (i & 1)] = pack2_rne(x[0], x[1]);
         pw[2 * kb + (i >> 1)][2 * (i & 1) + 1] = pack2_rne(x[2], x[3]);
       }
@@ -573,48 +549,81 @@ __global__ void __launch_bounds__(kManyWaves * 64, 2) kv8_many_kernel(const DecA
 }
 
 // ------------------------------------------------------------------ join
-// One wavefront a row (b, t, query head): its pieces, prefix first, weighed by their
+// The pieces of a row: `n` of them, `step` rows of results apart.
+struct Pieces { int64_t at; int n; int64_t step; };
+template <bool PRE>
+__device__ __forceinline__ Pieces pieces_of(const DecArgs& a, int seg, int h, int r) {
+  Pieces p{0, 0, a.rows[PRE]};
+  if (a.n_max[PRE] == 0) return p;
+  if (a.workers[PRE]) {
+    const int n_seg = PRE ? a.n_groups : a.s.B, total = a.first[PRE][n_seg];
+    const int from = a.first[PRE][seg], to = a.first[PRE][seg + 1];
+    if (to > from) {
+      const int run = run_pages(total * a.Hkv, a.workers[PRE]);
+      const int w0 = (h * total + from) / run, w1 = (h * total + to - 1) / run;
+      p.n = w1 - w0 + 1;
+      p.at = ((int64_t)w0 + (int64_t)h * n_seg + seg) * a.rows[PRE] + r;
+    }
+  } else {
+    p.n = sight<PRE>(a, seg).n;
+    p.at = ((int64_t)seg * a.Hkv + h) * a.n_max[PRE] * a.rows[PRE] + r;
+  }
+  return p;
+}
+
+// WAVES wavefronts a row (b, t, query head): its pieces, prefix first, weighed by their
 // maxima. Half a wavefront reads a piece's 128 values.
+template <int WAVES>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) float lds_o[4][kKv8Hd];
+  __shared__ float lds_l[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t i = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+  const int part = wave % WAVES;  // of the row's wavefronts
   const int Hq = a.Hkv * a.G;
   if (i >= (int64_t)a.s.B * a.s.T * Hq) return;
   const int64_t tok = i / Hq;
   const int hq = (int)(i % Hq), b = (int)(tok / a.s.T), t = (int)(tok % a.s.T), h = hq / a.G;
   const Kv8Len len = kv8_len(a.s, b);
-  int n[2] = {0, 0};
-  int64_t slot[2] = {0, 0};  // of the first piece
+  Pieces p[2] = {{0, 0, 0}, {0, 0, 0}};
   if (t < len.fresh) {
     const int r = t * a.G + hq % a.G;
-    n[0] = sight<false>(a, b).n;
-    slot[0] = ((int64_t)b * a.Hkv + h) * a.n_max[0] * a.rows[0] + r;
-    if (a.n_groups) {
-      const int grp = b / a.gs;
-      n[1] = sight<true>(a, grp).n;
-      slot[1] = ((int64_t)grp * a.Hkv + h) * a.n_max[1] * a.rows[1] + (int64_t)(b % a.gs) * a.s.T * a.G + r;
-    }
+    p[0] = pieces_of<false>(a, b, h, r);
+    if (a.n_groups) p[1] = pieces_of<true>(a, b / a.gs, h, (b % a.gs) * a.s.T * a.G + r);
   }
   float M = kNoMax;
 #pragma unroll
   for (int k = 1; k >= 0; --k)
-    for (int x = lane; x < n[k]; x += 64) M = fmax_nc(M, a.part_m[k][2 * (slot[k] + (int64_t)x * a.rows[k])]);
+    for (int x = lane; x < p[k].n; x += 64) M = fmax_nc(M, a.part_m[k][2 * (p[k].at + x * p[k].step)]);
   M = quad_max(M);
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) M = fmax_nc(M, __shfl_xor(M, o));
   f32x4 acc{};
   float L = 0.f;
 #pragma unroll
-  for (int k = 1; k >= 0; --k)
-    for (int x = lane >> 5; x < n[k]; x += 2) {
-      const int64_t at = slot[k] + (int64_t)x * a.rows[k];
+  for (int k = 1; k >= 0; --k) {
+#pragma unroll 4
+    for (int x = 2 * part + (lane >> 5); x < p[k].n; x += 2 * WAVES) {
+      const int64_t at = p[k].at + x * p[k].step;
       const float wgt = __builtin_amdgcn_exp2f(a.part_m[k][2 * at] - M);
       L += a.part_m[k][2 * at + 1] * wgt;
       acc += *reinterpret_cast<const f32x4*>(a.part_o[k] + at * kKv8Hd + 4 * (lane & 31)) * wgt;
     }
+  }
   L = pair_sum(L);
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] = pair_sum(acc[e]);
+  if (WAVES > 1) {
+    if (lane < 32) *reinterpret_cast<f32x4*>(&lds_o[wave][4 * lane]) = acc;
+    if (lane == 0) lds_l[wave] = L;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      acc += *reinterpret_cast<const f32x4*>(&lds_o[wave + w][4 * (lane & 31)]);
+      L += lds_l[wave + w];
+    }
+  }
   const float f = L == 0.f ? 0.f : 1.0f / L;  // nothing seen: zeros and -inf; NaN stays
   if (lane < 32)
     *reinterpret_cast<u32x2a*>(a.out + tok * a.o_ld + (int64_t)hq * kKv8Hd + 4 * lane) =
@@ -627,49 +636,49 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
 // ------------------------------------------------------------------ host
 constexpr int kFewRows = 32;  // rows that kv8_few_kernel takes
 
-// Pages of a piece and the most pieces that a segment has, of n keys at most of
-// which a window of `span` (0 = none) and the first `sinks` are seen.
-struct Cut { int chunk, n_max; };
-Cut cut(int64_t n_table, int64_t span, int64_t sinks, int64_t rows, int64_t segments_heads) {
-  if (n_table == 0) return {1, 0};
-  int64_t pages = n_table;
-  if (span) pages = std::min(pages, (span + kPage - 2) / kPage + 1 + (sinks + kPage - 1) / kPage);
-  int64_t c;
+// How a kind of segments is cut: n_table pages at most, of which a window of `span`
+// keys (0 = none) and the first `sinks` are seen. The chip's size is taken as it is
+// (256 CUs): the workspace's size must not depend on the device that asks.
+struct Cut { int chunk, n_max, workers; int64_t slots; };
+Cut cut(int64_t n_table, int64_t span, int64_t sinks, int64_t rows, int64_t segments, int64_t heads) {
+  if (n_table == 0 || segments == 0 || rows == 0) return {1, 0, 0, 0};
+  auto most = [&](int64_t c) {  // pieces of c pages
+    const int64_t n = cdiv(n_table, c);
+    return span ? std::min(n, (span + c * kPage - 2) / (c * kPage) + 1 + cdiv(sinks, c * kPage)) : n;
+  };
   if (rows <= kFewRows) {
-    c = std::max<int64_t>(4, cdiv(cdiv(pages, 64), 4) * 4);
-  } else {
-    const int64_t groups = segments_heads * cdiv(rows, kManyRows);
-    const int64_t want = std::max<int64_t>(1, cdiv(1024, groups));
-    c = std::max<int64_t>(4, cdiv(pages, want));
+    const int64_t pages = segments * heads * most(1), per_cu = kFewWaves * (rows <= 16 ? 3 : 2);
+    const int workers = (int)(cdiv(std::min<int64_t>(pages, 256 * per_cu), kFewWaves) * kFewWaves);
+    return {1, (int)most(1), workers, workers + segments * heads};
   }
-  int64_t n = cdiv(n_table, c);
-  if (span) n = std::min(n, (span + c * kPage - 2) / (c * kPage) + 1 + cdiv(sinks, c * kPage));
-  return {(int)c, (int)n};
+  const int64_t groups = segments * heads * cdiv(rows, kManyRows);
+  const int64_t c = std::max<int64_t>(4, cdiv(most(1), std::max<int64_t>(1, cdiv(1024, groups))));
+  return {(int)c, (int)most(c), 0, segments * heads * most(c)};
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Sizes of both kinds of segments and the workspace's parts.
 struct Plan {
   Cut c[2];
-  int64_t rows[2], slots[2];
-  size_t o_at[2], m_at[2], bytes;
+  int64_t rows[2];
+  size_t o_at[2], m_at[2], first_at[2], bytes;
 };
 Plan plan(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d) {
   Plan p{};
-  const int64_t G = d->n_q_heads / c->n_kv_heads, S = d->sinks;
-  const int64_t gs = d->n_groups ? s->B / d->n_groups : 0;
+  const int64_t G = d->n_q_heads / c->n_kv_heads, S = d->sinks, H = c->n_kv_heads;
+  const int64_t gs = d->n_groups ? s->B / d->n_groups : 0, segs[2] = {s->B, d->n_groups};
   p.rows[0] = (int64_t)s->T * G;
   p.rows[1] = gs * s->T * G;
   // keys that the rows of a segment see between them, at most
-  p.c[0] = cut(s->n_table, d->window ? (int64_t)d->window + s->T - 1 : 0, S, p.rows[0], (int64_t)s->B * c->n_kv_heads);
-  p.c[1] = d->n_groups ? cut(d->n_prefix_table, d->window, S, p.rows[1], (int64_t)d->n_groups * c->n_kv_heads) : Cut{1, 0};
-  const int64_t segs[2] = {s->B, d->n_groups};
+  p.c[0] = cut(s->n_table, d->window ? (int64_t)d->window + s->T - 1 : 0, S, p.rows[0], segs[0], H);
+  p.c[1] = cut(d->n_prefix_table, d->window, S, p.rows[1], segs[1], H);
   for (int k = 0; k < 2; ++k) {
-    p.slots[k] = segs[k] * c->n_kv_heads * p.c[k].n_max * p.rows[k];
     p.o_at[k] = p.bytes;
-    p.bytes += round256((size_t)p.slots[k] * kKv8Hd * 4);
+    p.bytes += round256((size_t)p.c[k].slots * p.rows[k] * kKv8Hd * 4);
     p.m_at[k] = p.bytes;
-    p.bytes += round256((size_t)p.slots[k] * 8);
+    p.bytes += round256((size_t)p.c[k].slots * p.rows[k] * 8);
+    p.first_at[k] = p.bytes;
+    p.bytes += p.c[k].workers ? round256((segs[k] + 1) * 4) : 0;
   }
   return p;
 }
@@ -698,29 +707,26 @@ glt_status check_attn(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_k
   if (s->B == 0 || s->T == 0) return GLT_OK;
   const Plan p = plan(c, s, d);
   for (int k = 0; k < 2; ++k) {
-    const int64_t segs = k ? d->n_groups : s->B;
-    GLT_CHECK(segs * c->n_kv_heads * cdiv(p.rows[k], kManyRows) * p.c[k].n_max < (1 << 24), GLT_ERR_SHAPE,
-              "%s: B=%d T=%d and tables of %d and %d pages", who, s->B, s->T, s->n_table, d->n_prefix_table);
+    const int64_t segs = k ? d->n_groups : s->B, groups = segs * c->n_kv_heads;
+    GLT_CHECK(p.c[k].workers ? groups * p.c[k].n_max < INT32_MAX - (1 << 16)
+                             : groups * cdiv(p.rows[k], kManyRows) * p.c[k].n_max < (1 << 24),
+              GLT_ERR_SHAPE, "%s: B=%d T=%d and tables of %d and %d pages", who, s->B, s->T, s->n_table, d->n_prefix_table);
   }
   return GLT_OK;
 }
 
 template <int NB, bool PRE>
-glt_status launch_few(const DecArgs& a, int cus, hipStream_t st) {
-  const int64_t segs = PRE ? a.n_groups : a.s.B;
-  const int64_t most = segs * a.n_max[PRE] * a.Hkv;
-  const size_t lds = few_lds(NB) + segs * 4;
-  const unsigned grid = (unsigned)std::min<int64_t>(most, (int64_t)cus * 3);
-  GLT_LAUNCH("kv8_few", (kv8_few_kernel<NB, PRE>), dim3(grid), dim3(kFewWaves * 64), lds, st, a);
+glt_status launch_few(const DecArgs& a, hipStream_t st) {
+  const size_t lds = (size_t)(PRE ? a.n_groups : a.s.B) * 4;
+  GLT_LAUNCH("kv8_few", (kv8_few_kernel<NB, PRE>), dim3(a.workers[PRE] / kFewWaves), dim3(kFewWaves * 64), lds, st, a);
   GLT_LAUNCH_CHECK("kv8_few");
   return GLT_OK;
 }
 
 template <bool PRE>
-glt_status launch_part(const DecArgs& a, int cus, hipStream_t st) {
+glt_status launch_part(const DecArgs& a, hipStream_t st) {
   if (a.n_max[PRE] == 0) return GLT_OK;
-  if (a.rows[PRE] <= 16) return launch_few<1, PRE>(a, cus, st);
-  if (a.rows[PRE] <= kFewRows) return launch_few<2, PRE>(a, cus, st);
+  if (a.workers[PRE]) return a.rows[PRE] <= 16 ? launch_few<1, PRE>(a, st) : launch_few<2, PRE>(a, st);
   const int64_t segs = PRE ? a.n_groups : a.s.B;
   const int64_t grid = segs * a.n_max[PRE] * cdiv(a.rows[PRE], kManyRows) * a.Hkv;
   GLT_LAUNCH("kv8_many", kv8_many_kernel<PRE>, dim3((unsigned)grid), dim3(kManyWaves * 64), kManyLds, st, a);
@@ -772,16 +778,12 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
   int dev = 0;
   GLT_TRY_HIP(hipGetDevice(&dev));
   GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "%s: device index %d out of range", who, dev);
-  static std::atomic<int> cu_count[64];  // 0: the kernels' LDS limit is not set yet
-  int cus = cu_count[dev].load(std::memory_order_acquire);
-  if (cus == 0) {
-    GLT_TRY_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-    const void* few[] = {(const void*)kv8_few_kernel<1, false>, (const void*)kv8_few_kernel<2, false>,
-                         (const void*)kv8_few_kernel<1, true>, (const void*)kv8_few_kernel<2, true>};
-    for (const void* f : few) GLT_TRY_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(2) + 8192 * 4));
-    GLT_TRY_HIP(hipFuncSetAttribute((const void*)kv8_many_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, kManyLds));
-    GLT_TRY_HIP(hipFuncSetAttribute((const void*)kv8_many_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, kManyLds));
-    cu_count[dev].store(cus, std::memory_order_release);
+  // the dynamic-LDS limit is a per-device attribute of the kernels
+  static std::atomic<bool> attr_set[64];
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    for (const void* f : {(const void*)kv8_many_kernel<false>, (const void*)kv8_many_kernel<true>})
+      GLT_TRY_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kManyLds));
+    attr_set[dev].store(true, std::memory_order_release);
   }
 
   DecArgs a{};
@@ -809,16 +811,21 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
   for (int k = 0; k < 2; ++k) {
     a.chunk[k] = p.c[k].chunk;
     a.n_max[k] = p.c[k].n_max;
+    a.workers[k] = p.c[k].workers;
+    a.first[k] = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.first_at[k]);
     a.rows[k] = (int)p.rows[k];
     a.part_o[k] = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_at[k]);
     a.part_m[k] = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.m_at[k]);
   }
   const hipStream_t st = as_stream(stream);
-  glt_status e = launch_part<true>(a, cus, st);
-  if (e == GLT_OK) e = launch_part<false>(a, cus, st);
+  glt_status e = launch_part<true>(a, st);
+  if (e == GLT_OK) e = launch_part<false>(a, st);
   if (e != GLT_OK) return e;
   const int64_t rows = tokens * d->n_q_heads;
-  GLT_LAUNCH("kv8_join", kv8_join_kernel, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
+  if (rows <= 4096)  // few rows of many pieces, mostly
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
+  else
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
   GLT_LAUNCH_CHECK("kv8_join");
   return GLT_OK;
 }

@@ -140,8 +140,10 @@ def test_sizes():
 
     def ws(**kw):
         return lib.glt_kv8_attention_workspace_size(*descs(kw))
-    # a window bounds the pieces whatever the table's width; the table's width does without one
-    assert ws(n_table=100000, pages_ld=100000, window=1000) < 2 * ws(n_table=40, pages_ld=40)
-    # at most 64 pieces of a sequence with few rows: an output, a maximum and a sum of each row
-    assert ws(n_table=100000, pages_ld=100000) <= 4 * 2 * 64 * 12 * (512 + 8) + 1024
+    # with few rows: a piece for each wavefront of the chip and for each sequence's head, whatever the table's
+    # width (an output, a maximum and a sum of each row), and the sequences' pages
+    assert ws(n_table=100000, pages_ld=100000) <= (256 * 12 + 4 * 2) * 12 * (512 + 8) + 4 * 5 + 1024
+    # with many, a window bounds the pieces
+    big = dict(T=64, n_table=100000, pages_ld=100000)
+    assert ws(window=1000, **big) < 2 * ws(T=64, n_table=40, pages_ld=40)
     assert ws(**PREFIX) > ws()
