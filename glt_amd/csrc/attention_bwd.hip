@@ -68,15 +68,16 @@ struct BwdArgs {
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
-  float* part;         // Hq > Hkv: dk, dv by query head, [2][B, T, Hq, 128]
+  float* part;         // parts > 1: dk, dv of each part, [2][B, T, Hkv * parts, 128]
   const int32_t* seq_lens;
   int64_t q_ld, k_ld, v_ld, o_ld;
   int B, T, Hq, Hkv, causal;
+  int parts;           // that a kv head's query heads come in, a workgroup of attn_dkdv_kernel each
   float scale;
   // WIN: causal, and of the keys before it a row reads those less than `window`
   // back and the first `sinks`, which lie in sink_blocks blocks of keys
   int window, sinks, sink_blocks, sink_cuts;
-  float* sink_part;  // dk, dv of these blocks by query head and cut, [B, Hq, block, cut][2][128][128]
+  float* sink_part;  // dk, dv of these blocks by part and cut, [B, Hkv * parts, block, cut][2][128][128]
 };
 
 // D of the lane's row: the diagonal of out . dout^T.
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
   const int nqb = (a.T + kRows - 1) / kRows;
   const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
   const int id = blockIdx.x, hb = id % nhb;
-  const int qb = nqb - 1 - id / nhb;
+  const int qb = WIN ? id / nhb : nqb - 1 - id / nhb;
   const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
   const int q0 = qb * kRows, wq0 = q0 + 32 * wave, myq = wq0 + lq;
   const int len = seq_len(a.seq_lens, b, a.T);
@@ -307,7 +308,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
+  // query heads h0 .. + heads - 1 (without a window one, as by the comment above)
+  const int parts = WIN ? a.parts : a.Hq / a.Hkv, heads = WIN ? a.Hq / a.Hkv / parts : 1;
+  const int nhb = a.Hkv * parts * a.B;
   const int id = blockIdx.x, hb = id % nhb;
   int kb = id / nhb, cut = 0;
   if (WIN && a.sink_blocks) {
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       kb -= extra;
     }
   }
-  const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
+  const int g = hb % a.Hkv, hp = g * parts + (hb / a.Hkv) % parts, h0 = hp * heads, b = hb / (a.Hkv * parts);
   const int k0 = kb * kRows, wk0 = k0 + 32 * wave;
   const int len = seq_len(a.seq_lens, b, a.T);
 
@@ -348,19 +351,22 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
   const uint32_t qb_ld = (uint32_t)(a.q_ld * 2), ob_ld = (uint32_t)(a.o_ld * 2);  // bytes
   // rows at or past len read as zeros, lse and D too: p = 1 there, dp - D = 0
   // and dout = 0, so they add nothing
-  const __amdgpu_buffer_rsrc_t rq = uni_rsrc_a(a.q + (int64_t)b * a.T * a.q_ld + (int64_t)h * kHd, rows_extent(len, a.q_ld));
-  const __amdgpu_buffer_rsrc_t rdo = uni_rsrc_a(a.dout + (int64_t)b * a.T * a.o_ld + (int64_t)h * kHd, rows_extent(len, a.o_ld));
-  const __amdgpu_buffer_rsrc_t rs = uni_rsrc_a(a.stats + ((wave & 1) * (int64_t)a.B * a.Hq + (int64_t)b * a.Hq + h) * a.T, (uint32_t)len * 4);
+  // (a row past the end starts behind the last head's last row)
+  const uint32_t more = (uint32_t)(heads - 1) * kHd * 2;
+  const __amdgpu_buffer_rsrc_t rq = uni_rsrc_a(a.q + (int64_t)b * a.T * a.q_ld + (int64_t)h0 * kHd, rows_extent(len, a.q_ld) + (len > 0 ? more : 0));
+  const __amdgpu_buffer_rsrc_t rdo = uni_rsrc_a(a.dout + (int64_t)b * a.T * a.o_ld + (int64_t)h0 * kHd, rows_extent(len, a.o_ld) + (len > 0 ? more : 0));
+  const float* const stat = a.stats + ((wave & 1) * (int64_t)a.B * a.Hq + (int64_t)b * a.Hq + h0) * a.T;
   lds_char* const lds = (lds_char*)smem;
-  auto load = [&](int qt, lds_char* dst) {
+  auto load = [&](int qt, int hd, lds_char* dst) {  // tile qt of head h0 + hd
     const int l = opaque(threadIdx.x) & 63;
-    load_tile<kWaves>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld);
-    load_tile<kWaves>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld);
+    load_tile<kWaves>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld + hd * kHd * 2);
+    load_tile<kWaves>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld + hd * kHd * 2);
     if (wave < 2)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + 2 * kTileB + wave * kTile * 4), 4,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(uni_rsrc_a(stat + (int64_t)hd * a.T, (uint32_t)len * 4),
+                                               (lds_void*)(dst + 2 * kTileB + wave * kTile * 4), 4,
                                                (uint32_t)(qt * kTile + l) * 4, 0, 0, 0);
   };
-  if (qt0 < qt1) load(qt0, lds);
+  if (qt0 < qt1) load(qt0, 0, lds);
 
   const uint32_t ro = row_frag_off(lane), co = col_frag_off(lane);
   f32x16 dk[4], dv[4];
@@ -368,9 +374,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
   for (int i = 0; i < 4; ++i) dk[i] = dv[i] = f32x16{};
   const float scale_log2 = a.scale * kLog2e;
 
-  // tile qt, in rd (Q, dout, lse, D); tile qt + 1 into wr
-  auto step = [&](int qt, const lds_char* __restrict__ rd, lds_char* __restrict__ wr) {
-    if (qt + 1 < qt1) load(qt + 1, wr);
+  // the lane, worked out again where a window leaves no register for what follows from it
+  auto again = [&] { return WIN ? (int)(opaque(threadIdx.x) & 63) : lane; };
+  // tile qt of head h0 + hd, in rd (Q, dout, lse, D); the next one into wr
+  auto step = [&](int qt, int hd, const lds_char* __restrict__ rd, lds_char* __restrict__ wr) {
+    if (qt + 1 < qt1) load(qt + 1, hd, wr);
+    else if (WIN && hd + 1 < heads) load(qt0, hd + 1, wr);
     const int q0t = qt * kTile;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
@@ -378,7 +387,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       if (q0 >= len || (a.causal && q0 + 31 < wk0)) continue;
       if (WIN && q0 >= wk0 + 31 + a.window && wk0 >= a.sinks) continue;
       f32x16 s{}, dp;
-      const lds_char* row = rd + opaque(ro + qb * 8 * kGroupB);
+      const lds_char* row = rd + opaque((WIN ? row_frag_off(again()) : ro) + qb * 8 * kGroupB);
       score_product<kDkdvAhead>(row, kf, s, [](int) {});
       if (WIN && q0 + 31 >= wk0 + a.window && wk0 + 32 > a.sinks) {  // and those that its window leaves
         const int l = opaque(threadIdx.x) & 63, key = wk0 + (l & 31);
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       }
       // the exponentials beside the other product; elements 4 i .. + 3 are
       // query rows 8 i + 4 lh .. + 3
-      const lds_char* st = rd + opaque(2 * kTileB + 128 * qb + 16 * (lane >> 5));
+      const lds_char* st = rd + opaque(2 * kTileB + 128 * qb + 16 * (again() >> 5));
       // the product starts at -D (16 subtractions less)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -422,7 +431,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      const lds_char* col = rd + opaque(co + qb * 8 * kGroupB);
+      const lds_char* col = rd + opaque((WIN ? col_frag_off(again()) : co) + qb * 8 * kGroupB);
       __builtin_amdgcn_s_setprio(1);
       bf16x8 oa[kGradAhead], qa[kGradAhead];  // step i: 16 query rows i >> 2, d block i & 3
 #pragma unroll
@@ -443,12 +452,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       __builtin_amdgcn_s_setprio(0);
     }
   };
-  for (int qt = qt0; qt < qt1; ++qt) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
-    phase_barrier();  // tile qt is whole, and every wavefront is done with tile qt - 1
-    const int cur = (qt - qt0) & 1;
-    step(qt, lds + cur * kDkdvBuf, lds + (cur ^ 1) * kDkdvBuf);
-  }
+  int cur = 0;
+  for (int hd = 0; hd < heads; ++hd)
+    for (int qt = qt0; qt < qt1; ++qt) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
+      phase_barrier();  // the tile is whole, and every wavefront is done with the one before
+      step(qt, hd, lds + cur * kDkdvBuf, lds + (cur ^ 1) * kDkdvBuf);
+      cur ^= 1;
+    }
   // the output rows' addresses are worked out again here: kept across the
   // loop they cost registers that it does not have
   const int tid = opaque(threadIdx.x);
@@ -463,15 +474,15 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
     for (int i = 0; i < 4; ++i) dk[i] *= 0.f;
   float *pk, *pv;
   if (WIN && kb < a.sink_blocks) {
-    pk = a.sink_part + (((((int64_t)b * a.Hq + h) * a.sink_blocks + kb) * a.sink_cuts + cut) * 2 * kRows + (myk - k0)) * kHd + 4 * lh;
+    pk = a.sink_part + (((((int64_t)b * a.Hkv * parts + hp) * a.sink_blocks + kb) * a.sink_cuts + cut) * 2 * kRows + (myk - k0)) * kHd + 4 * lh;
     pv = pk + kRows * kHd;
-  } else if (rep == 1) {
+  } else if (parts == 1) {
     store_rows(a.dk + tok * a.k_ld + (int64_t)g * kHd, dk, a.scale, lh);
     store_rows(a.dv + tok * a.v_ld + (int64_t)g * kHd, dv, 1.0f, lh);
     return;
   } else {
-    pk = a.part + (tok * a.Hq + h) * kHd + 4 * lh;
-    pv = pk + (int64_t)a.B * a.T * a.Hq * kHd;
+    pk = a.part + (tok * a.Hkv * parts + hp) * kHd + 4 * lh;
+    pv = pk + (int64_t)a.B * a.T * a.Hkv * parts * kHd;
   }
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -486,14 +497,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
 // order, rounded once; a thread takes 8 elements of a token's kv head.
 __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int rep = a.Hq / a.Hkv, cols = a.Hkv * (kHd / 8);
+  const int cols = a.Hkv * (kHd / 8);
   if (i >= (int64_t)a.B * a.T * cols) return;
   const int64_t row = i / cols;
   if (a.sink_blocks && row % a.T < a.sink_blocks * kRows) return;  // attn_sink_sum_kernel's
   const int c = (int)(i - row * cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
-  const float* p = a.part + ((blockIdx.y ? (int64_t)a.B * a.T : 0) + row) * a.Hq * kHd + (int64_t)g * rep * kHd + e;
+  const float* p = a.part + ((blockIdx.y ? (int64_t)a.B * a.T : 0) + row) * a.Hkv * a.parts * kHd + (int64_t)g * a.parts * kHd + e;
   f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
-  for (int s = 1; s < rep; ++s) {
+  for (int s = 1; s < a.parts; ++s) {
     x += *reinterpret_cast<const f32x4*>(p + s * kHd);
     y += *reinterpret_cast<const f32x4*>(p + s * kHd + 4);
   }
@@ -504,13 +515,13 @@ __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
             pack2_rne(y[2] * f, y[3] * f)};
 }
 
-// The keys of the sink blocks: parts added by query head, then by cut.
+// The keys of the sink blocks: the parts of their query heads, each by cut.
 __global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
   const int cols = a.Hkv * (kHd / 8), rows = min(a.sink_blocks * kRows, a.T);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (int64_t)a.B * rows * cols) return;
   const int c = (int)(i % cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
-  const int t = (int)(i / cols % rows), b = (int)(i / cols / rows), kb = t / kRows, rep = a.Hq / a.Hkv;
+  const int t = (int)(i / cols % rows), b = (int)(i / cols / rows), kb = t / kRows;
   const int len = seq_len(a.seq_lens, b, a.T), k0 = kb * kRows;
   int cuts = 1;
   if (k0 < len) {
@@ -518,11 +529,12 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
     cuts += (all - window_tiles(k0, a.window, all) + kSinkTiles - 1) / kSinkTiles;
   }
   f32x4 x{}, y{};
-  for (int s = 0; s < rep; ++s)
+  for (int s = 0; s < a.parts; ++s)
+#pragma unroll 4
     for (int cut = 0; cut < cuts; ++cut) {
       const float* p = a.sink_part +
-                       (((((int64_t)b * a.Hq + g * rep + s) * a.sink_blocks + kb) * a.sink_cuts + cut) * 2 * kRows +
-                        (blockIdx.y ? kRows : 0) + t - k0) * kHd + e;
+                       (((((int64_t)b * a.Hkv + g) * a.parts + s) * a.sink_blocks + kb) * a.sink_cuts + cut) * 2 * kRows * kHd +
+                       ((blockIdx.y ? kRows : 0) + t - k0) * kHd + e;
       x += *reinterpret_cast<const f32x4*>(p);
       y += *reinterpret_cast<const f32x4*>(p + 4);
     }
@@ -536,8 +548,21 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t stats_bytes(const glt_attn_desc* d) { return round256((size_t)2 * d->B * d->n_q_heads * d->T * sizeof(float)); }
-size_t part_bytes(const glt_attn_desc* d) {
-  return d->n_q_heads > d->n_kv_heads ? (size_t)2 * d->B * d->T * d->n_q_heads * kHd * sizeof(float) : 0;
+size_t part_bytes(const glt_attn_desc* d, int parts) {
+  return parts > 1 ? (size_t)2 * d->B * d->T * d->n_kv_heads * parts * kHd * sizeof(float) : 0;
+}
+// Parts of a kv head's query heads: one each, or with a window, where blocks are of
+// nearly one length (up to half of T), as few as leave two workgroups for each of 256
+// CUs: no f32 parts then. dkdv and sums in us at 2 x 4096, 32 query and 8 kv heads,
+// one each against all together: window 128 156, 59; 1024 304, 242; 2048 448, 416;
+// 4095 585, 661.
+int dkdv_parts(const glt_attn_desc* d, int32_t window) {
+  const int rep = d->n_q_heads / d->n_kv_heads;
+  if (window <= 0 || window > d->T / 2) return rep;
+  const int64_t blocks = cdiv(d->T, kRows) * d->n_kv_heads * d->B;
+  for (int parts = 1; parts < rep; ++parts)
+    if (rep % parts == 0 && blocks * parts >= 512) return parts;
+  return rep;
 }
 
 // Blocks of keys that hold sinks, and the cuts that their queries come in at most.
@@ -547,8 +572,8 @@ SinkCut sink_cut(const glt_attn_desc* d, int32_t window, int32_t sinks) {
   const int64_t tiles = cdiv(d->T, kTile), in = std::min<int64_t>(cdiv((int64_t)kRows - 1 + window, kTile), tiles);
   return {(int)cdiv(std::min(sinks, d->T), kRows), 1 + (int)cdiv(tiles - in, kSinkTiles)};
 }
-size_t sink_bytes(const glt_attn_desc* d, SinkCut c) {
-  return (size_t)d->B * d->n_q_heads * c.blocks * c.cuts * 2 * kRows * kHd * sizeof(float);
+size_t sink_bytes(const glt_attn_desc* d, SinkCut c, int parts) {
+  return (size_t)d->B * d->n_kv_heads * parts * c.blocks * c.cuts * 2 * kRows * kHd * sizeof(float);
 }
 
 template <bool WIN>
@@ -569,10 +594,10 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   GLT_LAUNCH(WIN ? "attn_window_dq" : "attn_dq", attn_dq_kernel<WIN>, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDqLds, st, a);
   GLT_LAUNCH_CHECK("attn_dq");
   const unsigned blocks = nb + (WIN && a.sink_blocks ? (unsigned)(a.sink_blocks * (a.sink_cuts - 1)) : 0u);
-  GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", attn_dkdv_kernel<WIN>, dim3(blocks * a.Hq * a.B), dim3(kWaves * 64),
-             kDkdvLds, st, a);
+  GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", attn_dkdv_kernel<WIN>, dim3(blocks * a.Hkv * a.parts * a.B),
+             dim3(kWaves * 64), kDkdvLds, st, a);
   GLT_LAUNCH_CHECK("attn_dkdv");
-  if (a.Hq > a.Hkv) {
+  if (a.parts > 1) {
     const int64_t chunks = (int64_t)a.B * a.T * a.Hkv * (kHd / 8);
     GLT_LAUNCH("attn_dkdv_sum", attn_dkdv_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
     GLT_LAUNCH_CHECK("attn_dkdv_sum");
@@ -585,7 +610,9 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   return GLT_OK;
 }
 
-size_t bwd_bytes(const glt_attn_desc* d, SinkCut c) { return stats_bytes(d) + part_bytes(d) + sink_bytes(d, c); }
+size_t bwd_bytes(const glt_attn_desc* d, SinkCut c, int parts) {
+  return stats_bytes(d) + part_bytes(d, parts) + sink_bytes(d, c, parts);
+}
 
 glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q, const void* k, const void* v,
                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
@@ -599,7 +626,8 @@ glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, cons
   const SinkCut cut = sink_cut(d, window, sinks);
   GLT_CHECK((cdiv(d->T, kRows) + (int64_t)cut.blocks * cut.cuts) * d->B < (1 << 24) / d->n_q_heads, GLT_ERR_SHAPE,
             "%s: B=%d T=%d n_q_heads=%d sinks=%d", who, d->B, d->T, d->n_q_heads, sinks);
-  const size_t need = bwd_bytes(d, cut);
+  const int parts = dkdv_parts(d, window);
+  const size_t need = bwd_bytes(d, cut, parts);
   GLT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, GLT_ERR_WORKSPACE,
             "%s: needs %zu workspace bytes, 256-byte aligned", who, need);
   // every kernel reads inputs after others have written gradients
@@ -634,7 +662,8 @@ glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, cons
   a.sinks = sinks;
   a.sink_blocks = cut.blocks;
   a.sink_cuts = cut.cuts;
-  a.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(d) + part_bytes(d));
+  a.parts = parts;
+  a.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(d) + part_bytes(d, parts));
   return window > 0 ? launch_bwd<true>(a, as_stream(stream)) : launch_bwd<false>(a, as_stream(stream));
 }
 
@@ -650,7 +679,8 @@ extern "C" size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d) {
 
 extern "C" size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks) {
   if (!d || d->B <= 0 || d->T <= 0 || d->n_q_heads <= 0 || d->n_kv_heads <= 0) return 256;
-  return bwd_bytes(d, window < d->T && sinks <= kMaxSinks ? sink_cut(d, window, sinks) : SinkCut{0, 0});
+  if (d->n_q_heads % d->n_kv_heads || window < 0 || window >= d->T) window = 0;
+  return bwd_bytes(d, sinks <= kMaxSinks ? sink_cut(d, window, sinks) : SinkCut{0, 0}, dkdv_parts(d, window));
 }
 
 extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
   const int nqb = (a.T + kRows - 1) / kRows;
   const int rep = a.Hq / a.Hkv, nhb = a.Hq * a.B;
   const int id = blockIdx.x, hb = id % nhb;
-  const int qb = nqb - 1 - id / nhb;
+  const int qb = WIN ? id / nhb : nqb - 1 - id / nhb;
   const int g = hb % a.Hkv, h = g * rep + (hb / a.Hkv) % rep, b = hb / a.Hq;
   const int q0 = qb * kRows, wq0 = q0 + 32 * wave, myq = wq0 + lq;
   const int len = seq_len(a.seq_lens, b, a.T);

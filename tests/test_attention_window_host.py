@@ -46,6 +46,9 @@ def test_workspace():
     one = 2 * 4 * 2 * 128 * 128 * 4
     assert size(d, 100, 1) == size(d, 100, 128) == plain + 3 * one
     assert size(d, 100, 129) == plain + 6 * one
+    # where key blocks fill the chip, a kv head's query heads need no parts
+    big = desc(B=20, T=2000)
+    assert size(big, 100, 0) < lib.glt_attention_bwd_workspace_size(ctypes.byref(big)) // 50
     assert bwd(d, 100, 1, nbytes=plain + 3 * one - 1) == 5
     assert bwd(d, 100, 1, ws=None) == 5
     assert lib.glt_attention_window_bwd_workspace_size(None, 1, 1) == 256
