@@ -7,10 +7,12 @@
 //   s = (q . code_k) step_k scale,   o += (p step_v) . code_v
 // need one rounding, of p step_v, and no value of k or v is formed.
 //
-// A segment's keys are cut into pieces; a piece's output, maximum and sum go into the
-// workspace, and a last kernel joins each row's pieces in order. Few rows a segment
-// (new tokens x query heads of a kv head: kv8_few_kernel) or many
-// (kv8_many_kernel); how each is cut stands there.
+// Everything that the new tokens have to read is a list of tiles of work, dealt out in
+// equal runs (deal() below): whatever the lengths, each wavefront or workgroup gets its
+// share. Where a run ends inside of a segment its rows come in pieces: a piece's output,
+// maximum and sum go into the workspace, and a last kernel joins each row's pieces in
+// order. Few rows a segment (new tokens x query heads of a kv head: few_rows) or many
+// (many_rows); the kinds of a call's own tokens and prefixes run in one launch.
 #include <algorithm>
 #include <atomic>
 
@@ -25,6 +27,15 @@ namespace {
 constexpr float kSlack = 8.0f;      // running-max slack (log2 units)
 constexpr float kNoMax = -3.0e38f;  // maximum of a row that has seen nothing
 
+// A kind of segments, [0] the sequences' own tokens, [1] prefixes.
+struct Part {
+  int rows;        // of a segment and head
+  int workers;     // wavefronts (few rows) or workgroups (many) that the work is dealt to
+  int blocks;      // workgroups of the launch
+  int* first;      // tiles of work before each segment, and in all
+  float* o;        // pieces' results by slot and row: 128 each
+  float* m;        // maximum (log2 units) and sum
+};
 struct DecArgs {
   const uint8_t* cache;
   int64_t n_pages;
@@ -39,25 +50,18 @@ struct DecArgs {
   uint16_t* out;
   float* lse;
   int64_t q_ld, o_ld;
-  // [0] the sequences' own tokens, [1] prefixes: rows of a segment and head, pages
-  // of a piece (1: kv8_few_kernel cuts by itself), pieces that a segment has at most,
-  // and the pieces' results by slot and row
-  int rows[2], chunk[2], n_max[2];
-  int workers[2];      // wavefronts of kv8_few_kernel, 0 where kv8_many_kernel runs
-  int* first[2];       // its pages before each segment, and in all
-  float* part_o[2];    // 128 each
-  float* part_m[2];    // maximum (log2 units) and sum
+  Part part[2];
 };
 
 __device__ __forceinline__ int prefix_len(const DecArgs& a, int b) {
   return a.n_groups ? min(max(a.plens[b / a.gs], 0), a.n_prefix_table * kPage) : 0;
 }
 
-// What the segment's rows see of it: its first `hi` keys, of which those from `lo`
-// on and the first `sunk`; the pieces ns before the window's and the window's from c0.
+// What the segment's rows see of it: of its first `hi` keys those from `lo` on and the
+// first `sunk`; a list of n pages, ns that hold sinks and then those from c0 on.
 struct Sight {
   int hi, ns, c0, n;
-  __device__ __forceinline__ int chunk_at(int piece) const { return piece < ns ? piece : c0 + piece - ns; }
+  __device__ __forceinline__ int page(int i) const { return i < ns ? i : c0 + i - ns; }
 };
 template <bool PRE>
 __device__ __forceinline__ Sight sight(const DecArgs& a, int seg) {
@@ -82,12 +86,11 @@ __device__ __forceinline__ Sight sight(const DecArgs& a, int seg) {
       sunk = min(max(a.S - prefix_len(a, seg), 0), hi);
     }
   }
-  const int keys = a.chunk[PRE] * kPage;
   Sight r;
   r.hi = hi;
-  const int end = (hi + keys - 1) / keys;
-  r.c0 = min(lo / keys, end);
-  r.ns = min((sunk + keys - 1) / keys, r.c0);
+  const int end = (hi + kPage - 1) / kPage;
+  r.c0 = min(lo / kPage, end);
+  r.ns = min((sunk + kPage - 1) / kPage, r.c0);
   r.n = r.ns + end - r.c0;
   return r;
 }
@@ -95,7 +98,7 @@ __device__ __forceinline__ Sight sight(const DecArgs& a, int seg) {
 // A row's sight within a segment: key j is seen if j < hi and (j >= lo or j < sunk).
 struct Row {
   int hi, lo, sunk;
-  int64_t q_row;  // (b * T + t) and its head, for q and the outputs
+  int64_t q_row;  // b * T + t, and its head, for q and the outputs
   int head;
 };
 template <bool PRE>
@@ -117,8 +120,14 @@ __device__ __forceinline__ Row row_of(const DecArgs& a, int seg, int h, int r, i
 }
 
 template <bool PRE>
-__device__ __forceinline__ int64_t page_id(const DecArgs& a, int seg, int p) {
+__device__ __forceinline__ int page_id(const DecArgs& a, int seg, int p) {
   return PRE ? a.ppages[seg * a.prefix_ld + p] : a.s.pages[seg * a.s.pages_ld + p];
+}
+// Where a page's head lies; a page outside the pool is not followed (its steps count as
+// NaN).
+__device__ __forceinline__ bool page_ok(const DecArgs& a, int id) { return id >= 0 && id < a.n_pages; }
+__device__ __forceinline__ const uint8_t* page_at(const DecArgs& a, int id, int h) {
+  return a.cache + ((int64_t)(page_ok(a, id) ? id : 0) * a.Hkv + h) * kHeadB;
 }
 
 // Eight codes as bf16 (exact: the upper halves of their f32 values).
@@ -141,34 +150,44 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// -------------------------------------------------------------- few rows
-// Up to 16 NB rows a segment and head. The pages that the segments' rows see, of all
-// heads, are one list, of which each wavefront takes an equal run whatever the
-// lengths; where a run enters another segment or head, a piece ends. A wavefront loads a
-// page's codes with 16-byte loads straight into the operands of
-//   S^T[key][row] = K . Q^T,  O^T[channel][row] += V^T . P^T
-// (16 x 16 x 32), with the softmax between: no LDS, no barrier, and every code is
-// converted once.
-//
-// Lane l: row l & 15 of a block of 16, g = l >> 4. The keys of score block (beta, a) are
-// numbered so that the accumulators are the second product's operand as they stand:
-// element e of lane group g is key 16 g + 8 a + 4 beta + e of the page.
-constexpr int kFewWaves = 4;
+// A finished row's lse and output: nothing seen gives -inf and zeros, NaN stays.
+__device__ __forceinline__ void write_lse(const DecArgs& a, const Row& w, float m, float l) {
+  const int64_t b = w.q_row / a.s.T, t = w.q_row - b * a.s.T;
+  a.lse[(b * a.Hkv * a.G + w.head) * a.s.T + t] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+// N groups of four channels from 4 lane on, STEP apart, of this lane
+template <int STEP, int N>
+__device__ __forceinline__ void write_row(const DecArgs& a, const Row& w, const f32x4* o, float m, float l, int lane) {
+  const float f = l == 0.f ? 0.f : 1.0f / l;
+  uint16_t* to = a.out + w.q_row * a.o_ld + (int64_t)w.head * kKv8Hd + 4 * lane;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    *reinterpret_cast<u32x2a*>(to + STEP * i) = u32x2a{pack2_rne(o[i][0] * f, o[i][1] * f), pack2_rne(o[i][2] * f, o[i][3] * f)};
+  if (lane == 0) write_lse(a, w, m, l);
+}
 
-// Pages of a wavefront's run.
-__device__ __forceinline__ int run_pages(int total, int workers) { return max((total + workers - 1) / workers, 1); }
+// ---------------------------------------------------------------- dealing
+constexpr int kManyRows = 128;  // rows of a workgroup of many_rows
+constexpr int kFewRows = 32;    // rows that few_rows takes
 
-template <int NB, bool PRE>
-__global__ void __launch_bounds__(kFewWaves * 64, NB == 1 ? 3 : 2) kv8_few_kernel(const DecArgs a) {
-  extern __shared__ int first[];  // pages before each segment, and in all
-  __shared__ int wave_sum[kFewWaves];
-  const int tid = threadIdx.x, lane = tid & 63, r15 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n_seg = PRE ? a.n_groups : a.s.B, R = a.rows[PRE];
+// Row blocks of a segment that hold new tokens.
+template <bool PRE, bool MANY>
+__device__ __forceinline__ int row_blocks(const DecArgs& a, int seg) {
+  if (!MANY) return 1;
+  return ((PRE ? a.part[1].rows : kv8_len(a.s, seg).fresh * a.G) + kManyRows - 1) / kManyRows;
+}
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// first[s]: tiles of work (pages x row blocks) before segment s, first[n_seg] in all, by
+// a workgroup of 256 in LDS, and by workgroup 0 of the kind for the join.
+template <bool PRE, bool MANY>
+__device__ __forceinline__ int deal(const DecArgs& a, int* first, int block) {
+  __shared__ int wave_sum[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int n_seg = PRE ? a.n_groups : a.s.B;
   int total = 0;
-  for (int s0 = 0; s0 < n_seg; s0 += kFewWaves * 64) {
-    const int s = s0 + tid, n = s < n_seg ? sight<PRE>(a, s).n : 0;
+  for (int s0 = 0; s0 < n_seg; s0 += 256) {
+    const int s = s0 + tid, n = s < n_seg ? sight<PRE>(a, s).n * row_blocks<PRE, MANY>(a, s) : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -179,197 +198,291 @@ __global__ void __launch_bounds__(kFewWaves * 64, NB == 1 ? 3 : 2) kv8_few_kerne
     __syncthreads();
     int before = total;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
+    for (int w = 0; w < 4; ++w) {
       if (w < wave) before += wave_sum[w];
       total += wave_sum[w];
     }
     if (s < n_seg) first[s] = before + x - n;
+    if (s == n_seg - 1) first[n_seg] = total;
     __syncthreads();
   }
-  total = __builtin_amdgcn_readfirstlane(total);
-  if (blockIdx.x == 0) {  // for the join
-    for (int s = tid; s < n_seg; s += kFewWaves * 64) a.first[PRE][s] = first[s];
-    if (tid == 0) a.first[PRE][n_seg] = total;
+  if (block == 0)
+    for (int s = tid; s <= n_seg; s += 256) a.part[PRE].first[s] = first[s];
+  return uni(total);
+}
+// Tiles of a run.
+template <bool MANY>
+__device__ __forceinline__ int run_tiles(int all, int workers) {
+  return max((all + workers - 1) / workers, MANY ? 2 : 1);
+}
+// The segment that tile `pos` of a head lies in: the last one that starts at or before it.
+__device__ __forceinline__ int find_segment(const int* first, int n_seg, int pos) {
+  int seg = 0;
+  for (int end = n_seg; end - seg > 1;) {
+    const int mid = (seg + end) >> 1;
+    if (uni(first[mid]) <= pos) seg = mid;
+    else end = mid;
   }
+  return seg;
+}
+// Slot of a piece of a column (segment, head, row block). A worker has one piece that
+// goes on with a column (its first) and one that begins a column without ending it (its
+// last); where prefixes' pieces have to be joined to them, whole columns need a slot
+// too: workers and columns both rise along the list.
+template <bool PRE>
+__device__ __forceinline__ int64_t slot_of(const DecArgs& a, int worker, int64_t column, bool begins) {
+  return PRE || a.n_groups ? worker + column : 2 * (int64_t)worker + begins;
+}
 
-  const int worker = blockIdx.x * kFewWaves + wave, all = total * a.Hkv, run = run_pages(all, a.workers[PRE]);
-  int at = worker * run;  // workers * run stays below all + workers
-  const int stop = min(at + run, all);
-  while (at < stop) {
-    const int h = at / total, pos = at - h * total;
-    int seg = 0;  // the last segment that starts at or before pos
-    for (int end = n_seg; end - seg > 1;) {
-      const int mid = (seg + end) >> 1;
-      if (__builtin_amdgcn_readfirstlane(first[mid]) <= pos) seg = mid;
-      else end = mid;
-    }
-    const Sight si = sight<PRE>(a, seg);
-    const int i0 = pos - __builtin_amdgcn_readfirstlane(first[seg]), i1 = min(si.n, i0 + stop - at);  // of the segment's list
-    at += i1 - i0;
+// -------------------------------------------------------------- few rows
+// Up to 16 NB rows a segment and head: a tile is a page of a head, and the workers are
+// wavefronts. A wavefront loads a page's codes with 16-byte loads straight into the operands of
+//   S^T[key][row] = K . Q^T,  O^T[channel][row] += V^T . P^T
+// (16 x 16 x 32), with the softmax between: no LDS, no barrier, and every code is
+// converted once.
+//
+// Lane l: row l & 15 of a block of 16, g = l >> 4. The keys of score block (beta, a) are
+// numbered so that the accumulators are the second product's operand as they stand:
+// element e of lane group g is key 16 g + 8 a + 4 beta + e of the page.
+constexpr int kFewWaves = 4;
 
-    // (what depends on the lane is worked out for each run: kept, it costs registers
-    // that there are not)
-    const int l1 = (int)opaque(threadIdx.x) & 63;
-    Row row[NB];
-    bf16x8 qf[NB][4];
+template <int NB>
+struct Few {
+  Row row[NB];
+  bf16x8 qf[NB][4];
+  f32x4 o[NB][8];
+  float m[NB], l[NB];
+
+  // (what depends on the lane is worked out for each run: kept, it costs registers
+  // that there are not)
+  template <bool PRE>
+  __device__ __forceinline__ void begin(const DecArgs& a, int seg, int h, int seg_hi) {
+    const int lane = (int)opaque(threadIdx.x) & 63, R = a.part[PRE].rows;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int r = 16 * nb + (l1 & 15);
-      row[nb] = row_of<PRE>(a, seg, h, min(r, R - 1), si.hi);
-      const uint16_t* qp = a.q + row[nb].q_row * a.q_ld + (int64_t)row[nb].head * kKv8Hd + 16 * (l1 >> 4);
+      row[nb] = row_of<PRE>(a, seg, h, min(16 * nb + (lane & 15), R - 1), seg_hi);
+      const uint16_t* qp = a.q + row[nb].q_row * a.q_ld + (int64_t)row[nb].head * kKv8Hd + 16 * (lane >> 4);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        qf[nb][s] = __builtin_bit_cast(bf16x8, row[nb].hi > 0 ? *reinterpret_cast<const u32x4*>(qp + 64 * (s >> 1) + 8 * (s & 1))
-                                                              : u32x4{0u, 0u, 0u, 0u});
-    }
-    f32x4 o[NB][8];
-    float m_run[NB], l_run[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      m_run[nb] = kNoMax;
-      l_run[nb] = 0.f;
+        qf[nb][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qp + 64 * (s >> 1) + 8 * (s & 1)));
+      m[nb] = kNoMax;
+      l[nb] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[nb][i] = f32x4{};
     }
+  }
 
-    int ids = 0;  // lane x: the id of the run's page i0 + x, 64 at a time
-    for (int i = i0; i < i1; ++i) {
-      const int x = (i - i0) & 63;
-      if (x == 0) ids = i + lane < i1 ? (int)page_id<PRE>(a, seg, si.chunk_at(i + lane)) : 0;
-      const int64_t id = __builtin_amdgcn_readlane(ids, x);
-      const int p = si.chunk_at(i);
-      const bool ok = id >= 0 && id < a.n_pages;
-      const uint8_t* pg = a.cache + ((ok ? id : 0) * a.Hkv + h) * kHeadB;
-      u32x4 kx[8], vx[8], kst[2], vst[2];
-      const uint8_t* kp = pg + (uint32_t)((16 * (r15 >> 2) + (r15 & 3)) * kKv8Hd + 16 * g);
+  // page p of the segment, at pg
+  __device__ __forceinline__ void page(const DecArgs& a, const uint8_t* pg, bool ok, int p) {
+    const int lane = (int)(NB > 1 ? opaque(threadIdx.x) : threadIdx.x) & 63, r15 = lane & 15, g = lane >> 4;
+    u32x4 kx[8], vx[8], kst[2], vst[2];
+    const uint8_t* kp = pg + (uint32_t)((16 * (r15 >> 2) + (r15 & 3)) * kKv8Hd + 16 * g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)  // block (beta = i >> 2, a = (i >> 1) & 1), channels 64 (i & 1) + 16 g ..
-        kx[i] = *reinterpret_cast<const u32x4*>(kp + (8 * ((i >> 1) & 1) + 4 * (i >> 2)) * kKv8Hd + 64 * (i & 1));
+    for (int i = 0; i < 8; ++i)  // block (beta = i >> 2, a = (i >> 1) & 1), channels 64 (i & 1) + 16 g ..
+      kx[i] = *reinterpret_cast<const u32x4*>(kp + (8 * ((i >> 1) & 1) + 4 * (i >> 2)) * kKv8Hd + 64 * (i & 1));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kst[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kKStepOff + 32 * g + 16 * i));
-        vst[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVStepOff + 32 * g + 16 * i));
-      }
-      auto load_v = [&](int from, int to) {
+    for (int i = 0; i < 2; ++i) {
+      kst[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kKStepOff + 32 * g + 16 * i));
+      vst[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVStepOff + 32 * g + 16 * i));
+    }
+    auto load_v = [&](int from, int to) {
 #pragma unroll
-        for (int i = from; i < to; ++i) vx[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + (16 * i + r15) * kPage + 16 * g));
-      };
-      if (NB == 1) load_v(0, 8);
-      if (!ok)
+      for (int i = from; i < to; ++i) vx[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + (16 * i + r15) * kPage + 16 * g));
+    };
+    if (NB == 1) load_v(0, 8);
+    if (!ok)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) kst[i] = vst[i] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-      // steps of keys 16 g + i
-      auto step = [](const u32x4* x, int i) {
-        const uint32_t w = x[i >> 3][(i & 7) >> 1];
-        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-      };
+      for (int i = 0; i < 2; ++i) kst[i] = vst[i] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    // steps of keys 16 g + i
+    auto step = [](const u32x4* x, int i) {
+      const uint32_t w = x[i >> 3][(i & 7) >> 1];
+      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    };
 
-      f32x4 s[NB][4];  // block 2 beta + a
+    f32x4 s[NB][4];  // block 2 beta + a
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk) {
+    for (int blk = 0; blk < 4; ++blk) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[nb][blk] = f32x4{};
+      for (int nb = 0; nb < NB; ++nb) s[nb][blk] = f32x4{};
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const u32x4 x = kx[2 * blk + (st >> 1)];
-          const bf16x8 ka = codes8(x[2 * (st & 1)], x[2 * (st & 1) + 1]);
+      for (int st = 0; st < 4; ++st) {
+        const u32x4 x = kx[2 * blk + (st >> 1)];
+        const bf16x8 ka = codes8(x[2 * (st & 1)], x[2 * (st & 1) + 1]);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) s[nb][blk] = mfma16(ka, qf[nb][st], s[nb][blk]);
-        }
-        if (NB > 1) __builtin_amdgcn_sched_barrier(0);
+        for (int nb = 0; nb < NB; ++nb) s[nb][blk] = mfma16(ka, qf[nb][st], s[nb][blk]);
       }
-      if (NB > 1) {  // no registers for both, nor for all of v
-        __builtin_amdgcn_sched_barrier(0);
-        load_v(0, 4);
-      }
-      bf16x8 pf[NB][2];
+      if (NB > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (NB > 1) {  // no registers for both, nor for all of v
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(0, 4);
+    }
+    bf16x8 pf[NB][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const Row& w = row[nb];
-        const int key0 = p * kPage + 16 * g;
-        // the lanes' rows see the whole page (of others, lanes' columns are zeros)
-        const bool whole = __all(p * kPage + kPage <= w.hi && (p * kPage >= w.lo || p * kPage + kPage <= w.sunk));
+    for (int nb = 0; nb < NB; ++nb) {
+      const Row& w = row[nb];
+      const int key0 = p * kPage + 16 * g;
+      // every row sees the whole page, but for rows that come to nothing
+      const bool whole = __all((w.hi == 0) | ((p * kPage + kPage <= w.hi) & ((p * kPage >= w.lo) | (p * kPage + kPage <= w.sunk))));
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nb][blk][e] *= step(kst, 8 * (blk & 1) + 4 * (blk >> 1) + e) * a.scale_log2;
+      if (!whole)
 #pragma unroll
         for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nb][blk][e] *= step(kst, 8 * (blk & 1) + 4 * (blk >> 1) + e) * a.scale_log2;
-        if (!whole)
+          for (int e = 0; e < 4; ++e) {
+            const int j = key0 + 8 * (blk & 1) + 4 * (blk >> 1) + e;
+            const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
+            s[nb][blk][e] = in ? s[nb][blk][e] : -INFINITY;
+          }
+      float mt = s[nb][0][0];
 #pragma unroll
-          for (int blk = 0; blk < 4; ++blk)
+      for (int i = 1; i < 16; ++i) mt = fmax_nc(mt, s[nb][i >> 2][i & 3]);
+      mt = quad_max(mt);
+      // (each row's moves by itself: no other row's values touch it)
+      const bool up = mt > m[nb] + kSlack;
+      if (__any(up)) {
+        const float m_new = up ? mt : m[nb];
+        const float alpha = __builtin_amdgcn_exp2f(m[nb] - m_new);
+        m[nb] = m_new;
+        l[nb] *= alpha;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = key0 + 8 * (blk & 1) + 4 * (blk >> 1) + e;
-              const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
-              s[nb][blk][e] = in ? s[nb][blk][e] : -INFINITY;
-            }
-        float mt = s[nb][0][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mt = fmax_nc(mt, s[nb][i >> 2][i & 3]);
-        mt = quad_max(mt);
-        if (__any(mt > m_run[nb] + kSlack)) {
-          const float m_new = fmax_nc(m_run[nb], mt);
-          const float alpha = __builtin_amdgcn_exp2f(m_run[nb] - m_new);
-          m_run[nb] = m_new;
-          l_run[nb] *= alpha;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[nb][i] *= alpha;
-        }
-        float pv[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = __builtin_amdgcn_exp2f(s[nb][i >> 2][i & 3] - m_run[nb]);
-          l_run[nb] += x;
-          pv[i] = x * step(vst, 8 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3));
-        }
-        if (!whole)  // an unseen key's step may be anything
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pv[i] = s[nb][i >> 2][i & 3] == -INFINITY ? 0.f : pv[i];
-#pragma unroll
-        for (int beta = 0; beta < 2; ++beta) {
-          const float* x = pv + 8 * beta;
-          pf[nb][beta] = __builtin_bit_cast(bf16x8, u32x4{pack2_rne(x[0], x[1]), pack2_rne(x[2], x[3]), pack2_rne(x[4], x[5]),
-                                                          pack2_rne(x[6], x[7])});
-        }
+        for (int i = 0; i < 8; ++i) o[nb][i] *= alpha;
       }
+      float pv[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (NB > 1 && i == 0) load_v(4, 8);
+      for (int i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(s[nb][i >> 2][i & 3] - m[nb]);
+        l[nb] += x;
+        pv[i] = x * step(vst, 8 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3));
+      }
+      if (!whole)  // an unseen key's step may be anything
 #pragma unroll
-        for (int beta = 0; beta < 2; ++beta) {
-          const bf16x8 va = codes8(vx[i][2 * beta], vx[i][2 * beta + 1]);
+        for (int i = 0; i < 16; ++i) pv[i] = s[nb][i >> 2][i & 3] == -INFINITY ? 0.f : pv[i];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) o[nb][i] = mfma16(va, pf[nb][beta], o[nb][i]);
-        }
+      for (int beta = 0; beta < 2; ++beta) {
+        const float* x = pv + 8 * beta;
+        pf[nb][beta] = __builtin_bit_cast(bf16x8, u32x4{pack2_rne(x[0], x[1]), pack2_rne(x[2], x[3]), pack2_rne(x[4], x[5]),
+                                                        pack2_rne(x[6], x[7])});
       }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (NB > 1 && i == 0) load_v(4, 8);
+#pragma unroll
+      for (int beta = 0; beta < 2; ++beta) {
+        const bf16x8 va = codes8(vx[i][2 * beta], vx[i][2 * beta + 1]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) o[nb][i] = mfma16(va, pf[nb][beta], o[nb][i]);
+      }
+    }
+  }
+};
 
+template <int NB, bool PRE>
+__device__ __forceinline__ void few_rows(const DecArgs& a, int* first, int block) {
+  const int n_seg = PRE ? a.n_groups : a.s.B, R = a.part[PRE].rows;
+  const int total = deal<PRE, false>(a, first, block);
+  const int worker = block * kFewWaves + uni(threadIdx.x >> 6), all = total * a.Hkv;
+  const int run = run_tiles<false>(all, a.part[PRE].workers);
+  int at = worker * run;  // workers * run stays below all + workers
+  const int stop = min(at + run, all);
+  while (at < stop) {
+    const int h = at / total, pos = at - h * total, seg = find_segment(first, n_seg, pos);
+    const int i0 = pos - uni(first[seg]), n = uni(first[seg + 1]) - uni(first[seg]), i1 = min(n, i0 + stop - at);
+    at += i1 - i0;
+    const Sight si = sight<PRE>(a, seg);
+    Few<NB> f;
+    f.template begin<PRE>(a, seg, h, si.hi);
+    int ids = 0;  // lane x: the id of the run's page i0 + x, 64 at a time
+    for (int i = i0; i < i1; ++i) {
+      const int x = (i - i0) & 63, lane = threadIdx.x & 63;
+      if (x == 0) ids = i + lane < i1 ? page_id<PRE>(a, seg, a.W ? si.page(i + lane) : i + lane) : 0;
+      const int id = __builtin_amdgcn_readlane(ids, x);
+      f.page(a, page_at(a, id, h), page_ok(a, id), a.W ? si.page(i) : i);
+    }
     const int l2 = (int)opaque(threadIdx.x) & 63, c15 = l2 & 15, cg = l2 >> 4;
-    const int64_t slot = (int64_t)worker + (int64_t)h * n_seg + seg;
+    const bool done = !PRE && !a.n_groups && i1 - i0 == n;  // the rows' only piece
+    const int64_t slot = slot_of<PRE>(a, worker, (int64_t)h * n_seg + seg, i0 == 0);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float l = quad_sum(l_run[nb]);
+      const float l = quad_sum(f.l[nb]);
       const int r = 16 * nb + c15;
-      if (r < R) {
-        float* to = a.part_o[PRE] + (slot * R + r) * kKv8Hd + 4 * cg;
+      if (r >= R) continue;
+      if (done) {
+        const Row w = row_of<PRE>(a, seg, h, r, si.hi);
+        if (w.hi) write_row<16, 8>(a, w, f.o[nb], f.m[nb], l, cg);  // (else the join does)
+        continue;
+      }
+      float* to = a.part[PRE].o + (slot * R + r) * kKv8Hd + 4 * cg;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<f32x4*>(to + 16 * i) = o[nb][i];
-        if (cg == 0) {
-          a.part_m[PRE][2 * (slot * R + r)] = m_run[nb];
-          a.part_m[PRE][2 * (slot * R + r) + 1] = l;
-        }
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<f32x4*>(to + 16 * i) = f.o[nb][i];
+      if (cg == 0) {
+        a.part[PRE].m[2 * (slot * R + r)] = f.m[nb];
+        a.part[PRE].m[2 * (slot * R + r) + 1] = l;
       }
     }
   }
 }
 
+// One workgroup a sequence and head, its pages dealt to WAVES wavefronts and joined in
+// LDS: where the pages are few this one launch ends sooner than pieces and their join.
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) kv8_whole_kernel(const DecArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int R = a.part[0].rows, wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int h = blockIdx.x % a.Hkv, seg = blockIdx.x / a.Hkv;
+  const Sight si = sight<false>(a, seg);
+  Few<1> f;
+  f.template begin<false>(a, seg, h, si.hi);
+  for (int i = wave; i < si.n; i += WAVES) {
+    const int p = si.page(i), id = uni(page_id<false>(a, seg, p));
+    f.page(a, page_at(a, id, h), page_ok(a, id), p);
+  }
+  float* const ml = reinterpret_cast<float*>(smem);             // [WAVES][2][R]
+  f32x4* const ov = reinterpret_cast<f32x4*>(smem + WAVES * 128);  // [WAVES][R][32]
+  const float l = quad_sum(f.l[0]);
+  const int r15 = lane & 15, g = lane >> 4;
+  if (r15 < R) {
+    if (g == 0) {
+      ml[wave * 32 + r15] = f.m[0];
+      ml[wave * 32 + 16 + r15] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ov[(wave * R + r15) * 32 + 4 * i + g] = f.o[0][i];
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < R * 32; x += WAVES * 64) {
+    const int r = x >> 5;
+    float M = ml[r], L = 0.f;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) M = fmax_nc(M, ml[w * 32 + r]);
+    f32x4 acc{};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float c = __builtin_amdgcn_exp2f(ml[w * 32 + r] - M);
+      L += ml[w * 32 + 16 + r] * c;
+      acc += ov[(w * R + r) * 32 + (x & 31)] * c;
+    }
+    const Row w = row_of<false>(a, seg, h, r, si.hi);
+    if (w.hi == 0) {  // padding: zeros and -inf
+      acc = f32x4{};
+      L = 0.f;
+    }
+    write_row<4, 1>(a, w, &acc, M, L, x & 31);
+  }
+}
+
 // ------------------------------------------------------------- many rows
-// One workgroup of four wavefronts per (segment, head, 128 rows, piece); a wavefront
-// owns 32 rows as in attention for training (attention_train.hip). A page is the tile:
-// the workgroup's threads load its codes into registers while the tile before is worked
-// on, convert them and write them to LDS in the order in which the products' operands are
-// read (1 KB of 64 lanes each, padded so that the writes spread over the banks).
+// A column is 128 rows of a segment and head, a tile one of its pages, and the workers are
+// workgroups of four wavefronts; a wavefront owns 32 rows as in attention for training
+// (attention_train.hip). The workgroup's threads load a page's codes into registers while
+// the tile before is worked on, convert them and write them to LDS in the order in which
+// the products' operands are read (1 KB of 64 lanes each, padded so that the writes spread
+// over the banks).
 constexpr int kManyWaves = 4;
-constexpr int kManyRows = 32 * kManyWaves;
 constexpr int kKFrag = 1040, kVFrag = 1056;           // bytes of an operand of 64 lanes
 constexpr int kVTile = 16 * kKFrag;                   // after the 16 of k
 constexpr int kSteps = kVTile + 16 * kVFrag;          // f32 steps of k (times scale) and v
@@ -377,291 +490,377 @@ constexpr int kManyBuf = kSteps + 2 * kPage * 4;      // 34,048 bytes
 constexpr int kManyLds = 2 * kManyBuf;
 
 template <bool PRE>
-__global__ void __launch_bounds__(kManyWaves * 64, 2) kv8_many_kernel(const DecArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, lh = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int R = a.rows[PRE], nrb = (R + kManyRows - 1) / kManyRows;
-  int id = blockIdx.x;
-  const int h = id % a.Hkv;
-  id /= a.Hkv;
-  const int rb = id % nrb;
-  id /= nrb;
-  const int piece = id % a.n_max[PRE], seg = id / a.n_max[PRE];
-  const Sight si = sight<PRE>(a, seg);
-  if (piece >= si.n) return;
-  const int chunk = si.chunk_at(piece);
-
-  const int r = rb * kManyRows + 32 * wave + lq;
-  const Row w = row_of<PRE>(a, seg, h, min(r, R - 1), si.hi);
-  const bool live = r < R && w.hi > 0;
-  // pages that the workgroup's rows read of the piece: the last of their keys
-  int last = live ? w.hi : 0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) last = max(last, __shfl_xor(last, o));
-  int* const lasts = reinterpret_cast<int*>(smem);
-  if (lane == 0) lasts[wave] = last;
-  __syncthreads();
-  last = max(max(lasts[0], lasts[1]), max(lasts[2], lasts[3]));
-  __syncthreads();
-  const int p0 = chunk * a.chunk[PRE], p1 = min(min(p0 + a.chunk[PRE], (si.hi + kPage - 1) / kPage), (last + kPage - 1) / kPage);
-
-  bf16x8 qf[8];
-  load_rows(qf, a.q + w.q_row * a.q_ld + (int64_t)w.head * kKv8Hd, live, lh);
-  f32x16 o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = f32x16{};
-  float m_run = kNoMax, l_run = 0.f;
-
+__device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int block) {
+  const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, lh = lane >> 5, wave = uni(tid >> 6);
+  const int n_seg = PRE ? a.n_groups : a.s.B, R = a.part[PRE].rows, all_rb = (R + kManyRows - 1) / kManyRows;
+  int* const first = reinterpret_cast<int*>(smem + kManyLds);
+  const int total = deal<PRE, true>(a, first, block), all = total * a.Hkv;
+  const int run = run_tiles<true>(all, a.part[PRE].workers);
   lds_char* const lds = (lds_char*)smem;
-  u32x4 kx[2], vx[2];
-  uint32_t st = 0;
-  auto fetch = [&](int p) {
-    const int64_t pid = __builtin_amdgcn_readfirstlane((int)page_id<PRE>(a, seg, p));
-    const bool ok = pid >= 0 && pid < a.n_pages;
-    const uint8_t* pg = a.cache + ((ok ? pid : 0) * a.Hkv + h) * kHeadB;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      kx[i] = *reinterpret_cast<const u32x4*>(pg + 16 * (tid + 256 * i));
-      vx[i] = *reinterpret_cast<const u32x4*>(pg + kVOff + 16 * (tid + 256 * i));
-    }
-    if (tid < 2 * kPage) {
-      st = *reinterpret_cast<const uint16_t*>(pg + kKStepOff + 2 * tid);
-      if (!ok) st = 0x7fc0u;
-    }
-  };
-  // 16 codes of token q >> 3, channels 16 (q & 7) .., or of channel q >> 2 and 16 tokens
-  auto stage = [&](lds_char* to) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = tid + 256 * i;
-      {
-        const int key = q >> 3, s = q & 7;
-        lds_char* x = to + ((key >> 5) * 8 + s) * kKFrag + (key & 31) * 16;
-        *(lds_bf16x8*)x = codes8(kx[i][0], kx[i][1]);
-        *(lds_bf16x8*)(x + 512) = codes8(kx[i][2], kx[i][3]);
-      }
-      {
-        const int d = q >> 2, s2 = q & 3;
-        lds_char* x = to + kVTile + ((d >> 5) * 4 + s2) * kVFrag + (d & 31) * 16;
-        *(lds_bf16x8*)x = codes8(vx[i][0], vx[i][1]);
-        *(lds_bf16x8*)(x + 512) = codes8(vx[i][2], vx[i][3]);
+  int at = block * run;
+  const int stop = min(at + run, all);
+  while (at < stop) {
+    const int h = at / total, pos = at - h * total, seg = find_segment(first, n_seg, pos);
+    const int nrb = uni(row_blocks<PRE, true>(a, seg)), n = (uni(first[seg + 1]) - uni(first[seg])) / nrb;
+    const int rem = pos - uni(first[seg]), rb = rem / n, i0 = rem - rb * n, i1 = min(n, i0 + stop - at);
+    at += i1 - i0;
+    const Sight si = sight<PRE>(a, seg);
+    const int r = rb * kManyRows + 32 * wave + lq;
+    const Row w = row_of<PRE>(a, seg, h, min(r, R - 1), si.hi);
+    const bool live = r < R && w.hi > 0;
+    // of the list, what the block's rows see: to the last row's own key, from the first row's window on
+    int from = i0, to = i1;
+    if (!PRE) {
+      const Kv8Len ln = kv8_len(a.s, seg);
+      const int t0 = rb * kManyRows / a.G, t1 = min((rb * kManyRows + kManyRows - 1) / a.G, ln.fresh - 1);
+      const int p1 = (ln.len - ln.fresh + t1) / kPage + 1;  // pages that hold keys up to t1's
+      to = uni(min(to, si.ns + max(p1 - si.c0, 0)));
+      if (a.W) {
+        const int skip = si.ns + max(max(ln.len - ln.fresh + t0 - a.W + 1, 0) / kPage - si.c0, 0);
+        // (a list without pages of its own for sinks may hold some)
+        if (from >= si.ns && from < skip && si.page(from) * kPage >= a.S - prefix_len(a, seg)) from = skip;
+        from = uni(from);
       }
     }
-    if (tid < 2 * kPage) {
-      const float f = __uint_as_float(st << 16);
-      *(__attribute__((address_space(3))) float*)(to + kSteps + 4 * tid) = tid < kPage ? f * a.scale_log2 : f;
-    }
-  };
 
-  auto step = [&](int p, const lds_char* rd) {
-    const int key0 = p * kPage;
-    f32x16 s[2] = {f32x16{}, f32x16{}};
-    const lds_char* kr = rd + lane * 16;
+    bf16x8 qf[8];
+    load_rows(qf, a.q + w.q_row * a.q_ld + (int64_t)w.head * kKv8Hd, true, lh);
+    f32x16 o[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      s[i & 1] = mfma(*(const lds_bf16x8*)(kr + ((i & 1) * 8 + (i >> 1)) * kKFrag), qf[i >> 1], s[i & 1]);
-    const lds_char* sp = rd + kSteps + 16 * lh;  // steps of keys 32 kb + 8 i + 4 lh + e
+    for (int i = 0; i < 4; ++i) o[i] = f32x16{};
+    float m_run = kNoMax, l_run = 0.f;
+
+    u32x4 kx[2], vx[2];
+    uint32_t st = 0;
+    int ids = 0;
+    auto fetch = [&](int i) {
+      const int x = (i - from) & 63;
+      if (x == 0) ids = i + lane < to ? page_id<PRE>(a, seg, a.W ? si.page(i + lane) : i + lane) : 0;
+      const int id = __builtin_amdgcn_readlane(ids, x);
+      const uint8_t* pg = page_at(a, id, h);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 f = *(const lds_f32x4*)(sp + 128 * kb + 32 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[kb][4 * i + e] *= f[e];
+      for (int y = 0; y < 2; ++y) {
+        kx[y] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(16 * (tid + 256 * y)));
+        vx[y] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + 16 * (tid + 256 * y)));
       }
-    const bool whole = __all(!live || (key0 + kPage <= w.hi && (key0 >= w.lo || key0 + kPage <= w.sunk)));
-    if (!whole)
+      if (tid < 2 * kPage) {
+        st = *reinterpret_cast<const uint16_t*>(pg + (uint32_t)(kKStepOff + 2 * tid));
+        if (!page_ok(a, id)) st = 0x7fc0u;
+      }
+    };
+    // 16 codes of token q >> 3, channels 16 (q & 7) .., or of channel q >> 2 and 16 tokens
+    auto stage = [&](lds_char* to) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q = tid + 256 * i;
+        {
+          const int key = q >> 3, s = q & 7;
+          lds_char* x = to + ((key >> 5) * 8 + s) * kKFrag + (key & 31) * 16;
+          *(lds_bf16x8*)x = codes8(kx[i][0], kx[i][1]);
+          *(lds_bf16x8*)(x + 512) = codes8(kx[i][2], kx[i][3]);
+        }
+        {
+          const int d = q >> 2, s2 = q & 3;
+          lds_char* x = to + kVTile + ((d >> 5) * 4 + s2) * kVFrag + (d & 31) * 16;
+          *(lds_bf16x8*)x = codes8(vx[i][0], vx[i][1]);
+          *(lds_bf16x8*)(x + 512) = codes8(vx[i][2], vx[i][3]);
+        }
+      }
+      if (tid < 2 * kPage) {
+        const float f = __uint_as_float(st << 16);
+        *(__attribute__((address_space(3))) float*)(to + kSteps + 4 * tid) = tid < kPage ? f * a.scale_log2 : f;
+      }
+    };
+
+    auto step = [&](int p, const lds_char* rd) {
+      const int key0 = p * kPage;
+      f32x16 s[2] = {f32x16{}, f32x16{}};
+      const lds_char* kr = rd + lane * 16;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        s[i & 1] = mfma(*(const lds_bf16x8*)(kr + ((i & 1) * 8 + (i >> 1)) * kKFrag), qf[i >> 1], s[i & 1]);
+      const lds_char* sp = rd + kSteps + 16 * lh;  // steps of keys 32 kb + 8 i + 4 lh + e
+      // Scores relative to the maximum so far, in one instruction each (to 0 before a row
+      // has seen anything: its maximum then moves whatever it is).
+      const bool unset = m_run == kNoMax;
+      const float base = unset ? 0.f : m_run;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = key0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
-          const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
-          s[kb][e] = in ? s[kb][e] : -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 f = *(const lds_f32x4*)(sp + 128 * kb + 32 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[kb][4 * i + e] = __builtin_fmaf(s[kb][4 * i + e], f[e], -base);
         }
-    float m2[2];
+      const bool whole = __all(!live | ((key0 + kPage <= w.hi) & ((key0 >= w.lo) | (key0 + kPage <= w.sunk))));
+      if (!whole)
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      m2[kb] = s[kb][0];
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int e = 1; e < 16; ++e) m2[kb] = fmax_nc(m2[kb], s[kb][e]);
-    }
-    const float mt = pair_max(fmax_nc(m2[0], m2[1]));
-    if (__any(mt > m_run + kSlack)) {
-      const float m_new = fmax_nc(m_run, mt);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-      m_run = m_new;
-      l_run *= alpha;
+          for (int e = 0; e < 16; ++e) {
+            const int j = key0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
+            const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
+            s[kb][e] = in ? s[kb][e] : -INFINITY;
+          }
+      float m2[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= alpha;
-    }
-    u32x4 pw[4];
+      for (int kb = 0; kb < 2; ++kb) {
+        m2[kb] = s[kb][0];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 f = *(const lds_f32x4*)(sp + kPage * 4 + 128 * kb + 32 * i);
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = __builtin_amdgcn_exp2f(s[kb][4 * i + e] - m_run);
-          l_run += y;
-          x[e] = y * f[e];
-        }
-        if (!whole)  // an unseen key's step may be anything
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = s[kb][4 * i + e] == -INFINITY ? 0.f : x[e];
-        pw[2 * kb + (i >> 1)][2 * (i & 1)] = pack2_rne(x[0], x[1]);
-        pw[2 * kb + (i >> 1)][2 * (i & 1) + 1] = pack2_rne(x[2], x[3]);
+        for (int e = 1; e < 16; ++e) m2[kb] = fmax_nc(m2[kb], s[kb][e]);
       }
-    const lds_char* vr = rd + kVTile + lane * 16;
+      const float mt = pair_max(fmax_nc(m2[0], m2[1]));
+      const bool up = mt > (unset ? -INFINITY : kSlack);
+      if (__any(up)) {  // each row's moves by itself
+        const float m_new = up ? base + mt : m_run, by = up ? m_new - base : 0.f;
+        const float alpha = unset ? 1.f : __builtin_amdgcn_exp2f(-by);
+        m_run = m_new;
+        l_run *= alpha;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      o[i & 3] = mfma(*(const lds_bf16x8*)(vr + ((i & 3) * 4 + (i >> 2)) * kVFrag), __builtin_bit_cast(bf16x8, pw[i >> 2]), o[i & 3]);
-  };
+        for (int i = 0; i < 4; ++i) o[i] *= alpha;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[kb][e] -= by;
+      }
+      u32x4 pw[4];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 f = *(const lds_f32x4*)(sp + kPage * 4 + 128 * kb + 32 * i);
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = __builtin_amdgcn_exp2f(s[kb][4 * i + e]);
+            l_run += y;
+            x[e] = y * f[e];
+          }
+          if (!whole)  // an unseen key's step may be anything
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = s[kb][4 * i + e] == -INFINITY ? 0.f : x[e];
+          pw[2 * kb + (i >> 1)][2 * (i & 1)] = pack2_rne(x[0], x[1]);
+          pw[2 * kb + (i >> 1)][2 * (i & 1) + 1] = pack2_rne(x[2], x[3]);
+        }
+      const lds_char* vr = rd + kVTile + lane * 16;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        o[i & 3] = mfma(*(const lds_bf16x8*)(vr + ((i & 3) * 4 + (i >> 2)) * kVFrag), __builtin_bit_cast(bf16x8, pw[i >> 2]), o[i & 3]);
+    };
 
-  if (p0 < p1) {
-    fetch(p0);
-    stage(lds);
-  }
-  for (int p = p0; p < p1; ++p) {
-    __syncthreads();  // tile p is whole, and every wavefront is done with tile p - 1
-    lds_char *x = lds + ((p - p0) & 1) * kManyBuf, *y = lds + (~(p - p0) & 1) * kManyBuf;
-    if (p + 1 < p1) fetch(p + 1);
-    step(p, x);
-    if (p + 1 < p1) stage(y);
-  }
+    __syncthreads();  // every wavefront is done with the run before
+    if (from < to) {
+      fetch(from);
+      stage(lds);
+    }
+    for (int i = from; i < to; ++i) {
+      __syncthreads();  // tile i is whole, and every wavefront is done with tile i - 1
+      lds_char *x = lds + ((i - from) & 1) * kManyBuf, *y = lds + (~(i - from) & 1) * kManyBuf;
+      if (i + 1 < to) fetch(i + 1);
+      step(a.W ? si.page(i) : i, x);
+      if (i + 1 < to) stage(y);
+    }
 
-  const float l = pair_sum(l_run);
-  if (r >= R) return;
-  const int64_t slot = (((int64_t)seg * a.Hkv + h) * a.n_max[PRE] + piece) * R + r;
-  if (lh == 0) {
-    a.part_m[PRE][2 * slot] = m_run;
-    a.part_m[PRE][2 * slot + 1] = l;
+    const float l = pair_sum(l_run);
+    if (!PRE && !a.n_groups && i1 - i0 == n) {  // the rows' only piece
+      if (live) {
+        store_rows(a.out + w.q_row * a.o_ld + (int64_t)w.head * kKv8Hd, o, l == 0.f ? 0.f : 1.0f / l, lh);
+        if (lh == 0) write_lse(a, w, m_run, l);
+      }
+    } else if (r < R) {
+      const int64_t column = ((int64_t)h * n_seg + seg) * all_rb + rb;
+      const int64_t slot = slot_of<PRE>(a, block, column, i0 == 0) * kManyRows + 32 * wave + lq;
+      if (lh == 0) {
+        a.part[PRE].m[2 * slot] = m_run;
+        a.part[PRE].m[2 * slot + 1] = l;
+      }
+      float* po = a.part[PRE].o + slot * kKv8Hd + 4 * lh;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4*>(po + 32 * db + 8 * i) =
+              f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+    }
   }
-  float* to = a.part_o[PRE] + slot * kKv8Hd + 4 * lh;
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4*>(to + 32 * db + 8 * i) = f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+}
+
+// How a part's rows are worked on.
+enum Kind { kNone, kFew16, kFew32, kMany };
+
+// The own tokens' workgroups first: with a prefix of many rows theirs wait for memory
+// while the others compute.
+template <Kind PREFIX, Kind OWN>
+__global__ void __launch_bounds__(256, PREFIX <= kFew16 && OWN == kFew16 ? 3 : 2) kv8_pieces_kernel(const DecArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int block = blockIdx.x;
+  if (PREFIX == kNone || block < a.part[0].blocks) {
+    if constexpr (OWN == kMany) many_rows<false>(a, smem, block);
+    if constexpr (OWN == kFew16) few_rows<1, false>(a, reinterpret_cast<int*>(smem), block);
+    if constexpr (OWN == kFew32) few_rows<2, false>(a, reinterpret_cast<int*>(smem), block);
+  } else {
+    const int b = block - a.part[0].blocks;
+    if constexpr (PREFIX == kMany) many_rows<true>(a, smem, b);
+    if constexpr (PREFIX == kFew16) few_rows<1, true>(a, reinterpret_cast<int*>(smem), b);
+    if constexpr (PREFIX == kFew32) few_rows<2, true>(a, reinterpret_cast<int*>(smem), b);
+  }
 }
 
 // ------------------------------------------------------------------ join
-// The pieces of a row: `n` of them, `step` rows of results apart.
-struct Pieces { int64_t at; int n; int64_t step; };
+// The pieces of a row: `n` of them, of the workers from w0 on.
+struct Pieces {
+  int n = 0, w0 = 0, rows = 0, r = 0;  // rows of a slot, and the row's place in it
+  int64_t column = 0;
+};
 template <bool PRE>
 __device__ __forceinline__ Pieces pieces_of(const DecArgs& a, int seg, int h, int r) {
-  Pieces p{0, 0, a.rows[PRE]};
-  if (a.n_max[PRE] == 0) return p;
-  if (a.workers[PRE]) {
-    const int n_seg = PRE ? a.n_groups : a.s.B, total = a.first[PRE][n_seg];
-    const int from = a.first[PRE][seg], to = a.first[PRE][seg + 1];
-    if (to > from) {
-      const int run = run_pages(total * a.Hkv, a.workers[PRE]);
-      const int w0 = (h * total + from) / run, w1 = (h * total + to - 1) / run;
-      p.n = w1 - w0 + 1;
-      p.at = ((int64_t)w0 + (int64_t)h * n_seg + seg) * a.rows[PRE] + r;
-    }
-  } else {
-    p.n = sight<PRE>(a, seg).n;
-    p.at = ((int64_t)seg * a.Hkv + h) * a.n_max[PRE] * a.rows[PRE] + r;
+  Pieces p;
+  const Part& k = a.part[PRE];
+  if (k.workers == 0) return p;
+  const int n_seg = PRE ? a.n_groups : a.s.B, total = k.first[n_seg], from = k.first[seg], to = k.first[seg + 1];
+  if (to == from) return p;
+  const bool many = k.rows > kFewRows;
+  int begin = h * total + from, n = to - from, rb = 0;
+  if (many) {
+    n /= row_blocks<PRE, true>(a, seg);
+    rb = r / kManyRows;
+    begin += rb * n;
   }
+  const int run = many ? run_tiles<true>(total * a.Hkv, k.workers) : run_tiles<false>(total * a.Hkv, k.workers);
+  p.w0 = begin / run;
+  p.n = (begin + n - 1) / run - p.w0 + 1;
+  p.rows = many ? kManyRows : k.rows;
+  p.r = r - rb * kManyRows;
+  p.column = ((int64_t)h * n_seg + seg) * (many ? (k.rows + kManyRows - 1) / kManyRows : 1) + rb;
   return p;
 }
+template <bool PRE>
+__device__ __forceinline__ int64_t piece_row(const DecArgs& a, const Pieces& p, int x) {
+  return slot_of<PRE>(a, p.w0 + x, p.column, x == 0) * p.rows + p.r;
+}
 
-// WAVES wavefronts a row (b, t, query head): its pieces, prefix first, weighed by their
-// maxima. Half a wavefront reads a piece's 128 values.
+// WAVES wavefronts a row (b, t, query head): half a wavefront reads a piece's 128 values,
+// weighed by their maxima.
 template <int WAVES>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
   __shared__ __attribute__((aligned(16))) float lds_o[4][kKv8Hd];
-  __shared__ float lds_l[4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t i = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
-  const int part = wave % WAVES;  // of the row's wavefronts
+  __shared__ float lds_m[4], lds_l[4];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+  const int share = wave % WAVES;  // of the row's wavefronts
   const int Hq = a.Hkv * a.G;
-  if (i >= (int64_t)a.s.B * a.s.T * Hq) return;
-  const int64_t tok = i / Hq;
-  const int hq = (int)(i % Hq), b = (int)(tok / a.s.T), t = (int)(tok % a.s.T), h = hq / a.G;
-  const Kv8Len len = kv8_len(a.s, b);
-  Pieces p[2] = {{0, 0, 0}, {0, 0, 0}};
-  if (t < len.fresh) {
-    const int r = t * a.G + hq % a.G;
-    p[0] = pieces_of<false>(a, b, h, r);
-    if (a.n_groups) p[1] = pieces_of<true>(a, b / a.gs, h, (b % a.gs) * a.s.T * a.G + r);
+  if (row >= (int64_t)a.s.B * a.s.T * Hq) return;
+  Row w;
+  w.q_row = row / Hq;
+  w.head = (int)(row % Hq);
+  const int b = (int)(w.q_row / a.s.T), t = (int)(w.q_row % a.s.T), h = w.head / a.G;
+  Pieces own, pre;
+  if (t < kv8_len(a.s, b).fresh) {
+    const int r = t * a.G + w.head % a.G;
+    own = pieces_of<false>(a, b, h, r);
+    if (a.n_groups) pre = pieces_of<true>(a, b / a.gs, h, (b % a.gs) * a.s.T * a.G + r);
+    else if (own.n == 1) return;  // written already
   }
-  float M = kNoMax;
-#pragma unroll
-  for (int k = 1; k >= 0; --k)
-    for (int x = lane; x < p[k].n; x += 64) M = fmax_nc(M, a.part_m[k][2 * (p[k].at + x * p[k].step)]);
-  M = quad_max(M);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) M = fmax_nc(M, __shfl_xor(M, o));
+  float M = kNoMax, L = 0.f;
   f32x4 acc{};
-  float L = 0.f;
+  const int all = pre.n + own.n;
+  constexpr int kAhead = 4;
+  for (int x0 = 2 * share + (lane >> 5); x0 < all; x0 += 2 * WAVES * kAhead) {
+    float m[kAhead], l[kAhead];
+    f32x4 o[kAhead];
 #pragma unroll
-  for (int k = 1; k >= 0; --k) {
-#pragma unroll 4
-    for (int x = 2 * part + (lane >> 5); x < p[k].n; x += 2 * WAVES) {
-      const int64_t at = p[k].at + x * p[k].step;
-      const float wgt = __builtin_amdgcn_exp2f(a.part_m[k][2 * at] - M);
-      L += a.part_m[k][2 * at + 1] * wgt;
-      acc += *reinterpret_cast<const f32x4*>(a.part_o[k] + at * kKv8Hd + 4 * (lane & 31)) * wgt;
+    for (int y = 0; y < kAhead; ++y) {
+      const int x = x0 + 2 * WAVES * y;
+      m[y] = kNoMax;
+      l[y] = 0.f;
+      o[y] = f32x4{};
+      if (x < all) {
+        const bool p = x < pre.n;
+        const int64_t at = p ? piece_row<true>(a, pre, x) : piece_row<false>(a, own, x - pre.n);
+        const float* const ml = (p ? a.part[1].m : a.part[0].m) + 2 * at;
+        m[y] = ml[0];
+        l[y] = ml[1];
+        o[y] = *reinterpret_cast<const f32x4*>((p ? a.part[1].o : a.part[0].o) + at * kKv8Hd + 4 * (lane & 31));
+      }
+    }
+    float m_new = M;
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) m_new = fmax_nc(m_new, m[y]);
+    const float alpha = __builtin_amdgcn_exp2f(M - m_new);
+    L *= alpha;
+    acc *= alpha;
+    M = m_new;
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const float c = __builtin_amdgcn_exp2f(m[y] - M);
+      L += l[y] * c;
+      acc += o[y] * c;
     }
   }
-  L = pair_sum(L);
+  const float both = pair_max(M), c = __builtin_amdgcn_exp2f(M - both);
+  M = both;
+  L = pair_sum(L * c);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] = pair_sum(acc[e]);
+  for (int e = 0; e < 4; ++e) acc[e] = pair_sum(acc[e] * c);
   if (WAVES > 1) {
     if (lane < 32) *reinterpret_cast<f32x4*>(&lds_o[wave][4 * lane]) = acc;
-    if (lane == 0) lds_l[wave] = L;
+    if (lane == 0) {
+      lds_m[wave] = M;
+      lds_l[wave] = L;
+    }
     __syncthreads();
-    if (part) return;
+    if (share) return;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) {
-      acc += *reinterpret_cast<const f32x4*>(&lds_o[wave + w][4 * (lane & 31)]);
-      L += lds_l[wave + w];
+    for (int x = 1; x < WAVES; ++x) M = fmax_nc(M, lds_m[wave + x]);
+    L = 0.f;
+    acc = f32x4{};
+#pragma unroll
+    for (int x = 0; x < WAVES; ++x) {
+      const float f = __builtin_amdgcn_exp2f(lds_m[wave + x] - M);
+      L += lds_l[wave + x] * f;
+      acc += *reinterpret_cast<const f32x4*>(&lds_o[wave + x][4 * (lane & 31)]) * f;
     }
   }
-  const float f = L == 0.f ? 0.f : 1.0f / L;  // nothing seen: zeros and -inf; NaN stays
-  if (lane < 32)
-    *reinterpret_cast<u32x2a*>(a.out + tok * a.o_ld + (int64_t)hq * kKv8Hd + 4 * lane) =
-        u32x2a{pack2_rne(acc[0] * f, acc[1] * f), pack2_rne(acc[2] * f, acc[3] * f)};
-  if (lane == 0)
-    a.lse[((int64_t)b * Hq + hq) * a.s.T + t] =
-        L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
+  if (lane < 32) write_row<4, 1>(a, w, &acc, M, L, lane);
 }
 
 // ------------------------------------------------------------------ host
-constexpr int kFewRows = 32;  // rows that kv8_few_kernel takes
-
-// How a kind of segments is cut: n_table pages at most, of which a window of `span`
-// keys (0 = none) and the first `sinks` are seen. The chip's size is taken as it is
-// (256 CUs): the workspace's size must not depend on the device that asks.
-struct Cut { int chunk, n_max, workers; int64_t slots; };
-Cut cut(int64_t n_table, int64_t span, int64_t sinks, int64_t rows, int64_t segments, int64_t heads) {
-  if (n_table == 0 || segments == 0 || rows == 0) return {1, 0, 0, 0};
-  auto most = [&](int64_t c) {  // pieces of c pages
-    const int64_t n = cdiv(n_table, c);
-    return span ? std::min(n, (span + c * kPage - 2) / (c * kPage) + 1 + cdiv(sinks, c * kPage)) : n;
-  };
-  if (rows <= kFewRows) {
-    const int64_t pages = segments * heads * most(1), per_cu = kFewWaves * (rows <= 16 ? 3 : 2);
-    const int workers = (int)(cdiv(std::min<int64_t>(pages, 256 * per_cu), kFewWaves) * kFewWaves);
-    return {1, (int)most(1), workers, workers + segments * heads};
+// The work of a kind of segments: n_table pages at most, of which a window of `span`
+// keys (0 = none) and the first `sinks` are seen. The chip is taken as it is (256 CUs), so
+// that the workspace's size does not depend on the device that asks.
+struct Deal {
+  Kind kind = kNone;
+  int64_t tiles = 0;  // at most
+  int workers = 0, blocks = 0;
+  int64_t slots = 0, slot_rows = 0, pages = 0;
+};
+Deal deal_of(int64_t n_table, int64_t span, int64_t sinks, int64_t rows, int64_t segments, int64_t heads, bool prefixes,
+             bool beside_many) {
+  Deal d;
+  if (n_table == 0 || segments == 0 || rows == 0) return d;
+  d.pages = span ? std::min(n_table, (span + kPage - 2) / kPage + 1 + cdiv(sinks, kPage)) : n_table;
+  d.kind = rows <= 16 ? kFew16 : rows <= kFewRows ? kFew32 : kMany;
+  const int64_t row_blocks = d.kind == kMany ? cdiv(rows, kManyRows) : 1, columns = segments * heads * row_blocks;
+  d.tiles = columns * d.pages;
+  if (d.kind == kMany) {
+    d.blocks = d.workers = (int)std::min<int64_t>(cdiv(d.tiles, 2), 512);  // two workgroups a CU
+    d.slot_rows = kManyRows;
+  } else {
+    d.blocks = (int)std::min<int64_t>(cdiv(d.tiles, kFewWaves), 256 * (beside_many ? 1 : d.kind == kFew16 ? 3 : 2));
+    d.workers = d.blocks * kFewWaves;
+    d.slot_rows = rows;
   }
-  const int64_t groups = segments * heads * cdiv(rows, kManyRows);
-  const int64_t c = std::max<int64_t>(4, cdiv(most(1), std::max<int64_t>(1, cdiv(1024, groups))));
-  return {(int)c, (int)most(c), 0, segments * heads * most(c)};
+  d.slots = prefixes ? d.workers + columns : 2 * (int64_t)d.workers;
+  return d;
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-// Sizes of both kinds of segments and the workspace's parts.
+// Both kinds of segments and the workspace's parts.
 struct Plan {
-  Cut c[2];
+  Deal d[2];
   int64_t rows[2];
   size_t o_at[2], m_at[2], first_at[2], bytes;
+  int whole;  // wavefronts of kv8_whole_kernel, 0: pieces and their join
 };
 Plan plan(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d) {
   Plan p{};
@@ -670,15 +869,23 @@ Plan plan(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d) 
   p.rows[0] = (int64_t)s->T * G;
   p.rows[1] = gs * s->T * G;
   // keys that the rows of a segment see between them, at most
-  p.c[0] = cut(s->n_table, d->window ? (int64_t)d->window + s->T - 1 : 0, S, p.rows[0], segs[0], H);
-  p.c[1] = cut(d->n_prefix_table, d->window, S, p.rows[1], segs[1], H);
+  p.d[1] = deal_of(d->n_prefix_table, d->window, S, p.rows[1], segs[1], H, true, false);
+  p.d[0] = deal_of(s->n_table, d->window ? (int64_t)d->window + s->T - 1 : 0, S, p.rows[0], segs[0], H, d->n_groups > 0,
+                   p.d[1].kind == kMany);
+  // One workgroup a sequence and head reads 16 pages in the time of a launch more.
+  if (d->n_groups == 0 && p.d[0].kind == kFew16 && p.d[0].pages <= 16) {
+    p.whole = s->B * H <= 256 ? 8 : 4;
+    return p;
+  }
   for (int k = 0; k < 2; ++k) {
+    if (p.d[k].kind == kNone) continue;
+    const size_t rows = (size_t)p.d[k].slots * p.d[k].slot_rows;
     p.o_at[k] = p.bytes;
-    p.bytes += round256((size_t)p.c[k].slots * p.rows[k] * kKv8Hd * 4);
+    p.bytes += round256(rows * kKv8Hd * 4);
     p.m_at[k] = p.bytes;
-    p.bytes += round256((size_t)p.c[k].slots * p.rows[k] * 8);
+    p.bytes += round256(rows * 8);
     p.first_at[k] = p.bytes;
-    p.bytes += p.c[k].workers ? round256((segs[k] + 1) * 4) : 0;
+    p.bytes += round256((segs[k] + 1) * 4);
   }
   return p;
 }
@@ -706,31 +913,64 @@ glt_status check_attn(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_k
   GLT_CHECK(rows < (1 << 25) / c->n_kv_heads, GLT_ERR_SHAPE, "%s: B=%d T=%d n_q_heads=%d", who, s->B, s->T, d->n_q_heads);
   if (s->B == 0 || s->T == 0) return GLT_OK;
   const Plan p = plan(c, s, d);
-  for (int k = 0; k < 2; ++k) {
-    const int64_t segs = k ? d->n_groups : s->B, groups = segs * c->n_kv_heads;
-    GLT_CHECK(p.c[k].workers ? groups * p.c[k].n_max < INT32_MAX - (1 << 16)
-                             : groups * cdiv(p.rows[k], kManyRows) * p.c[k].n_max < (1 << 24),
-              GLT_ERR_SHAPE, "%s: B=%d T=%d and tables of %d and %d pages", who, s->B, s->T, s->n_table, d->n_prefix_table);
+  for (int k = 0; k < 2; ++k)
+    GLT_CHECK(p.d[k].tiles < INT32_MAX - (1 << 16), GLT_ERR_SHAPE, "%s: B=%d T=%d and tables of %d and %d pages", who, s->B,
+              s->T, s->n_table, d->n_prefix_table);
+  return GLT_OK;
+}
+
+typedef void (*Kernel)(DecArgs);
+Kernel pieces_kernel(Kind prefix, Kind own) {
+  // [prefix][own]: a prefix has at least its sequences' rows
+  static const Kernel k[4][4] = {
+      {nullptr, kv8_pieces_kernel<kNone, kFew16>, kv8_pieces_kernel<kNone, kFew32>, kv8_pieces_kernel<kNone, kMany>},
+      {kv8_pieces_kernel<kFew16, kNone>, kv8_pieces_kernel<kFew16, kFew16>, nullptr, nullptr},
+      {kv8_pieces_kernel<kFew32, kNone>, kv8_pieces_kernel<kFew32, kFew16>, kv8_pieces_kernel<kFew32, kFew32>, nullptr},
+      {kv8_pieces_kernel<kMany, kNone>, kv8_pieces_kernel<kMany, kFew16>, kv8_pieces_kernel<kMany, kFew32>,
+       kv8_pieces_kernel<kMany, kMany>}};
+  return k[prefix][own];
+}
+
+// The dynamic-LDS limit is a per-device attribute of the kernels.
+constexpr int kMaxSegLds = (8192 + 1) * 4;
+glt_status set_limits(const char* who) {
+  static std::atomic<bool> set[64];
+  int dev = 0;
+  GLT_TRY_HIP(hipGetDevice(&dev));
+  GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "%s: device index %d out of range", who, dev);
+  if (set[dev].load(std::memory_order_acquire)) return GLT_OK;
+  for (int p = kNone; p <= kMany; ++p)
+    for (int o = kNone; o <= kMany; ++o)
+      if (const Kernel f = pieces_kernel((Kind)p, (Kind)o); f && (p == kMany || o == kMany))
+        GLT_TRY_HIP(hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, kManyLds + kMaxSegLds));
+  GLT_TRY_HIP(hipFuncSetAttribute((const void*)kv8_whole_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * (128 + 16 * 512)));
+  set[dev].store(true, std::memory_order_release);
+  return GLT_OK;
+}
+
+glt_status launch(DecArgs& a, const Plan& p, const char* who, hipStream_t st) {
+  const int64_t rows = (int64_t)a.s.B * a.s.T * a.Hkv * a.G;
+  const glt_status r = set_limits(who);
+  if (r != GLT_OK) return r;
+  if (p.whole) {
+    const size_t lds = p.whole * (128 + p.rows[0] * 512);
+    const dim3 grid((unsigned)(a.s.B * a.Hkv));
+    if (p.whole == 8) GLT_LAUNCH("kv8_whole", kv8_whole_kernel<8>, grid, dim3(512), lds, st, a);
+    else GLT_LAUNCH("kv8_whole", kv8_whole_kernel<4>, grid, dim3(256), lds, st, a);
+    GLT_LAUNCH_CHECK("kv8_whole");
+    return GLT_OK;
   }
-  return GLT_OK;
-}
-
-template <int NB, bool PRE>
-glt_status launch_few(const DecArgs& a, hipStream_t st) {
-  const size_t lds = (size_t)(PRE ? a.n_groups : a.s.B) * 4;
-  GLT_LAUNCH("kv8_few", (kv8_few_kernel<NB, PRE>), dim3(a.workers[PRE] / kFewWaves), dim3(kFewWaves * 64), lds, st, a);
-  GLT_LAUNCH_CHECK("kv8_few");
-  return GLT_OK;
-}
-
-template <bool PRE>
-glt_status launch_part(const DecArgs& a, hipStream_t st) {
-  if (a.n_max[PRE] == 0) return GLT_OK;
-  if (a.workers[PRE]) return a.rows[PRE] <= 16 ? launch_few<1, PRE>(a, st) : launch_few<2, PRE>(a, st);
-  const int64_t segs = PRE ? a.n_groups : a.s.B;
-  const int64_t grid = segs * a.n_max[PRE] * cdiv(a.rows[PRE], kManyRows) * a.Hkv;
-  GLT_LAUNCH("kv8_many", kv8_many_kernel<PRE>, dim3((unsigned)grid), dim3(kManyWaves * 64), kManyLds, st, a);
-  GLT_LAUNCH_CHECK("kv8_many");
+  if (const Kernel f = pieces_kernel(p.d[1].kind, p.d[0].kind)) {
+    const int segs = std::max(p.d[0].kind ? a.s.B : 0, p.d[1].kind ? a.n_groups : 0);
+    const size_t lds = (p.d[0].kind == kMany || p.d[1].kind == kMany ? kManyLds : 0) + (segs + 1) * 4;
+    GLT_LAUNCH("kv8_pieces", f, dim3((unsigned)(p.d[0].blocks + p.d[1].blocks)), dim3(256), lds, st, a);
+    GLT_LAUNCH_CHECK("kv8_pieces");
+  }
+  if (rows <= 4096)  // few rows of many pieces, mostly
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
+  else
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
+  GLT_LAUNCH_CHECK("kv8_join");
   return GLT_OK;
 }
 
@@ -775,17 +1015,6 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
       GLT_CHECK(!overlap(all[i], all[j]), GLT_ERR_INVALID_ARG,
                 "%s: out, lse and workspace must overlap neither each other nor q nor the cache", who);
 
-  int dev = 0;
-  GLT_TRY_HIP(hipGetDevice(&dev));
-  GLT_CHECK(dev >= 0 && dev < 64, GLT_ERR_HIP, "%s: device index %d out of range", who, dev);
-  // the dynamic-LDS limit is a per-device attribute of the kernels
-  static std::atomic<bool> attr_set[64];
-  if (!attr_set[dev].load(std::memory_order_acquire)) {
-    for (const void* f : {(const void*)kv8_many_kernel<false>, (const void*)kv8_many_kernel<true>})
-      GLT_TRY_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kManyLds));
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-
   DecArgs a{};
   a.cache = static_cast<const uint8_t*>(c->data);
   a.n_pages = c->n_pages;
@@ -809,23 +1038,9 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
   a.q_ld = q_ld;
   a.o_ld = o_ld;
   for (int k = 0; k < 2; ++k) {
-    a.chunk[k] = p.c[k].chunk;
-    a.n_max[k] = p.c[k].n_max;
-    a.workers[k] = p.c[k].workers;
-    a.first[k] = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.first_at[k]);
-    a.rows[k] = (int)p.rows[k];
-    a.part_o[k] = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_at[k]);
-    a.part_m[k] = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.m_at[k]);
+    char* const ws = static_cast<char*>(workspace);
+    a.part[k] = {(int)p.rows[k], p.d[k].workers, p.d[k].blocks, reinterpret_cast<int*>(ws + p.first_at[k]),
+                 reinterpret_cast<float*>(ws + p.o_at[k]), reinterpret_cast<float*>(ws + p.m_at[k])};
   }
-  const hipStream_t st = as_stream(stream);
-  glt_status e = launch_part<true>(a, st);
-  if (e == GLT_OK) e = launch_part<false>(a, st);
-  if (e != GLT_OK) return e;
-  const int64_t rows = tokens * d->n_q_heads;
-  if (rows <= 4096)  // few rows of many pieces, mostly
-    GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
-  else
-    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
-  GLT_LAUNCH_CHECK("kv8_join");
-  return GLT_OK;
+  return launch(a, p, who, as_stream(stream));
 }

@@ -140,10 +140,12 @@ def test_sizes():
 
     def ws(**kw):
         return lib.glt_kv8_attention_workspace_size(*descs(kw))
-    # with few rows: a piece for each wavefront of the chip and for each sequence's head, whatever the table's
-    # width (an output, a maximum and a sum of each row), and the sequences' pages
-    assert ws(n_table=100000, pages_ld=100000) <= (256 * 12 + 4 * 2) * 12 * (512 + 8) + 4 * 5 + 1024
-    # with many, a window bounds the pieces
-    big = dict(T=64, n_table=100000, pages_ld=100000)
-    assert ws(window=1000, **big) < 2 * ws(T=64, n_table=40, pages_ld=40)
+    # the pieces that a wavefront of the chip begins and goes on with, whatever the table's width (an output, a
+    # maximum and a sum of each row), and the sequences' tiles
+    wide = dict(n_table=100000, pages_ld=100000)
+    assert ws(**wide) <= 2 * 256 * 12 * 12 * (512 + 8) + 4 * 5 + 1024
+    assert ws(T=500, **wide) <= 2 * 512 * 128 * (512 + 8) + 4 * 5 + 1024
+    # a few pages a sequence, in a table or a window: one launch, nothing between
+    assert ws(n_table=16, pages_ld=16) == ws(window=900, **wide) == 256
+    assert ws(n_table=17, pages_ld=17) > 256
     assert ws(**PREFIX) > ws()
