@@ -430,21 +430,22 @@ def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=Non
     return dq, dk, dv
 
 
-def _ints_on(name, t, shape, device):
-    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous int32 {list(shape)} on {device}")
-
-
-def _table_ld(name, t, rows, device):
+def _table_ld(name, t, rows, index):
     """Elements between the rows of a page table int32 [rows, pages]."""
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.device != device:
-        raise ValueError(f"{name}: int32 [{rows}, pages] on {device}")
-    n = t.shape[1]
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != 2 or shape[0] != rows or t.get_device() != index:
+        raise ValueError(f"{name}: int32 [{rows}, pages] on GPU {index}")
+    n = shape[1]
     ld, step = t.stride()
-    if rows <= 1 or n == 0:
-        ld = n
-    _need((n <= 1 or step == 1) and ld >= n, f"{name}: strides {t.stride()} (a row's pages contiguous, rows apart)")
-    return ld
+    if step == 1 and ld >= n:
+        return ld
+    _need((n <= 1 or step == 1) and (rows <= 1 or n == 0), f"{name}: strides {t.stride()} (a row's pages contiguous, rows apart)")
+    return n
+
+
+def _check_ints(name, t, n, index):
+    if t.dtype is not torch.int32 or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 [{n}] on GPU {index}")
 
 
 class Kv8Cache:
@@ -463,40 +464,43 @@ class Kv8Cache:
         self.data = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _need(self.data.is_cuda, "Kv8Cache: a GPU device")
         self.n_pages, self.n_kv_heads, self.head_dim = n_pages, n_kv_heads, head_dim
+        self._index, self._device = self.data.get_device(), self.data.device
+        self._heads = (n_kv_heads, head_dim)
         self._c = F.Kv8Cache(self.data.data_ptr(), n_pages, n_kv_heads, head_dim)
+        self._ref = ctypes.byref(self._c)
 
     def _seqs(self, B, T, pages, lens, new_lens):
-        dev = self.data.device
-        ld = _table_ld("pages", pages, B, dev)
-        _ints_on("lens", lens, (B,), dev)
+        index = self._index
+        ld = _table_ld("pages", pages, B, index)
+        _check_ints("lens", lens, B, index)
         if new_lens is not None:
-            _ints_on("new_lens", new_lens, (B,), dev)
-        return F.Kv8Seqs(B, T, pages.data_ptr(), ld, pages.shape[1], lens.data_ptr(), _a(new_lens))
-
-    def _tokens(self, k, v):
-        _need(k.dim() == 4 and k.shape[2:] == (self.n_kv_heads, self.head_dim) and k.shape == v.shape,
-              f"k, v: [B, T, {self.n_kv_heads}, {self.head_dim}]")
-        B, T = k.shape[:2]
-        dev = self.data.device
-        return B, T, _heads_ld("k", k, B, T, dev), _heads_ld("v", v, B, T, dev)
+            _check_ints("new_lens", new_lens, B, index)
+            new_lens = new_lens.data_ptr()
+        return F.Kv8Seqs(B, T, pages.data_ptr(), ld, pages.shape[1], lens.data_ptr(), new_lens)
 
     def write(self, k, v, pages, lens, new_lens=None):
         """The new tokens' k and v [B, T, n_kv_heads, 128] bf16, also as views of
         one projection output, into the cache."""
-        B, T, k_ld, v_ld = self._tokens(k, v)
-        s = self._seqs(B, T, pages, lens, new_lens)
-        _call_on(self.data, "glt_kv8_write", ctypes.byref(self._c), ctypes.byref(s), k.data_ptr(), k_ld, v.data_ptr(), v_ld)
+        self._tokens("glt_kv8_write", k, v, pages, lens, new_lens)
 
     def read(self, pages, lens, T, new_lens=None, out=None):
         """(k, v) bf16 [B, T, n_kv_heads, 128] of the last new_lens[b] (None: T)
         tokens, into `out` where it is given; zeros past them."""
-        shape = (pages.shape[0], T, self.n_kv_heads, self.head_dim)
-        k, v = out or (torch.empty(shape, dtype=torch.bfloat16, device=self.data.device) for _ in range(2))
-        B, T, k_ld, v_ld = self._tokens(k, v)
-        _need(k.shape == shape, f"out: {list(shape)}")
+        if out is None:
+            k = torch.empty((pages.shape[0], T, *self._heads), dtype=torch.bfloat16, device=self._device)
+            out = k, torch.empty_like(k)
+        else:
+            _need(out[0].shape[:2] == (pages.shape[0], T), f"out: {pages.shape[0]} x {T} tokens")
+        self._tokens("glt_kv8_read", *out, pages, lens, new_lens)
+        return out
+
+    def _tokens(self, name, k, v, pages, lens, new_lens):
+        shape = k.shape
+        _need(len(shape) == 4 and shape[2:] == self._heads and shape == v.shape, f"k, v: [B, T, {self.n_kv_heads}, {self.head_dim}]")
+        B, T, dev = shape[0], shape[1], self._device
+        k_ld, v_ld = _heads_ld("k", k, B, T, dev), _heads_ld("v", v, B, T, dev)
         s = self._seqs(B, T, pages, lens, new_lens)
-        _call_on(self.data, "glt_kv8_read", ctypes.byref(self._c), ctypes.byref(s), k.data_ptr(), k_ld, v.data_ptr(), v_ld)
-        return k, v
+        _call_on(self.data, name, self._ref, ctypes.byref(s), k.data_ptr(), k_ld, v.data_ptr(), v_ld)
 
     def attention(self, q, pages, lens, new_lens=None, scale=None, window=None, sinks=0, prefix=None, workspace=None):
         """Attention of the new tokens q [B, T, Hq, 128] bf16 (written before)
@@ -507,24 +511,28 @@ class Kv8Cache:
         read once for the group. Rows past new_lens: zeros and -inf. workspace: a
         uint8 tensor of glt_kv8_attention_workspace_size bytes instead of a new
         one."""
-        _need(q.dim() == 4 and q.shape[3] == self.head_dim, f"q: [B, T, heads, {self.head_dim}]")
-        B, T, Hq, hd = q.shape
-        dev = self.data.device
+        shape = q.shape
+        _need(len(shape) == 4 and shape[3] == self.head_dim, f"q: [B, T, heads, {self.head_dim}]")
+        B, T, Hq, hd = shape
+        dev, index = self._device, self._index
         q_ld = _heads_ld("q", q, B, T, dev)
-        _need(window is None or window > 0, f"window {window} (None, or at least 1)")
+        if window is None:
+            window = 0
+        else:
+            _need(window > 0, f"window {window} (None, or at least 1)")
         s = self._seqs(B, T, pages, lens, new_lens)
-        d = F.Kv8Attn(Hq, hd ** -0.5 if scale is None else scale, window or 0, sinks)
+        d = F.Kv8Attn(Hq, hd ** -0.5 if scale is None else scale, window, sinks)
         if prefix is not None:
             ppages, plens = prefix
-            d.n_groups = ppages.shape[0]
-            _need(d.n_groups > 0 or B == 0, "prefix: no groups")
-            d.prefix_ld = _table_ld("prefix pages", ppages, d.n_groups, dev)
-            _ints_on("prefix lens", plens, (d.n_groups,), dev)
+            groups = d.n_groups = ppages.shape[0]
+            _need(groups > 0 or B == 0, "prefix: no groups")
+            d.prefix_ld = _table_ld("prefix pages", ppages, groups, index)
+            _check_ints("prefix lens", plens, groups, index)
             d.prefix_pages, d.n_prefix_table, d.prefix_lens = ppages.data_ptr(), ppages.shape[1], plens.data_ptr()
-        refs = ctypes.byref(self._c), ctypes.byref(s), ctypes.byref(d)
+        refs = self._ref, ctypes.byref(s), ctypes.byref(d)
         workspace = _workspace(workspace, F.load().glt_kv8_attention_workspace_size(*refs), dev)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        lse = torch.empty(B, Hq, T, dtype=torch.float32, device=dev)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
         _call_on(self.data, "glt_kv8_attention", *refs, q.data_ptr(), q_ld, out.data_ptr(), Hq * hd, lse.data_ptr(),
                  workspace.data_ptr(), workspace.numel())
         return out, lse
