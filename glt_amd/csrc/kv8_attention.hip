@@ -123,7 +123,7 @@ template <bool PRE>
 __device__ __forceinline__ int page_id(const DecArgs& a, int seg, int p) {
   return PRE ? a.ppages[seg * a.prefix_ld + p] : a.s.pages[seg * a.s.pages_ld + p];
 }
-// Where a page's head lies; a page outside the pool is not followed (its steps count as
+// Where a page's head lies; a page outside the pool is not followed (its scores count as
 // NaN).
 __device__ __forceinline__ bool page_ok(const DecArgs& a, int id) { return id >= 0 && id < a.n_pages; }
 __device__ __forceinline__ const uint8_t* page_at(const DecArgs& a, int id, int h) {
@@ -290,9 +290,7 @@ struct Few {
       for (int i = from; i < to; ++i) vx[i] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + (16 * i + r15) * kPage + 16 * g));
     };
     if (NB == 1) load_v(0, 8);
-    if (!ok)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) kst[i] = vst[i] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    const float scale = ok ? a.scale_log2 : NAN;
     // steps of keys 16 g + i
     auto step = [](const u32x4* x, int i) {
       const uint32_t w = x[i >> 3][(i & 7) >> 1];
@@ -327,7 +325,7 @@ struct Few {
 #pragma unroll
       for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nb][blk][e] *= step(kst, 8 * (blk & 1) + 4 * (blk >> 1) + e) * a.scale_log2;
+        for (int e = 0; e < 4; ++e) s[nb][blk][e] *= step(kst, 8 * (blk & 1) + 4 * (blk >> 1) + e) * scale;
       if (!whole)
 #pragma unroll
         for (int blk = 0; blk < 4; ++blk)
@@ -430,7 +428,7 @@ __device__ __forceinline__ void few_rows(const DecArgs& a, int* first, int block
 // One workgroup a sequence and head, its pages dealt to WAVES wavefronts and joined in
 // LDS: where the pages are few this one launch ends sooner than pieces and their join.
 template <int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) kv8_whole_kernel(const DecArgs a) {
+__global__ void __launch_bounds__(WAVES * 64, 3) kv8_whole_kernel(const DecArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int R = a.part[0].rows, wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int h = blockIdx.x % a.Hkv, seg = blockIdx.x / a.Hkv;
@@ -532,6 +530,7 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
 
     u32x4 kx[2], vx[2];
     uint32_t st = 0;
+    float scale = 0.f;
     int ids = 0;
     auto fetch = [&](int i) {
       const int x = (i - from) & 63;
@@ -543,10 +542,9 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
         kx[y] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(16 * (tid + 256 * y)));
         vx[y] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + 16 * (tid + 256 * y)));
       }
-      if (tid < 2 * kPage) {
-        st = *reinterpret_cast<const uint16_t*>(pg + (uint32_t)(kKStepOff + 2 * tid));
-        if (!page_ok(a, id)) st = 0x7fc0u;
-      }
+      // (every thread: a branch around a load waits for all of them)
+      st = *reinterpret_cast<const uint16_t*>(pg + (uint32_t)(kKStepOff + 2 * (tid & 127)));
+      scale = page_ok(a, id) ? a.scale_log2 : NAN;
     };
     // 16 codes of token q >> 3, channels 16 (q & 7) .., or of channel q >> 2 and 16 tokens
     auto stage = [&](lds_char* to) {
@@ -568,17 +566,27 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
       }
       if (tid < 2 * kPage) {
         const float f = __uint_as_float(st << 16);
-        *(__attribute__((address_space(3))) float*)(to + kSteps + 4 * tid) = tid < kPage ? f * a.scale_log2 : f;
+        *(__attribute__((address_space(3))) float*)(to + kSteps + 4 * tid) = tid < kPage ? f * scale : f;
       }
     };
 
     auto step = [&](int p, const lds_char* rd) {
       const int key0 = p * kPage;
       f32x16 s[2] = {f32x16{}, f32x16{}};
-      const lds_char* kr = rd + lane * 16;
+      {
+        const lds_char* kr = rd + lane * 16;
+        constexpr int kAhead = 4;
+        bf16x8 ka[kAhead];
+        auto get = [&](int i) { return *(const lds_bf16x8*)(kr + ((i & 1) * 8 + (i >> 1)) * kKFrag); };
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[i & 1] = mfma(*(const lds_bf16x8*)(kr + ((i & 1) * 8 + (i >> 1)) * kKFrag), qf[i >> 1], s[i & 1]);
+        for (int i = 0; i < kAhead; ++i) ka[i] = get(i);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[i & 1] = mfma(ka[i % kAhead], qf[i >> 1], s[i & 1]);
+          if (i + kAhead < 16) ka[i % kAhead] = get(i + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
       const lds_char* sp = rd + kSteps + 16 * lh;  // steps of keys 32 kb + 8 i + 4 lh + e
       // Scores relative to the maximum so far, in one instruction each (to 0 before a row
       // has seen anything: its maximum then moves whatever it is).
@@ -624,28 +632,43 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
           for (int e = 0; e < 16; ++e) s[kb][e] -= by;
       }
       u32x4 pw[4];
+      float ls[2] = {l_run, 0.f};
+      auto probs = [&](bool masked) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 f = *(const lds_f32x4*)(sp + kPage * 4 + 128 * kb + 32 * i);
-          float x[4];
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 f = *(const lds_f32x4*)(sp + kPage * 4 + 128 * kb + 32 * i);
+            float x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = __builtin_amdgcn_exp2f(s[kb][4 * i + e]);
-            l_run += y;
-            x[e] = y * f[e];
+            for (int e = 0; e < 4; ++e) {
+              const float z = s[kb][4 * i + e], y = __builtin_amdgcn_exp2f(z);
+              ls[kb] += y;
+              x[e] = masked && z == -INFINITY ? 0.f : y * f[e];  // an unseen key's step may be anything
+            }
+            pw[2 * kb + (i >> 1)][2 * (i & 1)] = pack2_rne(x[0], x[1]);
+            pw[2 * kb + (i >> 1)][2 * (i & 1) + 1] = pack2_rne(x[2], x[3]);
           }
-          if (!whole)  // an unseen key's step may be anything
+      };
+      if (whole) probs(false);
+      else probs(true);
+      l_run = ls[0] + ls[1];
+      {
+        const lds_char* vr = rd + kVTile + lane * 16;
+        constexpr int kAhead = 4;
+        bf16x8 va[kAhead];
+        auto get = [&](int i) { return *(const lds_bf16x8*)(vr + ((i & 3) * 4 + (i >> 2)) * kVFrag); };
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = s[kb][4 * i + e] == -INFINITY ? 0.f : x[e];
-          pw[2 * kb + (i >> 1)][2 * (i & 1)] = pack2_rne(x[0], x[1]);
-          pw[2 * kb + (i >> 1)][2 * (i & 1) + 1] = pack2_rne(x[2], x[3]);
+        for (int i = 0; i < kAhead; ++i) va[i] = get(i);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          o[i & 3] = mfma(va[i % kAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), o[i & 3]);
+          if (i + kAhead < 16) va[i % kAhead] = get(i + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
         }
-      const lds_char* vr = rd + kVTile + lane * 16;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        o[i & 3] = mfma(*(const lds_bf16x8*)(vr + ((i & 3) * 4 + (i >> 2)) * kVFrag), __builtin_bit_cast(bf16x8, pw[i >> 2]), o[i & 3]);
+        __builtin_amdgcn_s_setprio(0);
+      }
     };
 
     __syncthreads();  // every wavefront is done with the run before
@@ -653,6 +676,7 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
       fetch(from);
       stage(lds);
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));  // q too: no product has to wait for the next page
     for (int i = from; i < to; ++i) {
       __syncthreads();  // tile i is whole, and every wavefront is done with tile i - 1
       lds_char *x = lds + ((i - from) & 1) * kManyBuf, *y = lds + (~(i - from) & 1) * kManyBuf;
