@@ -167,7 +167,7 @@ __device__ __forceinline__ void write_row(const DecArgs& a, const Row& w, const 
 }
 
 // ---------------------------------------------------------------- dealing
-constexpr int kManyRows = 128;  // rows of a workgroup of many_rows
+constexpr int kManyRows = 256;  // rows of a workgroup of many_rows
 constexpr int kFewRows = 32;    // rows that few_rows takes
 
 // Row blocks of a segment that hold new tokens.
@@ -179,14 +179,14 @@ __device__ __forceinline__ int row_blocks(const DecArgs& a, int seg) {
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // first[s]: tiles of work (pages x row blocks) before segment s, first[n_seg] in all, by
-// a workgroup of 256 in LDS, and by workgroup 0 of the kind for the join.
-template <bool PRE, bool MANY>
+// a workgroup in LDS, and by workgroup 0 of the kind for the join.
+template <int WAVES, bool PRE, bool MANY>
 __device__ __forceinline__ int deal(const DecArgs& a, int* first, int block) {
-  __shared__ int wave_sum[4];
+  __shared__ int wave_sum[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int n_seg = PRE ? a.n_groups : a.s.B;
   int total = 0;
-  for (int s0 = 0; s0 < n_seg; s0 += 256) {
+  for (int s0 = 0; s0 < n_seg; s0 += WAVES * 64) {
     const int s = s0 + tid, n = s < n_seg ? sight<PRE>(a, s).n * row_blocks<PRE, MANY>(a, s) : 0;
     int x = n;
 #pragma unroll
@@ -198,7 +198,7 @@ __device__ __forceinline__ int deal(const DecArgs& a, int* first, int block) {
     __syncthreads();
     int before = total;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       if (w < wave) before += wave_sum[w];
       total += wave_sum[w];
     }
@@ -207,7 +207,7 @@ __device__ __forceinline__ int deal(const DecArgs& a, int* first, int block) {
     __syncthreads();
   }
   if (block == 0)
-    for (int s = tid; s <= n_seg; s += 256) a.part[PRE].first[s] = first[s];
+    for (int s = tid; s <= n_seg; s += WAVES * 64) a.part[PRE].first[s] = first[s];
   return uni(total);
 }
 // Tiles of a run.
@@ -244,8 +244,6 @@ __device__ __forceinline__ int64_t slot_of(const DecArgs& a, int worker, int64_t
 // Lane l: row l & 15 of a block of 16, g = l >> 4. The keys of score block (beta, a) are
 // numbered so that the accumulators are the second product's operand as they stand:
 // element e of lane group g is key 16 g + 8 a + 4 beta + e of the page.
-constexpr int kFewWaves = 4;
-
 template <int NB>
 struct Few {
   Row row[NB];
@@ -379,11 +377,11 @@ struct Few {
   }
 };
 
-template <int NB, bool PRE>
+template <int WAVES, int NB, bool PRE>
 __device__ __forceinline__ void few_rows(const DecArgs& a, int* first, int block) {
   const int n_seg = PRE ? a.n_groups : a.s.B, R = a.part[PRE].rows;
-  const int total = deal<PRE, false>(a, first, block);
-  const int worker = block * kFewWaves + uni(threadIdx.x >> 6), all = total * a.Hkv;
+  const int total = deal<WAVES, PRE, false>(a, first, block);
+  const int worker = block * WAVES + uni(threadIdx.x >> 6), all = total * a.Hkv;
   const int run = run_tiles<false>(all, a.part[PRE].workers);
   int at = worker * run;  // workers * run stays below all + workers
   const int stop = min(at + run, all);
@@ -474,25 +472,32 @@ __global__ void __launch_bounds__(WAVES * 64, 3) kv8_whole_kernel(const DecArgs 
 }
 
 // ------------------------------------------------------------- many rows
-// A column is 128 rows of a segment and head, a tile one of its pages, and the workers are
-// workgroups of four wavefronts; a wavefront owns 32 rows as in attention for training
-// (attention_train.hip). The workgroup's threads load a page's codes into registers while
-// the tile before is worked on, convert them and write them to LDS in the order in which
-// the products' operands are read (1 KB of 64 lanes each, padded so that the writes spread
+// A column is 256 rows of a segment and head, a tile one of its pages, and the workers are
+// workgroups of eight wavefronts; a wavefront owns 32 rows as in attention for training
+// (attention_train.hip), two share a SIMD. Converted codes lie in LDS in the order in which the
+// products' operands are read (1 KB of 64 lanes each, padded so that the writes spread
 // over the banks).
-constexpr int kManyWaves = 4;
+//
+// A tile costs a wavefront as much vector arithmetic (the softmax, the codes'
+// conversion) as matrix products, and one depends on the other. So the two
+// wavefronts of a SIMD alternate: between two barriers one runs its products
+//   M(j): o += V(j - 1) . P(j - 1)^T,  S(j) = K(j) . Q^T
+// while the other turns S(j - 1) into P(j - 1) and converts its half of the next
+// operands, and then they change places. The first four wavefronts (turn 0) are a phase
+// ahead of the others: in phases 2 j and 2 j + 1 M(j) runs and K(j + 1), V(j) are written,
+// so that two buffers of each are enough; the steps of four tiles are kept.
+constexpr int kManyWaves = 8;
 constexpr int kKFrag = 1040, kVFrag = 1056;           // bytes of an operand of 64 lanes
-constexpr int kVTile = 16 * kKFrag;                   // after the 16 of k
-constexpr int kSteps = kVTile + 16 * kVFrag;          // f32 steps of k (times scale) and v
-constexpr int kManyBuf = kSteps + 2 * kPage * 4;      // 34,048 bytes
-constexpr int kManyLds = 2 * kManyBuf;
+constexpr int kKTile = 16 * kKFrag, kVTile = 16 * kVFrag;
+constexpr int kVAt = 2 * kKTile, kStepAt = kVAt + 2 * kVTile;
+constexpr int kManyLds = kStepAt + 4 * 2 * kPage * 4;  // f32 steps of k (times scale) and v: 69,120 bytes
 
 template <bool PRE>
 __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int block) {
-  const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, lh = lane >> 5, wave = uni(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, lh = lane >> 5, wave = uni(tid >> 6), turn = wave >> 2;
   const int n_seg = PRE ? a.n_groups : a.s.B, R = a.part[PRE].rows, all_rb = (R + kManyRows - 1) / kManyRows;
   int* const first = reinterpret_cast<int*>(smem + kManyLds);
-  const int total = deal<PRE, true>(a, first, block), all = total * a.Hkv;
+  const int total = deal<kManyWaves, PRE, true>(a, first, block), all = total * a.Hkv;
   const int run = run_tiles<true>(all, a.part[PRE].workers);
   lds_char* const lds = (lds_char*)smem;
   int at = block * run;
@@ -503,9 +508,9 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
     const int rem = pos - uni(first[seg]), rb = rem / n, i0 = rem - rb * n, i1 = min(n, i0 + stop - at);
     at += i1 - i0;
     const Sight si = sight<PRE>(a, seg);
-    const int r = rb * kManyRows + 32 * wave + lq;
-    const Row w = row_of<PRE>(a, seg, h, min(r, R - 1), si.hi);
-    const bool live = r < R && w.hi > 0;
+    Row w = row_of<PRE>(a, seg, h, min(rb * kManyRows + 32 * wave + lq, R - 1), si.hi);
+    if (rb * kManyRows + 32 * wave + lq >= R) w.hi = 0;
+    const bool works = __any(w.hi > 0);
     // of the list, what the block's rows see: to the last row's own key, from the first row's window on
     int from = i0, to = i1;
     if (!PRE) {
@@ -520,74 +525,105 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
         from = uni(from);
       }
     }
+    const int tiles = max(to - from, 0);
 
     bf16x8 qf[8];
     load_rows(qf, a.q + w.q_row * a.q_ld + (int64_t)w.head * kKv8Hd, true, lh);
-    f32x16 o[4];
+    f32x16 o[4], s[2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = f32x16{};
+    u32x4 pw[4];
     float m_run = kNoMax, l_run = 0.f;
 
-    u32x4 kx[2], vx[2];
+    auto page_of = [&](int j) { return a.W ? si.page(from + j) : from + j; };
+    int ids = 0;  // lane x: the id of tile x, 64 at a time
+    auto id_of = [&](int j) {
+      if ((j & 63) == 0) ids = j + lane < tiles ? page_id<PRE>(a, seg, page_of(j + lane)) : 0;
+      return __builtin_amdgcn_readlane(ids, j & 63);
+    };
+    // this thread's 16 codes of each tile: token q >> 3, channels 16 (q & 7) .., or
+    // channel q >> 2 and 16 tokens
+    const uint32_t q = tid;
+    u32x4 kx, vx;
     uint32_t st = 0;
     float scale = 0.f;
-    int ids = 0;
-    auto fetch = [&](int i) {
-      const int x = (i - from) & 63;
-      if (x == 0) ids = i + lane < to ? page_id<PRE>(a, seg, a.W ? si.page(i + lane) : i + lane) : 0;
-      const int id = __builtin_amdgcn_readlane(ids, x);
-      const uint8_t* pg = page_at(a, id, h);
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        kx[y] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(16 * (tid + 256 * y)));
-        vx[y] = *reinterpret_cast<const u32x4*>(pg + (uint32_t)(kVOff + 16 * (tid + 256 * y)));
-      }
+    const uint8_t* pg = nullptr;  // of the tile whose v is next
+    auto fetch_k = [&](int j) {
+      const int id = id_of(j);
+      pg = page_at(a, id, h);
+      kx = *reinterpret_cast<const u32x4*>(pg + 16 * q);
       // (every thread: a branch around a load waits for all of them)
-      st = *reinterpret_cast<const uint16_t*>(pg + (uint32_t)(kKStepOff + 2 * (tid & 127)));
+      st = *reinterpret_cast<const uint16_t*>(pg + kKStepOff + 2 * (q & 127));
       scale = page_ok(a, id) ? a.scale_log2 : NAN;
     };
-    // 16 codes of token q >> 3, channels 16 (q & 7) .., or of channel q >> 2 and 16 tokens
-    auto stage = [&](lds_char* to) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int q = tid + 256 * i;
-        {
-          const int key = q >> 3, s = q & 7;
-          lds_char* x = to + ((key >> 5) * 8 + s) * kKFrag + (key & 31) * 16;
-          *(lds_bf16x8*)x = codes8(kx[i][0], kx[i][1]);
-          *(lds_bf16x8*)(x + 512) = codes8(kx[i][2], kx[i][3]);
-        }
-        {
-          const int d = q >> 2, s2 = q & 3;
-          lds_char* x = to + kVTile + ((d >> 5) * 4 + s2) * kVFrag + (d & 31) * 16;
-          *(lds_bf16x8*)x = codes8(vx[i][0], vx[i][1]);
-          *(lds_bf16x8*)(x + 512) = codes8(vx[i][2], vx[i][3]);
-        }
-      }
-      if (tid < 2 * kPage) {
-        const float f = __uint_as_float(st << 16);
-        *(__attribute__((address_space(3))) float*)(to + kSteps + 4 * tid) = tid < kPage ? f * scale : f;
-      }
+    auto stage_k = [&](int j) {
+      const int key = q >> 3, c = q & 7;
+      lds_char* x = lds + (j & 1) * kKTile + ((key >> 5) * 8 + c) * kKFrag + (key & 31) * 16;
+      *(lds_bf16x8*)x = codes8(kx[0], kx[1]);
+      *(lds_bf16x8*)(x + 512) = codes8(kx[2], kx[3]);
+      // the second half's threads write the steps
+      const float f = __uint_as_float(st << 16);
+      if (q >= 256 && q < 384)
+        *(__attribute__((address_space(3))) float*)(lds + kStepAt + (j & 3) * 2 * kPage * 4 + 4 * (q & 127)) =
+            (q & 127) < kPage ? f * scale : f;
+    };
+    // What is written beside M(j): K(j + 1) and V(j). (Past the end the last page once
+    // more, into buffers that nothing reads then: branches around the loads cost more.)
+    auto fetch = [&](int j) {
+      vx = *reinterpret_cast<const u32x4*>(pg + kVOff + 16 * q);
+      fetch_k(min(j + 1, tiles - 1));
+    };
+    auto stage = [&](int j) {
+      const int d = q >> 2, s2 = q & 3;
+      lds_char* x = lds + kVAt + (j & 1) * kVTile + ((d >> 5) * 4 + s2) * kVFrag + (d & 31) * 16;
+      *(lds_bf16x8*)x = codes8(vx[0], vx[1]);
+      *(lds_bf16x8*)(x + 512) = codes8(vx[2], vx[3]);
+      stage_k(j + 1);
     };
 
-    auto step = [&](int p, const lds_char* rd) {
-      const int key0 = p * kPage;
-      f32x16 s[2] = {f32x16{}, f32x16{}};
-      {
-        const lds_char* kr = rd + lane * 16;
-        constexpr int kAhead = 4;
-        bf16x8 ka[kAhead];
-        auto get = [&](int i) { return *(const lds_bf16x8*)(kr + ((i & 1) * 8 + (i >> 1)) * kKFrag); };
+    auto values = [&](int j) {  // o += V(j) . P^T
+      const lds_char* vr = lds + kVAt + (j & 1) * kVTile + lane * 16;
+      constexpr int kAhead = 4;
+      bf16x8 va[kAhead];
+      auto get = [&](int i) { return *(const lds_bf16x8*)(vr + ((i & 3) * 4 + (i >> 2)) * kVFrag); };
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) ka[i] = get(i);
+      for (int i = 0; i < kAhead; ++i) va[i] = get(i);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i & 1] = mfma(ka[i % kAhead], qf[i >> 1], s[i & 1]);
-          if (i + kAhead < 16) ka[i % kAhead] = get(i + kAhead);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      for (int i = 0; i < 16; ++i) {
+        o[i & 3] = mfma(va[i % kAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), o[i & 3]);
+        if (i + kAhead < 16) va[i % kAhead] = get(i + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const lds_char* sp = rd + kSteps + 16 * lh;  // steps of keys 32 kb + 8 i + 4 lh + e
+    };
+    // Steps of keys 32 kb + 8 i + 4 lh + e of a tile (k's times scale, or v's), read well
+    // before they are used (v's by halves: there are no registers for all of them).
+    f32x4 f[8];
+    auto steps = [&](int j, int v, int kb) {
+      const lds_char* sp = lds + kStepAt + (2 * (j & 3) + v) * kPage * 4 + 16 * lh;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[4 * kb + i] = *(const lds_f32x4*)(sp + 128 * kb + 32 * i);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto scores = [&](int j) {
+      const lds_char* kr = lds + (j & 1) * kKTile + lane * 16;
+      constexpr int kAhead = 4;
+      bf16x8 ka[kAhead];
+      auto get = [&](int i) { return *(const lds_bf16x8*)(kr + ((i & 1) * 8 + (i >> 1)) * kKFrag); };
+      s[0] = s[1] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ka[i] = get(i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i & 1] = mfma(ka[i % kAhead], qf[i >> 1], s[i & 1]);
+        if (i + kAhead < 16) ka[i % kAhead] = get(i + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      steps(j, 0, 0);
+      steps(j, 0, 1);
+    };
+    auto softmax = [&](int j) {
+      const int key0 = page_of(j) * kPage;
       // Scores relative to the maximum so far, in one instruction each (to 0 before a row
       // has seen anything: its maximum then moves whatever it is).
       const bool unset = m_run == kNoMax;
@@ -595,20 +631,19 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 f = *(const lds_f32x4*)(sp + 128 * kb + 32 * i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[kb][4 * i + e] = __builtin_fmaf(s[kb][4 * i + e], f[e], -base);
-        }
-      const bool whole = __all(!live | ((key0 + kPage <= w.hi) & ((key0 >= w.lo) | (key0 + kPage <= w.sunk))));
+        for (int e = 0; e < 16; ++e) s[kb][e] = __builtin_fmaf(s[kb][e], f[4 * kb + (e >> 2)][e & 3], -base);
+      steps(j, 1, 0);
+      const bool whole = __all((w.hi == 0) | ((key0 + kPage <= w.hi) & ((key0 >= w.lo) | (key0 + kPage <= w.sunk))));
+      auto in = [&](int i) {  // whether the row sees key i + 4 lh of the page
+        const int x = key0 + 4 * lh + i;
+        return (x < w.hi) & ((x >= w.lo) | (x < w.sunk));
+      };
       if (!whole)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int j = key0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
-            const bool in = (j < w.hi) & ((j >= w.lo) | (j < w.sunk));
-            s[kb][e] = in ? s[kb][e] : -INFINITY;
+            s[kb][e] = in(32 * kb + 8 * (e >> 2) + (e & 3)) ? s[kb][e] : -INFINITY;
           }
       float m2[2];
 #pragma unroll
@@ -631,74 +666,85 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[kb][e] -= by;
       }
-      u32x4 pw[4];
       float ls[2] = {l_run, 0.f};
       auto probs = [&](bool masked) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb) {
+          if (kb == 0) steps(j, 1, 1);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const f32x4 f = *(const lds_f32x4*)(sp + kPage * 4 + 128 * kb + 32 * i);
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float z = s[kb][4 * i + e], y = __builtin_amdgcn_exp2f(z);
+              const float y = __builtin_amdgcn_exp2f(s[kb][4 * i + e]);
               ls[kb] += y;
-              x[e] = masked && z == -INFINITY ? 0.f : y * f[e];  // an unseen key's step may be anything
+              x[e] = y * (!masked || in(32 * kb + 8 * i + e) ? f[4 * kb + i][e] : 0.f);  // an unseen key's step may be anything
             }
             pw[2 * kb + (i >> 1)][2 * (i & 1)] = pack2_rne(x[0], x[1]);
             pw[2 * kb + (i >> 1)][2 * (i & 1) + 1] = pack2_rne(x[2], x[3]);
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       };
       if (whole) probs(false);
       else probs(true);
       l_run = ls[0] + ls[1];
-      {
-        const lds_char* vr = rd + kVTile + lane * 16;
-        constexpr int kAhead = 4;
-        bf16x8 va[kAhead];
-        auto get = [&](int i) { return *(const lds_bf16x8*)(vr + ((i & 3) * 4 + (i >> 2)) * kVFrag); };
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) va[i] = get(i);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          o[i & 3] = mfma(va[i % kAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), o[i & 3]);
-          if (i + kAhead < 16) va[i % kAhead] = get(i + kAhead);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        __builtin_amdgcn_s_setprio(0);
-      }
     };
 
-    __syncthreads();  // every wavefront is done with the run before
-    if (from < to) {
-      fetch(from);
-      stage(lds);
-    }
-    __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));  // q too: no product has to wait for the next page
-    for (int i = from; i < to; ++i) {
-      __syncthreads();  // tile i is whole, and every wavefront is done with tile i - 1
-      lds_char *x = lds + ((i - from) & 1) * kManyBuf, *y = lds + (~(i - from) & 1) * kManyBuf;
-      if (i + 1 < to) fetch(i + 1);
-      step(a.W ? si.page(i) : i, x);
-      if (i + 1 < to) stage(y);
+    // (the run before: its last phase reads V and the turns' barriers match, so nothing that
+    // is written before the next barrier is still read)
+    if (tiles > 0) {
+      fetch_k(0);
+      stage_k(0);
+      if (turn) fetch(0);
+      __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));  // q too: no product has to wait for a page
+      phase_barrier();
+      if (turn) {
+        stage(0);
+        phase_barrier();
+      }
+      fetch(turn);
+      if (works) {
+        scores(0);
+        for (int j = 0; j < tiles; ++j) {
+          phase_barrier();
+          softmax(j);
+          stage(j + turn);
+          phase_barrier();
+          fetch(j + 1 + turn);
+          __builtin_amdgcn_s_setprio(1);
+          values(j);
+          scores(j + 1);  // (the last one's go nowhere)
+          __builtin_amdgcn_s_setprio(0);
+        }
+      } else {
+        for (int j = 0; j < tiles; ++j) {
+          phase_barrier();
+          stage(j + turn);
+          phase_barrier();
+          fetch(j + 1 + turn);
+        }
+      }
+      if (!turn) phase_barrier();
     }
 
+    // (worked out again: kept across the pages it costs registers that there are not)
+    const int l2 = (int)opaque(threadIdx.x) & 63, lh2 = l2 >> 5, r = rb * kManyRows + 32 * wave + (l2 & 31);
     const float l = pair_sum(l_run);
     if (!PRE && !a.n_groups && i1 - i0 == n) {  // the rows' only piece
-      if (live) {
-        store_rows(a.out + w.q_row * a.o_ld + (int64_t)w.head * kKv8Hd, o, l == 0.f ? 0.f : 1.0f / l, lh);
-        if (lh == 0) write_lse(a, w, m_run, l);
+      const Row x = row_of<PRE>(a, seg, h, min(r, R - 1), si.hi);
+      if (r < R && x.hi > 0) {
+        store_rows(a.out + x.q_row * a.o_ld + (int64_t)x.head * kKv8Hd, o, l == 0.f ? 0.f : 1.0f / l, lh2);
+        if (lh2 == 0) write_lse(a, x, m_run, l);
       }
     } else if (r < R) {
       const int64_t column = ((int64_t)h * n_seg + seg) * all_rb + rb;
-      const int64_t slot = slot_of<PRE>(a, block, column, i0 == 0) * kManyRows + 32 * wave + lq;
-      if (lh == 0) {
+      const int64_t slot = slot_of<PRE>(a, block, column, i0 == 0) * kManyRows + 32 * wave + (l2 & 31);
+      if (lh2 == 0) {
         a.part[PRE].m[2 * slot] = m_run;
         a.part[PRE].m[2 * slot + 1] = l;
       }
-      float* po = a.part[PRE].o + slot * kKv8Hd + 4 * lh;
+      float* po = a.part[PRE].o + slot * kKv8Hd + 4 * lh2;
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -712,21 +758,27 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
 // How a part's rows are worked on.
 enum Kind { kNone, kFew16, kFew32, kMany };
 
+// Wavefronts of a workgroup.
+constexpr int waves_of(Kind prefix, Kind own) { return prefix == kMany || own == kMany ? kManyWaves : 4; }
+
 // The own tokens' workgroups first: with a prefix of many rows theirs wait for memory
 // while the others compute.
 template <Kind PREFIX, Kind OWN>
-__global__ void __launch_bounds__(256, PREFIX <= kFew16 && OWN == kFew16 ? 3 : 2) kv8_pieces_kernel(const DecArgs a) {
+__global__ void __launch_bounds__(waves_of(PREFIX, OWN) * 64, PREFIX <= kFew16 && OWN == kFew16 ? 3 : 2)
+    kv8_pieces_kernel(const DecArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int W = waves_of(PREFIX, OWN);
+  int* const few = reinterpret_cast<int*>(smem);
   const int block = blockIdx.x;
   if (PREFIX == kNone || block < a.part[0].blocks) {
     if constexpr (OWN == kMany) many_rows<false>(a, smem, block);
-    if constexpr (OWN == kFew16) few_rows<1, false>(a, reinterpret_cast<int*>(smem), block);
-    if constexpr (OWN == kFew32) few_rows<2, false>(a, reinterpret_cast<int*>(smem), block);
+    if constexpr (OWN == kFew16) few_rows<W, 1, false>(a, few, block);
+    if constexpr (OWN == kFew32) few_rows<W, 2, false>(a, few, block);
   } else {
     const int b = block - a.part[0].blocks;
     if constexpr (PREFIX == kMany) many_rows<true>(a, smem, b);
-    if constexpr (PREFIX == kFew16) few_rows<1, true>(a, reinterpret_cast<int*>(smem), b);
-    if constexpr (PREFIX == kFew32) few_rows<2, true>(a, reinterpret_cast<int*>(smem), b);
+    if constexpr (PREFIX == kFew16) few_rows<W, 1, true>(a, few, b);
+    if constexpr (PREFIX == kFew32) few_rows<W, 2, true>(a, few, b);
   }
 }
 
@@ -867,11 +919,12 @@ Deal deal_of(int64_t n_table, int64_t span, int64_t sinks, int64_t rows, int64_t
   const int64_t row_blocks = d.kind == kMany ? cdiv(rows, kManyRows) : 1, columns = segments * heads * row_blocks;
   d.tiles = columns * d.pages;
   if (d.kind == kMany) {
-    d.blocks = d.workers = (int)std::min<int64_t>(cdiv(d.tiles, 2), 512);  // two workgroups a CU
+    d.blocks = d.workers = (int)std::min<int64_t>(cdiv(d.tiles, 2), 256);  // a workgroup a CU
     d.slot_rows = kManyRows;
   } else {
-    d.blocks = (int)std::min<int64_t>(cdiv(d.tiles, kFewWaves), 256 * (beside_many ? 1 : d.kind == kFew16 ? 3 : 2));
-    d.workers = d.blocks * kFewWaves;
+    const int waves = beside_many ? kManyWaves : 4;
+    d.blocks = (int)std::min<int64_t>(cdiv(d.tiles, waves), 256 * (beside_many ? 1 : d.kind == kFew16 ? 3 : 2));
+    d.workers = d.blocks * waves;
     d.slot_rows = rows;
   }
   d.slots = prefixes ? d.workers + columns : 2 * (int64_t)d.workers;
@@ -987,7 +1040,8 @@ glt_status launch(DecArgs& a, const Plan& p, const char* who, hipStream_t st) {
   if (const Kernel f = pieces_kernel(p.d[1].kind, p.d[0].kind)) {
     const int segs = std::max(p.d[0].kind ? a.s.B : 0, p.d[1].kind ? a.n_groups : 0);
     const size_t lds = (p.d[0].kind == kMany || p.d[1].kind == kMany ? kManyLds : 0) + (segs + 1) * 4;
-    GLT_LAUNCH("kv8_pieces", f, dim3((unsigned)(p.d[0].blocks + p.d[1].blocks)), dim3(256), lds, st, a);
+    GLT_LAUNCH("kv8_pieces", f, dim3((unsigned)(p.d[0].blocks + p.d[1].blocks)), dim3(waves_of(p.d[1].kind, p.d[0].kind) * 64),
+               lds, st, a);
     GLT_LAUNCH_CHECK("kv8_pieces");
   }
   if (rows <= 4096)  // few rows of many pieces, mostly

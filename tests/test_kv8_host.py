@@ -144,7 +144,7 @@ def test_sizes():
     # maximum and a sum of each row), and the sequences' tiles
     wide = dict(n_table=100000, pages_ld=100000)
     assert ws(**wide) <= 2 * 256 * 12 * 12 * (512 + 8) + 4 * 5 + 1024
-    assert ws(T=500, **wide) <= 2 * 512 * 128 * (512 + 8) + 4 * 5 + 1024
+    assert ws(T=500, **wide) <= 2 * 256 * 256 * (512 + 8) + 4 * 5 + 1024
     # a few pages a sequence, in a table or a window: one launch, nothing between
     assert ws(n_table=16, pages_ld=16) == ws(window=900, **wide) == 256
     assert ws(n_table=17, pages_ld=17) > 256
