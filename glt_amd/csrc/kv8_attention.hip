@@ -177,53 +177,80 @@ __device__ __forceinline__ int row_blocks(const DecArgs& a, int seg) {
   return ((PRE ? a.part[1].rows : kv8_len(a.s, seg).fresh * a.G) + kManyRows - 1) / kManyRows;
 }
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// first[s]: tiles of work (pages x row blocks) before segment s, first[n_seg] in all, by
-// a workgroup in LDS, and by workgroup 0 of the kind for the join.
-template <int WAVES, bool PRE, bool MANY>
-__device__ __forceinline__ int deal(const DecArgs& a, int* first, int block) {
-  __shared__ int wave_sum[WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-  const int n_seg = PRE ? a.n_groups : a.s.B;
-  int total = 0;
-  for (int s0 = 0; s0 < n_seg; s0 += WAVES * 64) {
-    const int s = s0 + tid, n = s < n_seg ? sight<PRE>(a, s).n * row_blocks<PRE, MANY>(a, s) : 0;
-    int x = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 63) wave_sum[wave] = x;
-    __syncthreads();
-    int before = total;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) before += wave_sum[w];
-      total += wave_sum[w];
-    }
-    if (s < n_seg) first[s] = before + x - n;
-    if (s == n_seg - 1) first[n_seg] = total;
-    __syncthreads();
-  }
-  if (block == 0)
-    for (int s = tid; s <= n_seg; s += WAVES * 64) a.part[PRE].first[s] = first[s];
-  return uni(total);
+// Sum over this and the lanes before.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // rows of 16, shifted by 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // a row's last lane to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+  return x;
 }
+
+// Tiles of work (pages x row blocks) before each segment and in all, for a workgroup; its
+// first one writes them for the join too. Up to 64 segments every wavefront keeps in a
+// register, a lane each: no barrier, and one comparison finds a tile's segment.
+template <int WAVES, bool PRE, bool MANY>
+struct Dealt {
+  int* lds;   // [n_seg + 1] of more than 64 segments
+  int mine;   // before segment `lane`
+  int n_seg, total;
+
+  __device__ __forceinline__ Dealt(const DecArgs& a, int* at, int block) : lds(at) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    n_seg = PRE ? a.n_groups : a.s.B;
+    auto tiles = [&](int s) { return s < n_seg ? sight<PRE>(a, s).n * row_blocks<PRE, MANY>(a, s) : 0; };
+    if (n_seg <= 64) {
+      const int n = tiles(lane), x = wave_scan(n);
+      mine = x - n;
+      total = __builtin_amdgcn_readlane(x, 63);
+      if (block == 0 && wave == 0) {
+        if (lane < n_seg) a.part[PRE].first[lane] = mine;
+        if (lane == 0) a.part[PRE].first[n_seg] = total;
+      }
+      return;
+    }
+    __shared__ int wave_sum[WAVES];
+    total = 0;
+    for (int s0 = 0; s0 < n_seg; s0 += WAVES * 64) {
+      const int n = tiles(s0 + tid), x = wave_scan(n);
+      if (lane == 63) wave_sum[wave] = x;
+      __syncthreads();
+      int before = total;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += wave_sum[w];
+        total += wave_sum[w];
+      }
+      if (s0 + tid < n_seg) lds[s0 + tid] = before + x - n;
+      if (s0 + tid == n_seg - 1) lds[n_seg] = total;
+      __syncthreads();
+    }
+    total = uni(total);
+    if (block == 0)
+      for (int s = tid; s <= n_seg; s += WAVES * 64) a.part[PRE].first[s] = lds[s];
+  }
+  __device__ __forceinline__ int first(int seg) const {
+    if (n_seg > 64) return uni(lds[seg]);
+    return seg < n_seg ? __builtin_amdgcn_readlane(mine, seg) : total;
+  }
+  // The segment that tile `pos` of a head lies in: the last one that starts at or before it.
+  __device__ __forceinline__ int find(int pos) const {
+    if (n_seg <= 64) return uni(__popcll(__ballot((int)(threadIdx.x & 63) < n_seg && mine <= pos)) - 1);
+    int seg = 0;
+    for (int end = n_seg; end - seg > 1;) {
+      const int mid = (seg + end) >> 1;
+      if (first(mid) <= pos) seg = mid;
+      else end = mid;
+    }
+    return seg;
+  }
+};
 // Tiles of a run.
 template <bool MANY>
 __device__ __forceinline__ int run_tiles(int all, int workers) {
   return max((all + workers - 1) / workers, MANY ? 2 : 1);
-}
-// The segment that tile `pos` of a head lies in: the last one that starts at or before it.
-__device__ __forceinline__ int find_segment(const int* first, int n_seg, int pos) {
-  int seg = 0;
-  for (int end = n_seg; end - seg > 1;) {
-    const int mid = (seg + end) >> 1;
-    if (uni(first[mid]) <= pos) seg = mid;
-    else end = mid;
-  }
-  return seg;
 }
 // Slot of a piece of a column (segment, head, row block). A worker has one piece that
 // goes on with a column (its first) and one that begins a column without ending it (its
@@ -380,14 +407,15 @@ struct Few {
 template <int WAVES, int NB, bool PRE>
 __device__ __forceinline__ void few_rows(const DecArgs& a, int* first, int block) {
   const int n_seg = PRE ? a.n_groups : a.s.B, R = a.part[PRE].rows;
-  const int total = deal<WAVES, PRE, false>(a, first, block);
+  const Dealt<WAVES, PRE, false> deal(a, first, block);
+  const int total = deal.total;
   const int worker = block * WAVES + uni(threadIdx.x >> 6), all = total * a.Hkv;
   const int run = run_tiles<false>(all, a.part[PRE].workers);
   int at = worker * run;  // workers * run stays below all + workers
   const int stop = min(at + run, all);
   while (at < stop) {
-    const int h = at / total, pos = at - h * total, seg = find_segment(first, n_seg, pos);
-    const int i0 = pos - uni(first[seg]), n = uni(first[seg + 1]) - uni(first[seg]), i1 = min(n, i0 + stop - at);
+    const int h = at / total, pos = at - h * total, seg = deal.find(pos);
+    const int i0 = pos - deal.first(seg), n = deal.first(seg + 1) - deal.first(seg), i1 = min(n, i0 + stop - at);
     at += i1 - i0;
     const Sight si = sight<PRE>(a, seg);
     Few<NB> f;
@@ -424,7 +452,10 @@ __device__ __forceinline__ void few_rows(const DecArgs& a, int* first, int block
 }
 
 // One workgroup a sequence and head, its pages dealt to WAVES wavefronts and joined in
-// LDS: where the pages are few this one launch ends sooner than pieces and their join.
+// LDS: where the pages are few this one launch ends sooner than pieces and their join. us
+// of one against the other, 32 query and 8 kv heads: 1 sequence of 1500 tokens 14.2, 15.9; 8 of
+// up to 1600 14.5, 16.1; 8 of 2000 19.0, 16.3; 48 with a window of 1024 24.7, 30.0; 64 of
+// 2000 44.7, 51.2; 200 of up to 1800 84, 103; 64 of up to 4000 77, 52.
 template <int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 3) kv8_whole_kernel(const DecArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -496,16 +527,16 @@ template <bool PRE>
 __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int block) {
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, lh = lane >> 5, wave = uni(tid >> 6), turn = wave >> 2;
   const int n_seg = PRE ? a.n_groups : a.s.B, R = a.part[PRE].rows, all_rb = (R + kManyRows - 1) / kManyRows;
-  int* const first = reinterpret_cast<int*>(smem + kManyLds);
-  const int total = deal<kManyWaves, PRE, true>(a, first, block), all = total * a.Hkv;
+  const Dealt<kManyWaves, PRE, true> deal(a, reinterpret_cast<int*>(smem + kManyLds), block);
+  const int total = deal.total, all = total * a.Hkv;
   const int run = run_tiles<true>(all, a.part[PRE].workers);
   lds_char* const lds = (lds_char*)smem;
   int at = block * run;
   const int stop = min(at + run, all);
   while (at < stop) {
-    const int h = at / total, pos = at - h * total, seg = find_segment(first, n_seg, pos);
-    const int nrb = uni(row_blocks<PRE, true>(a, seg)), n = (uni(first[seg + 1]) - uni(first[seg])) / nrb;
-    const int rem = pos - uni(first[seg]), rb = rem / n, i0 = rem - rb * n, i1 = min(n, i0 + stop - at);
+    const int h = at / total, pos = at - h * total, seg = deal.find(pos);
+    const int nrb = uni(row_blocks<PRE, true>(a, seg)), n = (deal.first(seg + 1) - deal.first(seg)) / nrb;
+    const int rem = pos - deal.first(seg), rb = rem / n, i0 = rem - rb * n, i1 = min(n, i0 + stop - at);
     at += i1 - i0;
     const Sight si = sight<PRE>(a, seg);
     Row w = row_of<PRE>(a, seg, h, min(rb * kManyRows + 32 * wave + lq, R - 1), si.hi);
@@ -635,8 +666,8 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
       steps(j, 1, 0);
       const bool whole = __all((w.hi == 0) | ((key0 + kPage <= w.hi) & ((key0 >= w.lo) | (key0 + kPage <= w.sunk))));
       auto in = [&](int i) {  // whether the row sees key i + 4 lh of the page
-        const int x = key0 + 4 * lh + i;
-        return (x < w.hi) & ((x >= w.lo) | (x < w.sunk));
+        const int at = key0 + 4 * lh;
+        return (i < w.hi - at) & ((i >= w.lo - at) | (i < w.sunk - at));
       };
       if (!whole)
 #pragma unroll
@@ -815,28 +846,33 @@ __device__ __forceinline__ int64_t piece_row(const DecArgs& a, const Pieces& p, 
   return slot_of<PRE>(a, p.w0 + x, p.column, x == 0) * p.rows + p.r;
 }
 
-// WAVES wavefronts a row (b, t, query head): half a wavefront reads a piece's 128 values,
-// weighed by their maxima.
+// A row (b, t, query head) and its pieces; false where it was written as its only piece.
+// (A call has less than 2^25 rows.)
+struct JoinRow { Row w; Pieces own, pre; };
+__device__ __forceinline__ bool find_row(const DecArgs& a, int row, JoinRow& j) {
+  const int Hq = a.Hkv * a.G, tok = row / Hq, b = tok / a.s.T, t = tok - b * a.s.T;
+  j.w.q_row = tok;
+  j.w.head = row - tok * Hq;
+  if (t >= kv8_len(a.s, b).fresh) return true;  // padding: no pieces, zeros and -inf
+  const int h = j.w.head / a.G, r = t * a.G + j.w.head - h * a.G;
+  j.own = pieces_of<false>(a, b, h, r);
+  if (a.n_groups == 0) return j.own.n != 1;
+  j.pre = pieces_of<true>(a, b / a.gs, h, (b % a.gs) * a.s.T * a.G + r);
+  return true;
+}
+
+// The row by WAVES wavefronts: half a wavefront reads a piece's 128 values, weighed by
+// their maxima.
 template <int WAVES>
-__global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
+__device__ __forceinline__ void join_row(const DecArgs& a, int row) {
   __shared__ __attribute__((aligned(16))) float lds_o[4][kKv8Hd];
   __shared__ float lds_m[4], lds_l[4];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
   const int share = wave % WAVES;  // of the row's wavefronts
-  const int Hq = a.Hkv * a.G;
-  if (row >= (int64_t)a.s.B * a.s.T * Hq) return;
-  Row w;
-  w.q_row = row / Hq;
-  w.head = (int)(row % Hq);
-  const int b = (int)(w.q_row / a.s.T), t = (int)(w.q_row % a.s.T), h = w.head / a.G;
-  Pieces own, pre;
-  if (t < kv8_len(a.s, b).fresh) {
-    const int r = t * a.G + w.head % a.G;
-    own = pieces_of<false>(a, b, h, r);
-    if (a.n_groups) pre = pieces_of<true>(a, b / a.gs, h, (b % a.gs) * a.s.T * a.G + r);
-    else if (own.n == 1) return;  // written already
-  }
+  JoinRow j;
+  if (!find_row(a, row, j)) return;
+  const Row& w = j.w;
+  const Pieces &own = j.own, &pre = j.pre;
   float M = kNoMax, L = 0.f;
   f32x4 acc{};
   const int all = pre.n + own.n;
@@ -899,6 +935,22 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
   }
   if (lane < 32) write_row<4, 1>(a, w, &acc, M, L, lane);
 }
+// WAVES 1: four rows a wavefront, one after the other. Where there are many rows most were
+// written as their only piece: a lane each looks.
+template <int WAVES>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
+  if (WAVES > 1) {
+    join_row<4>(a, blockIdx.x);
+    return;
+  }
+  const int rows = a.s.B * a.s.T * a.Hkv * a.G, row = (blockIdx.x * 4 + uni(threadIdx.x >> 6)) * 4, lane = threadIdx.x & 63;
+  bool todo = lane < 4 && row + lane < rows;
+  if (todo) {
+    JoinRow j;
+    todo = find_row(a, row + lane, j);
+  }
+  for (uint64_t m = __ballot(todo); m; m &= m - 1) join_row<1>(a, row + __builtin_ctzll(m));
+}
 
 // ------------------------------------------------------------------ host
 // The work of a kind of segments: n_table pages at most, of which a window of `span`
@@ -949,8 +1001,7 @@ Plan plan(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d) 
   p.d[1] = deal_of(d->n_prefix_table, d->window, S, p.rows[1], segs[1], H, true, false);
   p.d[0] = deal_of(s->n_table, d->window ? (int64_t)d->window + s->T - 1 : 0, S, p.rows[0], segs[0], H, d->n_groups > 0,
                    p.d[1].kind == kMany);
-  // One workgroup a sequence and head reads 16 pages in the time of a launch more.
-  if (d->n_groups == 0 && p.d[0].kind == kFew16 && p.d[0].pages <= 16) {
+  if (d->n_groups == 0 && p.d[0].kind == kFew16 && p.d[0].pages <= (s->B * H >= 256 ? 32 : 24)) {
     p.whole = s->B * H <= 256 ? 8 : 4;
     return p;
   }
@@ -1047,7 +1098,7 @@ glt_status launch(DecArgs& a, const Plan& p, const char* who, hipStream_t st) {
   if (rows <= 4096)  // few rows of many pieces, mostly
     GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
   else
-    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 16)), dim3(256), 0, st, a);
   GLT_LAUNCH_CHECK("kv8_join");
   return GLT_OK;
 }

@@ -146,6 +146,6 @@ def test_sizes():
     assert ws(**wide) <= 2 * 256 * 12 * 12 * (512 + 8) + 4 * 5 + 1024
     assert ws(T=500, **wide) <= 2 * 256 * 256 * (512 + 8) + 4 * 5 + 1024
     # a few pages a sequence, in a table or a window: one launch, nothing between
-    assert ws(n_table=16, pages_ld=16) == ws(window=900, **wide) == 256
-    assert ws(n_table=17, pages_ld=17) > 256
+    assert ws(n_table=24, pages_ld=24) == ws(window=1400, **wide) == 256
+    assert ws(n_table=25, pages_ld=25) > 256 and ws(B=200, n_table=32, pages_ld=32) == 256
     assert ws(**PREFIX) > ws()
