@@ -151,13 +151,18 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
     const int key0 = tiles.tile(t) * kTile + 32 * kb;
     score_product<kDqAhead>(row, qf, s, [](int) {});
     if (WIN) {
-      if (key0 + 32 > len || key0 + 31 > wq0 || (key0 <= wq0 + 31 - a.window && key0 + 32 > a.sinks)) {
-        const int base = key0 + 4 * lh;
-        const int hi = min(len, myq + 1) - base, lo = myq - a.window + 1 - base, sunk = a.sinks - base;
+      const int base = key0 + 4 * lh;
+      if (key0 + 32 > len || key0 + 31 > wq0) {
+        const int lim = min(len, myq + 1) - base;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < lim ? s[e] : -INFINITY;
+      }
+      if (key0 <= wq0 + 31 - a.window && key0 + 32 > a.sinks) {
+        const int from = myq - a.window + 1 - base, sunk = a.sinks - base;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int i = 8 * (e >> 2) + (e & 3);
-          s[e] = (i < hi) & ((i >= lo) | (i < sunk)) ? s[e] : -INFINITY;
+          s[e] = (i >= from) | (i < sunk) ? s[e] : -INFINITY;
         }
       }
     } else if (key0 + 32 > len || (a.causal && key0 + 31 > wq0)) {

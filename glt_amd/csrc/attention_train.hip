@@ -130,16 +130,31 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_train_fwd_kernel(const Fw
     // a window it may not: the maximum stays where it starts and the
     // probabilities are zeros.)
     if (WIN) {
-      if (key0 + kTile > len || key0 + kTile - 1 > wq0 || (key0 <= wq0 + 31 - a.window && key0 + kTile > a.sinks)) {
-        const int base = key0 + 4 * lh;
-        const int hi = min(len, myq + 1) - base, lo = myq - a.window + 1 - base, sunk = a.sinks - base;
+      // an edge at a time: few tiles have two
+      const int base = key0 + 4 * lh;
+      if (key0 + kTile > len || key0 + kTile - 1 > wq0) {
+        const int lim = min(len, myq + 1) - base;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int i = 32 * kb + 8 * (e >> 2) + (e & 3);
-            s[kb][e] = (i < hi) & ((i >= lo) | (i < sunk)) ? s[kb][e] : -INFINITY;
-          }
+          for (int e = 0; e < 16; ++e) s[kb][e] = (32 * kb + 8 * (e >> 2) + (e & 3)) < lim ? s[kb][e] : -INFINITY;
+      }
+      if (key0 <= wq0 + 31 - a.window && key0 + kTile > a.sinks) {
+        const int from = myq - a.window + 1 - base, sunk = a.sinks - base;
+        if (key0 >= a.sinks) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] = (32 * kb + 8 * (e >> 2) + (e & 3)) >= from ? s[kb][e] : -INFINITY;
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int i = 32 * kb + 8 * (e >> 2) + (e & 3);
+              s[kb][e] = (i >= from) | (i < sunk) ? s[kb][e] : -INFINITY;
+            }
+        }
       }
     } else if (key0 + kTile > len || (a.causal && key0 + kTile - 1 > wq0)) {
       const int lim = (a.causal ? min(len, myq + 1) : len) - (key0 + 4 * lh);

@@ -935,16 +935,17 @@ __device__ __forceinline__ void join_row(const DecArgs& a, int row) {
   }
   if (lane < 32) write_row<4, 1>(a, w, &acc, M, L, lane);
 }
-// WAVES 1: four rows a wavefront, one after the other. Where there are many rows most were
-// written as their only piece: a lane each looks.
-template <int WAVES>
+// A row by four wavefronts or one, or several rows a wavefront, one after the other: where
+// there are many most were written as their only piece, and a lane each looks.
+template <int WAVES, int ROWS>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
-  if (WAVES > 1) {
-    join_row<4>(a, blockIdx.x);
+  if (ROWS == 1) {
+    const int row = blockIdx.x * (4 / WAVES) + uni(threadIdx.x >> 6) / WAVES;
+    if (row < a.s.B * a.s.T * a.Hkv * a.G) join_row<WAVES>(a, row);
     return;
   }
-  const int rows = a.s.B * a.s.T * a.Hkv * a.G, row = (blockIdx.x * 4 + uni(threadIdx.x >> 6)) * 4, lane = threadIdx.x & 63;
-  bool todo = lane < 4 && row + lane < rows;
+  const int rows = a.s.B * a.s.T * a.Hkv * a.G, row = (blockIdx.x * 4 + uni(threadIdx.x >> 6)) * ROWS, lane = threadIdx.x & 63;
+  bool todo = lane < ROWS && row + lane < rows;
   if (todo) {
     JoinRow j;
     todo = find_row(a, row + lane, j);
@@ -1095,10 +1096,12 @@ glt_status launch(DecArgs& a, const Plan& p, const char* who, hipStream_t st) {
                lds, st, a);
     GLT_LAUNCH_CHECK("kv8_pieces");
   }
-  if (rows <= 4096)  // few rows of many pieces, mostly
-    GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
+  if (rows <= 4096)
+    GLT_LAUNCH("kv8_join", (kv8_join_kernel<4, 1>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else if (rows <= 32768)
+    GLT_LAUNCH("kv8_join", (kv8_join_kernel<1, 1>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
   else
-    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 16)), dim3(256), 0, st, a);
+    GLT_LAUNCH("kv8_join", (kv8_join_kernel<1, 8>), dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
   GLT_LAUNCH_CHECK("kv8_join");
   return GLT_OK;
 }
