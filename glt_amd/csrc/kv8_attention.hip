@@ -1115,8 +1115,8 @@ using namespace glt;
 extern "C" size_t glt_kv8_attention_workspace_size(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d) {
   if (!c || !s || !d || s->B <= 0 || s->T <= 0 || c->n_kv_heads <= 0 || d->n_q_heads < c->n_kv_heads || s->n_table < 0 ||
       d->n_groups < 0 || d->window < 0 || d->sinks < 0 || (d->n_groups > 0 && d->n_prefix_table < 0))
-    return 256;
-  return std::max<size_t>(plan(c, s, d).bytes, 256);
+    return 0;
+  return plan(c, s, d).bytes;
 }
 
 extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d, const void* q,
@@ -1133,8 +1133,8 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
   GLT_CHECK(((uintptr_t)q | (uintptr_t)out) % 16 == 0 && (uintptr_t)lse % 4 == 0, GLT_ERR_ALIGNMENT,
             "%s: tensors must be 16-byte aligned", who);
   const Plan p = plan(c, s, d);
-  const size_t need = std::max<size_t>(p.bytes, 256);
-  GLT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, GLT_ERR_WORKSPACE,
+  const size_t need = p.bytes;
+  GLT_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0), GLT_ERR_WORKSPACE,
             "%s: needs %zu workspace bytes, 256-byte aligned", who, need);
   const int64_t tokens = (int64_t)s->B * s->T, nq = 2 * kKv8Hd * (int64_t)d->n_q_heads;
   const ByteRows all[] = {{out, tokens, nq, 2 * o_ld},

@@ -348,6 +348,13 @@ def _heads_ld(name, t, B, T, device):
     return ld
 
 
+def _check_window(window, sinks):
+    if window is None:
+        _need(sinks == 0, "sinks: with a window")
+    elif not (1 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
+        raise ValueError(f"window {window} (None, or 1 to 2^31 - 1), sinks {sinks}")
+
+
 def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
     shape = q.shape
     _need(len(shape) == 4 and q.is_cuda, "q: [B, T, heads, head_dim] on a GPU")
@@ -372,7 +379,7 @@ def attention_train(q, k, v, causal=True, scale=None, seq_lens=None, window=None
     the lengths of a padded batch (rows past them: zero output, lse -inf).
     window=W: of the keys up to itself a row reads the last W (its own among
     them) and the first `sinks` of its sequence."""
-    _need(sinks == 0 or window is not None, "sinks: with a window")
+    _check_window(window, sinks)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     d, (B, T, Hq, _, _), _ = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
     lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device)
@@ -409,7 +416,7 @@ def attention_bwd(q, k, v, out, lse, dout, causal=True, scale=None, seq_lens=Non
     of one buffer where q, k, v are; `grads` gives them, overlapping no input).
     out and lse are the forward's; dout has out's shape and strides. workspace: a uint8 tensor of
     glt_attention_bwd_workspace_size (glt_attention_window_bwd_workspace_size) bytes to use instead of a new one."""
-    _need(sinks == 0 or window is not None, "sinks: with a window")
+    _check_window(window, sinks)
     d, shape, lds = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
     B, T, Hq, _, _ = shape
     dev = q.device
@@ -439,7 +446,8 @@ def _table_ld(name, t, rows, index):
     ld, step = t.stride()
     if step == 1 and ld >= n:
         return ld
-    _need((n <= 1 or step == 1) and (rows <= 1 or n == 0), f"{name}: strides {t.stride()} (a row's pages contiguous, rows apart)")
+    if (n > 1 and step != 1) or (rows > 1 and n != 0):
+        raise ValueError(f"{name}: strides {t.stride()} (a row's pages contiguous, rows apart)")
     return n
 
 
@@ -489,15 +497,17 @@ class Kv8Cache:
         if out is None:
             k = torch.empty((pages.shape[0], T, *self._heads), dtype=torch.bfloat16, device=self._device)
             out = k, torch.empty_like(k)
-        else:
-            _need(out[0].shape[:2] == (pages.shape[0], T), f"out: {pages.shape[0]} x {T} tokens")
+        elif out[0].shape[:2] != (pages.shape[0], T):
+            raise ValueError(f"out: {pages.shape[0]} x {T} tokens")
         self._tokens("glt_kv8_read", *out, pages, lens, new_lens)
         return out
 
     def _tokens(self, name, k, v, pages, lens, new_lens):
         shape = k.shape
-        _need(len(shape) == 4 and shape[2:] == self._heads and shape == v.shape, f"k, v: [B, T, {self.n_kv_heads}, {self.head_dim}]")
-        B, T, dev = shape[0], shape[1], self._device
+        if len(shape) != 4 or shape[2:] != self._heads or shape != v.shape:
+            raise ValueError(f"k, v: [B, T, {self.n_kv_heads}, {self.head_dim}]")
+        B, T, _, _ = shape
+        dev = self._device
         k_ld, v_ld = _heads_ld("k", k, B, T, dev), _heads_ld("v", v, B, T, dev)
         s = self._seqs(B, T, pages, lens, new_lens)
         _call_on(self.data, name, self._ref, ctypes.byref(s), k.data_ptr(), k_ld, v.data_ptr(), v_ld)
@@ -512,14 +522,17 @@ class Kv8Cache:
         uint8 tensor of glt_kv8_attention_workspace_size bytes instead of a new
         one."""
         shape = q.shape
-        _need(len(shape) == 4 and shape[3] == self.head_dim, f"q: [B, T, heads, {self.head_dim}]")
+        if len(shape) != 4 or shape[3] != self.head_dim:
+            raise ValueError(f"q: [B, T, heads, {self.head_dim}]")
         B, T, Hq, hd = shape
         dev, index = self._device, self._index
         q_ld = _heads_ld("q", q, B, T, dev)
         if window is None:
             window = 0
-        else:
-            _need(window > 0, f"window {window} (None, or at least 1)")
+        elif not 1 <= window < 2 ** 31:
+            raise ValueError(f"window {window} (None, or 1 to 2^31 - 1)")
+        if not 0 <= sinks < 2 ** 31:
+            raise ValueError(f"sinks {sinks} (0 to 2^31 - 1)")
         s = self._seqs(B, T, pages, lens, new_lens)
         d = F.Kv8Attn(Hq, hd ** -0.5 if scale is None else scale, window, sinks)
         if prefix is not None:
@@ -530,11 +543,15 @@ class Kv8Cache:
             _check_ints("prefix lens", plens, groups, index)
             d.prefix_pages, d.n_prefix_table, d.prefix_lens = ppages.data_ptr(), ppages.shape[1], plens.data_ptr()
         refs = self._ref, ctypes.byref(s), ctypes.byref(d)
-        workspace = _workspace(workspace, F.load().glt_kv8_attention_workspace_size(*refs), dev)
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        nbytes = F.load().glt_kv8_attention_workspace_size(*refs)
+        if nbytes:
+            workspace = _workspace(workspace, nbytes, dev)
+            ws = workspace.data_ptr(), workspace.numel()
+        else:  # one launch: nothing between
+            ws = None, 0
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=torch.bfloat16, device=dev)
         lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
-        _call_on(self.data, "glt_kv8_attention", *refs, q.data_ptr(), q_ld, out.data_ptr(), Hq * hd, lse.data_ptr(),
-                 workspace.data_ptr(), workspace.numel())
+        _call_on(self.data, "glt_kv8_attention", *refs, q.data_ptr(), q_ld, out.data_ptr(), Hq * hd, lse.data_ptr(), *ws)
         return out, lse
 
 

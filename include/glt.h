@@ -447,8 +447,8 @@ typedef struct {
 
 /* The new tokens' k and v [B, T, n_kv_heads, 128] bf16 (strides and alignment as
  * in glt_attn_desc) into the cache. Tokens t >= new_lens[b] are not read, and no other
- * byte of the pool is touched. Two sequences that write the same token leave
- * either's codes. */
+ * byte of the pool is touched. What a call writes twice, or two calls at once, holds a
+ * mixture of both. */
 glt_status glt_kv8_write(const glt_kv8_cache* c, const glt_kv8_seqs* s, const void* k, int64_t k_ld, const void* v,
                          int64_t v_ld, void* stream);
 /* The values that the cache holds of the new tokens, rounded to bf16 once; rows t
@@ -480,7 +480,7 @@ typedef struct {
  * new_lens[b] get zeros and -inf. |q| < 2^112 (the codes' products stay in f32). q
  * overlaps neither out, lse nor the workspace, nor any of them each other or the
  * cache. workspace: glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing
- * kept in it between calls. */
+ * kept in it between calls; where that is 0 it may be NULL. */
 size_t glt_kv8_attention_workspace_size(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d);
 glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d, const void* q,
                              int64_t q_ld, void* out, int64_t o_ld, float* lse, void* workspace,

@@ -82,6 +82,25 @@ def test_forward_and_backward_against_the_formula(dev, B, T, Hq, Hkv, window, si
             assert name == "lse" or not got[name][b, n:].any(), name
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,window,sinks,fused", [
+    (12, 1400, 16, 4, 100, 4, True),      # key blocks that fill the chip: a kv head's query heads in one workgroup
+    (12, 1400, 16, 4, 700, 0, False),
+    (12, 1400, 16, 4, 701, 0, False),     # in parts again
+    (6, 1400, 16, 4, 64, 130, False),     # in two parts
+    (24, 700, 6, 3, 90, 1, True),
+])
+def test_batches_that_fill_the_chip(dev, B, T, Hq, Hkv, window, sinks, fused):
+    q, k, v, dout = make(B, T, Hq, Hkv, 31, fused, 2.0)
+    lens = [T - (137 * i) % 900 if i % 3 else T for i in range(B)]
+    got = run(q, k, v, dout, seq_lens=torch.tensor(lens, dtype=torch.int32, device=dev), window=window, sinks=sinks)
+    lens = [max(n, 0) for n in lens]
+    for b in (1, B - 1):
+        one = [t[b:b + 1] for t in (q, k, v, dout)]
+        want = formula(*one, HD ** -0.5, lens[b:b + 1], window, sinks)
+        for name in want:
+            check(name, got[name][b:b + 1], want[name], lse_bound(one[0], one[1], HD ** -0.5, want["lse"]))
+
+
 @pytest.mark.parametrize("window", [333, 334, 5000, 2 ** 31 - 1])
 @pytest.mark.parametrize("sinks", [0, 7])
 def test_a_window_that_hides_nothing(dev, window, sinks):
@@ -182,16 +201,14 @@ def test_refusals(dev):
     from glt_amd import ops
     q, k, v, dout = make(2, 20, 4, 2, 19)
     out, lse = ops.attention_train(q, k, v, window=3)
-    for kw in (dict(window=0), dict(window=-1), dict(window=3, sinks=-1), dict(window=3, sinks=1025),
-               dict(window=3, causal=False)):
-        with pytest.raises(ops.F.GltError):
+    for kw, err in ((dict(window=3, sinks=1025), ops.F.GltError), (dict(window=3, causal=False), ops.F.GltError),
+                    (dict(window=0), ValueError), (dict(window=-1), ValueError), (dict(window=2 ** 32 + 5), ValueError),
+                    (dict(window=3, sinks=-1), ValueError), (dict(window=3, sinks=2 ** 32), ValueError),
+                    (dict(sinks=3), ValueError)):
+        with pytest.raises(err):
             ops.attention_train(q, k, v, **kw)
-        with pytest.raises(ops.F.GltError):
+        with pytest.raises(err):
             ops.attention_bwd(q, k, v, out, lse, dout, **kw)
-    with pytest.raises(ValueError):
-        ops.attention_train(q, k, v, sinks=3)
-    with pytest.raises(ValueError):
-        ops.attention_bwd(q, k, v, out, lse, dout, sinks=3)
 
 
 # ------------------------------------------------------- the set together

@@ -216,6 +216,92 @@ def test_prefixes(dev, T, Hq, Hkv, lens, new, plens, window, sinks):
     Setup(T, Hq, Hkv, lens, new, plens, seed=2).check(window, sinks)
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 70)])
+@pytest.mark.parametrize("T,Hq,Hkv,lens,new,plens", [
+    (300, 4, 1, [300, 777, 512], [300, 77, 0], None),        # five row blocks, in runs that end anywhere
+    (500, 8, 2, [1500], None, None),
+    (70, 12, 2, [70, 400, 90, 71], [70, 64, 1, 0], [900, 63]),
+    (33, 8, 1, [33, 200], None, [4000, 4000]),
+])
+def test_many_rows(dev, T, Hq, Hkv, lens, new, plens, window, sinks):
+    Setup(T, Hq, Hkv, lens, new, plens or (), seed=12).check(window, sinks)
+
+
+def test_many_sequences_of_many_rows(dev):
+    """More columns than workgroups: most rows are written as their only piece."""
+    lens = [40 + (97 * i) % 300 for i in range(70)]
+    Setup(40, 16, 4, lens, [(11 * i) % 41 for i in range(70)], seed=13, extra=0).check()
+
+
+@pytest.mark.parametrize("T,Hq,lens,new,plens", [
+    (4, 4, [300, 90], [4, 2], None), (4, 4, [3000, 90], [4, 2], None), (6, 8, [3000, 90], [6, 2], None),
+    (60, 8, [300, 90], [60, 2], None), (4, 4, [300, 90], [4, 2], [200]), (20, 8, [300, 90], [20, 2], [500]),
+])
+def test_a_bad_query_row_stays_alone(dev, T, Hq, lens, new, plens):
+    """NaN and infinity in padding and in one row: the other rows keep their bits."""
+    s = Setup(T, Hq, 1, lens, new, plens or (), seed=14)
+    a, al = s.run(window=200, sinks=3)
+    for bad in (float("nan"), float("inf"), -3e38):
+        q = s.q.clone()
+        s.q[1, 2:] = bad                    # padding
+        s.q[0, 1, 0] = bad
+        b, bl = s.run(window=200, sinks=3)
+        s.q.copy_(q)
+        assert torch.isnan(b[0, 1, 0]).all() or bad == -3e38
+        b[0, 1, 0], bl[0, 0, 1] = a[0, 1, 0], al[0, 0, 1]
+        assert torch.equal(a, b) and torch.equal(al, bl)
+
+
+@pytest.mark.parametrize("T,Hq", [(3, 2), (70, 4)])
+def test_lengths_outside_the_tables_are_clamped(dev, T, Hq):
+    s = Setup(T, Hq, 2, [128, 128, 30], extra=0, seed=15)
+    q, p = s.q, s.pages
+    a = s.cache.attention(q, p, ints([128, 0, 30]), new_lens=ints([T, 0, 2]))
+    b = s.cache.attention(q, p, ints([2 ** 31 - 1, -5, 30]), new_lens=ints([2 ** 31 - 1, T, 2]))
+    c = s.cache.attention(q, p, ints([500, 128, 30]), new_lens=ints([T + 1, -3, 2]))
+    for x in (b, c):
+        assert torch.equal(a[0], x[0]) and torch.equal(a[1], x[1])
+    k0, _ = s.cache.read(p, ints([128, 0, 30]), T, ints([T, 0, 2]))
+    k1, _ = s.cache.read(p, ints([2 ** 31 - 1, -5, 30]), T, ints([2 ** 31 - 1, T, 2]))
+    assert torch.equal(k0, k1)
+    pre = (s.table[:1], ints([2 ** 31 - 1]))
+    x = s.cache.attention(q, p, ints([128, 0, 30]), new_lens=ints([T, 0, 2]), prefix=pre)
+    y = s.cache.attention(q, p, ints([128, 0, 30]), new_lens=ints([T, 0, 2]), prefix=(s.table[:1], ints([128])))
+    assert torch.equal(x[0], y[0])
+    z = s.cache.attention(q, p, ints([128, 0, 30]), new_lens=ints([T, 0, 2]), prefix=(s.table[:1], ints([-1])))
+    R.check(z[0][2, :2], z[1][2, :, :2], R.attend(q[2, :2], s.k[2], s.v[2], torch.arange(28, 30), HD ** -0.5))
+
+
+def test_calls_at_once_on_two_streams(dev):
+    """Each with its own workspace, over one cache."""
+    s = Setup(1, 8, 2, [5000, 333, 64], seed=16)
+    t = Setup(50, 8, 2, [700, 90], plens=[900], seed=17)
+    want = s.run(), t.run()
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(sa):
+            a = s.run(), s.run(window=200, sinks=4)
+        with torch.cuda.stream(sb):
+            b = t.run()
+        got.append((a[0], b))
+    torch.cuda.synchronize()
+    for a, b in got:
+        for x, y in zip(a + b, want[0] + want[1]):
+            assert torch.equal(x, y)
+
+
+def test_no_sequences(dev):
+    cache = ops.Kv8Cache(2, 1)
+    none, q = torch.empty(0, 3, dtype=I32, device="cuda"), torch.empty(0, 1, 2, HD, dtype=BF, device="cuda")
+    out, lse = cache.attention(q, none, ints([]))
+    assert out.shape == (0, 1, 2, HD) and lse.shape == (0, 2, 1)
+    k = torch.empty(0, 1, 1, HD, dtype=BF, device="cuda")
+    cache.write(k, k, none, ints([]))
+    assert cache.read(none, ints([]), 1)[0].shape == (0, 1, 1, HD)
+
+
 @pytest.mark.parametrize("T,lens,window,sinks", [(1, [400, 100], 60, 2), (1, [400, 300], None, 0), (40, [400, 100], 60, 2)])
 def test_a_bad_token_reaches_the_rows_that_see_it(dev, T, lens, window, sinks):
     """Values of NaN at token 341 of the first sequence, and at one that no row sees."""
@@ -367,13 +453,14 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             cache.write(**a)
     for bad in (dict(q=q[..., :64]), dict(q=q.float()), dict(window=0), dict(window=-1),
+                dict(window=2 ** 32 + 5), dict(sinks=-1), dict(sinks=2 ** 32),
                 dict(prefix=(pages[:0], lens[:0])), dict(prefix=(pages, lens.long())),
-                dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))):
+                dict(prefix=(pages, lens), workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))):
         a = dict(q=q, pages=pages, lens=lens)
         a.update(bad)
         with pytest.raises(ValueError):
             cache.attention(**a)
-    for bad in (dict(q=q[:, :, :3].contiguous()), dict(scale=0.0), dict(scale=float("nan")), dict(sinks=-1),
+    for bad in (dict(q=q[:, :, :3].contiguous()), dict(scale=0.0), dict(scale=float("nan")),
                 dict(prefix=(ints([[0]] * 3), ints([1] * 3)))):
         a = dict(q=q, pages=pages, lens=lens)
         a.update(bad)

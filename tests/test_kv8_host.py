@@ -107,9 +107,10 @@ def test_attention_pointer_and_workspace_refusals():
         assert attn(**{n: v}) == 4
     for kw in (dict(q_ld=1016), dict(o_ld=1028), dict(q_ld=1 << 31)):
         assert attn(**kw) == 2
-    c, s, d = descs({})
+    kw = dict(n_table=40, pages_ld=40)
+    c, s, d = descs(kw)
     need = F.load().glt_kv8_attention_workspace_size(c, s, d)
-    assert attn(ws=None) == 5 and attn(nbytes=need - 1) == 5 and attn(ws=at(4) + 16) == 5
+    assert attn(kw, ws=None) == 5 and attn(kw, nbytes=need - 1) == 5 and attn(kw, ws=at(4) + 16) == 5
     lib = F.load()
     assert lib.glt_kv8_attention(None, s, d, P, 1024, P, 1024, P, P, 1 << 30, None) == 1
     assert lib.glt_kv8_attention(c, None, d, P, 1024, P, 1024, P, P, 1 << 30, None) == 1
@@ -121,7 +122,7 @@ def test_attention_pointer_and_workspace_refusals():
     dict(ws=at(2)), dict(out=P), dict(lse=P + 1024), dict(ws=P + 256), dict(ws=at(3)),
 ])
 def test_overlaps_are_refused(kw):
-    assert attn(**kw) == 1
+    assert attn(dict(n_table=40, pages_ld=40), **kw) == 1
     assert b"overlap" in F.load().glt_last_error_string()
 
 
@@ -136,7 +137,7 @@ def test_sizes():
     lib = F.load()
     assert lib.glt_kv8_size(10, 8, 128) == 10 * 8 * 64 * 260
     assert lib.glt_kv8_size(0, 8, 128) == 0 and lib.glt_kv8_size(10, 8, 64) == 0
-    assert lib.glt_kv8_attention_workspace_size(None, None, None) == 256
+    assert lib.glt_kv8_attention_workspace_size(None, None, None) == 0
 
     def ws(**kw):
         return lib.glt_kv8_attention_workspace_size(*descs(kw))
@@ -146,6 +147,6 @@ def test_sizes():
     assert ws(**wide) <= 2 * 256 * 12 * 12 * (512 + 8) + 4 * 5 + 1024
     assert ws(T=500, **wide) <= 2 * 256 * 256 * (512 + 8) + 4 * 5 + 1024
     # a few pages a sequence, in a table or a window: one launch, nothing between
-    assert ws(n_table=24, pages_ld=24) == ws(window=1400, **wide) == 256
-    assert ws(n_table=25, pages_ld=25) > 256 and ws(B=200, n_table=32, pages_ld=32) == 256
+    assert ws(n_table=24, pages_ld=24) == ws(window=1400, **wide) == 0
+    assert ws(n_table=25, pages_ld=25) > 0 and ws(B=200, n_table=32, pages_ld=32) == 0
     assert ws(**PREFIX) > ws()
