@@ -418,12 +418,18 @@ __device__ __forceinline__ void few_rows(const DecArgs& a, int* first, int block
     const int i0 = pos - deal.first(seg), n = deal.first(seg + 1) - deal.first(seg), i1 = min(n, i0 + stop - at);
     at += i1 - i0;
     const Sight si = sight<PRE>(a, seg);
+    // lane x: the id of the run's page i + x, 64 at a time, the first ones on their way
+    // while the rows are looked up
+    auto ids_from = [&](int i) {
+      const int x = i + (int)(threadIdx.x & 63);
+      return x < i1 ? page_id<PRE>(a, seg, a.W ? si.page(x) : x) : 0;
+    };
+    int ids = ids_from(i0);
     Few<NB> f;
     f.template begin<PRE>(a, seg, h, si.hi);
-    int ids = 0;  // lane x: the id of the run's page i0 + x, 64 at a time
     for (int i = i0; i < i1; ++i) {
-      const int x = (i - i0) & 63, lane = threadIdx.x & 63;
-      if (x == 0) ids = i + lane < i1 ? page_id<PRE>(a, seg, a.W ? si.page(i + lane) : i + lane) : 0;
+      const int x = (i - i0) & 63;
+      if (x == 0 && i > i0) ids = ids_from(i);
       const int id = __builtin_amdgcn_readlane(ids, x);
       f.page(a, page_at(a, id, h), page_ok(a, id), a.W ? si.page(i) : i);
     }
@@ -462,11 +468,13 @@ __global__ void __launch_bounds__(WAVES * 64, 3) kv8_whole_kernel(const DecArgs 
   const int R = a.part[0].rows, wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int h = blockIdx.x % a.Hkv, seg = blockIdx.x / a.Hkv;
   const Sight si = sight<false>(a, seg);
+  // lane x: the id of page wave + WAVES x (of at most 32)
+  const int own = wave + WAVES * lane, ids = own < si.n ? page_id<false>(a, seg, si.page(own)) : 0;
   Few<1> f;
   f.template begin<false>(a, seg, h, si.hi);
-  for (int i = wave; i < si.n; i += WAVES) {
-    const int p = si.page(i), id = uni(page_id<false>(a, seg, p));
-    f.page(a, page_at(a, id, h), page_ok(a, id), p);
+  for (int i = wave, x = 0; i < si.n; i += WAVES, ++x) {
+    const int id = __builtin_amdgcn_readlane(ids, x);
+    f.page(a, page_at(a, id, h), page_ok(a, id), si.page(i));
   }
   float* const ml = reinterpret_cast<float*>(smem);             // [WAVES][2][R]
   f32x4* const ov = reinterpret_cast<f32x4*>(smem + WAVES * 128);  // [WAVES][R][32]
@@ -539,9 +547,6 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
     const int rem = pos - deal.first(seg), rb = rem / n, i0 = rem - rb * n, i1 = min(n, i0 + stop - at);
     at += i1 - i0;
     const Sight si = sight<PRE>(a, seg);
-    Row w = row_of<PRE>(a, seg, h, min(rb * kManyRows + 32 * wave + lq, R - 1), si.hi);
-    if (rb * kManyRows + 32 * wave + lq >= R) w.hi = 0;
-    const bool works = __any(w.hi > 0);
     // of the list, what the block's rows see: to the last row's own key, from the first row's window on
     int from = i0, to = i1;
     if (!PRE) {
@@ -557,6 +562,13 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
       }
     }
     const int tiles = max(to - from, 0);
+    auto page_of = [&](int j) { return a.W ? si.page(from + j) : from + j; };
+    // lane x: the id of tile x, 64 at a time, the first ones on their way while the rows are looked up
+    auto ids_from = [&](int j) { return j + lane < tiles ? page_id<PRE>(a, seg, page_of(j + lane)) : 0; };
+    int ids = ids_from(0);
+    Row w = row_of<PRE>(a, seg, h, min(rb * kManyRows + 32 * wave + lq, R - 1), si.hi);
+    if (rb * kManyRows + 32 * wave + lq >= R) w.hi = 0;
+    const bool works = __any(w.hi > 0);
 
     bf16x8 qf[8];
     load_rows(qf, a.q + w.q_row * a.q_ld + (int64_t)w.head * kKv8Hd, true, lh);
@@ -566,10 +578,8 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
     u32x4 pw[4];
     float m_run = kNoMax, l_run = 0.f;
 
-    auto page_of = [&](int j) { return a.W ? si.page(from + j) : from + j; };
-    int ids = 0;  // lane x: the id of tile x, 64 at a time
     auto id_of = [&](int j) {
-      if ((j & 63) == 0) ids = j + lane < tiles ? page_id<PRE>(a, seg, page_of(j + lane)) : 0;
+      if ((j & 63) == 0 && j > 0) ids = ids_from(j);
       return __builtin_amdgcn_readlane(ids, j & 63);
     };
     // this thread's 16 codes of each tile: token q >> 3, channels 16 (q & 7) .., or
