@@ -9,6 +9,10 @@
 // codes. Those cross LDS into 16-byte stores (whole groups of tokens) or go out
 // byte by byte (a page's other tokens are never read or written: other streams
 // may hold them).
+//
+// Bound by memory: 8 sequences of up to 4096 new tokens, 8 kv heads: written in 26 us,
+// read back in 23 (269 MB in all, 5.5 TB/s); one token of 64 sequences 6 and 3.5, the
+// chain of lengths, table and rows.
 #include "kv8.hpp"
 #include "overlap.hpp"
 

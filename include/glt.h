@@ -402,11 +402,13 @@ glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* 
 /* The same with a window: row t reads, of the keys up to itself, those less than
  * `window` (at least 1) back and the first `sinks` (0 to 1024) of its sequence; d->causal
  * is 1. A window of T or more gives glt_attention_train_fwd's results. Tiles of 64 keys
- * that no row of a block reads are not visited: the work is T * (window + sinks), not T^2. */
+ * that no row of a block reads are not visited: the work is T * (window + sinks), not T^2.
+ * A NaN or infinity reaches rows that see a key of its tile, as without a window. */
 glt_status glt_attention_window_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
                                     const void* k, const void* v, void* out, float* lse, void* stream);
-/* Its backward, as glt_attention_bwd. The gradients of the sinks' keys are added from
- * every row of their sequence, in one fixed order. */
+/* Its backward, as glt_attention_bwd. The sums' order is fixed by the call's sizes (B, T,
+ * heads, window, sinks): the same call gives the same bits, and a sequence's dk and dv may
+ * round differently in a call of another size. */
 size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks);
 glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
                                     const void* k, const void* v, const void* out, const float* lse,
@@ -476,8 +478,9 @@ typedef struct {
 /* out = softmax(scale q . k^T) . v over the visible keys, [B, T, n_q_heads, 128]
  * bf16 (strides as in glt_attn_desc), lse [B, n_q_heads, T] f32. Scores are products of q
  * and the codes, scaled in f32; probabilities times the value's step are rounded to bf16 for
- * the second product; all sums and statistics are f32, in one fixed order. Rows t >=
- * new_lens[b] get zeros and -inf. |q| < 2^112 (the codes' products stay in f32). q
+ * the second product; all sums and statistics are f32, in an order that the call's sizes and
+ * lengths fix (the same call gives the same bits; a sequence's may round differently
+ * beside others). Rows t >= new_lens[b] get zeros and -inf. |q| < 2^112 (the codes' products stay in f32). q
  * overlaps neither out, lse nor the workspace, nor any of them each other or the
  * cache. workspace: glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing
  * kept in it between calls; where that is 0 it may be NULL. */
