@@ -572,11 +572,13 @@ int dkdv_parts(const glt_attn_desc* d, int32_t window) {
   return rep;
 }
 
-// Blocks of keys that hold sinks, and the cuts that their queries come in at most.
+// Blocks of keys that hold sinks, and the cuts that their queries come in at most (none
+// where no query is outside the blocks' own windows).
 struct SinkCut { int blocks, cuts; };
 SinkCut sink_cut(const glt_attn_desc* d, int32_t window, int32_t sinks) {
   if (window <= 0 || sinks <= 0) return {0, 0};
-  const int64_t tiles = cdiv(d->T, kTile), in = std::min<int64_t>(cdiv((int64_t)kRows - 1 + window, kTile), tiles);
+  const int64_t tiles = cdiv(d->T, kTile), in = cdiv((int64_t)kRows - 1 + window, kTile);
+  if (in >= tiles) return {0, 0};  // the first block's window reaches the end
   return {(int)cdiv(std::min(sinks, d->T), kRows), 1 + (int)cdiv(tiles - in, kSinkTiles)};
 }
 size_t sink_bytes(const glt_attn_desc* d, SinkCut c, int parts) {
@@ -604,7 +606,7 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", attn_dkdv_kernel<WIN>, dim3(blocks * a.Hkv * a.parts * a.B),
              dim3(kWaves * 64), kDkdvLds, st, a);
   GLT_LAUNCH_CHECK("attn_dkdv");
-  if (a.parts > 1) {
+  if (a.parts > 1 && a.sink_blocks * kRows < a.T) {
     const int64_t chunks = (int64_t)a.B * a.T * a.Hkv * (kHd / 8);
     GLT_LAUNCH("attn_dkdv_sum", attn_dkdv_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
     GLT_LAUNCH_CHECK("attn_dkdv_sum");

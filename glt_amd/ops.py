@@ -356,14 +356,15 @@ def _check_window(window, sinks):
 
 
 def _attn_train_desc(q, k, v, out, causal, scale, seq_lens):
+    """out None: a new dense one."""
     shape = q.shape
     _need(len(shape) == 4 and q.is_cuda, "q: [B, T, heads, head_dim] on a GPU")
     B, T, Hq, hd = shape
     dev = q.device
     lds = (_heads_ld("q", q, B, T, dev), _heads_ld("k", k, B, T, dev), _heads_ld("v", v, B, T, dev),
-           _heads_ld("out", out, B, T, dev))
+           Hq * hd if out is None else _heads_ld("out", out, B, T, dev))
     kshape = k.shape
-    _need(kshape == v.shape and kshape[3] == hd and out.shape == shape, "k, v and out do not fit q")
+    _need(kshape == v.shape and kshape[3] == hd and (out is None or out.shape == shape), "k, v and out do not fit q")
     if seq_lens is not None and not (seq_lens.dtype == torch.int32 and seq_lens.shape == (B,)
                                      and seq_lens.device == dev and seq_lens.is_contiguous()):
         raise ValueError(f"seq_lens: contiguous int32 [{B}] on {dev}")
@@ -380,9 +381,9 @@ def attention_train(q, k, v, causal=True, scale=None, seq_lens=None, window=None
     window=W: of the keys up to itself a row reads the last W (its own among
     them) and the first `sinks` of its sequence."""
     _check_window(window, sinks)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    d, (B, T, Hq, _, _), _ = _attn_train_desc(q, k, v, out, causal, scale, seq_lens)
-    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device)
+    d, (B, T, Hq, _, _), _ = _attn_train_desc(q, k, v, None, causal, scale, seq_lens)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
     name, sight = ("glt_attention_train_fwd", ()) if window is None else ("glt_attention_window_fwd", (window, sinks))
     _call_on(q, name, ctypes.byref(d), *sight, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
     return out, lse
@@ -399,6 +400,8 @@ def _attn_grad_buffers(q, k, v, shape, lds):
     B, T, Hq, Hkv, hd = shape
     ld, k_ld, v_ld, _ = lds
     rows, nq, nk = B * T, 2 * hd * Hq, 2 * hd * Hkv  # nq, nk: bytes of a token's heads
+    if ld == Hq * hd and k_ld == v_ld == Hkv * hd and rows > 1:  # dense, as they mostly come
+        return [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v)]
     if ld == k_ld == v_ld:
         pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
         (p0, n0), (p1, n1), (p2, n2) = sorted(((pq, nq), (pk, nk), (pv, nk)))
@@ -549,7 +552,7 @@ class Kv8Cache:
             ws = workspace.data_ptr(), workspace.numel()
         else:  # one launch: nothing between
             ws = None, 0
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
         _call_on(self.data, "glt_kv8_attention", *refs, q.data_ptr(), q_ld, out.data_ptr(), Hq * hd, lse.data_ptr(), *ws)
         return out, lse

@@ -58,3 +58,12 @@ def test_empty_batches_need_nothing():
     for kw in (dict(B=0), dict(T=0)):
         assert fwd(desc(**kw), q=None, k=None, v=None, out=None, lse=None) == 0
         assert bwd(desc(**kw), ws=None, nbytes=0) == 0
+
+
+def test_short_sequences_need_no_parts_for_sinks():
+    """Where the first block's window reaches the end, its own workgroup reads every query."""
+    lib = F.load()
+    for T, window, more in ((128, 2, False), (192, 2, False), (193, 2, True), (192, 65, False), (400, 300, False)):
+        d = desc(T=T)
+        plain = lib.glt_attention_bwd_workspace_size(ctypes.byref(d))
+        assert (lib.glt_attention_window_bwd_workspace_size(ctypes.byref(d), window, 4) > plain) == more, T
