@@ -21,7 +21,7 @@
 //
 // p and ds are rounded to bf16, as the matrix instructions take them, all sums are
 // f32: the gradients are off by 2.4 * 10^-3 in the 2-norm, of which their own
-// rounding is 1.6.
+// rounding is 1.6 (with a window dq 1.7 to 1.8, see kFineRows).
 //
 // Long rows: matrix instructions run 0.52 (dq) and 0.59 (dkdv) of the time, at the
 // power limit's 1.8 GHz. The rows in registers leave room for two wavefronts per
@@ -56,6 +56,21 @@ constexpr int kExactTiles = 8;
 // walk rows of one heavy key (T 700, scores of deviation 16) bring dq's error to
 // 3.0 * 2^-9 and dk's to 2.9 * 2^-9, with it to 2.0 and 1.2.
 constexpr float kOff = 0x1p-5f;
+
+// With a window dq takes ds in two bf16 parts, the rounding and what that left (16
+// bits), one product more: of long rows D's error, which a narrower window raises
+// against the rest, adds to ds's rounding. dq's error at 2 x 4096, 32 and 8 heads,
+// window 1024, 2.45 * 10^-3 in one part and 1.76 in two (1.66 is dq's own rounding to
+// bf16), the kernel 227 and 270 us; rows of at most kExactTiles tiles come to 1.66.
+// The two instructions on one accumulator after each other: in pairs of
+// accumulators, or the second part behind the first's four, 276 and 285.
+// dkdv, which gets D put right, takes two parts of ds and p in calls of at most
+// kFineRows tokens (one block of rows): few roundings do not average out there (7 to 11
+// tokens, 6 heads: dk 2.5 * 10^-3, in two parts 1.6) and the call is short (1 x 128, 32
+// and 8 heads, window 32, dkdv 11.8 and 12.5 us; 64 x 128 with every key 91 and 132).
+// In longer calls dk and dv stand at 2.35: two products of four more would be
+// needed for 1.66.
+constexpr int kFineRows = 128;
 
 struct BwdArgs {
   const uint16_t* q;
@@ -243,6 +258,16 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dq_kernel(const BwdArgs a
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const bf16x8 f = pack_frag(s, s2);
+        if constexpr (WIN) {  // and what the rounding left
+          const bf16x8 r = pack_rest(s, s2, f);
+#pragma unroll
+          for (int db = 0; db < 4; ++db) {
+            const bf16x8 k = col_frag(col, db, s2);
+            dq[db] = mfma(k, f, dq[db]);
+            dq[db] = mfma(k, r, dq[db]);
+          }
+          continue;
+        }
 #pragma unroll
         for (int db = 0; db < 4; ++db) dq[db] = mfma(col_frag(col, db, s2), f, dq[db]);
       }
@@ -301,17 +326,17 @@ constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
 // tiles, each with a workgroup of its own (launched first) that leaves an f32
 // part, the block's own window being cut 0; attn_sink_sum_kernel adds these parts by
 // head and cut. (Walked by the block's one workgroup they would be the longest
-// chain by far.) Window 1024 and 4 sinks at 2 x 4096, 32 query and 8 kv heads: dq 222 us,
-// dkdv 242, the sinks' sum 5; without sinks 229, 242. 1 x 12001, 16 and 4 heads, window 500
-// and 70 sinks: 128, 140, 26.
+// chain by far.) Window 1024 and 4 sinks at 2 x 4096, 32 query and 8 kv heads: dq 268 us,
+// dkdv 241, the sinks' sum 5; without sinks 273, 241. 1 x 12001, 16 and 4 heads, window 500
+// and 70 sinks: 153, 141, 26.
 constexpr int kSinkTiles = 16;
 // Query tiles that the window of the key block from k0 reaches, of `tiles` in all.
 __device__ __forceinline__ int window_tiles(int k0, int window, int tiles) {
   return min((k0 + kRows - 1 + window + kTile - 1) / kTile, tiles);
 }
 
-template <bool WIN>
-__global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs a) {
+template <bool WIN, bool FINE = false>
+__global__ void __launch_bounds__(kWaves * 64, FINE ? 1 : 2) attn_dkdv_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, lq = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -434,7 +459,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
         for (int e = 0; e < 4; e += 2) {
           const int x = 4 * i + e, w = 2 * (i & 1) + e / 2;
           pw[i >> 1][w] = pack2_rne(s[x], s[x + 1]);
-          dw[i >> 1][w] = pack2_rne(s[x] * dp[x], s[x + 1] * dp[x + 1]);
+          const float d0 = s[x] * dp[x], d1 = s[x + 1] * dp[x + 1];
+          dw[i >> 1][w] = pack2_rne(d0, d1);
+          if (FINE) dp[x] = d0, dp[x + 1] = d1;
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -450,6 +477,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) attn_dkdv_kernel(const BwdArgs
       for (int i = 0; i < 8; ++i) {
         dv[i & 3] = mfma(oa[i % kGradAhead], __builtin_bit_cast(bf16x8, pw[i >> 2]), dv[i & 3]);
         dk[i & 3] = mfma(qa[i % kGradAhead], __builtin_bit_cast(bf16x8, dw[i >> 2]), dk[i & 3]);
+        if constexpr (FINE) {
+          dv[i & 3] = mfma(oa[i % kGradAhead], pack_rest(s, i >> 2, __builtin_bit_cast(bf16x8, pw[i >> 2])), dv[i & 3]);
+          dk[i & 3] = mfma(qa[i % kGradAhead], pack_rest(dp, i >> 2, __builtin_bit_cast(bf16x8, dw[i >> 2])), dk[i & 3]);
+        }
         if (i + kGradAhead < 8) {
           oa[i % kGradAhead] = col_frag(col + kTileB, (i + kGradAhead) & 3, (i + kGradAhead) >> 2);
           qa[i % kGradAhead] = col_frag(col, (i + kGradAhead) & 3, (i + kGradAhead) >> 2);
@@ -585,7 +616,7 @@ size_t sink_bytes(const glt_attn_desc* d, SinkCut c, int parts) {
   return (size_t)d->B * d->n_kv_heads * parts * c.blocks * c.cuts * 2 * kRows * kHd * sizeof(float);
 }
 
-template <bool WIN>
+template <bool WIN, bool FINE = false>
 glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   constexpr int kDqLds = 4 * kTileB + 4 * kWaves, kDkdvLds = 2 * kDkdvBuf;
   // the dynamic-LDS limit is a per-device attribute of the kernels
@@ -596,14 +627,14 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   if (!attr_set[dev].load(std::memory_order_acquire)) {
     GLT_TRY_HIP(hipFuncSetAttribute((const void*)attn_dq_kernel<WIN>, hipFuncAttributeMaxDynamicSharedMemorySize, kDqLds));
     GLT_TRY_HIP(
-        hipFuncSetAttribute((const void*)attn_dkdv_kernel<WIN>, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
+        hipFuncSetAttribute((const void*)attn_dkdv_kernel<WIN, FINE>, hipFuncAttributeMaxDynamicSharedMemorySize, kDkdvLds));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const unsigned nb = (unsigned)cdiv(a.T, kRows);
   GLT_LAUNCH(WIN ? "attn_window_dq" : "attn_dq", attn_dq_kernel<WIN>, dim3(nb * a.Hq * a.B), dim3(kWaves * 64), kDqLds, st, a);
   GLT_LAUNCH_CHECK("attn_dq");
   const unsigned blocks = nb + (WIN && a.sink_blocks ? (unsigned)(a.sink_blocks * (a.sink_cuts - 1)) : 0u);
-  GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", attn_dkdv_kernel<WIN>, dim3(blocks * a.Hkv * a.parts * a.B),
+  GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", (attn_dkdv_kernel<WIN, FINE>), dim3(blocks * a.Hkv * a.parts * a.B),
              dim3(kWaves * 64), kDkdvLds, st, a);
   GLT_LAUNCH_CHECK("attn_dkdv");
   if (a.parts > 1 && a.sink_blocks * kRows < a.T) {
@@ -673,7 +704,8 @@ glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, cons
   a.sink_cuts = cut.cuts;
   a.parts = parts;
   a.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(d) + part_bytes(d, parts));
-  return window > 0 ? launch_bwd<true>(a, as_stream(stream)) : launch_bwd<false>(a, as_stream(stream));
+  const hipStream_t st = as_stream(stream);
+  return window <= 0 ? launch_bwd<false>(a, st) : a.T <= kFineRows ? launch_bwd<true, true>(a, st) : launch_bwd<true>(a, st);
 }
 
 }  // namespace
@@ -707,6 +739,7 @@ extern "C" glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t w
                                                size_t workspace_bytes, void* stream) {
   glt_status s = check_attn_desc(d, "glt_attention_window_bwd");
   if (s == GLT_OK) s = check_window(d, &window, &sinks, "glt_attention_window_bwd");
+  if (s == GLT_OK && window == 0 && d->T <= kFineRows) window = d->T;  // hides nothing, in two parts
   return s != GLT_OK ? s
                      : train_bwd(d, window, sinks, q, k, v, out, lse, dout, dq, dk, dv, workspace, workspace_bytes,
                                  stream, "glt_attention_window_bwd");

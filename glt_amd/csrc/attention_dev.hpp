@@ -194,6 +194,17 @@ __device__ __forceinline__ bf16x8 pack_frag(const f32x16& x, int s2) {
                                           pack2_rne(x[o + 4], x[o + 5]), pack2_rne(x[o + 6], x[o + 7])});
 }
 
+// What that rounding left, rounded: the two together hold 16 bits.
+__device__ __forceinline__ bf16x8 pack_rest(const f32x16& x, int s2, bf16x8 f) {
+  const int o = 8 * s2;
+  const u32x4 w = __builtin_bit_cast(u32x4, f);
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = pack2_rne(x[o + 2 * i] - __uint_as_float(w[i] << 16), x[o + 2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+  return __builtin_bit_cast(bf16x8, r);
+}
+
 // Score product of 32 walked rows: x += X . f^T over the 128 columns, the
 // fragments read AHEAD steps ahead; between(i) is arithmetic that the
 // scheduler may put beside step i's matrix instruction. (The fence per step

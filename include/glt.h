@@ -408,7 +408,8 @@ glt_status glt_attention_window_fwd(const glt_attn_desc* d, int32_t window, int3
                                     const void* k, const void* v, void* out, float* lse, void* stream);
 /* Its backward, as glt_attention_bwd. The sums' order is fixed by the call's sizes (B, T,
  * heads, window, sinks): the same call gives the same bits, and a sequence's dk and dv may
- * round differently in a call of another size. */
+ * round differently in a call of another size. dq takes its factor ds to 16 bits, and with
+ * T of at most 128 dk and dv take ds and p so, also where the window hides nothing. */
 size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks);
 glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
                                     const void* k, const void* v, const void* out, const float* lse,

@@ -153,6 +153,66 @@ def test_peaked_rows(dev, T, window, sinks, sharpness):
         check(name, got[name], want[name], lse_bound(q, k, scale, want["lse"]))
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,window,sinks,lens", [
+    (1, 2, 8, 1, 2, 0, None),
+    (1, 7, 6, 2, 3, 0, None),
+    (3, 11, 6, 2, 672, 0, None),                   # a window that hides nothing
+    (2, 65, 4, 4, 20, 3, (65, 30)),
+    (2, 128, 4, 1, 128, 0, None),
+    (1, 128, 2, 1, 127, 9, None),
+])
+def test_short_calls_round_once(dev, B, T, Hq, Hkv, window, sinks, lens):
+    """Up to 128 tokens p and ds go in two bf16 parts: the gradients are off by the
+    result's half step and what the rest leaves. e, the relative error of p: its
+    score's and lse's (a bound each), and the exponential's. dp and D are f32 sums of
+    at most 128 products of 16 bits, D's with p's error too; the parts hold 2^-16. The last
+    sum has as many terms as rows and heads, and 64 at most of rest and rounding each."""
+    q, k, v, dout = make(B, T, Hq, Hkv, 7, False, 2.0)
+    sl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+    got = run(q, k, v, dout, seq_lens=sl, window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    scale, rep = HD ** -0.5, Hq // Hkv
+    lens = lens or [T] * B
+    want = formula(q, k, v, dout, scale, lens, window, sinks)
+    e = 2 * lse_bound(q, k, scale, want["lse"]) + 2.0 ** -20
+    q, k, v, dout = (t.detach().cpu().double() for t in (q, k, v, dout))
+    names = ("dq", "dk", "dv")
+    tol, once = ({n: torch.zeros_like(want[n]) for n in names} for _ in range(2))
+    for b, n in enumerate(lens):
+        for h in range(Hq):
+            g = h // rep
+            Q, K, V, dO = q[b, :n, h], k[b, :n, g], v[b, :n, g], dout[b, :n, h]
+            p = torch.softmax((Q @ K.t() * scale).masked_fill(~visible(n, window, sinks), -math.inf), -1)
+            dp = dO @ V.t()
+            dp = dp - (p * dp).sum(-1, keepdim=True)
+            f32 = 127 * 2.0 ** -24 * (dO.abs() @ V.abs().t())
+            D = e * (p * dp.abs()).sum(-1, keepdim=True) + 2 * (p * f32).sum(-1, keepdim=True)
+            ds, sums = p * dp, 2.0 ** -16 + 2 * rep * n * 2.0 ** -24
+            eds, ep = ds.abs() * (e + sums) + p * (f32 + D), p * (e + sums)
+            tol["dq"][b, :n, h] = scale * eds @ K.abs()
+            tol["dk"][b, :n, g] += scale * eds.t() @ Q.abs()
+            tol["dv"][b, :n, g] += ep.t() @ dO.abs()
+            p, ds = p.to(BF).double(), ds.to(BF).double()
+            once["dq"][b, :n, h] = scale * ds @ K
+            once["dk"][b, :n, g] += scale * ds.t() @ Q
+            once["dv"][b, :n, g] += p.t() @ dO
+    for name in names:
+        tol[name] += (want[name].abs() + tol[name]).frexp().exponent.sub(9).double().exp2()
+        assert bool(((got[name].cpu().double() - want[name]).abs() <= tol[name]).all()), name
+        # one part does not hold that
+        assert T < 7 or not bool(((once[name].to(BF).double() - want[name]).abs() <= tol[name]).all()), name
+
+
+def test_long_rows_dq_in_two_parts(dev):
+    """dq takes ds in two parts at every length: in the 2-norm the result's rounding, 2^-9
+    as above, and D's share of out's, which adds in squares: a row's D is off by less than
+    half of what ds's own rounding would be, 2^-10 (a quarter of the square)."""
+    q, k, v, dout = make(1, 1500, 4, 2, 8, False, 2.0)
+    got = run(q, k, v, dout, window=600, sinks=4)
+    want = formula(q, k, v, dout, HD ** -0.5, [1500], 600, 4)["dq"]
+    assert float((got["dq"].cpu().double() - want).norm()) <= (2.0 ** -9) * 1.25 ** 0.5 * float(want.norm())
+
+
 def test_gradient_against_differences(dev):
     T, window, sinks = 150, 40, 3
     q, k, v, dout = make(1, T, 4, 2, 11)
