@@ -91,7 +91,7 @@ struct BwdArgs {
   float scale;
   // WIN: causal, and of the keys before it a row reads those less than `window`
   // back and the first `sinks`, which lie in sink_blocks blocks of keys
-  int window, sinks, sink_blocks, sink_cuts;
+  int window, sinks, sink_blocks, sink_cuts, sink_tiles;
   float* sink_part;  // dk, dv of these blocks by part and cut, [B, Hkv * parts, block, cut][2][128][128]
 };
 
@@ -322,14 +322,12 @@ constexpr int kDkdvBuf = 2 * kTileB + 2 * kTile * 4;
 
 //
 // WIN: a block's queries end with its last key's window. A block that holds sinks
-// is read by all queries after that too: they are cut into runs of kSinkTiles
+// is read by all queries after that too: they are cut into runs of sink_tiles
 // tiles, each with a workgroup of its own (launched first) that leaves an f32
 // part, the block's own window being cut 0; attn_sink_sum_kernel adds these parts by
 // head and cut. (Walked by the block's one workgroup they would be the longest
 // chain by far.) Window 1024 and 4 sinks at 2 x 4096, 32 query and 8 kv heads: dq 268 us,
-// dkdv 241, the sinks' sum 5; without sinks 273, 241. 1 x 12001, 16 and 4 heads, window 500
-// and 70 sinks: 153, 141, 26.
-constexpr int kSinkTiles = 16;
+// dkdv 241, the sinks' sum 5; without sinks 273, 241.
 // Query tiles that the window of the key block from k0 reaches, of `tiles` in all.
 __device__ __forceinline__ int window_tiles(int k0, int window, int tiles) {
   return min((k0 + kRows - 1 + window + kTile - 1) / kTile, tiles);
@@ -371,9 +369,9 @@ __global__ void __launch_bounds__(kWaves * 64, FINE ? 1 : 2) attn_dkdv_kernel(co
   if (WIN && k0 < len) {
     const int all = qt1, in = window_tiles(k0, a.window, all);
     if (cut > 0) {
-      qt0 = in + (cut - 1) * kSinkTiles;
+      qt0 = in + (cut - 1) * a.sink_tiles;
       if (qt0 >= all) return;
-      qt1 = min(qt0 + kSinkTiles, all);
+      qt1 = min(qt0 + a.sink_tiles, all);
     } else {
       qt1 = in;
     }
@@ -564,7 +562,7 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
   int cuts = 1;
   if (k0 < len) {
     const int all = (len + kTile - 1) / kTile;
-    cuts += (all - window_tiles(k0, a.window, all) + kSinkTiles - 1) / kSinkTiles;
+    cuts += (all - window_tiles(k0, a.window, all) + a.sink_tiles - 1) / a.sink_tiles;
   }
   f32x4 x{}, y{};
   for (int s = 0; s < a.parts; ++s)
@@ -593,24 +591,34 @@ size_t part_bytes(const glt_attn_desc* d, int parts) {
 // nearly one length (up to half of T), as few as leave two workgroups for each of 256
 // CUs: no f32 parts then. dkdv and sums in us at 2 x 4096, 32 query and 8 kv heads,
 // one each against all together: window 128 156, 59; 1024 304, 242; 2048 448, 416;
-// 4095 585, 661.
+// 4095 585, 661. Windows up to 1024 have 5 for each of 4 CUs, as what two would
+// save is less than the parts cost: 1 x 10240, 16 and 4 heads, all together against two parts,
+// window 500 122, 138, 2000 376, 379 (four parts 343); 1 x 12001 137, 154 and 407, 400
+// (387). Fewer leave CUs waiting: 1 x 2300, 64 and 16 heads, window 600 (288 workgroups)
+// 166, 130.
 int dkdv_parts(const glt_attn_desc* d, int32_t window) {
   const int rep = d->n_q_heads / d->n_kv_heads;
   if (window <= 0 || window > d->T / 2) return rep;
   const int64_t blocks = cdiv(d->T, kRows) * d->n_kv_heads * d->B;
   for (int parts = 1; parts < rep; ++parts)
-    if (rep % parts == 0 && blocks * parts >= 512) return parts;
+    if (rep % parts == 0 && blocks * parts >= (window <= 1024 ? 320 : 512)) return parts;
   return rep;
 }
 
 // Blocks of keys that hold sinks, and the cuts that their queries come in at most (none
 // where no query is outside the blocks' own windows).
-struct SinkCut { int blocks, cuts; };
+struct SinkCut { int blocks, cuts, tiles; };
 SinkCut sink_cut(const glt_attn_desc* d, int32_t window, int32_t sinks) {
-  if (window <= 0 || sinks <= 0) return {0, 0};
+  if (window <= 0 || sinks <= 0) return {0, 0, 1};
   const int64_t tiles = cdiv(d->T, kTile), in = cdiv((int64_t)kRows - 1 + window, kTile);
-  if (in >= tiles) return {0, 0};  // the first block's window reaches the end
-  return {(int)cdiv(std::min(sinks, d->T), kRows), 1 + (int)cdiv(tiles - in, kSinkTiles)};
+  if (in >= tiles) return {0, 0, 1};  // the first block's window reaches the end
+  // A run is as long as the block's own window, so that no workgroup is the longest,
+  // within limits: shorter runs write more parts, longer ones leave CUs empty. The backward in
+  // us with runs of 4, 8, 16 tiles: 1 x 12001, 16 and 4 heads, window 64 152, 158, 223,
+  // window 500 and 70 sinks (runs of 10: 294) 325, 292, 326; 2 x 4096, 32 and 8
+  // heads, window 64 197, 189, 250, window 1024 554, 538, 525.
+  const int64_t run = std::clamp<int64_t>(in, 8, 16);
+  return {(int)cdiv(std::min(sinks, d->T), kRows), 1 + (int)cdiv(tiles - in, run), (int)run};
 }
 size_t sink_bytes(const glt_attn_desc* d, SinkCut c, int parts) {
   return (size_t)d->B * d->n_kv_heads * parts * c.blocks * c.cuts * 2 * kRows * kHd * sizeof(float);
@@ -702,6 +710,7 @@ glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, cons
   a.sinks = sinks;
   a.sink_blocks = cut.blocks;
   a.sink_cuts = cut.cuts;
+  a.sink_tiles = cut.tiles;
   a.parts = parts;
   a.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(d) + part_bytes(d, parts));
   const hipStream_t st = as_stream(stream);
@@ -721,7 +730,7 @@ extern "C" size_t glt_attention_bwd_workspace_size(const glt_attn_desc* d) {
 extern "C" size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks) {
   if (!d || d->B <= 0 || d->T <= 0 || d->n_q_heads <= 0 || d->n_kv_heads <= 0) return 256;
   if (d->n_q_heads % d->n_kv_heads || window < 0 || window >= d->T) window = 0;
-  return bwd_bytes(d, sinks <= kMaxSinks ? sink_cut(d, window, sinks) : SinkCut{0, 0}, dkdv_parts(d, window));
+  return bwd_bytes(d, sinks <= kMaxSinks ? sink_cut(d, window, sinks) : SinkCut{0, 0, 1}, dkdv_parts(d, window));
 }
 
 extern "C" glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,

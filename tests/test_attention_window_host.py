@@ -42,14 +42,16 @@ def test_workspace():
     d = desc(T=2000)
     plain = lib.glt_attention_bwd_workspace_size(ctypes.byref(d))
     assert size(d, 100, 0) == size(d, 2000, 9) == size(d, 0, 0) == plain
-    # the parts of a block of 128 keys by head, its window and the queries after it 1024 by 1024
+    # the parts of a block of 128 keys by head, its window and the queries after it 512 by 512
     one = 2 * 4 * 2 * 128 * 128 * 4
-    assert size(d, 100, 1) == size(d, 100, 128) == plain + 3 * one
-    assert size(d, 100, 129) == plain + 6 * one
+    assert size(d, 100, 1) == size(d, 100, 128) == plain + 5 * one
+    assert size(d, 100, 129) == plain + 10 * one
+    # 10 tiles by 10 with a window of 500, 16 by 16 with one of 950
+    assert size(d, 500, 1) == plain + (1 + 3) * one and size(d, 950, 1) == plain + (1 + 1) * one
     # where key blocks fill the chip, a kv head's query heads need no parts
     big = desc(B=20, T=2000)
     assert size(big, 100, 0) < lib.glt_attention_bwd_workspace_size(ctypes.byref(big)) // 50
-    assert bwd(d, 100, 1, nbytes=plain + 3 * one - 1) == 5
+    assert bwd(d, 100, 1, nbytes=plain + 5 * one - 1) == 5
     assert bwd(d, 100, 1, ws=None) == 5
     assert lib.glt_attention_window_bwd_workspace_size(None, 1, 1) == 256
 

@@ -56,8 +56,8 @@ CASES = [
     (2, 450, 4, 2, 127, 65, None, True),           # a workgroup's rows
     (1, 515, 2, 2, 128, 128, None, False),
     (1, 515, 3, 1, 129, 129, None, False),         # sinks in two blocks
-    (1, 1500, 2, 1, 70, 4, None, True),            # sinks' queries in two cuts
-    (1, 3300, 4, 2, 200, 4, None, False),          # in four
+    (1, 1500, 2, 1, 70, 4, None, True),            # sinks' queries in cuts of eight tiles
+    (1, 3300, 4, 2, 200, 4, None, False),
     (1, 2500, 2, 1, 90, 300, None, False),         # of three blocks
     (1, 2300, 1, 1, 1000, 1024, None, False),
     (5, 300, 4, 2, 50, 2, (300, 0, 1, 64, 201), True),
