@@ -531,8 +531,7 @@ __global__ void __launch_bounds__(kWaves * 64, FINE ? 1 : 2) attn_dkdv_kernel(co
 
 // dk (blockIdx.y 0) or dv (1): the parts of a group's query heads added in head
 // order, rounded once; a thread takes 8 elements of a token's kv head.
-__global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void sum_parts(const BwdArgs& a, int64_t i) {
   const int cols = a.Hkv * (kHd / 8);
   if (i >= (int64_t)a.B * a.T * cols) return;
   const int64_t row = i / cols;
@@ -551,10 +550,13 @@ __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
             pack2_rne(y[2] * f, y[3] * f)};
 }
 
+__global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
+  sum_parts(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
+}
+
 // The keys of the sink blocks: the parts of their query heads, each by cut.
-__global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
+__device__ __forceinline__ void sum_sinks(const BwdArgs& a, int64_t i) {
   const int cols = a.Hkv * (kHd / 8), rows = min(a.sink_blocks * kRows, a.T);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (int64_t)a.B * rows * cols) return;
   const int c = (int)(i % cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
   const int t = (int)(i / cols % rows), b = (int)(i / cols / rows), kb = t / kRows;
@@ -580,6 +582,13 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a) {
   *reinterpret_cast<u32x4*>(dst + g * kHd + e) =
       u32x4{pack2_rne(x[0] * f, x[1] * f), pack2_rne(x[2] * f, x[3] * f), pack2_rne(y[0] * f, y[1] * f),
             pack2_rne(y[2] * f, y[3] * f)};
+}
+
+// Both: the first `others` workgroups take the other keys' parts, where there are any
+// (4 x 1029, 6 and 2 heads, window 82, 64 sinks: the backward 54 us, in two launches 57).
+__global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a, unsigned others) {
+  if (blockIdx.x < others) sum_parts(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
+  else sum_sinks(a, (int64_t)(blockIdx.x - others) * 256 + threadIdx.x);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -645,15 +654,15 @@ glt_status launch_bwd(const BwdArgs& a, hipStream_t st) {
   GLT_LAUNCH(WIN ? "attn_window_dkdv" : "attn_dkdv", (attn_dkdv_kernel<WIN, FINE>), dim3(blocks * a.Hkv * a.parts * a.B),
              dim3(kWaves * 64), kDkdvLds, st, a);
   GLT_LAUNCH_CHECK("attn_dkdv");
-  if (a.parts > 1 && a.sink_blocks * kRows < a.T) {
-    const int64_t chunks = (int64_t)a.B * a.T * a.Hkv * (kHd / 8);
-    GLT_LAUNCH("attn_dkdv_sum", attn_dkdv_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
-    GLT_LAUNCH_CHECK("attn_dkdv_sum");
-  }
+  auto sums = [&](int64_t rows) { return (unsigned)cdiv(a.B * rows * a.Hkv * (kHd / 8), 256); };
+  const unsigned others = a.parts > 1 && a.sink_blocks * kRows < a.T ? sums(a.T) : 0;
   if (WIN && a.sink_blocks) {
-    const int64_t chunks = (int64_t)a.B * std::min(a.sink_blocks * kRows, a.T) * a.Hkv * (kHd / 8);
-    GLT_LAUNCH("attn_sink_sum", attn_sink_sum_kernel, dim3((unsigned)cdiv(chunks, 256), 2), dim3(256), 0, st, a);
+    const unsigned sinks = sums(std::min(a.sink_blocks * kRows, a.T));
+    GLT_LAUNCH("attn_sink_sum", attn_sink_sum_kernel, dim3(others + sinks, 2), dim3(256), 0, st, a, others);
     GLT_LAUNCH_CHECK("attn_sink_sum");
+  } else if (others) {
+    GLT_LAUNCH("attn_dkdv_sum", attn_dkdv_sum_kernel, dim3(others, 2), dim3(256), 0, st, a);
+    GLT_LAUNCH_CHECK("attn_dkdv_sum");
   }
   return GLT_OK;
 }
