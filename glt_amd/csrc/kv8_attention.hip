@@ -968,22 +968,81 @@ __device__ __forceinline__ void join_row(const DecArgs& a, int row) {
   }
   if (lane < 32) write_row<4, 1>(a, w, &acc, M, L, lane);
 }
-// A row by four wavefronts or one, or several rows a wavefront, one after the other: where
-// there are many most were written as their only piece, and a lane each looks.
-template <int WAVES, int ROWS>
+// Many rows, without prefixes: eight by a wavefront. A lane each finds their pieces; half the
+// wavefront then reads four rows' values, two pieces of each on their way: a row's lengths,
+// pieces and values are loads that wait for each other.
+__global__ void __launch_bounds__(256) kv8_join_rows_kernel(const DecArgs a) {
+  constexpr int kEach = 4, kAhead = 2;
+  const int lane = threadIdx.x & 63, rows = a.s.B * a.s.T * a.Hkv * a.G;
+  const int row0 = (blockIdx.x * 4 + uni(threadIdx.x >> 6)) * 2 * kEach, row = row0 + (lane & (2 * kEach - 1));
+  JoinRow j{};
+  bool mine = row < rows;
+  if (mine) mine = find_row(a, row, j);
+  const uint32_t todo = (uint32_t)__ballot(mine);
+  if (!(todo & ((1 << 2 * kEach) - 1))) return;
+  const int64_t slot_rows = a.part[0].rows > kFewRows ? kManyRows : a.part[0].rows;
+  int n[kEach], w0[kEach], r[kEach], most = 0;
+  float M[kEach], L[kEach];
+  f32x4 acc[kEach];
+#pragma unroll
+  for (int y = 0; y < kEach; ++y) {
+    const int from = 2 * y + (lane >> 5);
+    n[y] = __shfl(j.own.n, from);
+    w0[y] = __shfl(j.own.w0, from);
+    r[y] = __shfl(j.own.r, from);
+    n[y] = (todo >> from) & 1 ? n[y] : 0;
+    most = max(most, n[y]);
+    M[y] = kNoMax;
+    L[y] = 0.f;
+    acc[y] = f32x4{};
+  }
+  for (int x0 = 0; __ballot(x0 < most); x0 += kAhead) {
+    float m[kEach][kAhead], l[kEach][kAhead];
+    f32x4 o[kEach][kAhead];
+#pragma unroll
+    for (int y = 0; y < kEach; ++y)
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        const int x = x0 + z;
+        m[y][z] = kNoMax;
+        l[y][z] = 0.f;
+        o[y][z] = f32x4{};
+        if (x < n[y]) {
+          const int64_t at = slot_of<false>(a, w0[y] + x, 0, x == 0) * slot_rows + r[y];
+          m[y][z] = a.part[0].m[2 * at];
+          l[y][z] = a.part[0].m[2 * at + 1];
+          o[y][z] = *reinterpret_cast<const f32x4*>(a.part[0].o + at * kKv8Hd + 4 * (lane & 31));
+        }
+      }
+#pragma unroll
+    for (int y = 0; y < kEach; ++y) {
+      const float m_new = fmax_nc(M[y], fmax_nc(m[y][0], m[y][1])), alpha = __builtin_amdgcn_exp2f(M[y] - m_new);
+      L[y] *= alpha;
+      acc[y] *= alpha;
+      M[y] = m_new;
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        const float c = __builtin_amdgcn_exp2f(m[y][z] - m_new);
+        L[y] += l[y][z] * c;
+        acc[y] += o[y][z] * c;
+      }
+    }
+  }
+#pragma unroll
+  for (int y = 0; y < kEach; ++y) {
+    const int from = 2 * y + (lane >> 5);
+    Row w{};
+    w.q_row = __shfl((int)j.w.q_row, from);
+    w.head = __shfl(j.w.head, from);
+    if ((todo >> from) & 1) write_row<4, 1>(a, w, &acc[y], M[y], L[y], lane & 31);
+  }
+}
+
+// A row by four wavefronts or one.
+template <int WAVES>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const DecArgs a) {
-  if (ROWS == 1) {
-    const int row = blockIdx.x * (4 / WAVES) + uni(threadIdx.x >> 6) / WAVES;
-    if (row < a.s.B * a.s.T * a.Hkv * a.G) join_row<WAVES>(a, row);
-    return;
-  }
-  const int rows = a.s.B * a.s.T * a.Hkv * a.G, row = (blockIdx.x * 4 + uni(threadIdx.x >> 6)) * ROWS, lane = threadIdx.x & 63;
-  bool todo = lane < ROWS && row + lane < rows;
-  if (todo) {
-    JoinRow j;
-    todo = find_row(a, row + lane, j);
-  }
-  for (uint64_t m = __ballot(todo); m; m &= m - 1) join_row<1>(a, row + __builtin_ctzll(m));
+  const int row = blockIdx.x * (4 / WAVES) + uni(threadIdx.x >> 6) / WAVES;
+  if (row < a.s.B * a.s.T * a.Hkv * a.G) join_row<WAVES>(a, row);
 }
 
 // ------------------------------------------------------------------ host
@@ -1129,12 +1188,15 @@ glt_status launch(DecArgs& a, const Plan& p, const char* who, hipStream_t st) {
                lds, st, a);
     GLT_LAUNCH_CHECK("kv8_pieces");
   }
+  // a wavefront a row against one for eight, us: 4160 rows 7.7, 10.6; 9600 9.5, 10.2; 16384
+  // 12.5, 9.4; 32768 21.8, 13.1; 65536 43 (rows one after the other), 19, with nothing to
+  // join 4.7 both
   if (rows <= 4096)
-    GLT_LAUNCH("kv8_join", (kv8_join_kernel<4, 1>), dim3((unsigned)rows), dim3(256), 0, st, a);
-  else if (rows <= 32768)
-    GLT_LAUNCH("kv8_join", (kv8_join_kernel<1, 1>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
+  else if (rows <= 12288 || a.n_groups)
+    GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
   else
-    GLT_LAUNCH("kv8_join", (kv8_join_kernel<1, 8>), dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
+    GLT_LAUNCH("kv8_join", kv8_join_rows_kernel, dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
   GLT_LAUNCH_CHECK("kv8_join");
   return GLT_OK;
 }

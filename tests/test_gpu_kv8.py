@@ -233,6 +233,33 @@ def test_many_sequences_of_many_rows(dev):
     Setup(40, 16, 4, lens, [(11 * i) % 41 for i in range(70)], seed=13, extra=0).check()
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 70)])
+@pytest.mark.parametrize("T,Hq,Hkv,lens,new", [
+    (413, 30, 2, [1500], None),                                  # five pieces a row, 12390 rows
+    (413, 30, 2, [1500, 500, 0], [413, 100, 0]),
+    (1, 28, 4, [1 + (613 * i) % 3000 for i in range(450)], [i % 7 != 0 for i in range(450)]),
+    (9, 32, 16, [9 + (613 * i) % 2500 for i in range(50)], [i % 10 for i in range(50)]),
+])
+def test_joins_of_many_rows(dev, T, Hq, Hkv, lens, new, window, sinks):
+    """More than 12288 rows: a wavefront joins eight, of pieces of several numbers, written
+    ones and padding."""
+    Setup(T, Hq, Hkv, lens, None if new is None else [int(n) for n in new], seed=15).check(window, sinks)
+
+
+def test_a_bad_query_row_stays_alone_among_many(dev):
+    s = Setup(120, 64, 1, [3000, 2000], [120, 50], seed=16)
+    a, al = s.run()
+    for bad in (float("nan"), float("inf")):
+        q = s.q.clone()
+        s.q[1, 50:] = bad                       # padding
+        s.q[0, 1, 0] = bad
+        b, bl = s.run()
+        s.q.copy_(q)
+        assert torch.isnan(b[0, 1, 0]).all()
+        b[0, 1, 0], bl[0, 0, 1] = a[0, 1, 0], al[0, 0, 1]
+        assert torch.equal(a, b) and torch.equal(al, bl)
+
+
 @pytest.mark.parametrize("T,Hq,lens,new,plens", [
     (4, 4, [300, 90], [4, 2], None), (4, 4, [3000, 90], [4, 2], None), (6, 8, [3000, 90], [6, 2], None),
     (60, 8, [300, 90], [60, 2], None), (4, 4, [300, 90], [4, 2], [200]), (20, 8, [300, 90], [20, 2], [500]),
