@@ -968,9 +968,10 @@ __device__ __forceinline__ void join_row(const DecArgs& a, int row) {
   }
   if (lane < 32) write_row<4, 1>(a, w, &acc, M, L, lane);
 }
-// Many rows, without prefixes: eight by a wavefront. A lane each finds their pieces; half the
-// wavefront then reads four rows' values, two pieces of each on their way: a row's lengths,
-// pieces and values are loads that wait for each other.
+// Many rows: eight by a wavefront. A lane each finds their pieces; half the wavefront
+// then reads four rows' values, two pieces of each on their way: a row's lengths, pieces and
+// values are loads that wait for each other.
+template <bool PRE>
 __global__ void __launch_bounds__(256) kv8_join_rows_kernel(const DecArgs a) {
   constexpr int kEach = 4, kAhead = 2;
   const int lane = threadIdx.x & 63, rows = a.s.B * a.s.T * a.Hkv * a.G;
@@ -980,16 +981,25 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(const DecArgs a) {
   if (mine) mine = find_row(a, row, j);
   const uint32_t todo = (uint32_t)__ballot(mine);
   if (!(todo & ((1 << 2 * kEach) - 1))) return;
-  const int64_t slot_rows = a.part[0].rows > kFewRows ? kManyRows : a.part[0].rows;
-  int n[kEach], w0[kEach], r[kEach], most = 0;
+  auto slot_rows = [&](int k) { return a.part[k].rows > kFewRows ? kManyRows : a.part[k].rows; };
+  const int own_rows = slot_rows(0), pre_rows = PRE ? slot_rows(1) : 0;
+  // pieces, of which the first n_pre are the prefix's; the first one's slot (less begins of slot_of)
+  const int own_first = (int)slot_of<false>(a, j.own.w0, j.own.column, false);
+  const int pre_first = PRE ? (int)slot_of<true>(a, j.pre.w0, j.pre.column, false) : 0;
+  int n[kEach], n_pre[kEach], own_at[kEach], pre_at[kEach], own_r[kEach], pre_r[kEach], most = 0;
   float M[kEach], L[kEach];
   f32x4 acc[kEach];
 #pragma unroll
   for (int y = 0; y < kEach; ++y) {
     const int from = 2 * y + (lane >> 5);
-    n[y] = __shfl(j.own.n, from);
-    w0[y] = __shfl(j.own.w0, from);
-    r[y] = __shfl(j.own.r, from);
+    n[y] = __shfl(j.own.n + j.pre.n, from);
+    own_at[y] = __shfl(own_first, from);
+    own_r[y] = __shfl(j.own.r, from);
+    if (PRE) {
+      n_pre[y] = __shfl(j.pre.n, from);
+      pre_at[y] = __shfl(pre_first, from);
+      pre_r[y] = __shfl(j.pre.r, from);
+    }
     n[y] = (todo >> from) & 1 ? n[y] : 0;
     most = max(most, n[y]);
     M[y] = kNoMax;
@@ -1008,10 +1018,14 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(const DecArgs a) {
         l[y][z] = 0.f;
         o[y][z] = f32x4{};
         if (x < n[y]) {
-          const int64_t at = slot_of<false>(a, w0[y] + x, 0, x == 0) * slot_rows + r[y];
-          m[y][z] = a.part[0].m[2 * at];
-          l[y][z] = a.part[0].m[2 * at + 1];
-          o[y][z] = *reinterpret_cast<const f32x4*>(a.part[0].o + at * kKv8Hd + 4 * (lane & 31));
+          const bool p = PRE && x < n_pre[y];
+          const int64_t at = p ? (int64_t)(pre_at[y] + x) * pre_rows + pre_r[y]
+                           : PRE ? (int64_t)(own_at[y] + x - n_pre[y]) * own_rows + own_r[y]
+                                 : (int64_t)(own_at[y] + 2 * x + (x == 0)) * own_rows + own_r[y];
+          const float* const ml = (p ? a.part[1].m : a.part[0].m) + 2 * at;
+          m[y][z] = ml[0];
+          l[y][z] = ml[1];
+          o[y][z] = *reinterpret_cast<const f32x4*>((p ? a.part[1].o : a.part[0].o) + at * kKv8Hd + 4 * (lane & 31));
         }
       }
 #pragma unroll
@@ -1190,13 +1204,15 @@ glt_status launch(DecArgs& a, const Plan& p, const char* who, hipStream_t st) {
   }
   // a wavefront a row against one for eight, us: 4160 rows 7.7, 10.6; 9600 9.5, 10.2; 16384
   // 12.5, 9.4; 32768 21.8, 13.1; 65536 43 (rows one after the other), 19, with nothing to
-  // join 4.7 both
+  // join 4.7 both; whole calls with prefixes, 15360 rows 70.5, 68, 102400 268, 219, 131072 460, 398
   if (rows <= 4096)
     GLT_LAUNCH("kv8_join", kv8_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, st, a);
-  else if (rows <= 12288 || a.n_groups)
+  else if (rows <= 12288)
     GLT_LAUNCH("kv8_join", kv8_join_kernel<1>, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a);
+  else if (a.n_groups)
+    GLT_LAUNCH("kv8_join", kv8_join_rows_kernel<true>, dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
   else
-    GLT_LAUNCH("kv8_join", kv8_join_rows_kernel, dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
+    GLT_LAUNCH("kv8_join", kv8_join_rows_kernel<false>, dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
   GLT_LAUNCH_CHECK("kv8_join");
   return GLT_OK;
 }

@@ -246,8 +246,20 @@ def test_joins_of_many_rows(dev, T, Hq, Hkv, lens, new, window, sinks):
     Setup(T, Hq, Hkv, lens, None if new is None else [int(n) for n in new], seed=15).check(window, sinks)
 
 
-def test_a_bad_query_row_stays_alone_among_many(dev):
-    s = Setup(120, 64, 1, [3000, 2000], [120, 50], seed=16)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 70)])
+@pytest.mark.parametrize("T,Hq,Hkv,lens,new,plens", [
+    (100, 32, 2, [150, 220, 101, 300], [100, 1, 60, 0], [700, 64]),
+    (100, 33, 3, [150, 220, 0, 3000], None, [5000]),
+    (1, 28, 4, [(61 * i) % 400 for i in range(500)], None, [(331 * i) % 1500 for i in range(10)]),
+    (1, 32, 4, [1 + (7 * i) % 90 for i in range(400)], [int(i % 9 != 0) for i in range(400)], [(77 * i) % 300 for i in range(100)]),
+])
+def test_joins_of_many_rows_with_prefixes(dev, T, Hq, Hkv, lens, new, plens, window, sinks):
+    Setup(T, Hq, Hkv, lens, new, plens, seed=17).check(window, sinks)
+
+
+@pytest.mark.parametrize("plens", [(), (900,)])
+def test_a_bad_query_row_stays_alone_among_many(dev, plens):
+    s = Setup(120, 64, 1, [3000, 2000], [120, 50], plens, seed=16)
     a, al = s.run()
     for bad in (float("nan"), float("inf")):
         q = s.q.clone()
