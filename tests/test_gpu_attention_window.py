@@ -60,6 +60,7 @@ CASES = [
     (1, 3300, 4, 2, 200, 4, None, False),
     (1, 2500, 2, 1, 90, 300, None, False),         # of three blocks
     (1, 2300, 1, 1, 1000, 1024, None, False),
+    (2, 2900, 4, 2, 500, 200, (2777, 700), False), # cuts of ten
     (5, 300, 4, 2, 50, 2, (300, 0, 1, 64, 201), True),
     (3, 1700, 2, 1, 64, 4, (1300, 1700, 17), False),
     (2, 100, 2, 1, 99, 0, None, False),            # all but one key
