@@ -386,13 +386,14 @@ __global__ void __launch_bounds__(kWaves * 64, FINE ? 1 : 2) attn_dkdv_kernel(co
   const __amdgpu_buffer_rsrc_t rq = uni_rsrc_a(a.q + (int64_t)b * a.T * a.q_ld + (int64_t)h0 * kHd, rows_extent(len, a.q_ld) + (len > 0 ? more : 0));
   const __amdgpu_buffer_rsrc_t rdo = uni_rsrc_a(a.dout + (int64_t)b * a.T * a.o_ld + (int64_t)h0 * kHd, rows_extent(len, a.o_ld) + (len > 0 ? more : 0));
   const float* const stat = a.stats + ((wave & 1) * (int64_t)a.B * a.Hq + (int64_t)b * a.Hq + h0) * a.T;
+  const __amdgpu_buffer_rsrc_t rs0 = uni_rsrc_a(stat, (uint32_t)len * 4);
   lds_char* const lds = (lds_char*)smem;
   auto load = [&](int qt, int hd, lds_char* dst) {  // tile qt of head h0 + hd
     const int l = opaque(threadIdx.x) & 63;
     load_tile<kWaves>(rq, dst, wave, tile_lane_off(wave, l, qb_ld), qb_ld, (uint32_t)qt * kTile * qb_ld + hd * kHd * 2);
     load_tile<kWaves>(rdo, dst + kTileB, wave, tile_lane_off(wave, l, ob_ld), ob_ld, (uint32_t)qt * kTile * ob_ld + hd * kHd * 2);
     if (wave < 2)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(uni_rsrc_a(stat + (int64_t)hd * a.T, (uint32_t)len * 4),
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(WIN ? uni_rsrc_a(stat + (int64_t)hd * a.T, (uint32_t)len * 4) : rs0,
                                                (lds_void*)(dst + 2 * kTileB + wave * kTile * 4), 4,
                                                (uint32_t)(qt * kTile + l) * 4, 0, 0, 0);
   };
@@ -488,13 +489,14 @@ __global__ void __launch_bounds__(kWaves * 64, FINE ? 1 : 2) attn_dkdv_kernel(co
       __builtin_amdgcn_s_setprio(0);
     }
   };
-  int cur = 0;
+  int next = 0;
   for (int hd = 0; hd < heads; ++hd)
     for (int qt = qt0; qt < qt1; ++qt) {
       __builtin_amdgcn_s_waitcnt(vmcnt_enc(0));
       phase_barrier();  // the tile is whole, and every wavefront is done with the one before
+      const int cur = WIN ? next : (qt - qt0) & 1;
+      next = cur ^ 1;
       step(qt, hd, lds + cur * kDkdvBuf, lds + (cur ^ 1) * kDkdvBuf);
-      cur ^= 1;
     }
   // the output rows' addresses are worked out again here: kept across the
   // loop they cost registers that it does not have
@@ -531,11 +533,12 @@ __global__ void __launch_bounds__(kWaves * 64, FINE ? 1 : 2) attn_dkdv_kernel(co
 
 // dk (blockIdx.y 0) or dv (1): the parts of a group's query heads added in head
 // order, rounded once; a thread takes 8 elements of a token's kv head.
+template <bool SINKS>
 __device__ __forceinline__ void sum_parts(const BwdArgs& a, int64_t i) {
   const int cols = a.Hkv * (kHd / 8);
   if (i >= (int64_t)a.B * a.T * cols) return;
   const int64_t row = i / cols;
-  if (a.sink_blocks && row % a.T < a.sink_blocks * kRows) return;  // attn_sink_sum_kernel's
+  if (SINKS && row % a.T < a.sink_blocks * kRows) return;  // attn_sink_sum_kernel's
   const int c = (int)(i - row * cols), g = c / (kHd / 8), e = c % (kHd / 8) * 8;
   const float* p = a.part + ((blockIdx.y ? (int64_t)a.B * a.T : 0) + row) * a.Hkv * a.parts * kHd + (int64_t)g * a.parts * kHd + e;
   f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
@@ -551,7 +554,7 @@ __device__ __forceinline__ void sum_parts(const BwdArgs& a, int64_t i) {
 }
 
 __global__ void __launch_bounds__(256) attn_dkdv_sum_kernel(const BwdArgs a) {
-  sum_parts(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
+  sum_parts<false>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
 // The keys of the sink blocks: the parts of their query heads, each by cut.
@@ -587,7 +590,7 @@ __device__ __forceinline__ void sum_sinks(const BwdArgs& a, int64_t i) {
 // Both: the first `others` workgroups take the other keys' parts, where there are any
 // (4 x 1029, 6 and 2 heads, window 82, 64 sinks: the backward 54 us, in two launches 57).
 __global__ void __launch_bounds__(256) attn_sink_sum_kernel(const BwdArgs a, unsigned others) {
-  if (blockIdx.x < others) sum_parts(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (blockIdx.x < others) sum_parts<true>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
   else sum_sinks(a, (int64_t)(blockIdx.x - others) * 256 + threadIdx.x);
 }
 
