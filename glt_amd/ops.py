@@ -530,14 +530,9 @@ class Kv8Cache:
         B, T, Hq, hd = shape
         dev, index = self._device, self._index
         q_ld = _heads_ld("q", q, B, T, dev)
-        if window is None:
-            window = 0
-        elif not 1 <= window < 2 ** 31:
-            raise ValueError(f"window {window} (None, or 1 to 2^31 - 1)")
-        if not 0 <= sinks < 2 ** 31:
-            raise ValueError(f"sinks {sinks} (0 to 2^31 - 1)")
+        _check_window(window, sinks)
         s = self._seqs(B, T, pages, lens, new_lens)
-        d = F.Kv8Attn(Hq, hd ** -0.5 if scale is None else scale, window, sinks)
+        d = F.Kv8Attn(Hq, hd ** -0.5 if scale is None else scale, window or 0, sinks)
         if prefix is not None:
             ppages, plens = prefix
             groups = d.n_groups = ppages.shape[0]

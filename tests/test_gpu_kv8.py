@@ -509,3 +509,12 @@ def test_refusals(dev):
         ops.Kv8Cache(4, 2, head_dim=64)
     with pytest.raises(ValueError):
         ops.Kv8Cache(0, 2)
+
+
+@pytest.mark.parametrize("sinks", [1, 3, 2 ** 31 - 1])
+def test_sinks_are_refused_without_a_window(dev, sinks):
+    """As in training: they say nothing where every token is seen, so the window was forgotten."""
+    s = Setup(1, 4, 2, [300], seed=18)
+    with pytest.raises(ValueError, match="sinks"):
+        s.run(sinks=sinks)
+    s.check(window=20, sinks=sinks)
