@@ -202,6 +202,9 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Args a) {
   }
 }
 
+// pages that T tokens from any place of a page lie in
+int64_t token_pages(const glt_kv8_seqs* s) { return (s->T + 2 * kPage - 2) / kPage; }
+
 glt_status check_tokens(const glt_kv8_cache* c, const glt_kv8_seqs* s, const void* k, int64_t k_ld, const void* v,
                         int64_t v_ld, const char* who) {
   const int64_t lds[2] = {k_ld, v_ld};
@@ -210,6 +213,9 @@ glt_status check_tokens(const glt_kv8_cache* c, const glt_kv8_seqs* s, const voi
               "%s: %c_ld %lld (at least %d heads of %d, a multiple of 8)", who, "kv"[i], (long long)lds[i], c->n_kv_heads, kKv8Hd);
   GLT_CHECK(k && v, GLT_ERR_INVALID_ARG, "%s: null pointer", who);
   GLT_CHECK(((uintptr_t)k | (uintptr_t)v) % 16 == 0, GLT_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", who);
+  // a launch holds less than 2^32 threads, 256 for a page and head
+  GLT_CHECK(token_pages(s) * s->B < (1 << 24) / c->n_kv_heads, GLT_ERR_SHAPE, "%s: B=%d T=%d n_kv_heads=%d", who, s->B, s->T,
+            c->n_kv_heads);
   return GLT_OK;
 }
 
@@ -225,9 +231,8 @@ Kv8Args pack_args(const glt_kv8_cache* c, const glt_kv8_seqs* s, void* k, int64_
   a.Hkv = c->n_kv_heads;
   return a;
 }
-// pages that T tokens from any place of a page lie in
 dim3 token_grid(const glt_kv8_cache* c, const glt_kv8_seqs* s) {
-  return dim3((unsigned)((s->T + 2 * kPage - 2) / kPage), (unsigned)c->n_kv_heads, (unsigned)s->B);
+  return dim3((unsigned)token_pages(s), (unsigned)c->n_kv_heads, (unsigned)s->B);
 }
 
 }  // namespace

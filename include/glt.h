@@ -438,7 +438,9 @@ size_t glt_kv8_size(int64_t n_pages, int32_t n_kv_heads, int32_t head_dim);
  * (device, NULL = T), padded to T in the call's tensors: new token t is token
  * lens[b] - new_lens[b] + t. Lengths are clamped: lens to [0, 64 n_table], new_lens to [0,
  * min(T, lens)]. A page id outside the pool is never followed: what would be written
- * there is dropped, what would be read is NaN. */
+ * there is dropped, what would be read is NaN. Refused (GLT_ERR_SHAPE) is what one launch
+ * does not hold: writes and reads of B * n_kv_heads * ((T + 126) / 64) >= 2^24,
+ * attention of B * T * n_q_heads >= 2^25. */
 typedef struct {
   int32_t B, T;
   const int32_t* pages;

@@ -150,3 +150,15 @@ def test_sizes():
     assert ws(n_table=24, pages_ld=24) == ws(window=1400, **wide) == 0
     assert ws(n_table=25, pages_ld=25) > 0 and ws(B=200, n_table=32, pages_ld=32) == 0
     assert ws(**PREFIX) > ws()
+
+
+@pytest.mark.parametrize("fn", ["glt_kv8_write", "glt_kv8_read"])
+@pytest.mark.parametrize("kw", [
+    dict(B=8192, T=1, n_kv_heads=2048), dict(B=8192, T=66, n_kv_heads=1024), dict(B=64, T=1 << 24, n_kv_heads=2),
+    dict(B=8192, T=1 << 24, n_kv_heads=4096),
+])
+def test_more_workgroups_than_a_launch_has_are_refused(fn, kw):
+    """256 threads each, of less than 2^32 in all; pages of 64 tokens from any place of the first."""
+    heads = 128 * kw["n_kv_heads"]
+    assert tokens(fn, kw, k_ld=heads, v_ld=heads) == 2
+    assert b"B=%d T=%d" % (kw["B"], kw["T"]) in F.load().glt_last_error_string()
