@@ -253,6 +253,15 @@ glt_status check_kv8(const glt_kv8_cache* c, const glt_kv8_seqs* s, const char* 
   return GLT_OK;
 }
 
+glt_status check_spared(const glt_kv8_seqs* s, const ByteRows* to, int n, const char* who) {
+  const ByteRows read[] = {table_bytes(s->pages, s->B, s->pages_ld, s->n_table), dense_bytes(s->lens, 4 * (int64_t)s->B),
+                           dense_bytes(s->new_lens, s->new_lens ? 4 * (int64_t)s->B : 0)};
+  for (int i = 0; i < n; ++i)
+    for (const ByteRows& x : read)
+      GLT_CHECK(!overlap(to[i], x), GLT_ERR_INVALID_ARG, "%s: results must overlap neither pages nor lengths", who);
+  return GLT_OK;
+}
+
 }  // namespace glt
 
 using namespace glt;
@@ -272,6 +281,8 @@ extern "C" glt_status glt_kv8_write(const glt_kv8_cache* c, const glt_kv8_seqs* 
   const ByteRows pool = dense_bytes(c->data, (int64_t)glt_kv8_size(c->n_pages, c->n_kv_heads, c->head_dim));
   GLT_CHECK(!overlap(pool, {k, tokens, w, 2 * k_ld}) && !overlap(pool, {v, tokens, w, 2 * v_ld}), GLT_ERR_INVALID_ARG,
             "glt_kv8_write: k and v must not overlap the cache");
+  r = check_spared(s, &pool, 1, "glt_kv8_write");
+  if (r != GLT_OK) return r;
   const Kv8Args a = pack_args(c, s, const_cast<void*>(k), k_ld, const_cast<void*>(v), v_ld);
   GLT_LAUNCH("kv8_write", kv8_write_kernel, token_grid(c, s), dim3(256), 0, as_stream(stream), a);
   GLT_LAUNCH_CHECK("kv8_write");
@@ -286,9 +297,11 @@ extern "C" glt_status glt_kv8_read(const glt_kv8_cache* c, const glt_kv8_seqs* s
   if (r != GLT_OK) return r;
   const int64_t tokens = (int64_t)s->B * s->T, w = 2 * kKv8Hd * (int64_t)c->n_kv_heads;
   const ByteRows pool = dense_bytes(c->data, (int64_t)glt_kv8_size(c->n_pages, c->n_kv_heads, c->head_dim));
-  const ByteRows rk{k, tokens, w, 2 * k_ld}, rv{v, tokens, w, 2 * v_ld};
-  GLT_CHECK(!overlap(pool, rk) && !overlap(pool, rv) && !overlap(rk, rv), GLT_ERR_INVALID_ARG,
+  const ByteRows to[] = {{k, tokens, w, 2 * k_ld}, {v, tokens, w, 2 * v_ld}};
+  GLT_CHECK(!overlap(pool, to[0]) && !overlap(pool, to[1]) && !overlap(to[0], to[1]), GLT_ERR_INVALID_ARG,
             "glt_kv8_read: k and v must overlap neither the cache nor each other");
+  r = check_spared(s, to, 2, "glt_kv8_read");
+  if (r != GLT_OK) return r;
   const Kv8Args a = pack_args(c, s, k, k_ld, v, v_ld);
   GLT_LAUNCH("kv8_read", kv8_read_kernel, token_grid(c, s), dim3(256), 0, as_stream(stream), a);
   GLT_LAUNCH_CHECK("kv8_read");

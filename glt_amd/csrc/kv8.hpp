@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "overlap.hpp"
 
 namespace glt {
 
@@ -27,6 +28,10 @@ __host__ __device__ constexpr int v_byte(int t) { return (t & 0x33) | ((t & 4) <
 
 // Refuses caches and page tables that no entry point serves (kv8.hip).
 glt_status check_kv8(const glt_kv8_cache* c, const glt_kv8_seqs* s, const char* who);
+// Refuses results (n of them) in the page table and lengths, which workgroups read after
+// others have written: a length that changed would lead past what was sized by it.
+glt_status check_spared(const glt_kv8_seqs* s, const ByteRows* to, int n, const char* who);
+inline ByteRows table_bytes(const int32_t* pages, int64_t rows, int64_t ld, int64_t n) { return {pages, rows, 4 * n, 4 * ld}; }
 
 // Tokens that sequence b holds and how many of them are the call's new ones.
 struct Kv8Len { int len, fresh; };

@@ -1234,7 +1234,7 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
                                         int64_t q_ld, void* out, int64_t o_ld, float* lse, void* workspace,
                                         size_t workspace_bytes, void* stream) {
   static const char* who = "glt_kv8_attention";
-  const glt_status r = check_attn(c, s, d, who);
+  glt_status r = check_attn(c, s, d, who);
   if (r != GLT_OK || s->B == 0 || s->T == 0) return r;
   const int64_t lds[2] = {q_ld, o_ld};
   for (int i = 0; i < 2; ++i)
@@ -1257,6 +1257,15 @@ extern "C" glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_se
     for (int j = i + 1; j < 5; ++j)
       GLT_CHECK(!overlap(all[i], all[j]), GLT_ERR_INVALID_ARG,
                 "%s: out, lse and workspace must overlap neither each other nor q nor the cache", who);
+  r = check_spared(s, all, 3, who);
+  if (r != GLT_OK) return r;
+  if (d->n_groups) {
+    const ByteRows prefix[] = {table_bytes(d->prefix_pages, d->n_groups, d->prefix_ld, d->n_prefix_table),
+                               dense_bytes(d->prefix_lens, 4 * (int64_t)d->n_groups)};
+    for (int i = 0; i < 3; ++i)
+      GLT_CHECK(!overlap(all[i], prefix[0]) && !overlap(all[i], prefix[1]), GLT_ERR_INVALID_ARG,
+                "%s: results must overlap neither a prefix's pages nor its length", who);
+  }
 
   DecArgs a{};
   a.cache = static_cast<const uint8_t*>(c->data);

@@ -440,7 +440,8 @@ size_t glt_kv8_size(int64_t n_pages, int32_t n_kv_heads, int32_t head_dim);
  * min(T, lens)]. A page id outside the pool is never followed: what would be written
  * there is dropped, what would be read is NaN. Refused (GLT_ERR_SHAPE) is what one launch
  * does not hold: writes and reads of B * n_kv_heads * ((T + 126) / 64) >= 2^24,
- * attention of B * T * n_q_heads >= 2^25. */
+ * attention of B * T * n_q_heads >= 2^25. No result (the pool of a write among them)
+ * overlaps tables or lengths. */
 typedef struct {
   int32_t B, T;
   const int32_t* pages;

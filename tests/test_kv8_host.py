@@ -162,3 +162,29 @@ def test_more_workgroups_than_a_launch_has_are_refused(fn, kw):
     heads = 128 * kw["n_kv_heads"]
     assert tokens(fn, kw, k_ld=heads, v_ld=heads) == 2
     assert b"B=%d T=%d" % (kw["B"], kw["T"]) in F.load().glt_last_error_string()
+
+
+# tables and lengths apart from the cache and each other
+APART = dict(pages=at(5), lens=at(6), new_lens=at(7), n_table=40, pages_ld=50)
+IN_TABLES = [at(5), at(5) + 4 * (3 * 50 + 38), at(6), at(7) - 368]
+
+
+@pytest.mark.parametrize("where", IN_TABLES)
+def test_results_in_tables_or_lengths_are_refused(where):
+    """At their start, in the table's last two pages, and from before the new lengths on."""
+    for n in ("out", "lse", "ws"):
+        assert attn(APART, **{n: where & ~255 if n == "ws" else where}) == 1, n
+        assert b"lengths" in F.load().glt_last_error_string()
+    for n in ("k", "v"):
+        assert tokens("glt_kv8_read", APART, **{n: where}) == 1, n
+        assert b"lengths" in F.load().glt_last_error_string()
+    assert tokens("glt_kv8_write", dict(APART, data=where)) == 1
+    assert b"lengths" in F.load().glt_last_error_string()
+
+
+def test_results_in_a_prefix_are_refused():
+    kw = dict(APART, n_groups=2, prefix_pages=at(8), prefix_ld=64, n_prefix_table=60, prefix_lens=at(9))
+    for where in (at(8), at(8) + 4 * 64, at(9)):
+        for n in ("out", "lse", "ws"):
+            assert attn(kw, **{n: where}) == 1, n
+            assert b"prefix" in F.load().glt_last_error_string()
