@@ -693,7 +693,8 @@ glt_status train_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, cons
   // every kernel reads inputs after others have written gradients
   const int64_t tokens = (int64_t)d->B * d->T, nq = 2 * kHd * d->n_q_heads, nk = 2 * kHd * d->n_kv_heads;
   const ByteRows in[] = {{q, tokens, nq, 2 * d->q_ld},   {k, tokens, nk, 2 * d->k_ld},    {v, tokens, nk, 2 * d->v_ld},
-                         {out, tokens, nq, 2 * d->o_ld}, {dout, tokens, nq, 2 * d->o_ld}, dense_bytes(lse, tokens * d->n_q_heads * 4)};
+                         {out, tokens, nq, 2 * d->o_ld}, {dout, tokens, nq, 2 * d->o_ld}, dense_bytes(lse, tokens * d->n_q_heads * 4),
+                         dense_bytes(d->seq_lens, d->seq_lens ? 4 * (int64_t)d->B : 0)};
   const ByteRows to[] = {{dq, tokens, nq, 2 * d->q_ld}, {dk, tokens, nk, 2 * d->k_ld}, {dv, tokens, nk, 2 * d->v_ld},
                          dense_bytes(workspace, (int64_t)need)};
   for (int i = 0; i < 4; ++i) {

@@ -296,6 +296,9 @@ glt_status train_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, cons
             GLT_ERR_INVALID_ARG, "%s: out must overlap no input (but q itself)", who);
   GLT_CHECK(!overlap(rl, rq) && !overlap(rl, rk) && !overlap(rl, rv) && !overlap(rl, ro), GLT_ERR_INVALID_ARG,
             "%s: lse must overlap no other tensor", who);
+  // workgroups read lengths after others have written
+  const ByteRows lens = dense_bytes(d->seq_lens, d->seq_lens ? 4 * (int64_t)d->B : 0);
+  GLT_CHECK(!overlap(ro, lens) && !overlap(rl, lens), GLT_ERR_INVALID_ARG, "%s: out and lse must not overlap seq_lens", who);
   // the dynamic-LDS limit is a per-device attribute of the kernel
   static std::atomic<bool> attr_set[64];
   int dev = 0;

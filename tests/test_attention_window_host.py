@@ -69,3 +69,13 @@ def test_short_sequences_need_no_parts_for_sinks():
         d = desc(T=T)
         plain = lib.glt_attention_bwd_workspace_size(ctypes.byref(d))
         assert (lib.glt_attention_window_bwd_workspace_size(ctypes.byref(d), window, 4) > plain) == more, T
+
+
+def test_results_over_the_lengths_are_refused():
+    d = desc(seq_lens=20 << 32)
+    for name in ("out", "lse"):
+        assert fwd(d, **{name: 20 << 32}) == 1, name
+        assert b"overlap" in F.load().glt_last_error_string()
+    for name in ("dq", "dk", "dv", "ws"):
+        assert bwd(d, **{name: 20 << 32}) == 1, name
+        assert b"overlap" in F.load().glt_last_error_string()
