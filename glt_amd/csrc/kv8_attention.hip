@@ -1100,6 +1100,7 @@ struct Plan {
 };
 Plan plan(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d) {
   Plan p{};
+  if (s->n_table == 0) return p;  // no tokens of their own, so no new ones: every row is padding
   const int64_t G = d->n_q_heads / c->n_kv_heads, S = d->sinks, H = c->n_kv_heads;
   const int64_t gs = d->n_groups ? s->B / d->n_groups : 0, segs[2] = {s->B, d->n_groups};
   p.rows[0] = (int64_t)s->T * G;
@@ -1156,13 +1157,12 @@ glt_status check_attn(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_k
 
 typedef void (*Kernel)(DecArgs);
 Kernel pieces_kernel(Kind prefix, Kind own) {
-  // [prefix][own]: a prefix has at least its sequences' rows
+  // [prefix][own]: a prefix has at least its sequences' rows, and none where they have no tokens
   static const Kernel k[4][4] = {
       {nullptr, kv8_pieces_kernel<kNone, kFew16>, kv8_pieces_kernel<kNone, kFew32>, kv8_pieces_kernel<kNone, kMany>},
-      {kv8_pieces_kernel<kFew16, kNone>, kv8_pieces_kernel<kFew16, kFew16>, nullptr, nullptr},
-      {kv8_pieces_kernel<kFew32, kNone>, kv8_pieces_kernel<kFew32, kFew16>, kv8_pieces_kernel<kFew32, kFew32>, nullptr},
-      {kv8_pieces_kernel<kMany, kNone>, kv8_pieces_kernel<kMany, kFew16>, kv8_pieces_kernel<kMany, kFew32>,
-       kv8_pieces_kernel<kMany, kMany>}};
+      {nullptr, kv8_pieces_kernel<kFew16, kFew16>, nullptr, nullptr},
+      {nullptr, kv8_pieces_kernel<kFew32, kFew16>, kv8_pieces_kernel<kFew32, kFew32>, nullptr},
+      {nullptr, kv8_pieces_kernel<kMany, kFew16>, kv8_pieces_kernel<kMany, kFew32>, kv8_pieces_kernel<kMany, kMany>}};
   return k[prefix][own];
 }
 

@@ -518,3 +518,13 @@ def test_sinks_are_refused_without_a_window(dev, sinks):
     with pytest.raises(ValueError, match="sinks"):
         s.run(sinks=sinks)
     s.check(window=20, sinks=sinks)
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+def test_no_tables_behind_prefixes(dev, T):
+    """Few, some and many rows that all come to nothing."""
+    s = Setup(1, 8, 2, [3, 3, 3, 3], plens=[500, 70], seed=19)
+    none = torch.empty(4, 0, dtype=I32, device="cuda")
+    q = rows((4, T, 8, HD), 1).cuda()
+    out, lse = s.cache.attention(q, none, ints([5, 0, 1, T]), prefix=s.prefix)
+    assert not out.any() and (lse == -torch.inf).all()

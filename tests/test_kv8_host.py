@@ -188,3 +188,12 @@ def test_results_in_a_prefix_are_refused():
         for n in ("out", "lse", "ws"):
             assert attn(kw, **{n: where}) == 1, n
             assert b"prefix" in F.load().glt_last_error_string()
+
+
+@pytest.mark.parametrize("T", [1, 6, 100])
+def test_sequences_without_a_table_need_no_workspace(T):
+    """They hold no tokens, so their prefix is read by no row."""
+    kw = dict(PREFIX, T=T, pages=None, pages_ld=0, n_table=0)
+    assert F.load().glt_kv8_attention_workspace_size(*descs(kw)) == 0
+    kw["n_table"] = kw["pages_ld"] = 1
+    assert F.load().glt_kv8_attention_workspace_size(*descs(kw)) > 0
