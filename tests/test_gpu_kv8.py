@@ -528,3 +528,48 @@ def test_no_tables_behind_prefixes(dev, T):
     q = rows((4, T, 8, HD), 1).cuda()
     out, lse = s.cache.attention(q, none, ints([5, 0, 1, T]), prefix=s.prefix)
     assert not out.any() and (lse == -torch.inf).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (50, 3), (150, 70), (300, 0)])
+@pytest.mark.parametrize("T,Hq,Hkv,lens,new,plens", [
+    (5, 8, 2, [5, 60, 9, 370], [5, 0, 2, 4], [1000]),           # 80 rows of a prefix, 20 of a sequence
+    (5, 8, 2, [5, 60, 9, 370], None, [1000, 64, 0, 333]),       # 20 and 20
+    (8, 12, 3, [8, 300, 70, 64, 9, 200], [8, 3, 0, 8, 1, 7], [130, 700]),  # 96, 32
+    (4, 8, 1, [700, 4], [4, 2], [63, 2000]),                    # 32, 32
+    (8, 4, 1, [20 + 3 * i for i in range(70)], [i % 9 for i in range(70)], [257]),  # more sequences than lanes
+])
+def test_two_row_blocks_behind_a_prefix(dev, T, Hq, Hkv, lens, new, plens, window, sinks):
+    """17 to 32 own rows a sequence and head beside a prefix's few or many."""
+    Setup(T, Hq, Hkv, lens, new, plens, seed=20).check(window, sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 70)])
+@pytest.mark.parametrize("T,plens", [
+    (5, [(97 * i) % 900 for i in range(20)]),                   # 200 rows of a prefix
+    (5, [(31 * i) % 400 for i in range(200)]),                  # 20
+])
+def test_joins_of_two_row_blocks_behind_a_prefix(dev, T, plens, window, sinks):
+    """16000 rows: eight joined by a wavefront."""
+    lens = [T + (53 * i) % 300 for i in range(200)]
+    Setup(T, 16, 4, lens, [i % (T + 1) for i in range(200)], plens, seed=21).check(window, sinks)
+
+
+@pytest.mark.parametrize("T,Hq,lens,new,plens", [
+    (6, 4, [3000, 90], [6, 2], None), (8, 4, [300, 90], [8, 2], None),      # 24, 32 rows
+    (6, 4, [300, 90], [6, 2], [200]), (8, 4, [300, 90], [8, 3], [500, 70]),  # beside 48 and 32 of a prefix
+])
+def test_a_bad_query_row_stays_alone_in_two_row_blocks(dev, T, Hq, lens, new, plens):
+    """NaN and infinity in padding and in a row of either block of 16."""
+    s = Setup(T, Hq, 1, lens, new, plens or (), seed=22)
+    a, al = s.run(window=200, sinks=3)
+    assert torch.isfinite(a).all()
+    for bad in (float("nan"), float("inf")):
+        for t, h in ((1, 0), (5, 3)):
+            q = s.q.clone()
+            s.q[1, 3:] = bad                    # padding
+            s.q[0, t, h] = bad
+            b, bl = s.run(window=200, sinks=3)
+            s.q.copy_(q)
+            assert torch.isnan(b[0, t, h]).all() and torch.isnan(bl[0, h, t])
+            b[0, t, h], bl[0, h, t] = a[0, t, h], al[0, h, t]
+            assert torch.equal(a, b) and torch.equal(al, bl)
