@@ -719,7 +719,11 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
       const float mt = pair_max(fmax_nc(m2[0], m2[1]));
       const bool up = mt > (unset ? -INFINITY : kSlack);
       if (__any(up)) {  // each row's moves by itself
-        const float m_new = up ? base + mt : m_run, by = up ? m_new - base : 0.f;
+        const float m_new = up ? base + mt : m_run;
+        // As the new maximum is rounded, unless that puts it more than 1 off (scores past
+        // 2^24): the largest probability would leave f32 or vanish.
+        float by = m_new - base;
+        by = !up ? 0.f : __builtin_fabsf(by - mt) > 1.f ? mt : by;
         const float alpha = unset ? 1.f : __builtin_amdgcn_exp2f(-by);
         m_run = m_new;
         l_run *= alpha;

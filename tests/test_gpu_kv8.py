@@ -573,3 +573,17 @@ def test_a_bad_query_row_stays_alone_in_two_row_blocks(dev, T, Hq, lens, new, pl
             assert torch.isnan(b[0, t, h]).all() and torch.isnan(bl[0, h, t])
             b[0, t, h], bl[0, h, t] = a[0, t, h], al[0, h, t]
             assert torch.equal(a, b) and torch.equal(al, bl)
+
+
+@pytest.mark.parametrize("q_std", [1e8, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("T,lens,plens", [(1, [700], ()), (1, [3000], ()), (8, [700], ()), (100, [700, 164], ()),
+                                          (100, [5000], ()), (60, [700], [500])])
+def test_scores_of_any_size(dev, T, lens, plens, q_std):
+    """Past 2^24 a step of f32 between two scores is more than a whole power of e: the weights
+    are those of a few keys (whichever rounding leaves in front), finite and no larger than the values."""
+    s = Setup(T, 4, 1, lens, None, plens, seed=23, q_std=q_std)
+    top = max(float(v.abs().max()) for v in s.v)
+    for sign in (1, -1):
+        s.q *= sign
+        out, lse = s.check(scale=1.0)
+        assert float(out.abs().max()) <= top * (1 + 2.0 ** -7)  # two roundings, of p and of the result
