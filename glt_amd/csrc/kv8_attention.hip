@@ -32,7 +32,7 @@ namespace glt {
 namespace {
 
 constexpr float kSlack = 8.0f;      // running-max slack (log2 units)
-constexpr float kNoMax = -3.0e38f;  // maximum of a row that has seen nothing
+constexpr float kNoMax = -3.4028234663852886e38f;  // maximum of a row that has seen nothing: below every score's
 
 // A kind of segments, [0] the sequences' own tokens, [1] prefixes.
 struct Part {

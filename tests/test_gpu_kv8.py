@@ -587,3 +587,15 @@ def test_scores_of_any_size(dev, T, lens, plens, q_std):
         s.q *= sign
         out, lse = s.check(scale=1.0)
         assert float(out.abs().max()) <= top * (1 + 2.0 ** -7)  # two roundings, of p and of the result
+
+
+@pytest.mark.parametrize("T,n", [(1, 1), (1, 40), (1, 3000), (8, 700), (100, 100), (100, 5000)])
+def test_scores_near_the_lowest_f32(dev, T, n):
+    """Every score the same, -3.2e38 in units of log2: the mean of the values."""
+    cache = stale(ops.Kv8Cache(80, 1))
+    pages = torch.arange(80, dtype=I32, device="cuda")[None]
+    k, v = torch.full((1, n, 1, HD), 8128.0, dtype=BF), rows((1, n, 1, HD), 24)  # 127 steps of 64
+    cache.write(k.cuda(), v.cuda(), pages, ints([n]))
+    q = torch.full((1, T, 4, HD), -2.0 ** 111, dtype=BF)
+    out, lse = cache.attention(q.cuda(), pages, ints([n]), scale=0.082)
+    R.check(out[0], lse[0], R.attend(q[0], R.values(k)[0], R.values(v)[0], torch.arange(n - T, n), 0.082))
