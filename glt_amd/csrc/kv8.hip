@@ -202,6 +202,11 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Args a) {
   }
 }
 
+// Caches that page ids and offsets reach.
+bool cache_sizes(int64_t n_pages, int n_kv_heads) {
+  return n_pages > 0 && n_pages <= INT32_MAX && n_kv_heads > 0 && n_kv_heads <= 4096;
+}
+
 // pages that T tokens from any place of a page lie in
 int64_t token_pages(const glt_kv8_seqs* s) { return (s->T + 2 * kPage - 2) / kPage; }
 
@@ -240,8 +245,8 @@ dim3 token_grid(const glt_kv8_cache* c, const glt_kv8_seqs* s) {
 glt_status check_kv8(const glt_kv8_cache* c, const glt_kv8_seqs* s, const char* who) {
   GLT_CHECK(c && s, GLT_ERR_INVALID_ARG, "%s: null descriptor", who);
   GLT_CHECK(c->head_dim == kKv8Hd, GLT_ERR_UNSUPPORTED, "%s: head_dim %d (only %d)", who, c->head_dim, kKv8Hd);
-  GLT_CHECK(c->n_pages > 0 && c->n_pages <= INT32_MAX && c->n_kv_heads > 0 && c->n_kv_heads <= 4096, GLT_ERR_SHAPE,
-            "%s: n_pages=%lld n_kv_heads=%d", who, (long long)c->n_pages, c->n_kv_heads);
+  GLT_CHECK(cache_sizes(c->n_pages, c->n_kv_heads), GLT_ERR_SHAPE, "%s: n_pages=%lld n_kv_heads=%d", who,
+            (long long)c->n_pages, c->n_kv_heads);
   GLT_CHECK(s->B >= 0 && s->B <= 8192 && s->T >= 0 && s->T <= (1 << 24), GLT_ERR_SHAPE, "%s: B=%d (at most 8192) T=%d", who,
             s->B, s->T);
   GLT_CHECK(s->n_table >= 0 && s->n_table <= (1 << 23) && s->pages_ld >= s->n_table, GLT_ERR_SHAPE,
@@ -267,7 +272,7 @@ glt_status check_spared(const glt_kv8_seqs* s, const ByteRows* to, int n, const 
 using namespace glt;
 
 extern "C" size_t glt_kv8_size(int64_t n_pages, int32_t n_kv_heads, int32_t head_dim) {
-  if (n_pages <= 0 || n_kv_heads <= 0 || head_dim != kKv8Hd) return 0;
+  if (!cache_sizes(n_pages, n_kv_heads) || head_dim != kKv8Hd) return 0;
   return (size_t)n_pages * n_kv_heads * kHeadB;
 }
 

@@ -422,8 +422,9 @@ glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t window, int3
  * aligned, laid out as the kernels read it. A token's head is held as
  *   step = bf16(max |x| / 127), in [2^-100, 2^121];  value = step * round(x / step)
  * (nearest, ties to even; NaN throughout where x holds NaN or infinity), so that
- * a value is within half a step of x, and a row of zeros stays one. head_dim is 128. The
- * pool needs no clearing: what no call has written is never looked at. */
+ * a value is within half a step of x, and a row of zeros stays one. head_dim is 128, n_pages
+ * less than 2^31, n_kv_heads at most 4096 (glt_kv8_size is 0 for others). The pool needs no
+ * clearing: what no call has written is never looked at. */
 typedef struct {
   void* data;
   int64_t n_pages;

@@ -197,3 +197,10 @@ def test_sequences_without_a_table_need_no_workspace(T):
     assert F.load().glt_kv8_attention_workspace_size(*descs(kw)) == 0
     kw["n_table"] = kw["pages_ld"] = 1
     assert F.load().glt_kv8_attention_workspace_size(*descs(kw)) > 0
+
+
+@pytest.mark.parametrize("n_pages,heads", [(1 << 31, 1), ((1 << 52) + 1, 16), (1 << 62, 8), (-1, 8), (10, 4097), (10, -1)])
+def test_no_size_for_caches_that_no_call_serves(n_pages, heads):
+    """Their bytes may pass 64 bits: 2^52 + 1 pages of 16 heads came to 266240."""
+    assert F.load().glt_kv8_size(n_pages, heads, 128) == 0
+    assert F.load().glt_kv8_size((1 << 31) - 1, 4096, 128) == ((1 << 31) - 1) * 4096 * 64 * 260
