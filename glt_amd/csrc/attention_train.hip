@@ -271,8 +271,9 @@ glt_status check_attn_desc(const glt_attn_desc* d, const char* who) {
 
 // Windows and sinks within a sequence of T; window 0 where it hides nothing.
 glt_status check_window(const glt_attn_desc* d, int32_t* window, int32_t* sinks, const char* who) {
-  GLT_CHECK(*window >= 1 && *sinks >= 0 && *sinks <= kMaxSinks, GLT_ERR_INVALID_ARG,
-            "%s: window %d (at least 1), sinks %d (0 to %d)", who, *window, *sinks, kMaxSinks);
+  GLT_CHECK(*window >= 1 && *sinks >= 0 && (*sinks <= kMaxSinks || *window >= d->T), GLT_ERR_INVALID_ARG,
+            "%s: window %d (at least 1), sinks %d (0 to %d, or any with a window of T = %d or more)", who, *window, *sinks,
+            kMaxSinks, d->T);
   GLT_CHECK(d->causal, GLT_ERR_UNSUPPORTED, "%s: a window is causal", who);
   if (*window >= d->T) *window = *sinks = 0;
   return GLT_OK;

@@ -401,8 +401,9 @@ glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* 
 
 /* The same with a window: row t reads, of the keys up to itself, those less than
  * `window` (at least 1) back and the first `sinks` (0 to 1024) of its sequence; d->causal
- * is 1. A window of T or more gives glt_attention_train_fwd's results. Tiles of 64 keys
- * that no row of a block reads are not visited: the work is T * (window + sinks), not T^2.
+ * is 1. A window of T or more, with any number of sinks, gives
+ * glt_attention_train_fwd's results. Tiles of 64 keys that no row of a block reads are not
+ * visited: the work is T * (window + sinks), not T^2.
  * A NaN or infinity reaches rows that see a key of its tile, as without a window. */
 glt_status glt_attention_window_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
                                     const void* k, const void* v, void* out, float* lse, void* stream);

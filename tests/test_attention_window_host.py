@@ -79,3 +79,11 @@ def test_results_over_the_lengths_are_refused():
     for name in ("dq", "dk", "dv", "ws"):
         assert bwd(d, **{name: 20 << 32}) == 1, name
         assert b"overlap" in F.load().glt_last_error_string()
+
+
+@pytest.mark.parametrize("window,sinks,taken", [(40, 1025, True), (2 ** 31 - 1, 2 ** 31 - 1, True), (39, 1024, True),
+                                                (39, 1025, False), (40, -1, False)])
+def test_any_sinks_where_the_window_hides_nothing(window, sinks, taken):
+    """40 tokens. (4: taken so far, and the operand's alignment refused.)"""
+    assert fwd(desc(), window, sinks, out=(1 << 32) + 8) == (4 if taken else 1)
+    assert bwd(desc(), window, sinks, out=(1 << 32) + 8) == (4 if taken else 1)

@@ -111,6 +111,13 @@ def test_a_window_that_hides_nothing(dev, window, sinks):
         assert torch.equal(a[name], b[name]), name
 
 
+def test_many_sinks_where_nothing_is_hidden(dev):
+    q, k, v, dout = make(1, 200, 4, 2, 3)
+    a, b = run(q, k, v, dout), run(q, k, v, dout, window=200, sinks=5000)
+    for name in a:
+        assert torch.equal(a[name], b[name]), name
+
+
 def test_what_no_row_of_the_tile_sees_takes_no_part(dev):
     """NaN and infinity in keys and values that lie whole tiles before every
     window, behind the sinks' tile, and in the padding."""
