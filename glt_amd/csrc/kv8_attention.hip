@@ -570,22 +570,23 @@ __device__ __forceinline__ void many_rows(const DecArgs& a, char* smem, int bloc
     const int rem = pos - deal.first(seg), rb = rem / n, i0 = rem - rb * n, i1 = min(n, i0 + stop - at);
     at += i1 - i0;
     const Sight si = sight<PRE>(a, seg);
-    // of the list, what the block's rows see: to the last row's own key, from the first row's window on
-    int from = i0, to = i1;
+    // Of the list, what the block's rows see: the first `sunk` pages, which hold sinks, and
+    // those from the first row's window on, to the last row's own key. (Of a prefix the list as it is.)
+    int sunk = si.ns, from = si.ns, to = n;
     if (!PRE) {
       const Kv8Len ln = kv8_len(a.s, seg);
       const int t0 = rb * kManyRows / a.G, t1 = min((rb * kManyRows + kManyRows - 1) / a.G, ln.fresh - 1);
       const int p1 = (ln.len - ln.fresh + t1) / kPage + 1;  // pages that hold keys up to t1's
-      to = uni(min(to, si.ns + max(p1 - si.c0, 0)));
+      to = si.ns + max(p1 - si.c0, 0);
       if (a.W) {
-        const int skip = si.ns + max(max(ln.len - ln.fresh + t0 - a.W + 1, 0) / kPage - si.c0, 0);
-        // (a list without pages of its own for sinks may hold some)
-        if (from >= si.ns && from < skip && si.page(from) * kPage >= a.S - prefix_len(a, seg)) from = skip;
-        from = uni(from);
+        from = si.ns + max(max(ln.len - ln.fresh + t0 - a.W + 1, 0) / kPage - si.c0, 0);
+        sunk = (min(max(a.S - prefix_len(a, seg), 0), si.hi) + kPage - 1) / kPage;  // (ns, or past where the window starts)
       }
     }
-    const int tiles = max(to - from, 0);
-    auto page_of = [&](int j) { return a.W ? si.page(from + j) : from + j; };
+    // the piece's part of both; where sinks lie the list's entries are the pages
+    const int head = uni(max(min(min(sunk, to), i1) - i0, 0)), rest = uni(max(max(from, i0), i0 + head));
+    const int tiles = uni(head + max(min(to, i1) - rest, 0)), tail = uni(si.c0 - si.ns + rest - head);
+    auto page_of = [&](int j) { return a.W ? j + (j < head ? i0 : tail) : i0 + j; };
     // lane x: the id of tile x, 64 at a time, the first ones on their way while the rows are looked up
     auto ids_from = [&](int j) { return j + lane < tiles ? page_id<PRE>(a, seg, page_of(j + lane)) : 0; };
     int ids = ids_from(0);

@@ -599,3 +599,34 @@ def test_scores_near_the_lowest_f32(dev, T, n):
     q = torch.full((1, T, 4, HD), -2.0 ** 111, dtype=BF)
     out, lse = cache.attention(q.cuda(), pages, ints([n]), scale=0.082)
     R.check(out[0], lse[0], R.attend(q[0], R.values(k)[0], R.values(v)[0], torch.arange(n - T, n), 0.082))
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 1), (33, 64), (64, 4), (128, 0), (128, 4), (100, 200), (500, 65), (600, 1000),
+                                          (128, 2 ** 31 - 1), (5000, 3)])
+@pytest.mark.parametrize("T,Hq,Hkv,lens,new,plens", [
+    (700, 4, 1, [2000, 701, 900], [700, 699, 3], ()),
+    (300, 6, 2, [1900], None, ()),
+    (300, 4, 2, [1500, 310], [300, 40], [50]),      # sinks of the prefix and behind it
+])
+def test_sinks_before_the_windows_of_many_rows(dev, T, Hq, Hkv, lens, new, plens, window, sinks):
+    """Row blocks whose windows start pages behind the sinks, on them, and before them."""
+    Setup(T, Hq, Hkv, lens, new, plens, seed=25).check(window, sinks)
+
+
+def test_sinks_leave_a_window_its_savings(dev):
+    """4096 new tokens with a window of 128: a few sinks are a page more for each row block (four
+    for three), not every page between them and its window as well (up to 65)."""
+    s = Setup(4096, 32, 8, [4096 + 64], seed=26)
+
+    def least(**kw):
+        t = []
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in "ab")
+            a.record()
+            for _ in range(4):
+                s.run(**kw)
+            b.record()
+            torch.cuda.synchronize()
+            t.append(a.elapsed_time(b))
+        return min(t)
+    assert least(window=128, sinks=4) < 3 * least(window=128)
