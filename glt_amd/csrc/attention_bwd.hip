@@ -65,11 +65,12 @@ constexpr float kOff = 0x1p-5f;
 // The two instructions on one accumulator after each other: in pairs of
 // accumulators, or the second part behind the first's four, 276 and 285.
 // dkdv, which gets D put right, takes two parts of ds and p in calls of at most
-// kFineRows tokens (one block of rows): few roundings do not average out there (7 to 11
-// tokens, 6 heads: dk 2.5 * 10^-3, in two parts 1.6) and the call is short (1 x 128, 32
-// and 8 heads, window 32, dkdv 11.8 and 12.5 us; 64 x 128 with every key 91 and 132).
-// In longer calls dk and dv stand at 2.35: two products of four more would be
-// needed for 1.66.
+// kFineRows tokens, one block of rows. What a part's rounding adds does not depend on T
+// (dk 1.66 * 10^-3 at 7 to 128 tokens, 2.34 at 129 to 1000): the bound is where the two
+// products more, of four, begin to cost. A few sequences leave most of the chip idle and
+// pay little (1 x 128, 32 and 8 heads, window 32, dkdv 11.8 and 12.5 us); many pay the
+// whole (64 x 128 with every key 91 and 132), but the rule leaves B out, so that a sequence
+// is rounded alike alone and in a batch.
 constexpr int kFineRows = 128;
 
 struct BwdArgs {

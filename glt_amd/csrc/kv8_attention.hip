@@ -544,7 +544,8 @@ __global__ void __launch_bounds__(WAVES * 64, 3) kv8_whole_kernel(const DecArgs 
 // 2048 over 8704 292 us, 0.88. Matrix instructions run 0.32 of the time and vector ones
 // 0.43: a SIMD overlaps them only in part (alone the products take 0.4 of the time, the softmax
 // 0.5, the conversion 0.1 and waiting for it 0.2). us at 512 and 2048 tokens, and of a prefix of
-// 16384 under 64 sequences, with the join: like this 118, 325, 58; two workgroups of
+// 16384 under 64 sequences, with the join, all before operands were read ahead: like this
+// 118, 325, 58; two workgroups of
 // four wavefronts a CU, each with its own converted pages, 125, 377, 56; both turns at once
 // 135, 428; conversion between the products 130, 365, 60; loads a phase earlier 130, 374,
 // 62; pages brought to L2 ahead 120, 323, 59; without raised priority 125, 370.

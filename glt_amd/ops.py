@@ -379,7 +379,7 @@ def attention_train(q, k, v, causal=True, scale=None, seq_lens=None, window=None
     as views of one projection output [B,T,(Hq+2Hkv)*hd]. seq_lens int32 [B]:
     the lengths of a padded batch (rows past them: zero output, lse -inf).
     window=W: of the keys up to itself a row reads the last W (its own among
-    them) and the first `sinks` of its sequence."""
+    them) and the first `sinks` of its sequence (up to 1024 where W < T)."""
     _check_window(window, sinks)
     d, (B, T, Hq, _, _), _ = _attn_train_desc(q, k, v, None, causal, scale, seq_lens)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -519,7 +519,7 @@ class Kv8Cache:
         """Attention of the new tokens q [B, T, Hq, 128] bf16 (written before)
         over the cache: (out [B, T, Hq, 128] bf16, lse [B, Hq, T] f32). Token p
         reads tokens j <= p, of which window=W leaves j > p - W and the first
-        `sinks`. prefix = (pages int32 [groups, m], lens int32 [groups]): each
+        `sinks` (0 without a window). prefix = (pages int32 [groups, m], lens int32 [groups]): each
         group of B / groups consecutive sequences continues these tokens, which are
         read once for the group. Rows past new_lens: zeros and -inf. workspace: a
         uint8 tensor of glt_kv8_attention_workspace_size bytes instead of a new

@@ -378,7 +378,8 @@ typedef struct {
  * log(sum exp) of each row's scaled scores. Statistics, sums and products in
  * f32; probabilities rounded to bf16 for the product with v. out may be q itself
  * (the same pointer and stride), otherwise it overlaps no input, and lse no other
- * tensor (GLT_ERR_INVALID_ARG). No workspace. */
+ * tensor (GLT_ERR_INVALID_ARG). Scaled scores stay below 2^28: past it f32's steps between
+ * scores leave the exponentials' range, and rows may come to NaN. No workspace. */
 glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
                                    void* out, float* lse, void* stream);
 
@@ -404,13 +405,16 @@ glt_status glt_attention_bwd(const glt_attn_desc* d, const void* q, const void* 
  * is 1. A window of T or more, with any number of sinks, gives
  * glt_attention_train_fwd's results. Tiles of 64 keys that no row of a block reads are not
  * visited: the work is T * (window + sinks), not T^2.
- * A NaN or infinity reaches rows that see a key of its tile, as without a window. */
+ * A NaN or infinity in k reaches the rows that see it. One in v, whose weight of 0 is
+ * multiplied, reaches each 32 rows of which one sees a key of its 64. */
 glt_status glt_attention_window_fwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
                                     const void* k, const void* v, void* out, float* lse, void* stream);
 /* Its backward, as glt_attention_bwd. The sums' order is fixed by the call's sizes (B, T,
  * heads, window, sinks): the same call gives the same bits, and a sequence's dk and dv may
  * round differently in a call of another size. dq takes its factor ds to 16 bits, and with
- * T of at most 128 dk and dv take ds and p so, also where the window hides nothing. */
+ * T of at most 128 dk and dv take ds and p so, also where the window hides nothing. A NaN
+ * or infinity of row t reaches dk and dv of each 32 keys of which one of t's 32 rows sees one;
+ * one in k or v reaches dq as v's do out, and through these rows their keys. */
 size_t glt_attention_window_bwd_workspace_size(const glt_attn_desc* d, int32_t window, int32_t sinks);
 glt_status glt_attention_window_bwd(const glt_attn_desc* d, int32_t window, int32_t sinks, const void* q,
                                     const void* k, const void* v, const void* out, const float* lse,
