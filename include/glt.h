@@ -378,8 +378,9 @@ typedef struct {
  * log(sum exp) of each row's scaled scores. Statistics, sums and products in
  * f32; probabilities rounded to bf16 for the product with v. out may be q itself
  * (the same pointer and stride), otherwise it overlaps no input, and lse no other
- * tensor (GLT_ERR_INVALID_ARG). Scaled scores stay below 2^28: past it f32's steps between
- * scores leave the exponentials' range, and rows may come to NaN. No workspace. */
+ * tensor (GLT_ERR_INVALID_ARG). Weights, and with them gradients, are off by some 2^-23 of
+ * the largest scaled score (f32), which stays below 2^28: past it rows may come to NaN.
+ * No workspace. */
 glt_status glt_attention_train_fwd(const glt_attn_desc* d, const void* q, const void* k, const void* v,
                                    void* out, float* lse, void* stream);
 
@@ -490,9 +491,9 @@ typedef struct {
  * and the codes, scaled in f32; probabilities times the value's step are rounded to bf16 for
  * the second product; all sums and statistics are f32, in an order that the call's sizes and
  * lengths fix (the same call gives the same bits; a sequence's may round differently
- * beside others). Rows t >= new_lens[b] get zeros and -inf. |q| < 2^112 (the codes' products stay in f32). q
- * overlaps neither out, lse nor the workspace, nor any of them each other or the
- * cache. workspace: glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing
+ * beside others). Rows t >= new_lens[b] get zeros and -inf. |q| < 2^112 (the codes'
+ * products stay in f32) and |v| < 2^88 (so do the sums before the division). q overlaps
+ * neither out, lse nor the workspace, nor any of them each other or the cache. workspace: glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing
  * kept in it between calls; where that is 0 it may be NULL. */
 size_t glt_kv8_attention_workspace_size(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d);
 glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d, const void* q,
