@@ -493,8 +493,9 @@ typedef struct {
  * lengths fix (the same call gives the same bits; a sequence's may round differently
  * beside others). Rows t >= new_lens[b] get zeros and -inf. |q| < 2^112 (the codes'
  * products stay in f32) and |v| < 2^88 (so do the sums before the division). q overlaps
- * neither out, lse nor the workspace, nor any of them each other or the cache. workspace: glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing
- * kept in it between calls; where that is 0 it may be NULL. */
+ * neither out, lse nor the workspace, nor any of them each other or the cache. workspace:
+ * glt_kv8_attention_workspace_size bytes, 256-byte aligned, nothing kept in it between
+ * calls; where that is 0 it may be NULL. */
 size_t glt_kv8_attention_workspace_size(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d);
 glt_status glt_kv8_attention(const glt_kv8_cache* c, const glt_kv8_seqs* s, const glt_kv8_attn* d, const void* q,
                              int64_t q_ld, void* out, int64_t o_ld, float* lse, void* workspace,
