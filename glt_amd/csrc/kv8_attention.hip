@@ -545,10 +545,13 @@ __global__ void __launch_bounds__(WAVES * 64, 3) kv8_whole_kernel(const DecArgs 
 // 0.43: a SIMD overlaps them only in part (alone the products take 0.4 of the time, the softmax
 // 0.5, the conversion 0.1 and waiting for it 0.2). us at 512 and 2048 tokens, and of a prefix of
 // 16384 under 64 sequences, with the join, all before operands were read ahead: like this
-// 118, 325, 58; two workgroups of
-// four wavefronts a CU, each with its own converted pages, 125, 377, 56; both turns at once
-// 135, 428; conversion between the products 130, 365, 60; loads a phase earlier 130, 374,
-// 62; pages brought to L2 ahead 120, 323, 59; without raised priority 125, 370.
+// 118, 325, 58; two workgroups of four wavefronts a CU, each with its own converted pages,
+// 125, 377, 56; both turns at once 135, 428; conversion between the products 130, 365, 60;
+// loads a phase earlier 130, 374, 62; pages brought to L2 ahead 120, 323, 59; without raised
+// priority 125, 370.
+//
+// With a window a row block walks the pages that hold sinks and those of its own window: 4096 new
+// tokens over 8192, window 128 53 us, with 4 sinks 59.
 constexpr int kManyWaves = 8;
 constexpr int kKFrag = 1040, kVFrag = 1056;           // bytes of an operand of 64 lanes
 constexpr int kKTile = 16 * kKFrag, kVTile = 16 * kVFrag;
